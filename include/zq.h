@@ -187,6 +187,74 @@ zq_status zq_dequantize(const zq_weight* w, float* out, void* stream);
  * Synchronous. */
 zq_status zq_dequantize_host(const zq_weight* w, float* out_host, void* stream);
 
+/* ---- operators around the matmul ---------------------------------------- */
+
+/* Element types of the operators below. */
+#define ZQ_DTYPE_F32 1
+#define ZQ_DTYPE_F16 2
+#define ZQ_DTYPE_BF16 3
+
+/* Root-mean-square norm with the residual's addition, ending in the codes
+ * that zq_matmul_codes multiplies.  For each of m rows of k elements:
+ *   s = x + residual, rounded to `dtype`, stored to residual_out
+ *       (s = x when residual is NULL)
+ *   r = fl32(1 / sqrt(mean(s^2) + eps)), the mean in 64 bits
+ *   v = fl32(fl32(s * r) * weight), stored to normed in `dtype`
+ *   q, row_scale = the activation quantizer's codes and scale of v
+ * so the codes and scales equal zq_quantize_rows over v bit for bit, and do
+ * not depend on the launch.  x, residual, residual_out and normed are
+ * [m][k] in `dtype` with row pitches in elements (>= k); weight is fp32 [k]
+ * or NULL (ones); q is int8 [m][ldq], ldq >= k, zeros in [k, ldq) (for
+ * zq_matmul_codes, ldq = zq_weight_padded_k); row_scale fp32 [m].  residual
+ * and residual_out go together; normed may be NULL.  An output may be the
+ * buffer of x or of residual (same pointer, same pitch); overlaps of any
+ * other kind are not allowed.  eps >= 0 and finite. */
+zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, size_t ldx, const void* residual,
+                               size_t ld_residual, const float* weight, double eps, void* residual_out,
+                               size_t ld_residual_out, void* normed, size_t ld_normed, int8_t* q, size_t ldq,
+                               float* row_scale, void* stream);
+
+/* Low-rank adapters of many requests added onto a shared projection's
+ * output: for each row i with 0 <= ids[i] < slots,
+ *   y[i] += scales[s] * B_s (A_s x[i]),   s = ids[i],
+ * over the first ranks[s] of max_rank (clamped to [0, max_rank]).  Rows with
+ * any other id are left as they are.  y is fp32 [m][n] with row pitch ldy
+ * (e.g. zq_matmul's output), x [m][k] of x_dtype with row pitch ldx; a
+ * [slots][max_rank][k] and b [slots][n][max_rank] contiguous, both w_dtype
+ * (ZQ_DTYPE_F16 or ZQ_DTYPE_BF16); ids int32 [m]; scales fp32 [slots] or NULL
+ * (ones); ranks int32 [slots] or NULL (max_rank).  The products are exact in
+ * the inputs' types and summed in fp32; A x is kept in fp32.  An infinite or
+ * NaN element of x[i] leaves y[i] infinite or NaN.  Each row's result depends on its own inputs only, not on the other rows of the call.
+ * max_rank <= ZQ_LOW_RANK_MAX, slots <= ZQ_LOW_RANK_MAX_SLOTS.  `workspace`
+ * (256-byte aligned) must hold zq_add_low_rank_workspace_bytes(m, slots)
+ * bytes (0 for few rows: NULL is then fine) and must not be shared by calls
+ * that may overlap on the GPU. */
+#define ZQ_LOW_RANK_MAX 256
+#define ZQ_LOW_RANK_MAX_SLOTS 8192
+size_t zq_add_low_rank_workspace_bytes(size_t m, size_t slots);
+zq_status zq_add_low_rank(float* y, size_t ldy, const void* x, int x_dtype, size_t ldx, size_t m, size_t k, size_t n,
+                          const void* a, const void* b, int w_dtype, size_t slots, size_t max_rank,
+                          const int32_t* ids, const float* scales, const int32_t* ranks, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/* Log probabilities over rows of logits [m][vocab] (`dtype`, row pitch ld):
+ *   logprobs[i][j] = log softmax(logits[i])[targets[i][j]]
+ *   entropy[i]     = -sum p log p (natural logarithm)
+ *   top_ids[i], top_logprobs[i]: the top_k most likely tokens in order; equal
+ *     logits go to the lower id
+ * all in fp32.  targets is int64 [m][n_targets] (n_targets may be 0); a
+ * negative target asks for nothing and gives 0, one >= vocab gives NaN.
+ * -inf logits are tokens that are not allowed; a row that allows none has
+ * every log probability -inf and entropy 0.  A NaN or +inf logit makes the
+ * row's log probabilities and entropy NaN; in the order of top_ids a NaN
+ * comes before every number.  entropy may be NULL; top_logprobs and top_ids
+ * are [m][top_k] and may be NULL when top_k is 0.
+ * top_k <= min(vocab, ZQ_LOGPROBS_MAX_TOP). */
+#define ZQ_LOGPROBS_MAX_TOP 32
+zq_status zq_token_logprobs(const void* logits, int dtype, size_t m, size_t vocab, size_t ld, const int64_t* targets,
+                            size_t n_targets, size_t top_k, float* logprobs, float* entropy, float* top_logprobs,
+                            int64_t* top_ids, void* stream);
+
 /* ---- column-sharded matmul over NCCL ------------------------------------ */
 
 /* Columns [*begin, *end) of rank `rank` when n_cols columns are split over

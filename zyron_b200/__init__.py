@@ -8,11 +8,15 @@ reference API used by the tests and the bench.  The C++20 drop-in lives in
 """
 from ._lib import (ZQCudaError, ZQDeviceTimeout, ZQError, ZQInvalidArgument, ZQOutOfRange, ZQOverflow,
                    ZQRuntimeError, lib)
+from .ops import (LowRankAdapters, NormQuantized, TokenLogprobs, add_low_rank, matmul_codes, rms_norm_quantize,
+                  token_logprobs)
 from .quantization import (QuantizedLinear, QuantizedMatrix, Type, device_error, matmul, quantize,
                            quantize_rows)
 
 __all__ = [
     "Type", "QuantizedMatrix", "QuantizedLinear", "quantize", "matmul", "quantize_rows", "device_error",
+    "rms_norm_quantize", "NormQuantized", "matmul_codes", "add_low_rank", "LowRankAdapters", "token_logprobs",
+    "TokenLogprobs",
     "ZQError", "ZQInvalidArgument", "ZQOutOfRange", "ZQOverflow", "ZQRuntimeError", "ZQCudaError",
     "ZQDeviceTimeout", "lib",
 ]

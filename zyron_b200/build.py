@@ -23,8 +23,8 @@ QLIB = os.path.join(HERE, "libzyron_quant.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
 CU_SOURCES = ["zq_api.cu", "zq_quant.cu", "zq_gemv.cu", "zq_gemm_sm100.cu", "zq_skinny_sm100.cu", "zq_noalloc.cu",
-              "zq_lm.cu", "zq_sharded.cu"]
-CU_HEADERS = ["zq_common.cuh", "zq_dot.cuh", "zq_tcgen05.cuh", "zq_kernels.h", "zq_internal.h"]
+              "zq_lm.cu", "zq_sharded.cu", "zq_norm.cu", "zq_lowrank.cu", "zq_logprobs.cu", "zq_ops.cu"]
+CU_HEADERS = ["zq_common.cuh", "zq_dot.cuh", "zq_elem.cuh", "zq_tcgen05.cuh", "zq_kernels.h", "zq_internal.h"]
 # Host-only C++ of the library, built by g++ with the reference's own Release
 # flags (-std=c++20 -O3 -DNDEBUG): zq_sample.cpp restates the reference's
 # token sampler, whose std::sort order and std::mt19937 draws come from the

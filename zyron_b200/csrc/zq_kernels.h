@@ -147,6 +147,55 @@ size_t skinny_scratch_bytes(int N, int M);
 cudaError_t launch_zero_words(int* p, int n, cudaStream_t stream);
 cudaError_t launch_skinny(const SkinnyArgs& a, cudaStream_t stream, bool pdl);
 
+// zq_rms_norm_quantize (zq_norm.cu); pitches in elements.
+struct NormArgs {
+    const void* x;
+    const void* residual;  // null: no addition
+    const float* weight;   // null: ones
+    void* residual_out;
+    void* normed;          // null: not written
+    int8_t* q;
+    float* row_scale;
+    long long ldx, ld_residual, ld_residual_out, ld_normed, ldq;
+    long long m;
+    int k;
+    double eps;
+};
+cudaError_t launch_rms_norm_quantize(const NormArgs& a, int dtype, cudaStream_t stream);
+
+// zq_token_logprobs (zq_logprobs.cu).
+constexpr int kTopMax = ZQ_LOGPROBS_MAX_TOP;
+struct LogprobArgs {
+    const void* logits;
+    long long ld;
+    long long m;
+    int vocab;
+    const int64_t* targets;  // [m][n_targets]
+    long long n_targets;
+    int top_k;
+    float* logprobs;
+    float* entropy;          // null: not written
+    float* top_logprobs;     // [m][top_k]
+    int64_t* top_ids;
+};
+cudaError_t launch_token_logprobs(const LogprobArgs& a, int dtype, cudaStream_t stream);
+
+// zq_add_low_rank (zq_lowrank.cu).
+struct LowRankArgs {
+    float* y;
+    const void* x;
+    const void* a;         // [slots][max_rank][k]
+    const void* b;         // [slots][n][max_rank]
+    const int32_t* ids;    // [m]
+    const float* scales;   // [slots], null: ones
+    const int32_t* ranks;  // [slots], null: max_rank
+    long long ldy, ldx;
+    long long m;
+    int k, n, slots, max_rank;
+};
+size_t low_rank_workspace_bytes(size_t m, size_t slots);
+cudaError_t launch_add_low_rank(const LowRankArgs& a, int x_dtype, int w_dtype, void* workspace, cudaStream_t stream);
+
 int gemm_block_n(int M, int N);
 
 // Multiprocessors of the current device available to the persistent kernels

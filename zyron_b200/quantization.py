@@ -350,7 +350,14 @@ class QuantizedLinear:
     def bias(self):
         return self._b
 
-    def forward(self, input, out=None, stream=None):
+    def forward(self, input, out=None, stream=None, adapters=None, adapter_ids=None):
+        """``adapters`` (ops.LowRankAdapters of this projection) with
+        ``adapter_ids`` (int32, input's leading dimensions) adds each row's
+        low-rank adapter onto the output; torch CUDA input only."""
+        if (adapters is None) != (adapter_ids is None):
+            raise _lib.ZQInvalidArgument("zyron_b200: adapters and adapter_ids go together")
+        if adapters is not None and isinstance(input, np.ndarray):
+            raise _lib.ZQInvalidArgument("zyron_b200: adapters need a CUDA tensor as input")
         ndim = input.ndim if isinstance(input, np.ndarray) else input.dim()
         if ndim < 2:
             raise _lib.ZQInvalidArgument("ZYRON QuantizedLinear: input rank must be >= 2")
@@ -359,6 +366,11 @@ class QuantizedLinear:
         bias = self._b
         if isinstance(input, np.ndarray) and bias is not None:
             bias = bias.cpu().numpy()
-        return matmul(input, self._w, bias=bias, out=out, stream=stream)
+        y = matmul(input, self._w, bias=bias, out=out, stream=stream)
+        if adapters is not None:
+            from .ops import add_low_rank
+
+            add_low_rank(y, input, *adapters[:2], adapter_ids, *adapters[2:], stream=stream)
+        return y
 
     __call__ = forward
