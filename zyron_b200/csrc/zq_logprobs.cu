@@ -688,20 +688,21 @@ cudaError_t launch(const LogprobArgs& a, int split, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, kTop, kWarps>, a, split);
 }
 
-#ifndef LP_SMALL
-#define LP_SMALL 4
-#endif
-#ifndef LP_FILL
-#define LP_FILL 8
-#endif
 template <class T, bool kTop>
 cudaError_t launch_rows(const LogprobArgs& a, cudaStream_t stream) {
-    if (a.m >= LP_SMALL * (long long)sm_count()) return launch<T, kTop, 4>(a, 1, stream);
-    // Enough CTAs to fill the SMs several times over, none with less than
-    // one full round of its threads' loads.
+    // Many rows: a block of 4 warps each, 6 rows an SM or more keep enough
+    // loads in flight and more rows are past their ends at any time (1024 x
+    // 150001 bf16, 8 alternatives: 78 us against 86 us with 8 warps; 600 x
+    // 100000: 46 us against 36 us).  The same where one round of 4 warps holds
+    // a row (600 x 2000 bf16: 9.4 us against 11.9 us).
+    const int sms = sm_count();
+    const long long packs = a.vocab / kElemsPer16<T>;
+    if (a.m >= 6LL * sms || packs <= 128 * kUnroll) return launch<T, kTop, 4>(a, 1, stream);
+    // Else CTAs of 8 warps, 4 an SM, none with less than a round: with 8 an SM
+    // the steps behind the pass cost more than the shorter passes save
+    // (300 x 100000 bf16, 8 alternatives: 24 us against 31 us).
     int split = 1;
-    const long long per_cta = 256LL * kUnroll * kElemsPer16<T>;
-    while (split < kMaxSplit && a.m * split < LP_FILL * (long long)sm_count() && a.vocab >= 2 * split * per_cta) split *= 2;
+    while (split < kMaxSplit && a.m * split < 4LL * sms && packs >= 2LL * split * 256 * kUnroll) split *= 2;
     return launch<T, kTop, 8>(a, split, stream);
 }
 
