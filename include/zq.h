@@ -224,14 +224,15 @@ zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, siz
  * (ZQ_DTYPE_F16 or ZQ_DTYPE_BF16); ids int32 [m]; scales fp32 [slots] or NULL
  * (ones); ranks int32 [slots] or NULL (max_rank).  The products are exact in
  * the inputs' types and summed in fp32; A x is kept in fp32.  An infinite or
- * NaN element of x[i] leaves y[i] infinite or NaN.  Each row's result depends on its own inputs only, not on the other rows of the call.
- * max_rank <= ZQ_LOW_RANK_MAX, slots <= ZQ_LOW_RANK_MAX_SLOTS.  `workspace`
- * (256-byte aligned) must hold zq_add_low_rank_workspace_bytes(m, slots)
- * bytes (0 for few rows: NULL is then fine) and must not be shared by calls
- * that may overlap on the GPU. */
+ * NaN element of x[i] leaves y[i] infinite or NaN.  A row's result depends
+ * on its own inputs and on the call's sizes, not on the other rows' values or
+ * their order.  max_rank <= ZQ_LOW_RANK_MAX, slots <= ZQ_LOW_RANK_MAX_SLOTS.
+ * `workspace` (256-byte aligned) must hold zq_add_low_rank_workspace_bytes
+ * bytes (on the same device) and must not be shared by calls that may overlap
+ * on the GPU. */
 #define ZQ_LOW_RANK_MAX 256
 #define ZQ_LOW_RANK_MAX_SLOTS 8192
-size_t zq_add_low_rank_workspace_bytes(size_t m, size_t slots);
+size_t zq_add_low_rank_workspace_bytes(size_t m, size_t k, size_t n, size_t slots, size_t max_rank);
 zq_status zq_add_low_rank(float* y, size_t ldy, const void* x, int x_dtype, size_t ldx, size_t m, size_t k, size_t n,
                           const void* a, const void* b, int w_dtype, size_t slots, size_t max_rank,
                           const int32_t* ids, const float* scales, const int32_t* ranks, void* workspace,

@@ -197,14 +197,14 @@ def test_matmul_codes_equals_matmul(zb, torch, m, k, n, qtype):
 def adapter_oracle(torch, y, x, a, b, ids, scales, ranks):
     """In 64 bits, with the bound that the kernel's roundings allow: one of
     2^-23 (the tensor cores may cut off) for each of the 16 products and the
-    carry of the MMAs that a sum goes through, one for each of the at most 16
-    partial sums of A x, and half of one each for the scaling and for the sum
-    with y.  Three-part products of fp32 and fp16 inputs are exact."""
+    carry of the MMAs that a sum goes through, at most all of k's, one for each
+    partial sum of A x, at most 16 or one for 32 of k, and half of one each for
+    the scaling and for the sum with y.  Products of parts are exact."""
     y64, x64 = y.double().clone(), x.double()
     tol = y64.abs() * 2.0**-24
     parts = {"float32": 3, "float16": 2, "bfloat16": 1}[str(x.dtype).split(".")[1]] * (2 if a.dtype == torch.float16 else 1)
     k, rank = a.shape[2], a.shape[1]
-    steps_a = -(-k // (32 * 64)) * 2 * parts * 17 + 16
+    steps_a = -(-k // 32) * 2 * parts * 17 + max(16, -(-k // 32))
     steps_b = -(-rank // 32) * 2 * 3 * (2 if a.dtype == torch.float16 else 1) * 17
     for i, s in enumerate(ids.tolist()):
         if not 0 <= s < a.shape[0]:
@@ -313,16 +313,22 @@ def test_adapters_infinities(zb, torch):
     assert ((got.double() - want).abs() <= tol)[rest].all()
 
 
-def test_adapters_rows_do_not_depend_on_others(zb, torch):
-    """A row's bits are the same alone, among few rows, among sorted many."""
-    y, x, a, b, ids, scales, ranks = adapter_case(torch, 600, 200, 100, 3, 24, "float32", "bfloat16", "mixed", False)
-    dev = [t.cuda() for t in (x, a, b, ids, scales)]
-    every = zb.add_low_rank(y.cuda(), *dev[:4], scales=dev[4])
-    again = zb.add_low_rank(y.cuda(), *dev[:4], scales=dev[4])
-    same_bits(torch, again, every, "twice")
-    for rows in (slice(5, 6), slice(0, 40), slice(100, 340)):
-        part = zb.add_low_rank(y[rows].cuda(), dev[0][rows], dev[1], dev[2], dev[3][rows], scales=dev[4])
-        same_bits(torch, part, every[rows], f"rows {rows}")
+@pytest.mark.parametrize("m", [200, 600])
+def test_adapters_rows_do_not_depend_on_others(zb, torch, m):
+    """A row's bits are the same twice, with the rows in another order, and
+    with other values and adapters in the other rows."""
+    y, x, a, b, ids, scales, ranks = adapter_case(torch, m, 200, 100, 3, 24, "float32", "bfloat16", "mixed", False)
+    y, x, a, b, ids, scales = (t.cuda() for t in (y, x, a, b, ids, scales))
+    every = zb.add_low_rank(y.clone(), x, a, b, ids, scales=scales)
+    same_bits(torch, zb.add_low_rank(y.clone(), x, a, b, ids, scales=scales), every, "twice")
+    order = torch.randperm(m, generator=torch.Generator().manual_seed(2)).cuda()
+    moved = zb.add_low_rank(y[order], x[order], a, b, ids[order], scales=scales)
+    same_bits(torch, moved, every[order], "in another order")
+    x2, ids2 = x * 3 + 1, (ids + 2) % 3
+    keep = torch.arange(m, device="cuda") % 7 == 3
+    x2[keep], ids2[keep] = x[keep], ids[keep]
+    part = zb.add_low_rank(y.clone(), x2, a, b, ids2.int(), scales=scales)
+    same_bits(torch, part[keep], every[keep], "among others")
 
 
 @pytest.mark.parametrize("m", [5, 400])

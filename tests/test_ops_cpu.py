@@ -66,12 +66,15 @@ def test_adapter_refusals(native_lib):
         refused(adapters(L, **{bad: None}), "null pointer")
     refused(adapters(L, n=1 << 31, ldy=1 << 31), "dimension too large", _lib.ZQ_ERR_OVERFLOW)
     refused(adapters(L, y=C.c_void_p(2)), "a pointer is not aligned to its element type")
-    need = L.zq_add_low_rank_workspace_bytes(5000, 2)
+    need = L.zq_add_low_rank_workspace_bytes(5000, 64, 32, 2, 8)
     assert need > 5000 * 4 and need % 256 == 0
+    assert L.zq_add_low_rank_workspace_bytes(1, 4096, 4096, 8, 16) > 0
+    for none in ((0, 64, 32, 2, 8), (5, 0, 32, 2, 8), (5, 64, 0, 2, 8), (5, 64, 32, 0, 8), (5, 64, 32, 2, 0),
+                 (5, 64, 32, 8193, 8), (5, 64, 32, 2, 257), (1 << 31, 64, 32, 2, 8)):
+        assert L.zq_add_low_rank_workspace_bytes(*none) == 0
     refused(adapters(L, m=5000), f"workspace too small (0 < {need} bytes)")
     refused(adapters(L, m=5000, ws=P, ws_bytes=need - 1), f"workspace too small ({need - 1} < {need} bytes)")
     refused(adapters(L, m=5000, ws=C.c_void_p((1 << 20) + 64), ws_bytes=need), "workspace must be 256-byte aligned")
-    assert L.zq_add_low_rank_workspace_bytes(1, 8192) == 0
 
 
 def logprobs(L, x=P, dtype=1, m=4, vocab=100, ld=100, targets=P, n=1, top=0, lp=P, ent=None, top_lp=None, top_ids=None):

@@ -193,7 +193,7 @@ struct LowRankArgs {
     long long m;
     int k, n, slots, max_rank;
 };
-size_t low_rank_workspace_bytes(size_t m, size_t slots);
+size_t low_rank_workspace_bytes(const LowRankArgs& a);  // m > 0
 cudaError_t launch_add_low_rank(const LowRankArgs& a, int x_dtype, int w_dtype, void* workspace, cudaStream_t stream);
 
 int gemm_block_n(int M, int N);

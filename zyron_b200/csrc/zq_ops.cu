@@ -74,9 +74,17 @@ zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, siz
     return e == cudaSuccess ? ZQ_OK : zq::cuda_error(e, "rms_norm_quantize");
 }
 
-size_t zq_add_low_rank_workspace_bytes(size_t m, size_t slots) {
-    if (m > kIntMax || slots > ZQ_LOW_RANK_MAX_SLOTS) return 0;
-    return zq::low_rank_workspace_bytes(m, slots);
+size_t zq_add_low_rank_workspace_bytes(size_t m, size_t k, size_t n, size_t slots, size_t max_rank) {
+    if (m == 0 || m > kIntMax || k == 0 || k > kIntMax / 2 || n == 0 || n > kIntMax / 2 || slots == 0 ||
+        slots > ZQ_LOW_RANK_MAX_SLOTS || max_rank == 0 || max_rank > ZQ_LOW_RANK_MAX)
+        return 0;
+    zq::LowRankArgs r{};
+    r.m = (long long)m;
+    r.k = (int)k;
+    r.n = (int)n;
+    r.slots = (int)slots;
+    r.max_rank = (int)max_rank;
+    return zq::low_rank_workspace_bytes(r);
 }
 
 zq_status zq_add_low_rank(float* y, size_t ldy, const void* x, int x_dtype, size_t ldx, size_t m, size_t k, size_t n,
@@ -105,13 +113,13 @@ zq_status zq_add_low_rank(float* y, size_t ldy, const void* x, int x_dtype, size
     if (!aligned(y, 4) || !aligned(x, size) || !aligned(a, 2) || !aligned(b, 2) || !aligned(ids, 4) ||
         !aligned(scales, 4) || !aligned(ranks, 4))
         return invalid("zyron_b200: a pointer is not aligned to its element type");
-    const size_t need = zq::low_rank_workspace_bytes(m, slots);
-    if (need && (!workspace || workspace_bytes < need)) {
+    const size_t need = zq_add_low_rank_workspace_bytes(m, k, n, slots, max_rank);
+    if (!workspace || workspace_bytes < need) {
         char buf[128];
         std::snprintf(buf, sizeof buf, "zyron_b200: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
         return invalid(buf);
     }
-    if (need && !aligned(workspace, 256)) return invalid("zyron_b200: workspace must be 256-byte aligned");
+    if (!aligned(workspace, 256)) return invalid("zyron_b200: workspace must be 256-byte aligned");
     zq::LowRankArgs r{};
     r.y = y;
     r.x = x;

@@ -243,11 +243,9 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
         xr, ldx = _rows(x, "x")
         ids = ids.contiguous()
         m = xr.shape[0]
-        need = lib().zq_add_low_rank_workspace_bytes(m, slots)
-        ws = base = None
-        if need:
-            ws = torch.empty(need + 256, dtype=torch.uint8, device=x.device)
-            base = (ws.data_ptr() + 255) & ~255
+        need = lib().zq_add_low_rank_workspace_bytes(m, k, n, slots, max_rank)
+        ws = torch.empty(need + 256, dtype=torch.uint8, device=x.device)
+        base = (ws.data_ptr() + 255) & ~255
         check(lib().zq_add_low_rank(yr.data_ptr(), ldy, xr.data_ptr(), xt, ldx, m, k, n, a.data_ptr(), b.data_ptr(),
                                     wt, slots, max_rank, ids.data_ptr(), _ptr(scales), _ptr(ranks), base, need, ptr))
     return y
