@@ -29,16 +29,23 @@ from .quantization import QuantizedMatrix, _torch
 if typing.TYPE_CHECKING:
     from torch import Tensor
 
-_DTYPES = None
 _NO_CONTEXT = contextlib.nullcontext()
 
 
-def _dtypes():
-    global _DTYPES
-    if _DTYPES is None:
-        torch = _torch()
-        _DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}  # ZQ_DTYPE_*
+def _setup():
+    """Element type codes (ZQ_DTYPE_*) and the current stream's raw handle by
+    device index; torch is imported at the first call."""
+    global _DTYPES, _raw_stream
+    torch = _torch()
+    _DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if _raw_stream is None:
+        _raw_stream = lambda index: torch.cuda.current_stream(index).cuda_stream  # noqa: E731
     return _DTYPES
+
+
+_DTYPES = None
+_raw_stream = None
 
 
 def _bad(msg):
@@ -46,30 +53,43 @@ def _bad(msg):
 
 
 def _dtype(t, name):
-    d = _dtypes().get(t.dtype)
+    d = (_DTYPES or _setup()).get(t.dtype)
     if d is None:
         raise _bad(f"{name} must be float32, float16 or bfloat16")
     return d
 
 
-def _same_device(first, **others):
-    if not first.is_cuda:
+def _device(first, **others):
+    """The CUDA device index that all tensors (or None) are on."""
+    index = first.get_device()
+    if index < 0:
         raise _bad("tensors must be on a CUDA device")
     for name, t in others.items():
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != index:
             raise _bad(f"{name} is on {t.device}, not on {first.device}")
+    return index
 
 
-def _context(device, stream):
-    """(context manager, stream pointer): inside, `device` is current and
+def _context(index, stream):
+    """(context manager, stream pointer): inside, the device is current and
     allocations belong to the stream."""
     torch = _torch()
     if stream is None:
-        ptr = torch.cuda.current_stream(device).cuda_stream
-        return (_NO_CONTEXT if torch.cuda.current_device() == device.index else torch.cuda.device(device)), ptr
-    if stream.device != device:
-        raise _bad(f"the stream is on {stream.device}, not on {device}")
+        return (_NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)), _raw_stream(index)
+    if stream.device.index != index:
+        raise _bad(f"the stream is on {stream.device}, not on cuda:{index}")
     return torch.cuda.stream(stream), stream.cuda_stream
+
+
+def _empty(shape, dtype, device):
+    """A new contiguous tensor.  Strides given make the cheapest allocating
+    call: at small sizes a call's time is its host time."""
+    torch = _torch()
+    if len(shape) == 1:
+        return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
+    if len(shape) == 2:
+        return torch.empty_strided(shape, (shape[1] or 1, 1), dtype=dtype, device=device)
+    return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _rows(t, name):
@@ -79,20 +99,22 @@ def _rows(t, name):
     k = t.shape[-1]
     if t.dim() != 2:
         t = t.reshape(-1, k) if k else t.reshape(0, 0)
-    if t.stride(1) != 1 and k > 1 or (t.shape[0] > 1 and t.stride(0) < k):
-        t = t.contiguous()
+    if t.is_contiguous():
+        return t, k
+    if (t.stride(1) != 1 and k > 1) or (t.shape[0] > 1 and t.stride(0) < k):
+        return t.contiguous(), k
     return t, (t.stride(0) if t.shape[0] > 1 else k)
 
 
 def _out_rows(t, name, shape, dtype):
     """An output given by the caller as rows; never copied."""
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
+    if t.shape != shape or t.dtype != dtype:
         raise _bad(f"{name} must have shape {tuple(shape)} and type {dtype}")
-    k = t.shape[-1]
+    k = shape[-1]
+    if t.is_contiguous():
+        return (t if t.dim() == 2 else t.view(-1, k)), k
     if t.dim() != 2:
-        if not t.is_contiguous():
-            raise _bad(f"{name} must be contiguous or rank 2")
-        t = t.view(-1, k)
+        raise _bad(f"{name} must be contiguous or rank 2")
     if (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < k):
         raise _bad(f"{name} must have contiguous rows that do not overlap")
     return t, (t.stride(0) if t.shape[0] > 1 else k)
@@ -122,36 +144,40 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
     ``normed=True`` also returns the normed rows, e.g. for adapters."""
     torch = _torch()
     dtype = _dtype(x, "x")
-    _same_device(x, weight=weight, residual=residual, residual_out=residual_out)
-    lead, k = x.shape[:-1], x.shape[-1] if x.dim() else 0
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise _bad("residual must have x's shape and type")
-    if residual is None and residual_out is not None:
+    index = _device(x, weight=weight, residual=residual, residual_out=residual_out)
+    shape = x.shape
+    lead, k = shape[:-1], shape[-1] if len(shape) else 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != x.dtype:
+            raise _bad("residual must have x's shape and type")
+    elif residual_out is not None:
         raise _bad("residual and residual_out go together")
-    if weight is not None and (weight.dtype != torch.float32 or weight.dim() != 1 or weight.shape[0] != k
-                               or not weight.is_contiguous()):
+    if weight is not None and (weight.dtype != torch.float32 or weight.shape != (k,) or not weight.is_contiguous()):
         raise _bad("weight must be contiguous float32 of x's last dimension")
-    context, ptr = _context(x.device, stream)
+    context, ptr = _context(index, stream)
     with context:
         xr, ldx = _rows(x, "x")
         m = xr.shape[0]
+        device = x.device
         rr = so = n = None
         ldr = lds = 0
         if residual is not None:
             rr, ldr = _rows(residual, "residual")
             if residual_out is None:
-                residual_out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-            so, lds = _out_rows(residual_out, "residual_out", x.shape, x.dtype)
+                so = residual_out = _empty(shape, x.dtype, device)
+                lds = k
+            else:
+                so, lds = _out_rows(residual_out, "residual_out", shape, x.dtype)
         if normed:
-            n = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            n = _empty(shape, x.dtype, device)
         kp = (k + 127) // 128 * 128
-        codes = torch.empty((m, kp), dtype=torch.int8, device=x.device)
-        scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+        codes = _empty((m, kp), torch.int8, device)
+        scale = _empty(lead, torch.float32, device)
         check(lib().zq_rms_norm_quantize(xr.data_ptr(), dtype, m, k, ldx, _ptr(rr), ldr, _ptr(weight), eps, _ptr(so),
                                          lds, _ptr(n), k, codes.data_ptr(), kp, scale.data_ptr(), ptr))
     if kp != k:
         codes = codes[:, :k]
-    if x.dim() != 2:
+    if len(shape) != 2:
         codes = codes.unflatten(0, lead) if lead else codes[0]
     return NormQuantized(codes, scale, residual_out, n)
 
@@ -170,15 +196,16 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
     lead = codes.shape[:-1]
     if codes.dtype != torch.int8 or row_scale.dtype != torch.float32 or row_scale.shape != lead:
         raise _bad("codes must be int8 [..., K] and row_scale float32 [...]")
-    _same_device(codes, row_scale=row_scale, bias=bias, out=out)
-    if weights._device != codes.device.index:
+    index = _device(codes, row_scale=row_scale, bias=bias, out=out)
+    if weights._device != index:
         raise _bad(f"the weights are on cuda:{weights._device}, not on {codes.device}")
     n = weights.cols()
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
         raise _bad("bias must be contiguous float32 of the output's last dimension")
     if out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (*lead, n) or not out.is_contiguous()):
         raise _bad("out must be contiguous float32 [..., N]")
-    context, ptr = _context(codes.device, stream)
+    _raw_stream or _setup()
+    context, ptr = _context(index, stream)
     with context:
         q, pitch = _rows(codes, "codes")
         m = q.shape[0]
@@ -190,9 +217,9 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
             q = padded
         scale = row_scale.contiguous()
         if out is None:
-            out = torch.empty((*lead, n), dtype=torch.float32, device=q.device)
+            out = _empty((*lead, n), torch.float32, q.device)
         need = lib().zq_matmul_workspace_bytes(weights.handle, m)
-        ws = torch.empty(need + 256, dtype=torch.uint8, device=q.device)
+        ws = _empty((need + 256,), torch.uint8, q.device)
         base = (ws.data_ptr() + 255) & ~255
         check(lib().zq_matmul_codes(weights.handle, q.data_ptr(), scale.data_ptr(), m, _ptr(bias), out.data_ptr(),
                                     base, need, ptr))
@@ -221,14 +248,17 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
     torch = _torch()
     xt = _dtype(x, "x")
     wt = _dtype(a, "a")
-    _same_device(x, y=y, a=a, b=b, ids=ids, scales=scales, ranks=ranks)
-    if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2]:
+    index = _device(x, y=y, a=a, b=b, ids=ids, scales=scales, ranks=ranks)
+    if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype:
         raise _bad("a must be [slots, max_rank, in] and b [slots, out, max_rank], of one type")
     slots, max_rank, k = a.shape
-    n = b.shape[1]
-    if x.dim() < 1 or x.shape[-1] != k:
+    b_slots, n, b_rank = b.shape
+    if slots != b_slots or max_rank != b_rank:
+        raise _bad("a must be [slots, max_rank, in] and b [slots, out, max_rank], of one type")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] != k:
         raise _bad("input/adapter dimension mismatch")
-    lead = x.shape[:-1]
+    lead = shape[:-1]
     if not a.is_contiguous() or not b.is_contiguous():
         raise _bad("a and b must be contiguous")
     if ids.dtype != torch.int32 or ids.shape != lead:
@@ -238,13 +268,14 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
     if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != (slots,) or not ranks.is_contiguous()):
         raise _bad("ranks must be contiguous int32 [slots]")
     yr, ldy = _out_rows(y, "y", (*lead, n), torch.float32)
-    context, ptr = _context(x.device, stream)
+    context, ptr = _context(index, stream)
     with context:
         xr, ldx = _rows(x, "x")
-        ids = ids.contiguous()
+        if not ids.is_contiguous():
+            ids = ids.contiguous()
         m = xr.shape[0]
         need = lib().zq_add_low_rank_workspace_bytes(m, k, n, slots, max_rank)
-        ws = torch.empty(need + 256, dtype=torch.uint8, device=x.device)
+        ws = _empty((need + 256,), torch.uint8, x.device)
         base = (ws.data_ptr() + 255) & ~255
         check(lib().zq_add_low_rank(yr.data_ptr(), ldy, xr.data_ptr(), xt, ldx, m, k, n, a.data_ptr(), b.data_ptr(),
                                     wt, slots, max_rank, ids.data_ptr(), _ptr(scales), _ptr(ranks), base, need, ptr))
@@ -271,34 +302,37 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=True, stream=None):
     none has log probabilities of -inf and entropy 0."""
     torch = _torch()
     dtype = _dtype(logits, "logits")
-    _same_device(logits, targets=targets)
-    if logits.dim() < 1:
+    index = _device(logits, targets=targets)
+    shape = logits.shape
+    if len(shape) < 1:
         raise _bad("logits rank must be >= 1")
-    lead, vocab = logits.shape[:-1], logits.shape[-1]
+    lead, vocab = shape[:-1], shape[-1]
     n = 0
     if targets is not None:
         if targets.dtype != torch.int64:
             raise _bad("targets must be int64")
         if targets.shape == lead:
             n = 1
-        elif targets.dim() == logits.dim() and targets.shape[:-1] == lead:
+        elif targets.dim() == len(shape) and targets.shape[:-1] == lead:
             n = targets.shape[-1]
         else:
             raise _bad("targets must have logits' leading dimensions, and one more at most")
     if top_k < 0:
         raise _bad("top_k must be >= 0")
-    context, ptr = _context(logits.device, stream)
+    context, ptr = _context(index, stream)
     with context:
         rows, ld = _rows(logits, "logits")
+        device = logits.device
         lp = ent = top_lp = top_ids = None
         if targets is not None:
-            targets = targets.contiguous()
-            lp = torch.empty(targets.shape, dtype=torch.float32, device=logits.device)
+            if not targets.is_contiguous():
+                targets = targets.contiguous()
+            lp = _empty(targets.shape, torch.float32, device)
         if entropy:
-            ent = torch.empty(lead, dtype=torch.float32, device=logits.device)
+            ent = _empty(lead, torch.float32, device)
         if top_k:
-            top_lp = torch.empty((*lead, top_k), dtype=torch.float32, device=logits.device)
-            top_ids = torch.empty((*lead, top_k), dtype=torch.int64, device=logits.device)
+            top_lp = _empty((*lead, top_k), torch.float32, device)
+            top_ids = _empty((*lead, top_k), torch.int64, device)
         check(lib().zq_token_logprobs(rows.data_ptr(), dtype, rows.shape[0], vocab, ld, _ptr(targets), n, top_k,
                                       _ptr(lp), _ptr(ent), _ptr(top_lp), _ptr(top_ids), ptr))
     return TokenLogprobs(lp, ent, top_lp, top_ids)
