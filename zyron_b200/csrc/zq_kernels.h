@@ -160,6 +160,9 @@ struct NormArgs {
     long long m;
     int k;
     double eps;
+    // filled in by the launcher
+    double inv_k = 0.0;
+    bool wide_codes = false;  // packs of codes lie on their own size
 };
 cudaError_t launch_rms_norm_quantize(const NormArgs& a, int dtype, cudaStream_t stream);
 

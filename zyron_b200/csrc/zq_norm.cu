@@ -12,9 +12,12 @@
 // every code -- does not depend on the launch shape: a last-bit change of r
 // would carry values across the codes' rounding borders.
 //
-// Bound: one read of x and residual and one write of the sum and the codes,
-// at about 20 operations an element, so memory bandwidth.  A row stays in the
-// registers of one group of threads from its load to its stores.
+// Bound: one read of x and residual and one write of the sum and the codes:
+// memory bandwidth, if an element takes few instructions (at 16 bits and 8192
+// columns there is time for about 25 of them).  So a row stays in the registers
+// of one group of threads from its load to its stores, 16-bit sums are added
+// in pairs, and a code is read off a sum with 1.5 * 2^23 unless it is near a
+// tie.
 #include "zq_common.cuh"
 #include "zq_elem.cuh"
 #include "zq_kernels.h"
@@ -56,22 +59,123 @@ __device__ __forceinline__ float group_max(float v, float* part) {
     return v;
 }
 
-__device__ __forceinline__ float row_rstd(double sum, int K, double eps) {
-    return (float)__ddiv_rn(1.0, __dsqrt_rn(sum / (double)K + eps));
+// fl32(1 / sqrt(sum / k + eps)).  Two Newton steps from the hardware's estimate
+// (2^-20) leave the 64-bit value within a few of its last bits: the fp32
+// rounding is that of the division's result unless it lies within 2^-50 of a
+// border between two fp32 values.
+__device__ __forceinline__ float row_rstd(double sum, double inv_k, double eps) {
+    const double a = fma(sum, inv_k, eps);
+    if (!(a > 1e-290 && a < 1e290)) return (float)__ddiv_rn(1.0, __dsqrt_rn(a));
+    double y;
+    asm("rsqrt.approx.ftz.f64 %0, %1;" : "=d"(y) : "d"(a));
+    const double h = 0.5 * a;
+    y = y * fma(-h * y, y, 1.5);
+    y = y * fma(-h * y, y, 1.5);
+    return (float)y;
 }
 
 __device__ __forceinline__ float norm_value(float s, float rstd, float w) {
     return __fmul_rn(__fmul_rn(s, rstd), w);
 }
 
-// A row of at most 32 * kWarps * kPacks packs of kN elements, held in the
-// registers of kWarps warps.  kN is what one memory access carries: 16 bytes
-// of T where every row and width allows it, else one element.
-template <class T, int kN, int kWarps, int kPacks>
-__global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256)
+// a + b, rounded to the type.  16-bit sums in pairs: rounding the exact sum
+// once equals rounding it to fp32 first, since a sum that fp32 cannot hold has
+// one term below the other's last 16-bit place.
+template <int kN>
+__device__ __forceinline__ void add_packs(Pack<float, kN>& a, const Pack<float, kN>& b) {
+#pragma unroll
+    for (int j = 0; j < kN; ++j) a.e[j] = __fadd_rn(a.e[j], b.e[j]);
+}
+template <int kN>
+__device__ __forceinline__ void add_packs(Pack<__half, kN>& a, const Pack<__half, kN>& b) {
+#pragma unroll
+    for (int j = 0; j + 1 < kN; j += 2) {
+        const __half2 s = __hadd2_rn(__halves2half2(a.e[j], a.e[j + 1]), __halves2half2(b.e[j], b.e[j + 1]));
+        a.e[j] = __low2half(s), a.e[j + 1] = __high2half(s);
+    }
+}
+template <int kN>
+__device__ __forceinline__ void add_packs(Pack<__nv_bfloat16, kN>& a, const Pack<__nv_bfloat16, kN>& b) {
+#pragma unroll
+    for (int j = 0; j + 1 < kN; j += 2) {
+        const __nv_bfloat162 s =
+            __hadd2_rn(__halves2bfloat162(a.e[j], a.e[j + 1]), __halves2bfloat162(b.e[j], b.e[j + 1]));
+        a.e[j] = __low2bfloat16(s), a.e[j + 1] = __high2bfloat16(s);
+    }
+}
+
+__device__ __noinline__ int divided_code(float n, float scale) { return zq_quantize_value(n, scale, 127); }
+
+// The codes of n[0..kN), as zq_quantize_value gives them.  y = n * rcp lies
+// within 2.3e-5 of the quotient that is to be rounded (zq_quantize_value_rcp),
+// and at most at 127 (1 + 2^-22).  y + 1.5 * 2^23 rounds y to a whole number,
+// which its low bits hold.  Nearer than 3e-5 to a tie, and for NaN, the
+// division decides.
+template <int kN>
+__device__ __forceinline__ Pack<int8_t, kN> codes_of(const float (&n)[kN], float scale, float rcp) {
+    constexpr float kMagic = 12582912.0f;
+    float t[kN];
+    bool clear = true;
+#pragma unroll
+    for (int j = 0; j < kN; ++j) {
+        const float y = __fmul_rn(n[j], rcp);
+        t[j] = __fadd_rn(y, kMagic);
+        clear = clear && fabsf(__fadd_rn(y, -__fadd_rn(t[j], -kMagic))) < 0.5f - 3.0e-5f;
+    }
+    Pack<int8_t, kN> c;
+    if (clear) {
+        if constexpr (kN % 4 == 0) {
+#pragma unroll
+            for (int j = 0; j < kN; j += 4) {
+                const uint32_t w = __byte_perm(__byte_perm(__float_as_uint(t[j]), __float_as_uint(t[j + 1]), 0x0040),
+                                               __byte_perm(__float_as_uint(t[j + 2]), __float_as_uint(t[j + 3]), 0x0040),
+                                               0x5410);
+                memcpy(&c.e[j], &w, 4);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) c.e[j] = (int8_t)__float_as_uint(t[j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) c.e[j] = (int8_t)divided_code(n[j], scale);
+    }
+    return c;
+}
+
+// The kN elements of a row from p * kN on, as far as k; zeros behind.  kAligned:
+// rows start on 16 bytes and k is a multiple of kN.  Else a lane's elements
+// come one by one, out of lines that its first access brought to L1.
+template <bool kAligned, class T, int kN>
+__device__ __forceinline__ Pack<T, kN> load_pack(const T* row, int p, int k) {
+    Pack<T, kN> v;
+    if (kAligned) {
+        v = reinterpret_cast<const Pack<T, kN>*>(row)[p];
+    } else {
+#pragma unroll
+        for (int j = 0; j < kN; ++j) v.e[j] = p * kN + j < k ? row[p * kN + j] : T(0.0f);
+    }
+    return v;
+}
+template <bool kAligned, class T, int kN>
+__device__ __forceinline__ void store_pack(T* row, int p, int k, const Pack<T, kN>& v) {
+    if (kAligned) {
+        reinterpret_cast<Pack<T, kN>*>(row)[p] = v;
+    } else {
+#pragma unroll
+        for (int j = 0; j < kN; ++j)
+            if (p * kN + j < k) row[p * kN + j] = v.e[j];
+    }
+}
+
+// A row of at most 32 * kWarps * kPacks packs of 16 bytes, held in the
+// registers of kWarps warps.
+template <class T, int kWarps, int kPacks, bool kAligned>
+__global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1 : 3)
     rms_norm_quantize_kernel(const NormArgs a) {
     pdl_launch_dependents();
     pdl_wait_primary();
+    constexpr int kN = kElemsPer16<T>;
     constexpr int kBlockWarps = kWarps > 8 ? kWarps : 8;
     constexpr int kThreads = 32 * kWarps;
     __shared__ double part_sum[kBlockWarps];
@@ -79,37 +183,35 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256)
     const long long row = (long long)blockIdx.x * (kBlockWarps / kWarps) + threadIdx.x / kThreads;
     const int t = threadIdx.x % kThreads;
     const bool live = row < a.m;
-    const int packs = a.k / kN;
+    const int packs = live ? (a.k + kN - 1) / kN : 0;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    const T* res = static_cast<const T*>(a.residual) + row * a.ld_residual;
+    T* sum_out = static_cast<T*>(a.residual_out) + row * a.ld_residual_out;
     using P = Pack<T, kN>;
-    const P* x = reinterpret_cast<const P*>(static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx);
-    const P* res = reinterpret_cast<const P*>(static_cast<const T*>(a.residual) + (live ? row : 0) * a.ld_residual);
-    P* sum_out = reinterpret_cast<P*>(static_cast<T*>(a.residual_out) + (live ? row : 0) * a.ld_residual_out);
 
     P v[kPacks];
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
         const int p = t + i * kThreads;
-        if (live && p < packs)
-            v[i] = x[p];
+        if (p < packs)
+            v[i] = load_pack<kAligned, T, kN>(x, p, a.k);
         else
 #pragma unroll
-            for (int j = 0; j < kN; ++j) v[i].e[j] = from_float<T>(0.0f);
+            for (int j = 0; j < kN; ++j) v[i].e[j] = T(0.0f);
     }
     if (a.residual) {
         P r[kPacks];
 #pragma unroll
         for (int i = 0; i < kPacks; ++i) {
             const int p = t + i * kThreads;
-            if (live && p < packs) r[i] = res[p];
+            if (p < packs) r[i] = load_pack<kAligned, T, kN>(res, p, a.k);
         }
 #pragma unroll
         for (int i = 0; i < kPacks; ++i) {
             const int p = t + i * kThreads;
-            if (live && p < packs) {
-#pragma unroll
-                for (int j = 0; j < kN; ++j)
-                    v[i].e[j] = from_float<T>(__fadd_rn(to_float(v[i].e[j]), to_float(r[i].e[j])));
-                sum_out[p] = v[i];
+            if (p < packs) {
+                add_packs(v[i], r[i]);
+                store_pack<kAligned, T, kN>(sum_out, p, a.k, v[i]);
             }
         }
     }
@@ -122,21 +224,24 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256)
             sum = __fma_rn(d, d, sum);
         }
     sum = group_sum<kWarps>(sum, part_sum);
-    const float rstd = row_rstd(sum, a.k, a.eps);
+    const float rstd = row_rstd(sum, a.inv_k, a.eps);
 
     float n[kPacks][kN];
     float absmax = 0.0f;
 #pragma unroll
     for (int i = 0; i < kPacks; ++i) {
         const int p = t + i * kThreads;
-        if (!live || p >= packs) continue;
-        Pack<float, kN == 1 ? 1 : 4> w[kN == 1 ? 1 : kN / 4];
+        if (p >= packs) continue;
+        Pack<float, 4> w[kN / 4];
 #pragma unroll
-        for (int j = 0; j < (kN == 1 ? 1 : kN / 4); ++j)
-            if (a.weight) w[j] = reinterpret_cast<const Pack<float, kN == 1 ? 1 : 4>*>(a.weight + (size_t)p * kN)[j];
+        for (int j = 0; j < kN / 4; ++j) {
+            w[j] = Pack<float, 4>{{1.0f, 1.0f, 1.0f, 1.0f}};
+            if (a.weight) w[j] = load_pack<kAligned, float, 4>(a.weight, p * (kN / 4) + j, a.k);
+        }
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
-            n[i][j] = norm_value(to_float(v[i].e[j]), rstd, a.weight ? w[j / 4].e[j % 4] : 1.0f);
+            n[i][j] = norm_value(to_float(v[i].e[j]), rstd, w[j / 4].e[j % 4]);
+            // behind the row 0 * rstd is NaN for an infinite rstd: no maximum
             absmax = fmaxf(absmax, fabsf(n[i][j]));
         }
     }
@@ -151,15 +256,17 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256)
     for (int i = 0; i < kPacks; ++i) {
         const int p = t + i * kThreads;
         if (p >= packs) continue;
-        Pack<int8_t, kN> c;
-        P o;
+        const Pack<int8_t, kN> c = codes_of(n[i], scale, rcp);
+        if (!kAligned && a.wide_codes && (p + 1) * kN <= a.k)  // rows of codes have a pitch of their own
+            store_pack<true, int8_t, kN>(q, p, a.k, c);
+        else
+            store_pack<kAligned, int8_t, kN>(q, p, a.k, c);
+        if (normed) {
+            P o;
 #pragma unroll
-        for (int j = 0; j < kN; ++j) {
-            c.e[j] = (int8_t)zq_quantize_value_rcp(n[i][j], scale, rcp, 127);
-            o.e[j] = from_float<T>(n[i][j]);
+            for (int j = 0; j < kN; ++j) o.e[j] = from_float<T>(n[i][j]);
+            store_pack<kAligned, T, kN>(normed, p, a.k, o);
         }
-        reinterpret_cast<Pack<int8_t, kN>*>(q)[p] = c;
-        if (normed) reinterpret_cast<P*>(normed)[p] = o;
     }
     for (int j = a.k + t; j < a.ldq; j += kThreads) q[j] = 0;
 }
@@ -187,7 +294,7 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
         const double d = (double)to_float(v);
         sum = __fma_rn(d, d, sum);
     }
-    const float rstd = row_rstd(group_sum<32>(sum, part_sum), a.k, a.eps);
+    const float rstd = row_rstd(group_sum<32>(sum, part_sum), a.inv_k, a.eps);
     const T* s = res ? sum_out : x;
     float absmax = 0.0f;
     for (int i = threadIdx.x; i < a.k; i += 1024)
@@ -206,25 +313,26 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
     for (long long i = a.k + threadIdx.x; i < a.ldq; i += 1024) q[i] = 0;
 }
 
-template <class T, int kN, int kWarps, int kPacks>
+template <class T, int kWarps, int kPacks, bool kAligned>
 cudaError_t launch_rows(const NormArgs& a, cudaStream_t stream) {
     constexpr int kRows = kWarps > 8 ? 1 : 8 / kWarps;
-    return launch_pdl_kernel(rms_norm_quantize_kernel<T, kN, kWarps, kPacks>,
+    return launch_pdl_kernel(rms_norm_quantize_kernel<T, kWarps, kPacks, kAligned>,
                              dim3((unsigned)((a.m + kRows - 1) / kRows)), dim3(kWarps > 8 ? kWarps * 32 : 256), 0,
                              stream, a);
 }
 
-template <class T, int kN>
+template <class T, int kPacks, bool kAligned>
 cudaError_t launch_width(const NormArgs& a, cudaStream_t stream) {
-    // Up to 32 elements a thread; the fewest warps that hold the row.
-    constexpr int kPacks = 32 / kN;
-    const int packs = a.k / kN;
-    if (packs <= 32 * kPacks) return launch_rows<T, kN, 1, kPacks>(a, stream);
-    if (packs <= 64 * kPacks) return launch_rows<T, kN, 2, kPacks>(a, stream);
-    if (packs <= 128 * kPacks) return launch_rows<T, kN, 4, kPacks>(a, stream);
-    if (packs <= 256 * kPacks) return launch_rows<T, kN, 8, kPacks>(a, stream);
-    if (packs <= 512 * kPacks) return launch_rows<T, kN, 16, kPacks>(a, stream);
-    if (packs <= 1024 * kPacks) return launch_rows<T, kN, 32, kPacks>(a, stream);
+    // The fewest warps that hold the row at kPacks packs a thread.
+    const int packs = (a.k + kElemsPer16<T> - 1) / kElemsPer16<T>;
+    if (packs <= 32 * kPacks) return launch_rows<T, 1, kPacks, kAligned>(a, stream);
+    if (packs <= 64 * kPacks) return launch_rows<T, 2, kPacks, kAligned>(a, stream);
+    if (packs <= 128 * kPacks) return launch_rows<T, 4, kPacks, kAligned>(a, stream);
+    if (packs <= 256 * kPacks) return launch_rows<T, 8, kPacks, kAligned>(a, stream);
+    if (packs <= 512 * kPacks) return launch_rows<T, 16, kPacks, kAligned>(a, stream);
+    if (packs <= 1024 * kPacks) return launch_rows<T, 32, kPacks, kAligned>(a, stream);
+    // 32 elements a thread reach furthest
+    if constexpr (kPacks < 32 / kElemsPer16<T>) return launch_width<T, 32 / kElemsPer16<T>, kAligned>(a, stream);
     return launch_pdl_kernel(rms_norm_quantize_long_kernel<T>, dim3((unsigned)a.m), dim3(1024), 0, stream, a);
 }
 
@@ -233,15 +341,24 @@ bool aligned(const void* p, long long pitch_bytes, size_t to) {
 }
 
 template <class T>
-cudaError_t launch_type(const NormArgs& a, cudaStream_t stream) {
+cudaError_t launch_type(NormArgs a, cudaStream_t stream) {
     constexpr int kN = kElemsPer16<T>;
     constexpr long long b = sizeof(T);
-    const bool wide = a.k % kN == 0 && aligned(a.x, a.ldx * b, 16) && aligned(a.q, a.ldq, kN) &&
-                      aligned(a.weight, 0, 16) &&
-                      (!a.residual ||
-                       (aligned(a.residual, a.ld_residual * b, 16) && aligned(a.residual_out, a.ld_residual_out * b, 16))) &&
-                      (!a.normed || aligned(a.normed, a.ld_normed * b, 16));
-    return wide ? launch_width<T, kN>(a, stream) : launch_width<T, 1>(a, stream);
+    const bool whole = a.k % kN == 0 && aligned(a.x, a.ldx * b, 16) && aligned(a.q, a.ldq, kN) &&
+                       aligned(a.weight, 0, 16) &&
+                       (!a.residual || (aligned(a.residual, a.ld_residual * b, 16) &&
+                                        aligned(a.residual_out, a.ld_residual_out * b, 16))) &&
+                       (!a.normed || aligned(a.normed, a.ld_normed * b, 16));
+    a.inv_k = 1.0 / a.k;
+    a.wide_codes = aligned(a.q, a.ldq, kN);
+    // Elements a thread.  Many rows: 32, since what a thread does once a row
+    // (two reductions, the root) then weighs least (8192 x 8192 bf16: 86 us, 16
+    // a thread 125 us, 64 a thread, with fewer loads under way, 111 us).  A row
+    // an SM or fewer: 8, the shortest chains (one row of 4096 fp32: 2.7 us
+    // against 3.4 us with 16).  Rows off the 16-byte grid: 16 (1537 x 4099
+    // fp32: 24 us, 8 a thread 40 us; 4000 x 4099 bf16: 81 us, 32 a thread 98).
+    if (!whole) return launch_width<T, 16 / kN, false>(a, stream);
+    return a.m <= sm_count() ? launch_width<T, 8 / kN, true>(a, stream) : launch_width<T, 32 / kN, true>(a, stream);
 }
 
 }  // namespace
