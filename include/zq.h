@@ -202,7 +202,11 @@ zq_status zq_dequantize_host(const zq_weight* w, float* out_host, void* stream);
  *   v = fl32(fl32(s * r) * weight), stored to normed in `dtype`
  *   q, row_scale = the activation quantizer's codes and scale of v
  * so the codes and scales equal zq_quantize_rows over v bit for bit, and do
- * not depend on the launch.  x, residual, residual_out and normed are
+ * not depend on the launch.  With reciprocal != 0 the scale is
+ * fl32(max|v| * fl32(1 / 127)) instead of the quotient max|v| / 127, a last
+ * bit apart in some rows: the scale of quantizers that multiply by the
+ * reciprocal (torch's absmax / 127.0 on a GPU does), for codes equal to
+ * theirs.  x, residual, residual_out and normed are
  * [m][k] in `dtype` with row pitches in elements (>= k); weight is fp32 [k]
  * or NULL (ones); q is int8 [m][ldq], ldq >= k, zeros in [k, ldq) (for
  * zq_matmul_codes, ldq = zq_weight_padded_k); row_scale fp32 [m].  residual
@@ -210,9 +214,9 @@ zq_status zq_dequantize_host(const zq_weight* w, float* out_host, void* stream);
  * buffer of x or of residual (same pointer, same pitch); overlaps of any
  * other kind are not allowed.  eps >= 0 and finite. */
 zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, size_t ldx, const void* residual,
-                               size_t ld_residual, const float* weight, double eps, void* residual_out,
-                               size_t ld_residual_out, void* normed, size_t ld_normed, int8_t* q, size_t ldq,
-                               float* row_scale, void* stream);
+                               size_t ld_residual, const float* weight, double eps, int reciprocal,
+                               void* residual_out, size_t ld_residual_out, void* normed, size_t ld_normed, int8_t* q,
+                               size_t ldq, float* row_scale, void* stream);
 
 /* Low-rank adapters of many requests added onto a shared projection's
  * output: for each row i with 0 <= ids[i] < slots,

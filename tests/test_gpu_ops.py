@@ -43,7 +43,7 @@ def same_bits(torch, got, want, what):
 
 # ---- norm -----------------------------------------------------------------------
 
-def norm_oracle(torch, x, residual, weight, eps):
+def norm_oracle(torch, x, residual, weight, eps, reciprocal=False):
     """The definition on the CPU.  Squares of fp32 values are exact in 64
     bits; the sum's rounding there cannot move the fp32 reciprocal root except
     within 1e-15 of a rounding border."""
@@ -56,7 +56,8 @@ def norm_oracle(torch, x, residual, weight, eps):
     r = (1.0 / torch.sqrt(mean + eps)).float()
     v = s * r * (1.0 if weight is None else weight)
     absmax = torch.nan_to_num(v.abs(), nan=0.0, posinf=math.inf).amax(-1, keepdim=True)
-    scale = torch.where(absmax > 0, absmax / 127.0, torch.ones_like(absmax))
+    quotient = absmax * torch.tensor(1.0 / 127.0) if reciprocal else absmax / torch.tensor(127.0)
+    scale = torch.where(absmax > 0, quotient, torch.ones_like(absmax))
     q = v / scale
     codes = torch.sign(q) * torch.floor(q.double().abs() + 0.5)
     codes = torch.where(q.isnan(), -127.0, codes.clamp(-127, 127))
@@ -114,6 +115,18 @@ def test_norm_codes_are_quantize_rows(zb, torch, m, k):
     codes, scale = zb.quantize_rows(got.normed)
     same_bits(torch, got.codes, codes, "codes")
     same_bits(torch, got.row_scale, scale, "row_scale")
+
+
+@pytest.mark.parametrize("m,k,dtype", [(700, 512, "float32"), (300, 1001, "bfloat16"), (4, 40000, "float16")])
+def test_norm_reciprocal_scale(zb, torch, m, k, dtype):
+    x, r, w = norm_case(torch, m, k, dtype, True)
+    codes, scale, _, _ = norm_oracle(torch, x, r, w, 1e-5, reciprocal=True)
+    got = zb.rms_norm_quantize(x.cuda(), w.cuda(), residual=r.cuda(), reciprocal=True)
+    same_bits(torch, got.row_scale, scale, "row_scale")
+    same_bits(torch, got.codes, codes, "codes")
+    other = zb.rms_norm_quantize(x.cuda(), w.cuda(), residual=r.cuda()).row_scale
+    assert m < 10 or (other != got.row_scale).any()  # the two rules differ in some rows
+    assert ((other - got.row_scale).abs() <= 2.0**-23 * other).all()
 
 
 @pytest.mark.parametrize("k", [24, 4099, 40000])

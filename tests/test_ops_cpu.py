@@ -17,8 +17,8 @@ def refused(rc, message, status=_lib.ZQ_ERR_INVALID_ARGUMENT):
 
 def norm(L, x=P, dtype=1, m=4, k=64, ldx=64, residual=None, ldr=0, weight=P, eps=1e-5, out=None, ldo=0, normed=None,
          ldn=0, q=P, ldq=128, scale=P):
-    return L.zq_rms_norm_quantize(x, dtype, m, k, ldx, residual, ldr, weight, eps, out, ldo, normed, ldn, q, ldq, scale,
-                                  None)
+    return L.zq_rms_norm_quantize(x, dtype, m, k, ldx, residual, ldr, weight, eps, 0, out, ldo, normed, ldn, q, ldq,
+                                  scale, None)
 
 
 def test_norm_refusals(native_lib):

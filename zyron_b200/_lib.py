@@ -111,7 +111,7 @@ SIGNATURES = {
     "zq_weight_set_option": (st, [vp, C.c_int, C.c_int, C.POINTER(C.c_int)]),
     "zq_test_decode_wait_timeout": (st, [vp, vp, vp, sz, vp, vp, sz, C.c_uint64, vp]),
     "zq_lm_set_option": (st, [vp, C.c_int, C.c_int, C.POINTER(C.c_int)]),
-    "zq_rms_norm_quantize": (st, [vp, C.c_int, sz, sz, sz, vp, sz, vp, C.c_double, vp, sz, vp, sz, vp, sz, vp, vp]),
+    "zq_rms_norm_quantize": (st, [vp, C.c_int, sz, sz, sz, vp, sz, vp, C.c_double, C.c_int, vp, sz, vp, sz, vp, sz, vp, vp]),
     "zq_add_low_rank_workspace_bytes": (sz, [sz, sz, sz, sz, sz]),
     "zq_add_low_rank": (st, [vp, sz, vp, C.c_int, sz, sz, sz, sz, vp, vp, C.c_int, sz, sz, vp, vp, vp, vp, sz, vp]),
     "zq_token_logprobs": (st, [vp, C.c_int, sz, sz, sz, vp, sz, sz, vp, vp, vp, vp, vp]),

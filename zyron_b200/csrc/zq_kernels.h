@@ -160,6 +160,7 @@ struct NormArgs {
     long long m;
     int k;
     double eps;
+    int reciprocal;  // the scale by multiplication
     // filled in by the launcher
     double inv_k = 0.0;
     bool wide_codes = false;  // packs of codes lie on their own size

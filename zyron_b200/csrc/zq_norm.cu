@@ -5,8 +5,10 @@
 //   r = fl32(1 / sqrt(mean(s^2) + eps))          mean in 64 bits
 //   v = fl32(fl32(s * r) * w)
 //   scale = max|v| / 127 (1 for a row of zeros), code = round(v / scale)
+//   (or scale = max|v| * fl32(1 / 127) where the caller asks for it)
 //
-// The codes and scales are those of quantize_rows over v, bit for bit.  The
+// With the quotient the codes and scales are those of quantize_rows over v, bit
+// for bit.  The
 // only quantity that depends on the order of a sum is the mean of squares.
 // It is summed in 64 bits, where fp32 squares are exact, so r -- and with it
 // every code -- does not depend on the launch shape: a last-bit change of r
@@ -72,6 +74,10 @@ __device__ __forceinline__ float row_rstd(double sum, double inv_k, double eps) 
     y = y * fma(-h * y, y, 1.5);
     y = y * fma(-h * y, y, 1.5);
     return (float)y;
+}
+
+__device__ __forceinline__ float row_scale_of(const NormArgs& a, float absmax) {
+    return a.reciprocal && absmax > 0.0f ? __fmul_rn(absmax, 1.0f / 127.0f) : zq_scale_from_absmax(absmax, 127.0f);
 }
 
 __device__ __forceinline__ float norm_value(float s, float rstd, float w) {
@@ -247,7 +253,7 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1
     }
     absmax = group_max<kWarps>(absmax, part_max);
     if (!live) return;
-    const float scale = zq_scale_from_absmax(absmax, 127.0f);
+    const float scale = row_scale_of(a, absmax);
     const float rcp = zq_quant_rcp(scale);
     if (t == 0) a.row_scale[row] = scale;
     int8_t* q = a.q + row * a.ldq;
@@ -300,7 +306,7 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
     for (int i = threadIdx.x; i < a.k; i += 1024)
         absmax = fmaxf(absmax, fabsf(norm_value(to_float(s[i]), rstd, a.weight ? a.weight[i] : 1.0f)));
     absmax = group_max<32>(absmax, part_max);
-    const float scale = zq_scale_from_absmax(absmax, 127.0f);
+    const float scale = row_scale_of(a, absmax);
     const float rcp = zq_quant_rcp(scale);
     if (threadIdx.x == 0) a.row_scale[row] = scale;
     int8_t* q = a.q + row * a.ldq;

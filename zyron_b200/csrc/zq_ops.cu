@@ -33,9 +33,9 @@ bool offsets_fit(size_t rows, size_t pitch, size_t size) {
 extern "C" {
 
 zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, size_t ldx, const void* residual,
-                               size_t ld_residual, const float* weight, double eps, void* residual_out,
-                               size_t ld_residual_out, void* normed, size_t ld_normed, int8_t* q, size_t ldq,
-                               float* row_scale, void* stream) {
+                               size_t ld_residual, const float* weight, double eps, int reciprocal,
+                               void* residual_out, size_t ld_residual_out, void* normed, size_t ld_normed, int8_t* q,
+                               size_t ldq, float* row_scale, void* stream) {
     const size_t size = dtype_bytes(dtype);
     if (size == 0) return invalid("zyron_b200: unsupported element type");
     if (k == 0) return invalid("zyron_b200: k must be > 0");
@@ -70,6 +70,7 @@ zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, siz
     a.m = (long long)m;
     a.k = (int)k;
     a.eps = eps;
+    a.reciprocal = reciprocal != 0;
     const cudaError_t e = zq::launch_rms_norm_quantize(a, dtype, as_stream(stream));
     return e == cudaSuccess ? ZQ_OK : zq::cuda_error(e, "rms_norm_quantize");
 }

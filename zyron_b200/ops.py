@@ -133,7 +133,7 @@ class NormQuantized(typing.NamedTuple):
     normed: Tensor | None  # the normed rows in x's type
 
 
-def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None, normed=False, stream=None):
+def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None, normed=False, reciprocal=False, stream=None):
     """Adds ``residual`` to ``x`` [..., k], norms the rows by their root mean
     square, scales them by ``weight`` (fp32 [k]) and quantizes them as
     ``quantize_rows`` does, bit for bit.
@@ -141,7 +141,10 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
     ``x`` and ``residual`` share a type (float32, float16 or bfloat16); the
     sum is rounded to it, and the norm reads the rounded sum.  The sum goes to
     ``residual_out`` (a new tensor when None; may be ``residual`` itself).
-    ``normed=True`` also returns the normed rows, e.g. for adapters."""
+    ``normed=True`` also returns the normed rows, e.g. for adapters.
+    ``reciprocal=True`` takes the row scale as max|v| times fp32's 1/127, as
+    torch computes absmax / 127.0 on a GPU, instead of the quotient: a last bit
+    apart in some rows, for codes equal to such a quantizer's."""
     torch = _torch()
     dtype = _dtype(x, "x")
     index = _device(x, weight=weight, residual=residual, residual_out=residual_out)
@@ -173,8 +176,8 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
         kp = (k + 127) // 128 * 128
         codes = _empty((m, kp), torch.int8, device)
         scale = _empty(lead, torch.float32, device)
-        check(lib().zq_rms_norm_quantize(xr.data_ptr(), dtype, m, k, ldx, _ptr(rr), ldr, _ptr(weight), eps, _ptr(so),
-                                         lds, _ptr(n), k, codes.data_ptr(), kp, scale.data_ptr(), ptr))
+        check(lib().zq_rms_norm_quantize(xr.data_ptr(), dtype, m, k, ldx, _ptr(rr), ldr, _ptr(weight), eps, reciprocal,
+                                         _ptr(so), lds, _ptr(n), k, codes.data_ptr(), kp, scale.data_ptr(), ptr))
     if kp != k:
         codes = codes[:, :k]
     if len(shape) != 2:
