@@ -188,7 +188,8 @@ def _norm(st):
     if own:
         import zyron_b200 as zb
 
-        r = zb.rms_norm_quantize(x, weight, residual=residual, eps=EPS, normed=st["normed"])
+        # torch takes absmax / 127.0 as a product with fp32's 1/127
+        r = zb.rms_norm_quantize(x, weight, residual=residual, eps=EPS, normed=st["normed"], reciprocal=True)
         return {"codes": r.codes, "row_scale": r.row_scale, "residual": r.residual, "normed": r.normed}
     s = x.float()
     total = None
