@@ -24,28 +24,26 @@ import typing
 
 from . import _lib
 from ._lib import check, lib
-from .quantization import QuantizedMatrix, _torch
+from .quantization import QuantizedMatrix
 
 if typing.TYPE_CHECKING:
     from torch import Tensor
 
 _NO_CONTEXT = contextlib.nullcontext()
+torch = None  # the module, from the first call on
+_DTYPES = {}  # torch type -> ZQ_DTYPE_*
+_raw_stream = None  # device index -> raw handle of its current stream
 
 
 def _setup():
-    """Element type codes (ZQ_DTYPE_*) and the current stream's raw handle by
-    device index; torch is imported at the first call."""
-    global _DTYPES, _raw_stream
-    torch = _torch()
-    _DTYPES = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
-    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    global torch, _raw_stream
+    import torch as module
+
+    _DTYPES.update({module.float32: 1, module.float16: 2, module.bfloat16: 3})
+    _raw_stream = getattr(module._C, "_cuda_getCurrentRawStream", None)
     if _raw_stream is None:
-        _raw_stream = lambda index: torch.cuda.current_stream(index).cuda_stream  # noqa: E731
-    return _DTYPES
-
-
-_DTYPES = None
-_raw_stream = None
+        _raw_stream = lambda index: module.cuda.current_stream(index).cuda_stream  # noqa: E731
+    torch = module
 
 
 def _bad(msg):
@@ -53,27 +51,27 @@ def _bad(msg):
 
 
 def _dtype(t, name):
-    d = (_DTYPES or _setup()).get(t.dtype)
+    d = _DTYPES.get(t.dtype)
     if d is None:
         raise _bad(f"{name} must be float32, float16 or bfloat16")
     return d
 
 
-def _device(first, **others):
-    """The CUDA device index that all tensors (or None) are on."""
+def _device(first, names, *others):
+    """The CUDA device index that all tensors (or None) are on; `names` are
+    the others'."""
     index = first.get_device()
     if index < 0:
         raise _bad("tensors must be on a CUDA device")
-    for name, t in others.items():
+    for i, t in enumerate(others):
         if t is not None and t.get_device() != index:
-            raise _bad(f"{name} is on {t.device}, not on {first.device}")
+            raise _bad(f"{names.split()[i]} is on {t.device}, not on {first.device}")
     return index
 
 
 def _context(index, stream):
     """(context manager, stream pointer): inside, the device is current and
     allocations belong to the stream."""
-    torch = _torch()
     if stream is None:
         return (_NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)), _raw_stream(index)
     if stream.device.index != index:
@@ -84,7 +82,6 @@ def _context(index, stream):
 def _empty(shape, dtype, device):
     """A new contiguous tensor.  Strides given make the cheapest allocating
     call: at small sizes a call's time is its host time."""
-    torch = _torch()
     if len(shape) == 1:
         return torch.empty_strided(shape, (1,), dtype=dtype, device=device)
     if len(shape) == 2:
@@ -145,9 +142,10 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
     ``reciprocal=True`` takes the row scale as max|v| times fp32's 1/127, as
     torch computes absmax / 127.0 on a GPU, instead of the quotient: a last bit
     apart in some rows, for codes equal to such a quantizer's."""
-    torch = _torch()
+    if torch is None:
+        _setup()
     dtype = _dtype(x, "x")
-    index = _device(x, weight=weight, residual=residual, residual_out=residual_out)
+    index = _device(x, "weight residual residual_out", weight, residual, residual_out)
     shape = x.shape
     lead, k = shape[:-1], shape[-1] if len(shape) else 0
     if residual is not None:
@@ -190,7 +188,8 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
     [..., K] and ``row_scale`` fp32 [...], as ``rms_norm_quantize`` or
     ``quantize_rows`` leave them.  Codes whose rows are not 128-aligned, as
     those of ``rms_norm_quantize`` are, are copied first."""
-    torch = _torch()
+    if torch is None:
+        _setup()
     if weights is None or weights.empty():
         raise _lib.ZQInvalidArgument("ZYRON quantization: weights are empty")
     k = weights.rows()
@@ -199,7 +198,7 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
     lead = codes.shape[:-1]
     if codes.dtype != torch.int8 or row_scale.dtype != torch.float32 or row_scale.shape != lead:
         raise _bad("codes must be int8 [..., K] and row_scale float32 [...]")
-    index = _device(codes, row_scale=row_scale, bias=bias, out=out)
+    index = _device(codes, "row_scale bias out", row_scale, bias, out)
     if weights._device != index:
         raise _bad(f"the weights are on cuda:{weights._device}, not on {codes.device}")
     n = weights.cols()
@@ -207,7 +206,6 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
         raise _bad("bias must be contiguous float32 of the output's last dimension")
     if out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (*lead, n) or not out.is_contiguous()):
         raise _bad("out must be contiguous float32 [..., N]")
-    _raw_stream or _setup()
     context, ptr = _context(index, stream)
     with context:
         q, pitch = _rows(codes, "codes")
@@ -248,10 +246,11 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
     ``ranks`` are the fields of ``LowRankAdapters``.  Rows whose id is not in
     [0, slots) are left as they are; only the first ``ranks[s]`` of an
     adapter's ranks count."""
-    torch = _torch()
+    if torch is None:
+        _setup()
     xt = _dtype(x, "x")
     wt = _dtype(a, "a")
-    index = _device(x, y=y, a=a, b=b, ids=ids, scales=scales, ranks=ranks)
+    index = _device(x, "y a b ids scales ranks", y, a, b, ids, scales, ranks)
     if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype:
         raise _bad("a must be [slots, max_rank, in] and b [slots, out, max_rank], of one type")
     slots, max_rank, k = a.shape
@@ -303,9 +302,10 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=True, stream=None):
     A negative target asks for nothing and gives 0; one behind the vocabulary
     gives NaN.  -inf logits are tokens that are not allowed; a row that allows
     none has log probabilities of -inf and entropy 0."""
-    torch = _torch()
+    if torch is None:
+        _setup()
     dtype = _dtype(logits, "logits")
-    index = _device(logits, targets=targets)
+    index = _device(logits, "targets", targets)
     shape = logits.shape
     if len(shape) < 1:
         raise _bad("logits rank must be >= 1")
