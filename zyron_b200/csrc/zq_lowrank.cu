@@ -149,8 +149,9 @@ template <class T>
 constexpr int kRaw = 8 / kElemsPer16<T>;
 
 // Elements [0, n) of p (n may be <= 0 or above 8) as raw packs, zeros behind
-// them.  kVec: p is 16-byte aligned and, where n > 0, all 8 may be read.
-template <class T, bool kVec>
+// them.  kVec: p is 16-byte aligned and, where n > 0, all 8 may be read; with
+// kWhole all 8 count.
+template <class T, bool kVec, bool kWhole = false>
 __device__ __forceinline__ void load8(const T* p, int n, uint4 (&raw)[kRaw<T>]) {
     constexpr int kN = kElemsPer16<T>;
     if (kVec) {
@@ -159,7 +160,7 @@ __device__ __forceinline__ void load8(const T* p, int n, uint4 (&raw)[kRaw<T>]) 
             raw[i] = make_uint4(0, 0, 0, 0);
             if (n > 0) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
         }
-        if (n > 0 && n < 8) {
+        if (!kWhole && n > 0 && n < 8) {
 #pragma unroll
             for (int i = 0; i < kRaw<T>; ++i) {
                 Pack<T, kN> v;
@@ -311,33 +312,37 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_kernel(const LowRankArgs a
     for (int r0 = 0; r0 < rank; r0 += kRankPass) {
         if (r0) __syncthreads();  // the pass before has been read
         float acc[kRankPass / 8][4] = {};
-        // One chunk of 32: with x's elements at hand, and the next chunk's
-        // fetched while its products run.  kTail: not all 32 exist.
-        uint4 raw_lo[kRaw<TX>], raw_hi[kRaw<TX>];
-        auto chunk = [&](int k0, auto columns, auto tail) {
+        // One chunk of 32: its elements are at hand, and the next chunk's are
+        // fetched into the places that its products leave; with 8 columns there
+        // are no registers for that, and A's come at the chunk's start (4096 x
+        // 4096 x 4096, rank 16: 51 us, without it 54; rank 64: 78 us, with it,
+        // spilling, 87).  k is a whole number of packs where kVec.
+        uint4 raw_lo[kRaw<TX>], raw_hi[kRaw<TX>], raw_a[kRankPass / 8][1];
+        auto fetch_x = [&](int k) {
+            load8<TX, kVec, kVec>(x_lo + k, k_end - k, raw_lo);
+            load8<TX, kVec, kVec>(x_hi + k, k_end - k, raw_hi);
+        };
+        auto fetch_a = [&](int k, int j) {
+            const int r = min(r0 + 8 * j + g, rank - 1);
+            load8<TW, kVec, kVec>(wa + (long long)r * a.k + k, k_end - k, raw_a[j]);
+        };
+        auto chunk = [&](int k0, auto columns) {
             constexpr int kN = decltype(columns)::value;  // 8-rank columns
-            constexpr bool kTail = decltype(tail)::value;
-            const int k = k0 + 8 * t;
-            uint4 raw_a[kN][1];
-#pragma unroll
-            for (int j = 0; j < kN; ++j) {
-                const int r = min(r0 + 8 * j + g, rank - 1);
-                load8<TW, kVec>(wa + (long long)r * a.k + k, kTail ? k_end - k : 8, raw_a[j]);
-            }
+            constexpr bool kAhead = kN < 8;
+            const int next = k0 + kStep + 8 * t;
             Pairs<TX> lo, hi;
             to_pairs(raw_lo, lo);
             to_pairs(raw_hi, hi);
-            if (!kTail) {
-                const int next = k + kStep;
-                if (k0 + kStep + 32 <= k_end) {
-                    load8<TX, kVec>(x_lo + next, 8, raw_lo);
-                    load8<TX, kVec>(x_hi + next, 8, raw_hi);
-                } else {
-                    load8<TX, kVec>(x_lo + next, k_end - next, raw_lo);
-                    load8<TX, kVec>(x_hi + next, k_end - next, raw_hi);
-                }
+            if (!kAhead) {
+#pragma unroll
+                for (int j = 0; j < kN; ++j) fetch_a(k0 + 8 * t, j);
             }
+            fetch_x(next);
             mma_chunk<TW, kN>(acc, lo.pair, hi.pair, raw_a);
+            if (kAhead) {
+#pragma unroll
+                for (int j = 0; j < kN; ++j) fetch_a(next, j);
+            }
         };
         // The sums so far to the warp's place in shared memory.  Tensor cores cut
         // sums off instead of rounding them, which adds up along a chain of
@@ -361,17 +366,20 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_kernel(const LowRankArgs a
         };
         auto share = [&](auto columns) {
             int k0 = k_begin + 32 * group;
-            load8<TX, kVec>(x_lo + k0 + 8 * t, k_end - k0 - 8 * t, raw_lo);
-            load8<TX, kVec>(x_hi + k0 + 8 * t, k_end - k0 - 8 * t, raw_hi);
+            fetch_x(k0 + 8 * t);
+            constexpr int kN = decltype(columns)::value;
+            if (kN < 8) {
+#pragma unroll
+                for (int j = 0; j < kN; ++j) fetch_a(k0 + 8 * t, j);
+            }
             bool add = false;
-            for (int n = 1; k0 + 32 <= k_end; k0 += kStep, ++n) {
-                chunk(k0, columns, std::false_type{});
+            for (int n = 1; k0 < k_end; k0 += kStep, ++n) {
+                chunk(k0, columns);
                 if (n % kChain == 0) {
                     put(columns, add);
                     add = true;
                 }
             }
-            if (k0 < k_end) chunk(k0, columns, std::true_type{});
             put(columns, add);
         };
         if (16 * mt < rows) {
@@ -479,20 +487,22 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
     constexpr int kStep = kWarpCols * kGroups;
     const int first = c_begin + kWarpCols * group;  // of the columns, kWarpCols at a time
     const TW* b_lane = wb + (long long)(first + 4 * (g >> 1) + (g & 1)) * a.max_rank;  // this lane's first
-    // d += this lane's h x kWarpCols columns of B over ranks r0 to r0 + 31.
+    // This lane's elements of kWarpCols columns of B over ranks r0 to r0 + 31.
     // kWhole: every pack of 8 ranks is inside the rank or outside; those
     // outside meet zeros of h, so the first pack stands in for them.  `cols`:
     // the columns that exist, of kWarpCols.
-    auto part_product = [&](float(&acc)[kWarpCols / 8][4], const TW* b0, int r0, int cols, auto whole) {
+    auto fetch_b = [&](uint4(&raw)[kWarpCols / 8][1], const TW* b0, int r0, int cols, auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
-        uint4 raw_b[kWarpCols / 8][1];
         const int r = r0 + 8 * t, at = kWhole && r >= rank ? 0 : r;
 #pragma unroll
         for (int j = 0; j < kWarpCols / 8; ++j) {
             const int bc = 16 * (j >> 1) + 2 * (j & 1);
             const bool in = kWhole || bc + 4 * (g >> 1) + (g & 1) < cols;
-            load8<TW, kVecB>(b0 + bc * a.max_rank + at, kWhole ? 8 : in ? rank - r : 0, raw_b[j]);
+            load8<TW, kVecB, kWhole>(b0 + bc * a.max_rank + at, kWhole ? 8 : in ? rank - r : 0, raw[j]);
         }
+    };
+    // d += this lane's h over those ranks x the columns
+    auto product = [&](float(&acc)[kWarpCols / 8][4], const uint4(&raw)[kWarpCols / 8][1], int r0) {
         uint32_t lo[3][4], hi[3][4];
 #pragma unroll
         for (int p = 0; p < 3; ++p) {
@@ -500,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
             memcpy(lo[p], __builtin_assume_aligned(h, 16), 16);
             memcpy(hi[p], __builtin_assume_aligned(h + 8 * pitch, 16), 16);
         }
-        mma_chunk<TW, kWarpCols / 8>(acc, lo, hi, raw_b);
+        mma_chunk<TW, kWarpCols / 8>(acc, lo, hi, raw);
     };
     auto store = [&](const float(&acc)[kWarpCols / 8][4], int c0, int cols) {
 #pragma unroll
@@ -521,16 +531,32 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
     };
     int c0 = first;
     const long long b_step = (long long)kStep * a.max_rank;
-    if (kVecB && rank % 8 == 0) {
+    if (kVecB && rank % 8 == 0 && c0 + kWarpCols <= c_end) {
+        // the next step's elements are fetched while this one's products run
+        uint4 raw[kWarpCols / 8][1];
+        fetch_b(raw, b_lane, 0, kWarpCols, std::true_type{});
         for (; c0 + kWarpCols <= c_end; c0 += kStep, b_lane += b_step) {
             float acc[kWarpCols / 8][4] = {};
-            for (int r0 = 0; r0 < rank; r0 += 32) part_product(acc, b_lane, r0, kWarpCols, std::true_type{});
+            for (int r0 = 0; r0 < rank; r0 += 32) {
+                uint4 next[kWarpCols / 8][1];
+                if (r0 + 32 < rank)
+                    fetch_b(next, b_lane, r0 + 32, kWarpCols, std::true_type{});
+                else if (c0 + kStep + kWarpCols <= c_end)
+                    fetch_b(next, b_lane + b_step, 0, kWarpCols, std::true_type{});
+                product(acc, raw, r0);
+#pragma unroll
+                for (int j = 0; j < kWarpCols / 8; ++j) raw[j][0] = next[j][0];
+            }
             store(acc, c0, kWarpCols);
         }
     }
     for (; c0 < c_end; c0 += kStep, b_lane += b_step) {
         float acc[kWarpCols / 8][4] = {};
-        for (int r0 = 0; r0 < rank; r0 += 32) part_product(acc, b_lane, r0, c_end - c0, std::false_type{});
+        for (int r0 = 0; r0 < rank; r0 += 32) {
+            uint4 raw[kWarpCols / 8][1];
+            fetch_b(raw, b_lane, r0, c_end - c0, std::false_type{});
+            product(acc, raw, r0);
+        }
         store(acc, c0, c_end - c0);
     }
 }
