@@ -52,11 +52,15 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLogUnroll = 2;
-constexpr int kUnroll = 1 << kLogUnroll;  // 16-byte packs that a thread loads ahead
+// 16-byte packs that a thread loads ahead, as a power of 2: 4; with fp32 rows in
+// blocks of 4 warps 8 (2048 x 32003, one alternative: 48 us against 53 us; at 16
+// bits the larger parts cost the second look more than the loads gain, 1024 x
+// 150001: 86 us against 78 us).
+template <class T, int kWarps>
+constexpr int kLogUnroll = sizeof(T) == 4 && kWarps == 4 ? 3 : 2;
 constexpr int kMaxSplit = 8;  // CTAs of a row
 constexpr int kStage = 128;   // packs that a warp looks at again at a time
-constexpr int kAhead = 2;  // rounds from a load to its prefetch
+constexpr int kAhead = 1;     // rounds from a load to its prefetch
 constexpr int kParts = 4;  // parts of a thread's loads that keep a maximum each
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -399,7 +403,7 @@ struct Warp {
     }
 };
 
-// How a thread's packs fall into kParts parts: rounds of kUnroll packs, 2^shift
+// How a thread's packs fall into kParts parts: rounds of its loads ahead, 2^shift
 // rounds a part.
 __device__ __forceinline__ int part_shift(int packs, int per_round) {
     const int rounds = (packs + per_round - 1) / per_round;
@@ -412,6 +416,7 @@ __device__ __forceinline__ int part_shift(int packs, int per_round) {
 template <class T, int kWarps>
 __device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int p1, int shift, float (&largest)[kParts]) {
     constexpr int kN = kElemsPer16<T>;
+    constexpr int kUnroll = 1 << kLogUnroll<T, kWarps>;
     constexpr int kThreads = kWarps * 32;
     constexpr int kRound = kThreads * kUnroll;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -480,7 +485,7 @@ __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const
     }
     __syncwarp();
     // All their packs, as many at a time as the stage holds.
-    const int log_each = shift + kLogUnroll;
+    const int log_each = shift + kLogUnroll<T, kWarps>;
     const int n = parts << log_each;
     for (int i0 = 0; i0 < n; i0 += kStage) {
         int at[kStage / 32];
@@ -557,7 +562,7 @@ __global__ void __launch_bounds__(kWarps * 32) token_logprobs_kernel(const Logpr
     const int packs = (a.vocab - head) / kN;
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
     const int p0 = (int)((long long)packs * part / split), p1 = (int)((long long)packs * (part + 1) / split);
-    const int shift = part_shift(p1 - p0, kThreads * kUnroll);
+    const int shift = part_shift(p1 - p0, kThreads << kLogUnroll<T, kWarps>);
     float largest[kParts];
     pass<T, kWarps>(w, body, p0, p1, shift, largest);
     if (kTop) find_top<T, kWarps>(top, sh, w, largest, body, p0, p1, shift, head, a.top_k);
@@ -697,12 +702,12 @@ cudaError_t launch_rows(const LogprobArgs& a, cudaStream_t stream) {
     // a row (600 x 2000 bf16: 9.4 us against 11.9 us).
     const int sms = sm_count();
     const long long packs = a.vocab / kElemsPer16<T>;
-    if (a.m >= 6LL * sms || packs <= 128 * kUnroll) return launch<T, kTop, 4>(a, 1, stream);
+    if (a.m >= 6LL * sms || packs <= 128 << kLogUnroll<T, 4>) return launch<T, kTop, 4>(a, 1, stream);
     // Else CTAs of 8 warps, 4 an SM, none with less than a round: with 8 an SM
     // the steps behind the pass cost more than the shorter passes save
     // (300 x 100000 bf16, 8 alternatives: 24 us against 31 us).
     int split = 1;
-    while (split < kMaxSplit && a.m * split < 4LL * sms && packs >= 2LL * split * 256 * kUnroll) split *= 2;
+    while (split < kMaxSplit && a.m * split < 4LL * sms && packs >= 2LL * split * 256 << kLogUnroll<T, 8>) split *= 2;
     return launch<T, kTop, 8>(a, split, stream);
 }
 
