@@ -160,6 +160,14 @@ def test_norm_in_place_and_shapes(zb, torch):
     same_bits(torch, rd.view(6, 320), total, "residual in place")
     same_bits(torch, got.codes.reshape(6, 320), codes, "codes")
     same_bits(torch, got.normed.view(6, 320), v, "normed")
+    # x's own buffer takes the sum as well, and x may be its own residual
+    xd = x.cuda()
+    again = zb.rms_norm_quantize(xd, w.cuda(), residual=r.cuda(), eps=1e-6, residual_out=xd)
+    same_bits(torch, xd, total, "residual into x")
+    same_bits(torch, again.codes, codes, "codes, residual into x")
+    twice = zb.rms_norm_quantize(x.cuda(), w.cuda(), residual=x.cuda(), eps=1e-6)
+    same_bits(torch, twice.codes, norm_oracle(torch, x, x, w, 1e-6)[0], "x twice")
+    xd = x.cuda().view(2, 3, 320)
     one = zb.rms_norm_quantize(x[0].cuda(), w.cuda(), eps=1e-6)  # a vector
     assert one.codes.shape == (320,) and one.row_scale.shape == ()
     none = zb.rms_norm_quantize(xd[:0], w.cuda())
@@ -390,6 +398,11 @@ def test_adapters_refusals_on_device(zb, torch):
         kw = {"y": y, "x": x, "a": a, "b": b, "ids": ids, **bad}
         with pytest.raises(ValueError, match=match):
             zb.add_low_rank(**kw)
+    lin = zb.QuantizedLinear(torch.zeros(32, 16, device="cuda"))
+    pool = zb.LowRankAdapters(a, b)
+    assert lin(x[:0], adapters=pool, adapter_ids=ids[:0]).shape == (0, 16)
+    with pytest.raises(ValueError, match="dimension mismatch"):
+        lin(x, adapters=zb.LowRankAdapters(a[:, :, :31].contiguous(), b), adapter_ids=ids)
     empty = zb.add_low_rank(y[:0], x[:0], a, b, ids[:0])
     assert empty.shape == (0, 16)
 
@@ -624,6 +637,33 @@ def test_step_in_graphs_and_streams(zb, torch, m):
             same_bits(torch, logits, wl, "logits")
             for a, b in zip(lp, wlp):
                 same_bits(torch, a, b, "log probabilities")
+
+
+def test_calls_from_threads(zb, torch):
+    """Calls from several threads at once, each on a stream of its own."""
+    import threading
+
+    step, _keep = make_step(zb, torch)
+    sets = [step_inputs(torch, m, seed=20 + i) for i, m in enumerate((3, 40, 300, 17))]
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    got = [None] * len(sets)
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got[i] = step(*sets[i])
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(sets))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for (logits, lp), (wl, wlp) in zip(got, want):
+        same_bits(torch, logits, wl, "logits")
+        for a, b in zip(lp, wlp):
+            same_bits(torch, a, b, "log probabilities")
 
 
 def test_stream_argument(zb, torch):

@@ -65,6 +65,8 @@ def test_adapter_refusals(native_lib):
     for bad in ("y", "x", "a", "b", "ids"):
         refused(adapters(L, **{bad: None}), "null pointer")
     refused(adapters(L, n=1 << 31, ldy=1 << 31), "dimension too large", _lib.ZQ_ERR_OVERFLOW)
+    refused(adapters(L, m=(1 << 31) - 4096), "dimension too large", _lib.ZQ_ERR_OVERFLOW)
+    refused(adapters(L, ldx=BIG), "matrix size overflow", _lib.ZQ_ERR_OVERFLOW)
     refused(adapters(L, y=C.c_void_p(2)), "a pointer is not aligned to its element type")
     need = L.zq_add_low_rank_workspace_bytes(5000, 64, 32, 2, 8)
     assert need > 5000 * 4 and need % 256 == 0

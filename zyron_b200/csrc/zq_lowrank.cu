@@ -498,9 +498,10 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
     const int first = c_begin + kWarpCols * group;  // of the columns, kWarpCols at a time
     const TW* b_lane = wb + (long long)(first + 4 * (g >> 1) + (g & 1)) * a.max_rank;  // this lane's first
     // This lane's elements of kWarpCols columns of B over ranks r0 to r0 + 31.
-    // kWhole: every pack of 8 ranks is inside the rank or outside; those
-    // outside meet zeros of h, so the first pack stands in for them.  `cols`:
-    // the columns that exist, of kWarpCols.
+    // kWhole: all columns exist and rows of B are whole packs; packs past the
+    // rank meet zeros of h, so the first pack stands in for them, and what a
+    // pack holds past the rank (`in_rank` masks the last step's) is made zero.
+    // `cols`: else the columns that exist, of kWarpCols.
     auto fetch_b = [&](uint4(&raw)[kWarpCols / 8][1], const TW* b0, int r0, int cols, auto whole) {
         constexpr bool kWhole = decltype(whole)::value;
         const int r = r0 + 8 * t, at = kWhole && r >= rank ? 0 : r;
@@ -511,6 +512,13 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
             load8<TW, kVecB, kWhole>(b0 + bc * a.max_rank + at, kWhole ? 8 : in ? rank - r : 0, raw[j]);
         }
     };
+    const bool ragged = rank % 8 != 0;
+    uint32_t in_rank[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = (rank - 1) / 32 * 32 + 8 * t + 2 * i;
+        in_rank[i] = (r < rank ? 0xFFFFu : 0u) | (r + 1 < rank ? 0xFFFF0000u : 0u);
+    }
     // d += this lane's h over those ranks x the columns
     auto product = [&](float(&acc)[kWarpCols / 8][4], const uint4(&raw)[kWarpCols / 8][1], int r0) {
         uint32_t lo[3][4], hi[3][4];
@@ -541,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
     };
     int c0 = first;
     const long long b_step = (long long)kStep * a.max_rank;
-    if (kVecB && rank % 8 == 0 && c0 + kWarpCols <= c_end) {
+    if (kVecB && c0 + kWarpCols <= c_end) {
         // the next step's elements are fetched while this one's products run
         uint4 raw[kWarpCols / 8][1];
         fetch_b(raw, b_lane, 0, kWarpCols, std::true_type{});
@@ -553,6 +561,13 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
                     fetch_b(next, b_lane, r0 + 32, kWarpCols, std::true_type{});
                 else if (c0 + kStep + kWarpCols <= c_end)
                     fetch_b(next, b_lane + b_step, 0, kWarpCols, std::true_type{});
+                if (ragged && r0 + 32 >= rank) {
+#pragma unroll
+                    for (int j = 0; j < kWarpCols / 8; ++j) {
+                        raw[j][0].x &= in_rank[0], raw[j][0].y &= in_rank[1];
+                        raw[j][0].z &= in_rank[2], raw[j][0].w &= in_rank[3];
+                    }
+                }
                 product(acc, raw, r0);
 #pragma unroll
                 for (int j = 0; j < kWarpCols / 8; ++j) raw[j][0] = next[j][0];

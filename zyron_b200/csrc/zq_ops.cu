@@ -13,6 +13,10 @@ namespace {
 
 constexpr size_t kIntMax = (size_t)std::numeric_limits<int>::max();
 
+// Rows of an adapter call: their 32-bit indices pass the last by up to two
+// rounds of the sorting block.
+constexpr size_t kMaxRows = kIntMax - 4096;
+
 zq_status invalid(const char* msg) { return zq::set_error(ZQ_ERR_INVALID_ARGUMENT, msg); }
 
 cudaStream_t as_stream(void* s) { return s ? static_cast<cudaStream_t>(s) : cudaStreamPerThread; }
@@ -76,7 +80,7 @@ zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, siz
 }
 
 size_t zq_add_low_rank_workspace_bytes(size_t m, size_t k, size_t n, size_t slots, size_t max_rank) {
-    if (m == 0 || m > kIntMax || k == 0 || k > kIntMax / 2 || n == 0 || n > kIntMax / 2 || slots == 0 ||
+    if (m == 0 || m > kMaxRows || k == 0 || k > kIntMax / 2 || n == 0 || n > kIntMax / 2 || slots == 0 ||
         slots > ZQ_LOW_RANK_MAX_SLOTS || max_rank == 0 || max_rank > ZQ_LOW_RANK_MAX)
         return 0;
     zq::LowRankArgs r{};
@@ -107,7 +111,7 @@ zq_status zq_add_low_rank(float* y, size_t ldy, const void* x, int x_dtype, size
     if (ldy < n || ldx < k) return invalid("zyron_b200: a row pitch is smaller than its row");
     if (m == 0) return ZQ_OK;
     if (!y || !x || !a || !b || !ids) return invalid("zyron_b200: null pointer");
-    if (m > kIntMax || k > kIntMax / 2 || n > kIntMax / 2)
+    if (m > kMaxRows || k > kIntMax / 2 || n > kIntMax / 2)
         return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: dimension too large");
     if (!offsets_fit(m, ldx, size) || !offsets_fit(m, ldy, 4))
         return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: matrix size overflow");
