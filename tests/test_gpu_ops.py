@@ -87,7 +87,7 @@ NORM_SIZES = [(1, 1), (1, 4096), (2, 7), (3, 31), (5, 32), (9, 33), (8, 256), (7
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,k", NORM_SIZES)
 def test_norm_bits(zb, torch, m, k, dtype):
-    for residual, pitch, normed in ((True, 0, True), (False, 0, False), (True, 8, False), (False, 3, True)):
+    for residual, pitch, normed in ((True, 0, True), (False, 0, False), (True, 8, False), (False, 3, True), (True, 5, True)):
         x, r, w = norm_case(torch, m, k, dtype, residual, pitch)
         codes, scale, total, v = norm_oracle(torch, x, r, w, 1e-5)
         dev = lambda t: None if t is None else torch.empty(t.shape[0], k + pitch, dtype=t.dtype, device="cuda")[:, :k].copy_(t)  # noqa: E731

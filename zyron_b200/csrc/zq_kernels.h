@@ -163,7 +163,8 @@ struct NormArgs {
     int reciprocal;  // the scale by multiplication
     // filled in by the launcher
     double inv_k = 0.0;
-    bool wide_codes = false;  // packs of codes lie on their own size
+    // whole packs of a row lie on their own size
+    bool wide_weight = false, wide_codes = false, wide_sum = false, wide_normed = false;
 };
 cudaError_t launch_rms_norm_quantize(const NormArgs& a, int dtype, cudaStream_t stream);
 

@@ -28,10 +28,11 @@
 // value of each of kParts parts.  k threads have a value at least as large as
 // the k-th largest of the threads' maxima (or a cheaper lower bound of it), so
 // the k largest lie in the parts of threads whose maximum reaches it: about k.
-// The loads of those are read again, mostly from L2, and the keys that beat the bar wait in the warp's queue
-// in shared memory; 32 at a time are sorted across the lanes and merged into
-// the warp's list of 32, one a lane in order, whose k-th is the new bar.  At
-// last the block counts for each key left the keys above it.
+// The loads of those are read again, mostly from L2, and the keys that beat the
+// bar wait in the warp's queue in shared memory; 32 at a time are sorted across
+// the lanes and merged into the warp's list of 32, one a lane in order, whose
+// k-th is the new bar.  At last the block counts for each key left the keys
+// above it.
 //
 // Bound: one read of the logits; 16 exponentials a clock and SM come next (at
 // 16-bit logits 0.7 of the read's time).  A row is split over the CTAs of a
@@ -61,7 +62,7 @@ constexpr int kLogUnroll = sizeof(T) == 4 && kWarps == 4 ? 3 : 2;
 constexpr int kMaxSplit = 8;  // CTAs of a row
 constexpr int kStage = 128;   // packs that a warp looks at again at a time
 constexpr int kAhead = 1;     // rounds from a load to its prefetch
-constexpr int kParts = 4;  // parts of a thread's loads that keep a maximum each
+constexpr int kParts = 4;     // parts of a thread's loads that keep a maximum each
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 8.0f;

@@ -426,7 +426,8 @@ __host__ __device__ int part_pitch(int max_rank) {
 }
 
 // y[0..4) += v, added in L2: nothing waits for y to arrive.  Each element is
-// added to once, so the result does not depend on any order.
+// added to once, so the result does not depend on any order.  (The addition in
+// L2 takes subnormal values as 0.)
 __device__ __forceinline__ void add4(float* y, float v0, float v1, float v2, float v3) {
     asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y), "f"(v0), "f"(v1), "f"(v2), "f"(v3) : "memory");
 }
@@ -671,7 +672,7 @@ Shape shape_of(const LowRankArgs& a) {
     s.mt = direct ? 1 : kSortedTiles;
     // Blocks a tile, so that each grid fills the SMs twice over, which is what
     // fits at once: a part of a third block an SM costs as much as a whole one
-    // (4096 x 4096 x 4096 of rank 64: 74 us, with 3 an SM 90 us, with 1 103
+    // (4096 x 4096 x 4096 of rank 64: 82 us, with 3 an SM 94 us, with 1 119
     // us).  No share is smaller than one chunk a warp.  How many tiles have
     // rows is only known on the device; full tiles and one in part for every
     // slot (for every second, where many rows are sorted) are taken for it.

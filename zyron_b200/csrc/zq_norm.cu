@@ -151,7 +151,9 @@ __device__ __forceinline__ Pack<int8_t, kN> codes_of(const float (&n)[kN], float
 
 // The kN elements of a row from p * kN on, as far as k; zeros behind.  kAligned:
 // rows start on 16 bytes and k is a multiple of kN.  Else a lane's elements
-// come one by one, out of lines that its first access brought to L1.
+// come one by one, out of lines that its first access brought to L1.  (Aligned
+// loads shifted into place with a neighbour's took longer: 94 us against 79 us
+// at 4000 x 4099 bf16.)
 template <bool kAligned, class T, int kN>
 __device__ __forceinline__ Pack<T, kN> load_pack(const T* row, int p, int k) {
     Pack<T, kN> v;
@@ -163,9 +165,10 @@ __device__ __forceinline__ Pack<T, kN> load_pack(const T* row, int p, int k) {
     }
     return v;
 }
+// kAligned or `wide`: whole packs of the row lie on their own size.
 template <bool kAligned, class T, int kN>
-__device__ __forceinline__ void store_pack(T* row, int p, int k, const Pack<T, kN>& v) {
-    if (kAligned) {
+__device__ __forceinline__ void store_pack(T* row, int p, int k, const Pack<T, kN>& v, bool wide) {
+    if (kAligned || (wide && (p + 1) * kN <= k)) {
         reinterpret_cast<Pack<T, kN>*>(row)[p] = v;
     } else {
 #pragma unroll
@@ -217,7 +220,7 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1
             const int p = t + i * kThreads;
             if (p < packs) {
                 add_packs(v[i], r[i]);
-                store_pack<kAligned, T, kN>(sum_out, p, a.k, v[i]);
+                store_pack<kAligned, T, kN>(sum_out, p, a.k, v[i], a.wide_sum);
             }
         }
     }
@@ -242,7 +245,15 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1
 #pragma unroll
         for (int j = 0; j < kN / 4; ++j) {
             w[j] = Pack<float, 4>{{1.0f, 1.0f, 1.0f, 1.0f}};
-            if (a.weight) w[j] = load_pack<kAligned, float, 4>(a.weight, p * (kN / 4) + j, a.k);
+            if (a.weight) {
+                const int from = p * kN + 4 * j;
+                if (kAligned || (a.wide_weight && from + 4 <= a.k)) {
+                    w[j] = *reinterpret_cast<const Pack<float, 4>*>(a.weight + from);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) w[j].e[u] = from + u < a.k ? a.weight[from + u] : 0.0f;
+                }
+            }
         }
 #pragma unroll
         for (int j = 0; j < kN; ++j) {
@@ -262,16 +273,12 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1
     for (int i = 0; i < kPacks; ++i) {
         const int p = t + i * kThreads;
         if (p >= packs) continue;
-        const Pack<int8_t, kN> c = codes_of(n[i], scale, rcp);
-        if (!kAligned && a.wide_codes && (p + 1) * kN <= a.k)  // rows of codes have a pitch of their own
-            store_pack<true, int8_t, kN>(q, p, a.k, c);
-        else
-            store_pack<kAligned, int8_t, kN>(q, p, a.k, c);
+        store_pack<kAligned, int8_t, kN>(q, p, a.k, codes_of(n[i], scale, rcp), a.wide_codes);
         if (normed) {
             P o;
 #pragma unroll
             for (int j = 0; j < kN; ++j) o.e[j] = from_float<T>(n[i][j]);
-            store_pack<kAligned, T, kN>(normed, p, a.k, o);
+            store_pack<kAligned, T, kN>(normed, p, a.k, o, a.wide_normed);
         }
     }
     for (int j = a.k + t; j < a.ldq; j += kThreads) q[j] = 0;
@@ -350,21 +357,25 @@ template <class T>
 cudaError_t launch_type(NormArgs a, cudaStream_t stream) {
     constexpr int kN = kElemsPer16<T>;
     constexpr long long b = sizeof(T);
-    const bool whole = a.k % kN == 0 && aligned(a.x, a.ldx * b, 16) && aligned(a.q, a.ldq, kN) &&
-                       aligned(a.weight, 0, 16) &&
-                       (!a.residual || (aligned(a.residual, a.ld_residual * b, 16) &&
-                                        aligned(a.residual_out, a.ld_residual_out * b, 16))) &&
-                       (!a.normed || aligned(a.normed, a.ld_normed * b, 16));
     a.inv_k = 1.0 / a.k;
+    a.wide_weight = aligned(a.weight, 0, 16);
     a.wide_codes = aligned(a.q, a.ldq, kN);
+    a.wide_sum = aligned(a.residual_out, a.ld_residual_out * b, 16);
+    a.wide_normed = aligned(a.normed, a.ld_normed * b, 16);
+    const bool whole = a.k % kN == 0 && aligned(a.x, a.ldx * b, 16) && a.wide_weight && a.wide_codes &&
+                       (!a.residual || (aligned(a.residual, a.ld_residual * b, 16) && a.wide_sum)) &&
+                       (!a.normed || a.wide_normed);
     // Elements a thread.  Many rows: 32, since what a thread does once a row
     // (two reductions, the root) then weighs least (8192 x 8192 bf16: 86 us, 16
-    // a thread 125 us, 64 a thread, with fewer loads under way, 111 us).  A row
-    // an SM or fewer: 8, the shortest chains (one row of 4096 fp32: 2.7 us
-    // against 3.4 us with 16).  Rows off the 16-byte grid: 16 (1537 x 4099
-    // fp32: 24 us, 8 a thread 40 us; 4000 x 4099 bf16: 81 us, 32 a thread 98).
-    if (!whole) return launch_width<T, 16 / kN, false>(a, stream);
-    return a.m <= sm_count() ? launch_width<T, 8 / kN, true>(a, stream) : launch_width<T, 32 / kN, true>(a, stream);
+    // a thread 125 us, 64 a thread, with fewer loads under way, 111 us; rows off
+    // the 16-byte grid, 1537 x 4099 fp32: 20 us, 16 a thread 26 us).  A row an SM
+    // or fewer: 8, the shortest chains (one row of 4096 fp32: 2.7 us against
+    // 3.4 us with 16).  Off the grid a warp's lanes should all have elements
+    // (30000 x 100 bf16: 20 us with 8, 27 us with 16, 41 us with 32).
+    const bool few = a.m <= sm_count();
+    if (whole) return few ? launch_width<T, 8 / kN, true>(a, stream) : launch_width<T, 32 / kN, true>(a, stream);
+    if (few || a.k <= 256) return launch_width<T, 8 / kN, false>(a, stream);
+    return a.k <= 512 ? launch_width<T, 16 / kN, false>(a, stream) : launch_width<T, 32 / kN, false>(a, stream);
 }
 
 }  // namespace
