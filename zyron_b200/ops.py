@@ -30,6 +30,10 @@ if typing.TYPE_CHECKING:
     from torch import Tensor
 
 _NO_CONTEXT = contextlib.nullcontext()
+# torch's default stream has the handle 0, which the library takes for the
+# thread's own default stream.  cudaStreamLegacy names the one that torch means:
+# the same order, and torch's launches need not look at a second stream.
+_LEGACY_STREAM = 1
 torch = None  # the module, from the first call on
 _DTYPES = {}  # torch type -> ZQ_DTYPE_*
 _raw_stream = None  # device index -> raw handle of its current stream
@@ -73,10 +77,11 @@ def _context(index, stream):
     """(context manager, stream pointer): inside, the device is current and
     allocations belong to the stream."""
     if stream is None:
-        return (_NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)), _raw_stream(index)
+        return (_NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)), \
+            _raw_stream(index) or _LEGACY_STREAM
     if stream.device.index != index:
         raise _bad(f"the stream is on {stream.device}, not on cuda:{index}")
-    return torch.cuda.stream(stream), stream.cuda_stream
+    return torch.cuda.stream(stream), stream.cuda_stream or _LEGACY_STREAM
 
 
 def _empty(shape, dtype, device):
