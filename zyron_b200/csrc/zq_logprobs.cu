@@ -54,15 +54,20 @@ namespace {
 namespace cg = cooperative_groups;
 
 // 16-byte packs that a thread loads ahead, as a power of 2: 4; with fp32 rows in
-// blocks of 4 warps 8 (2048 x 32003, one alternative: 48 us against 53 us; at 16
-// bits the larger parts cost the second look more than the loads gain, 1024 x
-// 150001: 86 us against 78 us).
+// blocks of 4 warps 8 (2048 x 32003, one alternative: 48 us against 53 us when it
+// was chosen; at 16 bits it gains nothing, 1024 x 150001 with 8 alternatives: 76
+// us against 73 us).
 template <class T, int kWarps>
 constexpr int kLogUnroll = sizeof(T) == 4 && kWarps == 4 ? 3 : 2;
 constexpr int kMaxSplit = 8;  // CTAs of a row
 constexpr int kStage = 128;   // packs that a warp looks at again at a time
 constexpr int kAhead = 1;     // rounds from a load to its prefetch
-constexpr int kParts = 4;     // parts of a thread's loads that keep a maximum each
+// Parts of a thread's loads that keep a maximum each.  A block of 4 warps has
+// long parts, which a second look reads whole (1024 x 150001 bf16: 8 alternatives
+// 71 us with 8 parts, 75 us with 4; 20 alternatives 76 and 84); with 8 warps the
+// registers are short (48 x 131072, 20 alternatives: 17.7 us with 8, 15.4 with 4).
+template <int kWarps>
+constexpr int kParts = kWarps == 4 ? 8 : 4;
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kHeadroom = 8.0f;
@@ -328,7 +333,7 @@ struct Shared {
     uint64_t queue[kWarps][64];
     uint4 stage[kWarps][kStage];        // packs looked at again, and where they are from
     int stage_at[kWarps][kStage];
-    uint8_t part[kWarps][kParts * 32];  // parts to look at again: part * 32 + lane
+    uint8_t part[kWarps][kParts<kWarps> * 32];  // parts to look at again: part * 32 + lane
     alignas(16) uint64_t keys[kWarps * kTopMax + 8];
     uint64_t best[kTopMax];             // this CTA's largest
     alignas(16) uint64_t gathered[kMaxSplit * kTopMax + 8];  // first CTA: every CTA's
@@ -404,27 +409,30 @@ struct Warp {
     }
 };
 
-// How a thread's packs fall into kParts parts: rounds of its loads ahead, 2^shift
-// rounds a part.
-__device__ __forceinline__ int part_shift(int packs, int per_round) {
+// Rounds of a thread's loads ahead that make one of its kParts parts; with 8
+// warps a power of 2, since a division's registers would cost the fifth block
+// an SM (300 x 100000 bf16, 8 alternatives: 26 us against 30 us).
+template <int kWarps>
+__device__ __forceinline__ int part_rounds(int packs, int per_round) {
     const int rounds = (packs + per_round - 1) / per_round;
-    return max(0, 32 - __clz((max(rounds, 1) - 1) / kParts));
+    const int each = max(1, (rounds + kParts<kWarps> - 1) / kParts<kWarps>);
+    return kWarps == 8 ? 1 << (32 - __clz(each - 1)) : each;
 }
 
 // The sums, and the thread's largest value (NaN passed over) of each part, over
 // the packs [p0, p1) of a row's body: a warp takes kUnroll packs a lane at a
 // time, every lane all packs of its place in the block.
 template <class T, int kWarps>
-__device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int p1, int shift, float (&largest)[kParts]) {
+__device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int p1, int per_part, float (&largest)[kParts<kWarps>]) {
     constexpr int kN = kElemsPer16<T>;
     constexpr int kUnroll = 1 << kLogUnroll<T, kWarps>;
     constexpr int kThreads = kWarps * 32;
     constexpr int kRound = kThreads * kUnroll;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) largest[i] = -INFINITY;
-    int round = 0;
-    for (int p = p0 + warp * 32; p < p1; p += kRound, ++round) {
+    for (int i = 0; i < kParts<kWarps>; ++i) largest[i] = -INFINITY;
+    int part = 0, left = per_part;
+    for (int p = p0 + warp * 32; p < p1; p += kRound) {
         if (threadIdx.x == 0) prefetch(body + p, kAhead * kRound, kRound, p1 - p);
         const bool whole = p + kRound - kThreads + 32 <= p1;
         uint4 v[kUnroll];
@@ -448,8 +456,12 @@ __device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int 
         if (__any_sync(kAll, w.far(most))) w.look(warp_max(most));
         w.take(v, whole);
 #pragma unroll
-        for (int i = 0; i < kParts; ++i)
-            if (round >> shift == i) largest[i] = fmaxf(largest[i], most);
+        for (int i = 0; i < kParts<kWarps>; ++i)
+            if (part == i) largest[i] = fmaxf(largest[i], most);
+        if (--left == 0) {
+            left = per_part;
+            ++part;
+        }
     }
 }
 
@@ -457,7 +469,7 @@ __device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int 
 // warps' lists and queues.
 template <class T, int kWarps>
 __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const Warp<T>& w,
-                                         const float (&largest)[kParts], const uint4* body, int p0, int p1, int shift,
+                                         const float (&largest)[kParts<kWarps>], const uint4* body, int p0, int p1, int per_part,
                                          int head, int k) {
     constexpr int kN = kElemsPer16<T>;
     constexpr int kThreads = kWarps * 32;
@@ -466,7 +478,7 @@ __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const
     // least of all warps' j-th, warps * j >= k.
     float most = largest[0];
 #pragma unroll
-    for (int i = 1; i < kParts; ++i) most = fmaxf(most, largest[i]);
+    for (int i = 1; i < kParts<kWarps>; ++i) most = fmaxf(most, largest[i]);
     const uint32_t sorted = sort_lanes(order(most));
     if (lane == 32 - k) atomicMax(&sh.kth, sorted);
     if (lane == 32 - (k + kWarps - 1) / kWarps) atomicMin(&sh.jth, sorted);
@@ -479,15 +491,15 @@ __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const
     const bool nan = __any_sync(kAll, isnan(s2.x + s2.y + w.slow.s));
     int parts = 0;
 #pragma unroll
-    for (int i = 0; i < kParts; ++i) {
+    for (int i = 0; i < kParts<kWarps>; ++i) {
         const uint32_t hits = __ballot_sync(kAll, nan || order(largest[i]) >= least);
         if (hits >> lane & 1) sh.part[warp][parts + __popc(hits & ((1u << lane) - 1))] = (uint8_t)(i * 32 + lane);
         parts += __popc(hits);
     }
     __syncwarp();
     // All their packs, as many at a time as the stage holds.
-    const int log_each = shift + kLogUnroll<T, kWarps>;
-    const int n = parts << log_each;
+    const int each = per_part << kLogUnroll<T, kWarps>;
+    const int n = parts * each;
     for (int i0 = 0; i0 < n; i0 += kStage) {
         int at[kStage / 32];
 #pragma unroll
@@ -495,8 +507,8 @@ __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const
             const int i = i0 + u * 32 + lane;
             at[u] = p1;
             if (i < n) {
-                const int what = sh.part[warp][i >> log_each];
-                const long long pack = ((long long)(what >> 5) << log_each) + (i & ((1 << log_each) - 1));
+                const int entry = kWarps == 8 ? i >> (31 - __clz(each)) : i / each, what = sh.part[warp][entry];
+                const long long pack = (long long)(what >> 5) * each + (i - entry * each);
                 if (pack * kThreads < p1 - first - (what & 31)) at[u] = first + (what & 31) + (int)pack * kThreads;
             }
             if (at[u] < p1)
@@ -532,7 +544,7 @@ __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const
 }
 
 template <class T, bool kTop, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32) token_logprobs_kernel(const LogprobArgs a, int split) {
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 5 : 8) token_logprobs_kernel(const LogprobArgs a, int split) {
     cg::cluster_group cluster = cg::this_cluster();
     if (split > 1) cluster.barrier_arrive();
     pdl_launch_dependents();
@@ -563,10 +575,10 @@ __global__ void __launch_bounds__(kWarps * 32) token_logprobs_kernel(const Logpr
     const int packs = (a.vocab - head) / kN;
     const uint4* body = reinterpret_cast<const uint4*>(x + head);
     const int p0 = (int)((long long)packs * part / split), p1 = (int)((long long)packs * (part + 1) / split);
-    const int shift = part_shift(p1 - p0, kThreads << kLogUnroll<T, kWarps>);
-    float largest[kParts];
-    pass<T, kWarps>(w, body, p0, p1, shift, largest);
-    if (kTop) find_top<T, kWarps>(top, sh, w, largest, body, p0, p1, shift, head, a.top_k);
+    const int per_part = part_rounds<kWarps>(p1 - p0, kThreads << kLogUnroll<T, kWarps>);
+    float largest[kParts<kWarps>];
+    pass<T, kWarps>(w, body, p0, p1, per_part, largest);
+    if (kTop) find_top<T, kWarps>(top, sh, w, largest, body, p0, p1, per_part, head, a.top_k);
     if (part == 0 && warp == 0) {
         const int tail = head + packs * kN;
         const int loose = head + (a.vocab - tail);  // at most 2 (kN - 1) < 32
@@ -698,15 +710,16 @@ template <class T, bool kTop>
 cudaError_t launch_rows(const LogprobArgs& a, cudaStream_t stream) {
     // Many rows: a block of 4 warps each, 6 rows an SM or more keep enough
     // loads in flight and more rows are past their ends at any time (1024 x
-    // 150001 bf16, 8 alternatives: 78 us against 86 us with 8 warps; 600 x
-    // 100000: 46 us against 36 us).  The same where one round of 4 warps holds
+    // 150001 bf16, 8 alternatives, both with 4 parts: 78 us against 86 us with
+    // 8 warps; 600 x 100000: 46 us against 36 us).  The same where one round of 4 warps holds
     // a row (600 x 2000 bf16: 9.4 us against 11.9 us).
     const int sms = sm_count();
     const long long packs = a.vocab / kElemsPer16<T>;
     if (a.m >= 6LL * sms || packs <= 128 << kLogUnroll<T, 4>) return launch<T, kTop, 4>(a, 1, stream);
     // Else CTAs of 8 warps, 4 an SM, none with less than a round: with 8 an SM
     // the steps behind the pass cost more than the shorter passes save
-    // (300 x 100000 bf16, 8 alternatives: 24 us against 31 us).
+    // (300 x 100000 bf16, 8 alternatives: 24 us against 31 us when it was
+    // chosen).
     int split = 1;
     while (split < kMaxSplit && a.m * split < 4LL * sms && packs >= 2LL * split * 256 << kLogUnroll<T, 8>) split *= 2;
     return launch<T, kTop, 8>(a, split, stream);
