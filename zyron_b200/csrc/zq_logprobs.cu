@@ -390,17 +390,23 @@ struct Warp {
             s = s0;
             t = t0;
         }
+        if (quick) {
+#pragma unroll
+            for (int u = 0; u < n; ++u)
+#pragma unroll
+                for (int j = 0; j < kPairs; ++j) {
+                    const float2 f = unpair(two_of<T>(v[u], j));
+                    add(pair(max_nan(f.x, kClamp<T>), max_nan(f.y, kClamp<T>)));
+                }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < n; ++u)
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
                 const float2 f = unpair(two_of<T>(v[u], j));
-                if (quick) {
-                    add(pair(max_nan(f.x, kClamp<T>), max_nan(f.y, kClamp<T>)));
-                } else {
-                    take_slow(slow, f.x);
-                    take_slow(slow, f.y);
-                }
+                take_slow(slow, f.x);
+                take_slow(slow, f.y);
             }
     }
     __device__ __forceinline__ Sums fast() const {
