@@ -416,8 +416,7 @@ struct Warp {
 };
 
 // Rounds of a thread's loads ahead that make one of its kParts parts; with 8
-// warps a power of 2, since a division's registers would cost the fifth block
-// an SM (300 x 100000 bf16, 8 alternatives: 26 us against 30 us).
+// warps a power of 2, which saves a division's registers.
 template <int kWarps>
 __device__ __forceinline__ int part_rounds(int packs, int per_round) {
     const int rounds = (packs + per_round - 1) / per_round;
@@ -549,8 +548,11 @@ __device__ __forceinline__ void find_top(TopList& top, Shared<kWarps>& sh, const
     }
 }
 
+// Blocks an SM: 8 of 4 warps; 4 of 8 warps, since 5 leave too few registers (48 x
+// 131072 bf16, 20 alternatives: 15.1 us against 17.4 us with 5, spilling; 300 x
+// 100000, where the fifth would hold the last blocks, 27.6 us against 24.7 us).
 template <class T, bool kTop, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 5 : 8) token_logprobs_kernel(const LogprobArgs a, int split) {
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 4 : 8) token_logprobs_kernel(const LogprobArgs a, int split) {
     cg::cluster_group cluster = cg::this_cluster();
     if (split > 1) cluster.barrier_arrive();
     pdl_launch_dependents();
