@@ -247,8 +247,9 @@ zq_status zq_add_low_rank(float* y, size_t ldy, const void* x, int x_dtype, size
  *   entropy[i]     = -sum p log p (natural logarithm)
  *   top_ids[i], top_logprobs[i]: the top_k most likely tokens in order; equal
  *     logits go to the lower id
- * all in fp32.  targets is int64 [m][n_targets] (n_targets may be 0); a
- * negative target asks for nothing and gives 0, one >= vocab gives NaN.
+ * all in fp32; no log probability is above 0 and no entropy below.  targets is
+ * int64 [m][n_targets] (n_targets may be 0); a negative target asks for nothing
+ * and gives 0, one >= vocab gives NaN.
  * -inf logits are tokens that are not allowed; a row that allows none has
  * every log probability -inf and entropy 0.  A NaN or +inf logit makes the
  * row's log probabilities and entropy NaN; in the order of top_ids a NaN

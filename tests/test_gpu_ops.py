@@ -510,6 +510,45 @@ def test_logprobs_orders(zb, torch, vocab):
     check_logprobs(zb, torch, x.cuda(), torch.zeros(4, 1, dtype=torch.int64), 32)
 
 
+@pytest.mark.parametrize("m,vocab", [(9, 70), (9, 40000), (300, 17000), (900, 9001)])
+@pytest.mark.parametrize("dtype,far", [("float32", (1e4, 1e9, 1e10, 1e12, 1e30)), ("bfloat16", (1e4, 1e9, 1e10, 1e12, 1e30)),
+                                       ("float16", (1e4, 6e4))])
+def test_logprobs_finite_masks_and_far_maxima(zb, torch, m, vocab, dtype, far):
+    """Masks of a finite value anywhere in the type's range, over whole rows,
+    whole shares of a row and single tokens, and maxima as far above the rest."""
+    t = getattr(torch, dtype)
+    targets = torch.arange(m).view(m, 1) % vocab
+    targets = torch.cat([targets, torch.full((m, 1), vocab // 2), torch.full((m, 1), vocab - 1)], 1)
+    base = randn(torch, vocab, m, vocab)
+    for c in far:
+        x = base.clone()
+        few = randn(torch, 1, vocab) > 2.0
+        few[vocab // 3] = True
+        for i in range(0, m - 8, 9):
+            x[i] = -c                                # every token masked
+            x[i + 1, ~few] = -c                      # most
+            x[i + 2, : vocab * 6 // 10] = -c         # the first ones
+            x[i + 3, vocab * 4 // 10 :] = -c         # the last ones
+            x[i + 4, :-1] = -c                       # all but the last
+            x[i + 5, vocab // 5] = c                 # one far above
+            x[i + 6, vocab // 3] = x[i + 6, -1] = c  # two
+            x[i + 7] = c                             # all
+            x[i + 8, ::2], x[i + 8, 1::2] = -c, c
+        check_logprobs(zb, torch, x.to(t).cuda(), targets, 3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,vocab", [(3000, 64), (1000, 3000), (40, 70000)])
+def test_logprobs_are_not_positive(zb, torch, m, vocab, dtype):
+    """Probabilities near 1, where the roundings of a log probability are larger than itself."""
+    likely = torch.arange(m) * 37 % vocab
+    g = torch.Generator().manual_seed(3)
+    x = randn(torch, vocab, m, vocab) - 40 * torch.rand(m, 1, generator=g)
+    x[torch.arange(m), likely] = 60 * torch.rand(m, generator=g)
+    got = check_logprobs(zb, torch, x.to(getattr(torch, dtype)).cuda(), likely[:, None], 4)
+    assert (got.logprobs <= 0).all() and (got.top_logprobs <= 0).all()
+
+
 def test_logprobs_shapes_and_views(zb, torch):
     x = randn(torch, 3, 2, 3, 1000)
     t = torch.randint(0, 1000, (2, 3), generator=torch.Generator().manual_seed(1))
