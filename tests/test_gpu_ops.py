@@ -150,6 +150,25 @@ def test_norm_extremes(zb, torch, k):
         same_bits(torch, got.codes, codes, "codes")
 
 
+@pytest.mark.parametrize("k", [8192, 70000])
+def test_norm_longest_code_rows(zb, torch, k):
+    """Padding up to the largest row pitch of the codes, where a 32-bit count of it would wrap."""
+    from zyron_b200 import _lib
+
+    ldq = 2**31 - 1
+    x = randn(torch, k, 1, k)
+    xd = x.cuda()
+    q = torch.full((ldq + 1,), 7, dtype=torch.int8, device="cuda")
+    scale = torch.empty(1, device="cuda")
+    _lib.check(_lib.lib().zq_rms_norm_quantize(xd.data_ptr(), 1, 1, k, k, None, 0, None, 1e-5, 0, None, 0, None, 0,
+                                               q.data_ptr(), ldq, scale.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    codes, want, _, _ = norm_oracle(torch, x, None, None, 1e-5)
+    same_bits(torch, q[:k], codes[0], "codes")
+    same_bits(torch, scale, want, "row_scale")
+    assert not q[k:ldq].any() and q[ldq] == 7
+
+
 def test_norm_in_place_and_shapes(zb, torch):
     x, r, w = norm_case(torch, 6, 320, "bfloat16", True)
     codes, scale, total, v = norm_oracle(torch, x, r, w, 1e-6)

@@ -281,7 +281,7 @@ __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1
             store_pack<kAligned, T, kN>(normed, p, a.k, o, a.wide_normed);
         }
     }
-    for (int j = a.k + t; j < a.ldq; j += kThreads) q[j] = 0;
+    for (long long j = a.k + t; j < a.ldq; j += kThreads) q[j] = 0;  // ldq may be the last int
 }
 
 // Rows too long for the registers: one block a row that reads the sum three
