@@ -662,6 +662,48 @@ def test_step_together(zb, torch, m):
     same_bits(torch, lp.top_ids, wids, "top_ids")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(6000, 5), (3000, 36), (500, 1001)])
+def test_chains_of_calls(zb, torch, m, k, dtype):
+    """Calls that follow one another without a pause, each on what the one
+    before wrote in place, rows sharing sectors of memory: the same bits as with
+    the device waited for after every call."""
+    t = getattr(torch, dtype)
+    w = (1 + 0.1 * randn(torch, 1, k)).cuda()
+    a = (randn(torch, 2, 3, 8, k) * k**-0.5).bfloat16().cuda()
+    b = (randn(torch, 3, 3, k, 8) * 8**-0.5).bfloat16().cuda()
+    ids = torch.randint(-1, 3, (m,), generator=torch.Generator().manual_seed(4), dtype=torch.int32).cuda()
+    W = zb.quantize((randn(torch, 5, k, k) * k**-0.5).cuda())
+
+    def chain(pause):
+        r = randn(torch, 6, m, k).to(t).cuda()
+        y = randn(torch, 7, m, k).cuda()
+        x = r * 2
+        for i in range(12):
+            h = zb.rms_norm_quantize(x, w, residual=r, residual_out=r, normed=True)
+            pause()
+            zb.add_low_rank(y, h.normed, a, b, ids)
+            pause()
+            n = zb.rms_norm_quantize(y, w, residual=y, residual_out=y, normed=True)
+            pause()
+            zb.add_low_rank(y, y, a, b, ids)  # x may be y: all of it is read before y is added to
+            pause()
+            z = zb.matmul_codes(n.codes, n.row_scale, W, out=y)
+            pause()
+            lp = zb.token_logprobs(y, top_k=2)
+            pause()
+            z = zb.matmul(y, W)
+            pause()
+            x = zb.rms_norm_quantize(z.to(t) if i % 2 else h.normed, w, residual=r, normed=True).normed
+            pause()
+        return r, y, z, lp.entropy, lp.top_ids
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(3):
+        for got, ref, what in zip(chain(lambda: None), want, ("residual", "y", "matmul", "entropy", "top_ids")):
+            same_bits(torch, got, ref, what)
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_step_in_graphs_and_streams(zb, torch, m):
     """Two captured graphs of the step, replayed in turn and on two streams at

@@ -11,6 +11,7 @@
 #pragma once
 
 #include <cstdint>
+#include <cstring>
 #include <cuda_runtime.h>
 
 namespace zq {
@@ -321,5 +322,43 @@ __device__ __forceinline__ uint4 ld_stream_u4(const void* p) {
                  : "l"(p));
     return v;
 }
+
+// Loads of data that earlier kernels of the stream wrote (launch_kernel has the
+// rule); they move neither across pdl_wait_primary nor across this thread's own
+// stores.  load_l2 and load_l2_once go past L1.  Which streams better differs:
+// rms_norm_quantize, 8192 x 8192 bf16, 85.1 us with load_l2, 86.1 with the other;
+// token_logprobs, 2048 x 32003 fp32, 54 and 48; add_low_rank, 4096 x 4096 x 4096
+// of rank 64, 78 and 74.  load_l1 may come from L1.
+#define ZQ_LOAD(NAME, OP)                                                          \
+    template <class T>                                                             \
+    __device__ __forceinline__ T NAME(const T* p) {                                \
+        static_assert(sizeof(T) == 16 || sizeof(T) == 4 || sizeof(T) == 2 || sizeof(T) == 8, "one load"); \
+        T v;                                                                       \
+        if constexpr (sizeof(T) == 16) {                                           \
+            uint4 r;                                                               \
+            asm volatile(OP ".v4.u32 {%0,%1,%2,%3}, [%4];"                         \
+                         : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)              \
+                         : "l"(p)                                                  \
+                         : "memory");                                              \
+            memcpy(&v, &r, 16);                                                    \
+        } else if constexpr (sizeof(T) == 8) {                                     \
+            uint64_t r;                                                            \
+            asm volatile(OP ".u64 %0, [%1];" : "=l"(r) : "l"(p) : "memory");       \
+            memcpy(&v, &r, 8);                                                     \
+        } else if constexpr (sizeof(T) == 4) {                                     \
+            uint32_t r;                                                            \
+            asm volatile(OP ".u32 %0, [%1];" : "=r"(r) : "l"(p) : "memory");       \
+            memcpy(&v, &r, 4);                                                     \
+        } else {                                                                   \
+            uint16_t r;                                                            \
+            asm volatile(OP ".u16 %0, [%1];" : "=h"(r) : "l"(p) : "memory");       \
+            memcpy(&v, &r, 2);                                                     \
+        }                                                                          \
+        return v;                                                                  \
+    }
+ZQ_LOAD(load_l2, "ld.global.cg")
+ZQ_LOAD(load_l2_once, "ld.relaxed.gpu.global.L1::no_allocate")
+ZQ_LOAD(load_l1, "ld.global")
+#undef ZQ_LOAD
 
 }  // namespace zq

@@ -509,7 +509,7 @@ __global__ void __launch_bounds__(threads_for<kW4>(), 1)
             tmem_fence_after();
             const int row0 = mt * kBM + quarter * 32;
             const int row = row0 + lane;
-            const float sr = row < M ? __ldg(row_scale + row) : 0.0f;
+            const float sr = row < M ? load_l2(row_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
             if constexpr (!kGather) {
                 store_tile_rows<BN>(taddr, row, row < M, nt * BN, N, sr, col_scale, bias, out.base[0], vec1, shift);
@@ -881,7 +881,7 @@ __global__ void __launch_bounds__((pair_threads<kW4, kGather>()), 1)
             tmem_fence_after();
             const int row0 = mt * 256 + (int)rank * 128 + quarter * 32;
             const int row = row0 + lane;
-            const float sr = row < M ? __ldg(row_scale + row) : 0.0f;
+            const float sr = row < M ? load_l2(row_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
             if constexpr (!kGather) {
                 store_tile_rows<256>(taddr, row, row < M, nt * 256, N, sr, col_scale, bias, out.base[0], vec1, shift);

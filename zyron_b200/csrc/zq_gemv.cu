@@ -108,12 +108,12 @@ __device__ __forceinline__ void quantize_row_staged(const float* __restrict__ x,
         const int k0 = gi * 8;
         float4 lo, hi;
         if (vec && k0 + 8 <= K) {
-            lo = __ldg(reinterpret_cast<const float4*>(x + k0));
-            hi = __ldg(reinterpret_cast<const float4*>(x + k0) + 1);
+            lo = load_l1(reinterpret_cast<const float4*>(x + k0));
+            hi = load_l1(reinterpret_cast<const float4*>(x + k0) + 1);
         } else {
             float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = k0 + j < K ? __ldg(x + k0 + j) : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = k0 + j < K ? load_l1(x + k0 + j) : 0.0f;
             lo = make_float4(v[0], v[1], v[2], v[3]);
             hi = make_float4(v[4], v[5], v[6], v[7]);
         }
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const uint8_t* __restric
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             const int i = b + u * kThreads;
-                            v[u] = i < K4 ? __ldg(x4 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            v[u] = i < K4 ? load_l1(x4 + i) : make_float4(0.f, 0.f, 0.f, 0.f);
                         }
 #pragma unroll
                         for (int u = 0; u < 2; ++u)
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const uint8_t* __restric
                                                        fmaxf(fabsf(v[u].z), fabsf(v[u].w))));
                     }
                 } else {
-                    for (int i = threadIdx.x; i < K; i += kThreads) mx[m] = fmaxf(mx[m], fabsf(__ldg(xr + i)));
+                    for (int i = threadIdx.x; i < K; i += kThreads) mx[m] = fmaxf(mx[m], fabsf(load_l1(xr + i)));
                 }
             }
 #pragma unroll
@@ -243,13 +243,13 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const uint8_t* __restric
             float v[8];
             const float* xk = x + (size_t)m * K + k0;
             if (m < M && vec && k0 + 8 <= K) {
-                const float4 lo = __ldg(reinterpret_cast<const float4*>(xk));
-                const float4 hi = __ldg(reinterpret_cast<const float4*>(xk) + 1);
+                const float4 lo = load_l1(reinterpret_cast<const float4*>(xk));
+                const float4 hi = load_l1(reinterpret_cast<const float4*>(xk) + 1);
                 v[0] = lo.x; v[1] = lo.y; v[2] = lo.z; v[3] = lo.w;
                 v[4] = hi.x; v[5] = hi.y; v[6] = hi.z; v[7] = hi.w;
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = (m < M && k0 + j < K) ? __ldg(xk + j) : 0.0f;
+                for (int j = 0; j < 8; ++j) v[j] = (m < M && k0 + j < K) ? load_l1(xk + j) : 0.0f;
             }
             uint32_t c[8];
             const float rcp = zq_quant_rcp(sm);
@@ -267,11 +267,11 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const uint8_t* __restric
         for (int i = threadIdx.x; i < kM * words; i += kThreads) {
             const int m = i / words;
             const int wi = i - m * words;
-            s4[i] = m < M ? q4[(size_t)m * words + wi] : 0u;
+            s4[i] = m < M ? load_l1(q4 + (size_t)m * words + wi) : 0u;
         }
     }
 #pragma unroll
-    for (int m = 0; m < kM; ++m) srow[m] = m < M ? row_scale[m] : 0.0f;
+    for (int m = 0; m < kM; ++m) srow[m] = m < M ? load_l1(row_scale + m) : 0.0f;
     }
     __syncthreads();
 

@@ -17,10 +17,19 @@ namespace zq {
 // Every kernel launched this way reads only immutable data (weight panels,
 // scales) before its griddepcontrol.wait, and reads or writes everything else
 // after it; the wait returns when the kernels before it have completed and
-// their memory is visible.
+// their memory is visible in L2.  An SM's L1 may still hold lines that another
+// kernel loaded before they were written, and ld.global.nc asks for data that
+// nothing writes while the kernel is resident.  So what earlier kernels of the
+// stream wrote is read through L2 (load_l2, load_l2_once, ld.global.cg, TMA), and
+// a kernel that needs L1 for it is launched with `early` false, after everything
+// before it has ended, and executes no launch_dependents: no kernel runs beside
+// it that could meet its lines.  The GEMV starts early and reads its activations
+// by load_l1: it lets no other start, and whatever runs beside it has brought no
+// such data to L1.  Weights, their scales, and ids, ranks and scales of adapters
+// are never the output of the library's own kernels; they may come from L1.
 template <class... Params, class... Args>
-cudaError_t launch_pdl_kernel(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
-                              Args... args) {
+cudaError_t launch_kernel(bool early, void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                          Args... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = block;
@@ -30,8 +39,13 @@ cudaError_t launch_pdl_kernel(void (*kern)(Params...), dim3 grid, dim3 block, si
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = early ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kern, static_cast<Params>(args)...);
+}
+template <class... Params, class... Args>
+cudaError_t launch_pdl_kernel(void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                              Args... args) {
+    return launch_kernel(true, kern, grid, block, smem, stream, args...);
 }
 
 constexpr int kGemvMaxRows = 8;

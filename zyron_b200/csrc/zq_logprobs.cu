@@ -453,7 +453,7 @@ __device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int 
         uint4 v[kUnroll];
         if (whole) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u] = ld_stream_u4(body + p + u * kThreads + lane);
+            for (int u = 0; u < kUnroll; ++u) v[u] = load_l2_once(body + p + u * kThreads + lane);
         } else {
             Pack<T, kN> none;
 #pragma unroll
@@ -462,7 +462,7 @@ __device__ __forceinline__ void pass(Warp<T>& w, const uint4* body, int p0, int 
             for (int u = 0; u < kUnroll; ++u) {
                 const int q = p + u * kThreads + lane;
                 if (q < p1)
-                    v[u] = ld_stream_u4(body + q);
+                    v[u] = load_l2_once(body + q);
                 else
                     memcpy(&v[u], &none, 16);
             }
@@ -601,7 +601,7 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 4 : 8) token_logpro
         const int tail = head + packs * kN;
         const int loose = head + (a.vocab - tail);  // at most 2 (kN - 1) < 32
         const int i = lane < head ? lane : tail + lane - head;
-        const float f = lane < loose ? to_float(x[i]) : -INFINITY;
+        const float f = lane < loose ? to_float(load_l2_once(x + i)) : -INFINITY;
         const float m = warp_max(f);
         if (w.far(m)) w.look(m);
         if (w.quick)
@@ -687,12 +687,12 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 8 ? 4 : 8) token_logpro
     }
     auto log_p = [&](float v) { return v - r.r - log_s; };
     for (long long i = threadIdx.x; i < a.n_targets; i += kThreads) {
-        const long long t = a.targets[row * a.n_targets + i];
+        const long long t = load_l2_once(reinterpret_cast<const long long*>(a.targets) + row * a.n_targets + i);
         float lp = 0.0f;  // no token asked for
         if (t >= a.vocab)
             lp = __uint_as_float(0x7FC00000u);
         else if (t >= 0)
-            lp = log_p(to_float(x[t]));
+            lp = log_p(to_float(load_l2_once(x + t)));
         a.logprobs[row * a.n_targets + i] = lp;
     }
     if (kTop && (int)threadIdx.x < a.top_k) {

@@ -27,8 +27,9 @@
 // global memory straight into fragments; the kMT warps of a block that share
 // weights and differ in rows meet in L1.
 //
-// Bound: the used adapters once, x once, y read and written.  Every block
-// prefetches its shares into L2 before it waits for anything else.
+// Bound: the used adapters once, x once, y read and written.  A block prefetches
+// its shares into L2 as soon as it knows its rows: in expand that is before h is
+// there.
 #include <type_traits>
 
 #include "zq_common.cuh"
@@ -150,15 +151,20 @@ constexpr int kRaw = 8 / kElemsPer16<T>;
 
 // Elements [0, n) of p (n may be <= 0 or above 8) as raw packs, zeros behind
 // them.  kVec: p is 16-byte aligned and, where n > 0, all 8 may be read; with
-// kWhole all 8 count.
-template <class T, bool kVec, bool kWhole = false>
+// kWhole all 8 count.  kL2: p is data of earlier kernels (one by one its
+// elements share lines in L1, and the kernel neither starts early nor lets
+// others; launch_kernel).
+template <class T, bool kVec, bool kWhole = false, bool kL2 = false>
 __device__ __forceinline__ void load8(const T* p, int n, uint4 (&raw)[kRaw<T>]) {
     constexpr int kN = kElemsPer16<T>;
     if (kVec) {
 #pragma unroll
         for (int i = 0; i < kRaw<T>; ++i) {
             raw[i] = make_uint4(0, 0, 0, 0);
-            if (n > 0) raw[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+            if (n > 0) {
+                const uint4* q = reinterpret_cast<const uint4*>(p) + i;
+                raw[i] = kL2 ? load_l2_once(q) : __ldg(q);
+            }
         }
         if (!kWhole && n > 0 && n < 8) {
 #pragma unroll
@@ -236,10 +242,10 @@ __device__ __forceinline__ int find_rows(const LowRankArgs& a, const Workspace& 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (kMT == 1 && a.m <= kDirectRows) {
         __shared__ uint32_t same[kWarps];
-        const int id = a.ids[tile];
+        const int id = load_l1(a.ids + tile);
         *slot = id;
         if (threadIdx.x < 16) row_of[threadIdx.x] = -1;
-        const bool mine = (int)threadIdx.x < a.m && a.ids[threadIdx.x] == id;
+        const bool mine = (int)threadIdx.x < a.m && load_l1(a.ids + threadIdx.x) == id;
         const uint32_t votes = __ballot_sync(0xffffffffu, mine);
         if (lane == 0) same[warp] = votes;
         __syncthreads();
@@ -258,16 +264,16 @@ __device__ __forceinline__ int find_rows(const LowRankArgs& a, const Workspace& 
         __syncthreads();
         return min(16, all - before);
     }
-    if (tile >= *ws.count) return 0;
-    const Tile t = ws.tiles[tile];
+    if (tile >= load_l2_once(ws.count)) return 0;
+    const Tile t = load_l2_once(ws.tiles + tile);
     *slot = t.slot;
-    if (threadIdx.x < 16 * kMT) row_of[threadIdx.x] = (int)threadIdx.x < t.rows ? ws.order[t.first + threadIdx.x] : -1;
+    if (threadIdx.x < 16 * kMT) row_of[threadIdx.x] = (int)threadIdx.x < t.rows ? load_l2_once(ws.order + t.first + threadIdx.x) : -1;
     __syncthreads();
     return t.rows;
 }
 
 __device__ __forceinline__ int rank_of(const LowRankArgs& a, int slot) {
-    return a.ranks ? min(max(a.ranks[slot], 0), a.max_rank) : a.max_rank;
+    return a.ranks ? min(max(load_l1(a.ranks + slot), 0), a.max_rank) : a.max_rank;
 }
 
 // ---- h = A x -----------------------------------------------------------------
@@ -280,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_kernel(const LowRankArgs a
     // The kernels before have completed when this one's blocks let expand
     // start, so expand may read everything but h before its own wait.
     pdl_wait_primary();
-    pdl_launch_dependents();
+    if (kVec) pdl_launch_dependents();
     constexpr int kGroups = kWarps / kMT;  // warps that split a tile's k
     __shared__ int row_of[16 * kMT];
     extern __shared__ float sums[];  // [kGroups][16 * kMT][width]
@@ -308,6 +314,7 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_kernel(const LowRankArgs a
     const int width = pass_width(a.max_rank), hp = rank_pitch(a.max_rank);
     const TX* x_lo = static_cast<const TX*>(a.x) + row_of[min(16 * mt + g, rows - 1)] * a.ldx;
     const TX* x_hi = static_cast<const TX*>(a.x) + row_of[min(16 * mt + g + 8, rows - 1)] * a.ldx;
+    const int hi_end = 16 * mt + 8 < rows ? k_end : 0;  // no loads for an upper half without rows
     constexpr int kStep = 32 * kGroups;
     for (int r0 = 0; r0 < rank; r0 += kRankPass) {
         if (r0) __syncthreads();  // the pass before has been read
@@ -319,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_kernel(const LowRankArgs a
         // spilling, 87).  k is a whole number of packs where kVec.
         uint4 raw_lo[kRaw<TX>], raw_hi[kRaw<TX>], raw_a[kRankPass / 8][1];
         auto fetch_x = [&](int k) {
-            load8<TX, kVec, kVec>(x_lo + k, k_end - k, raw_lo);
-            load8<TX, kVec, kVec>(x_hi + k, k_end - k, raw_hi);
+            load8<TX, kVec, kVec, true>(x_lo + k, k_end - k, raw_lo);
+            load8<TX, kVec, kVec, true>(x_hi + k, hi_end - k, raw_hi);
         };
         auto fetch_a = [&](int k, int j) {
             const int r = min(r0 + 8 * j + g, rank - 1);
@@ -425,11 +432,16 @@ __host__ __device__ int part_pitch(int max_rank) {
     return b % 128 == 64 ? b : b + 64;
 }
 
-// y[0..4) += v, added in L2: nothing waits for y to arrive.  Each element is
-// added to once, so the result does not depend on any order.  (The addition in
-// L2 takes subnormal values as 0.)
+// y[0..4) += v, added in L2: nothing waits for y to arrive, and no sector of y
+// that another block adds to comes to L1.  Each element is added to once, so the
+// result does not depend on any order.  (The addition in L2 takes subnormal
+// values as 0.)
 __device__ __forceinline__ void add4(float* y, float v0, float v1, float v2, float v3) {
     asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(y), "f"(v0), "f"(v1), "f"(v2), "f"(v3) : "memory");
+}
+
+__device__ __forceinline__ void add1(float* y, float v) {
+    asm volatile("red.global.add.f32 [%0], %1;" ::"l"(y), "f"(v) : "memory");
 }
 
 // kVecB: rows of B start on 16 bytes and are whole packs of 8; kVecY: 16-byte
@@ -455,12 +467,12 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
         if (kVecB && threadIdx.x == kThreads - 1)
             prefetch(wb + (long long)c_begin * a.max_rank, (long long)(c_end - c_begin) * a.max_rank * (long long)sizeof(TW));
     }
-    pdl_launch_dependents();
     pdl_wait_primary();
+    pdl_launch_dependents();  // no earlier: shrink may have brought x to L1
     if (rank == 0) return;
 
     // h: the shares' sum, scaled, as three bf16 parts
-    const float scale = a.scales ? a.scales[slot] : 1.0f;
+    const float scale = a.scales ? load_l1(a.scales + slot) : 1.0f;
     const int pitch = part_pitch(a.max_rank), hp = rank_pitch(a.max_rank);
     for (int r = threadIdx.x >> 3; r < 16 * kMT; r += kThreads / 8)
         for (int c = (threadIdx.x & 7) * 4; c < rank; c += 32) {
@@ -469,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
                 const float* h = ws.h + (size_t)row_of[r] * hp + c;
 #pragma unroll 8
                 for (int w = 0; w < shape.shares; ++w) {
-                    const float4 v = *reinterpret_cast<const float4*>(h + (size_t)w * a.m * hp);
+                    const float4 v = load_l2_once(reinterpret_cast<const float4*>(h + (size_t)w * a.m * hp));
                     s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
                 }
             }
@@ -542,8 +554,8 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    if (has_lo && at + i < cols) y_lo[col + i] += acc[2 * u + i / 2][i % 2];
-                    if (has_hi && at + i < cols) y_hi[col + i] += acc[2 * u + i / 2][2 + i % 2];
+                    if (has_lo && at + i < cols) add1(y_lo + col + i, acc[2 * u + i / 2][i % 2]);
+                    if (has_hi && at + i < cols) add1(y_hi + col + i, acc[2 * u + i / 2][2 + i % 2]);
                 }
             }
         }
@@ -605,7 +617,7 @@ __global__ void __launch_bounds__(kPlanThreads)
 #pragma unroll
     for (int u = 0; u < kPlanHeld; ++u) {
         const int i = u * kPlanThreads + threadIdx.x;
-        id[u] = i < m ? ids[i] : -1;
+        id[u] = i < m ? load_l1(ids + i) : -1;
         if (id[u] >= slots || id[u] < 0) id[u] = -1;
     }
     for (int s = threadIdx.x; s < slots; s += kPlanThreads) counts[s] = 0;
@@ -622,7 +634,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     for (int u = 0; u < kPlanHeld; ++u)
         if (u * kPlanThreads < m) place[u] = count(id[u]);
     for (int i = kPlanHeld * kPlanThreads + threadIdx.x; i < (m + 31) / 32 * 32; i += kPlanThreads) {
-        const int slot = i < m ? ids[i] : -1;
+        const int slot = i < m ? load_l1(ids + i) : -1;
         const int at = count(slot < 0 || slot >= slots ? -1 : slot);
         if (i < m) ws.place[i] = at;
     }
@@ -659,7 +671,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     for (int u = 0; u < kPlanHeld; ++u)
         if (u * kPlanThreads < m && id[u] >= 0) ws.order[counts[id[u]] + place[u]] = u * kPlanThreads + threadIdx.x;
     for (int i = kPlanHeld * kPlanThreads + threadIdx.x; i < m; i += kPlanThreads) {
-        const int slot = ids[i];
+        const int slot = load_l1(ids + i);
         if (slot >= 0 && slot < slots) ws.order[counts[slot] + ws.place[i]] = i;
     }
 }
@@ -693,13 +705,13 @@ Shape shape_of(const LowRankArgs& a) {
 }
 
 template <class Kern>
-cudaError_t launch_grid(Kern kern, dim3 grid, int smem, cudaStream_t stream, const LowRankArgs& a, void* ws,
+cudaError_t launch_grid(bool early, Kern kern, dim3 grid, int smem, cudaStream_t stream, const LowRankArgs& a, void* ws,
                         const Shape& shape) {
     if (smem > 47 * 1024) {  // with the static arrays past the 48 KiB that need no attribute
         const cudaError_t e = ensure_smem_attr(kern, (size_t)smem);
         if (e != cudaSuccess) return e;
     }
-    return launch_pdl_kernel(kern, grid, dim3(kThreads), (size_t)smem, stream, a, ws, shape);
+    return launch_kernel(early, kern, grid, dim3(kThreads), (size_t)smem, stream, a, ws, shape);
 }
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -709,8 +721,8 @@ cudaError_t launch_shrink(const LowRankArgs& a, void* ws, const Shape& shape, un
     const bool vec = a.k % 8 == 0 && on16(a.x) && a.ldx * sizeof(TX) % 16 == 0 && on16(a.a);
     const int smem = kWarps * 16 * pass_width(a.max_rank) * (int)sizeof(float);
     const dim3 grid(tiles, (unsigned)shape.shares);
-    return vec ? launch_grid(shrink_kernel<TX, TW, true, kMT>, grid, smem, stream, a, ws, shape)
-               : launch_grid(shrink_kernel<TX, TW, false, kMT>, grid, smem, stream, a, ws, shape);
+    return vec ? launch_grid(true, shrink_kernel<TX, TW, true, kMT>, grid, smem, stream, a, ws, shape)
+               : launch_grid(false, shrink_kernel<TX, TW, false, kMT>, grid, smem, stream, a, ws, shape);
 }
 
 template <class TW, int kMT>
@@ -719,10 +731,10 @@ cudaError_t launch_expand(const LowRankArgs& a, void* ws, const Shape& shape, un
     const bool vy = a.n % 4 == 0 && on16(a.y) && a.ldy % 4 == 0;
     const int smem = 3 * 16 * kMT * part_pitch(a.max_rank);
     const dim3 grid(tiles, (unsigned)shape.col_shares);
-    if (vb && vy) return launch_grid(expand_kernel<TW, true, true, kMT>, grid, smem, stream, a, ws, shape);
-    if (vb) return launch_grid(expand_kernel<TW, true, false, kMT>, grid, smem, stream, a, ws, shape);
-    if (vy) return launch_grid(expand_kernel<TW, false, true, kMT>, grid, smem, stream, a, ws, shape);
-    return launch_grid(expand_kernel<TW, false, false, kMT>, grid, smem, stream, a, ws, shape);
+    if (vb && vy) return launch_grid(true, expand_kernel<TW, true, true, kMT>, grid, smem, stream, a, ws, shape);
+    if (vb) return launch_grid(true, expand_kernel<TW, true, false, kMT>, grid, smem, stream, a, ws, shape);
+    if (vy) return launch_grid(true, expand_kernel<TW, false, true, kMT>, grid, smem, stream, a, ws, shape);
+    return launch_grid(true, expand_kernel<TW, false, false, kMT>, grid, smem, stream, a, ws, shape);
 }
 
 template <class TX, class TW>

@@ -151,14 +151,15 @@ __device__ __forceinline__ Pack<int8_t, kN> codes_of(const float (&n)[kN], float
 
 // The kN elements of a row from p * kN on, as far as k; zeros behind.  kAligned:
 // rows start on 16 bytes and k is a multiple of kN.  Else a lane's elements
-// come one by one, out of lines that its first access brought to L1.  (Aligned
+// come one by one, out of lines that its first access brought to L1 (such a kernel
+// neither starts early nor lets others; launch_kernel).  (Aligned
 // loads shifted into place with a neighbour's took longer: 94 us against 79 us
 // at 4000 x 4099 bf16.)
 template <bool kAligned, class T, int kN>
 __device__ __forceinline__ Pack<T, kN> load_pack(const T* row, int p, int k) {
     Pack<T, kN> v;
     if (kAligned) {
-        v = reinterpret_cast<const Pack<T, kN>*>(row)[p];
+        v = load_l2(reinterpret_cast<const Pack<T, kN>*>(row) + p);
     } else {
 #pragma unroll
         for (int j = 0; j < kN; ++j) v.e[j] = p * kN + j < k ? row[p * kN + j] : T(0.0f);
@@ -182,7 +183,7 @@ __device__ __forceinline__ void store_pack(T* row, int p, int k, const Pack<T, k
 template <class T, int kWarps, int kPacks, bool kAligned>
 __global__ void __launch_bounds__(kWarps > 8 ? kWarps * 32 : 256, kWarps > 8 ? 1 : 3)
     rms_norm_quantize_kernel(const NormArgs a) {
-    pdl_launch_dependents();
+    if (kAligned) pdl_launch_dependents();
     pdl_wait_primary();
     constexpr int kN = kElemsPer16<T>;
     constexpr int kBlockWarps = kWarps > 8 ? kWarps : 8;
@@ -299,9 +300,9 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
     T* sum_out = a.residual ? static_cast<T*>(a.residual_out) + row * a.ld_residual_out : nullptr;
     double sum = 0.0;
     for (int i = threadIdx.x; i < a.k; i += 1024) {
-        T v = x[i];
+        T v = load_l2(x + i);
         if (res) {
-            v = from_float<T>(__fadd_rn(to_float(v), to_float(res[i])));
+            v = from_float<T>(__fadd_rn(to_float(v), to_float(load_l2(res + i))));
             sum_out[i] = v;
         }
         const double d = (double)to_float(v);
@@ -311,7 +312,7 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
     const T* s = res ? sum_out : x;
     float absmax = 0.0f;
     for (int i = threadIdx.x; i < a.k; i += 1024)
-        absmax = fmaxf(absmax, fabsf(norm_value(to_float(s[i]), rstd, a.weight ? a.weight[i] : 1.0f)));
+        absmax = fmaxf(absmax, fabsf(norm_value(to_float(load_l2(s + i)), rstd, a.weight ? a.weight[i] : 1.0f)));
     absmax = group_max<32>(absmax, part_max);
     const float scale = row_scale_of(a, absmax);
     const float rcp = zq_quant_rcp(scale);
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
     int8_t* q = a.q + row * a.ldq;
     T* normed = a.normed ? static_cast<T*>(a.normed) + row * a.ld_normed : nullptr;
     for (int i = threadIdx.x; i < a.k; i += 1024) {
-        const float n = norm_value(to_float(s[i]), rstd, a.weight ? a.weight[i] : 1.0f);
+        const float n = norm_value(to_float(load_l2(s + i)), rstd, a.weight ? a.weight[i] : 1.0f);
         q[i] = (int8_t)zq_quantize_value_rcp(n, scale, rcp, 127);
         if (normed) normed[i] = from_float<T>(n);
     }
@@ -329,9 +330,9 @@ __global__ void __launch_bounds__(1024) rms_norm_quantize_long_kernel(const Norm
 template <class T, int kWarps, int kPacks, bool kAligned>
 cudaError_t launch_rows(const NormArgs& a, cudaStream_t stream) {
     constexpr int kRows = kWarps > 8 ? 1 : 8 / kWarps;
-    return launch_pdl_kernel(rms_norm_quantize_kernel<T, kWarps, kPacks, kAligned>,
-                             dim3((unsigned)((a.m + kRows - 1) / kRows)), dim3(kWarps > 8 ? kWarps * 32 : 256), 0,
-                             stream, a);
+    return launch_kernel(kAligned, rms_norm_quantize_kernel<T, kWarps, kPacks, kAligned>,
+                         dim3((unsigned)((a.m + kRows - 1) / kRows)), dim3(kWarps > 8 ? kWarps * 32 : 256), 0, stream,
+                         a);
 }
 
 template <class T, int kPacks, bool kAligned>

@@ -31,12 +31,12 @@ __device__ __forceinline__ void clear_words(int* zero, int n_zero) {
         for (int i = threadIdx.x; i < n_zero; i += blockDim.x) zero[i] = 0;
 }
 
+// Reads x twice, the second time from L1 where the row fits: neither starts
+// early nor lets others (launch_kernel).
 template <bool kVec>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const float* __restrict__ x, int M, int K,
                                                             int Kp, int8_t* __restrict__ q,
                                                             float* __restrict__ row_scale, int* zero, int n_zero) {
-    pdl_launch_dependents();
-    pdl_wait_primary();  // x may come from, and q / counters be read by, the kernels before
     clear_words(zero, n_zero);
     const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
     const int lane = threadIdx.x & 31;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const float* __r
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
             const int idx = t + i * kT;
-            v[i] = idx < k4 ? __ldg(x4 + idx) : make_float4(0.f, 0.f, 0.f, 0.f);
+            v[i] = idx < k4 ? load_l2(x4 + idx) : make_float4(0.f, 0.f, 0.f, 0.f);
             m = fmaxf(m, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
         }
     }
@@ -164,10 +164,10 @@ cudaError_t launch_quantize_rows(const float* x, int M, int K, int Kp, int8_t* q
     const bool vec = (K % 4 == 0) && (Kp % 4 == 0) && ((reinterpret_cast<uintptr_t>(x) & 15u) == 0) &&
                      ((reinterpret_cast<uintptr_t>(q) & 3u) == 0);
     if (vec)
-        return launch_pdl_kernel(quantize_rows_kernel<true>, grid, dim3(256), 0, stream, x, M, K, Kp, q, row_scale,
-                                 zero, n_zero);
-    return launch_pdl_kernel(quantize_rows_kernel<false>, grid, dim3(256), 0, stream, x, M, K, Kp, q, row_scale, zero,
-                             n_zero);
+        return launch_kernel(false, quantize_rows_kernel<true>, grid, dim3(256), 0, stream, x, M, K, Kp, q, row_scale,
+                             zero, n_zero);
+    return launch_kernel(false, quantize_rows_kernel<false>, grid, dim3(256), 0, stream, x, M, K, Kp, q, row_scale,
+                         zero, n_zero);
 }
 
 // ---------------------------------------------------------------------------
