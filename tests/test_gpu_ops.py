@@ -390,6 +390,32 @@ def test_adapters_strides(zb, torch, m):
     same_bits(torch, y3[0], want, "three dimensions")
 
 
+@pytest.mark.parametrize("m", [5, 300])
+def test_adapters_subnormal_outputs(zb, torch, m):
+    """Subnormal y, sums and additions count as zeros, wherever y lies; rows
+    without an adapter keep theirs."""
+    n, k = 40, 16
+    tiny = 2.0**-126
+    a = torch.zeros(2, 1, k).bfloat16()
+    b = torch.ones(2, n, 1).bfloat16()
+    a[0, 0, 0] = 1.0
+    x = torch.zeros(m, k)
+    y = torch.full((m, n), tiny / 8)
+    x[1, 0], y[1] = -tiny, 1.5 * tiny     # a normal sum's terms
+    x[2, 0], y[2] = tiny / 4, tiny        # a subnormal addition
+    x[3, 0], y[3] = 2.0**-100, tiny / 2   # beside a normal one
+    ids = torch.zeros(m, dtype=torch.int32)
+    ids[4:] = -1
+    want = y.clone()
+    want[0], want[1], want[2], want[3] = 0.0, 0.0, tiny, 2.0**-100
+    for start in (0, 1):
+        wide = torch.zeros(m, n + start, device="cuda")
+        got = wide[:, start:]
+        got.copy_(y)
+        zb.add_low_rank(got, x.cuda(), a.cuda(), b.cuda(), ids.cuda())
+        same_bits(torch, got.abs(), want, f"y at {start}")
+
+
 def test_adapters_linear_forward(zb, torch):
     w = randn(torch, 1, 96, 80) * 0.05
     lin = zb.QuantizedLinear(w.cuda(), randn(torch, 2, 80))
