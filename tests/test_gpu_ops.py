@@ -310,6 +310,96 @@ def test_adapters(zb, torch, m, k, n, slots, rank, dtype, wdtype):
         check_adapters(torch, zb, *adapter_case(torch, m, k, n, slots, rank, dtype, wdtype, layout, ragged))
 
 
+WDTYPES = ["bfloat16", "float16"]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wdtype", WDTYPES)
+@pytest.mark.parametrize("m,k,n,slots,rank", [(3, 96, 40, 2, 5), (40, 1000, 33, 3, 70), (300, 4096, 64, 3, 16),
+                                              (270, 333, 130, 2, 256)])
+def test_adapters_exact_products(zb, torch, m, k, n, slots, rank, dtype, wdtype):
+    """Sums that fp32 holds exactly, whatever the order, bit for bit: every
+    element's own bits through both products, and whole numbers whose sums of
+    absolute values stay below 2^24.  A part of a value that is lost shows."""
+    t, w = getattr(torch, dtype), getattr(torch, wdtype)
+    g = torch.Generator().manual_seed(m + k)
+    ids = torch.randint(-1, slots, (m,), generator=g, dtype=torch.int32)
+    live = ids >= 0
+
+    def run(y, x, a, b, scales=None):
+        yd = y.cuda()
+        zb.add_low_rank(yd, x.to(t).cuda(), a.to(w).cuda(), b.to(w).cuda(), ids.cuda(),
+                        scales=None if scales is None else scales.cuda())
+        return yd
+
+    # one element and one rank an output, weights and scales powers of two
+    x = randn(torch, k, m, k).to(t).float()
+    a, b = torch.zeros(slots, rank, k), torch.zeros(slots, n, rank)
+    col = torch.randint(0, k, (slots, rank), generator=g)
+    a.scatter_(2, col[:, :, None], 2.0 ** torch.randint(-3, 4, (slots, rank, 1), generator=g))
+    pick = torch.randint(0, rank, (slots, n), generator=g)
+    b.scatter_(2, pick[:, :, None], -(2.0 ** torch.randint(-3, 4, (slots, n, 1), generator=g)))
+    scales = 2.0 ** torch.arange(slots).float()
+    s = ids.clamp(min=0).long()
+    h = x.gather(1, col[s]) * a.gather(2, col[:, :, None])[s, :, 0]
+    want = scales[s][:, None] * h.gather(1, pick[s]) * b.gather(2, pick[:, :, None])[s, :, 0]
+    same_bits(torch, run(torch.zeros(m, n), x, a, b, scales), torch.where(live[:, None], want, 0.0), "single products")
+
+    # whole numbers
+    xlimit = {"float32": 1 << 24, "float16": 1 << 11, "bfloat16": 1 << 8}[dtype]
+    wlimit = {"float16": (1 << 11) - 1, "bfloat16": 1 << 8}[wdtype]
+    for amax, a_n, xmax, bmax, b_n in ((1, 8, 1 << 19, 1, 2), (wlimit, 8, 1 << 9, 1, 1), (1, 4, 1 << 10, wlimit, 1)):
+        xmax = min(xmax, xlimit)
+
+        def whole(shape, most):
+            return torch.randint(-most, most + 1, shape, generator=g).double()
+
+        x = whole((m, k), xmax)
+        a, b = torch.zeros(slots, rank, k).double(), torch.zeros(slots, n, rank).double()
+        a.scatter_(2, torch.randint(0, k, (slots, rank, a_n), generator=g), whole((slots, rank, a_n), amax))
+        b.scatter_(2, torch.randint(0, rank, (slots, n, b_n), generator=g), whole((slots, n, b_n), bmax))
+        y = whole((m, n), 1 << 21)
+        h = torch.einsum("mk,mrk->mr", x, a[s])
+        want = y + live[:, None] * torch.einsum("mr,mnr->mn", h, b[s])
+        assert want.abs().max() < 1 << 24
+        same_bits(torch, run(y.float(), x, a, b), want.float(), f"whole numbers to {xmax}, {amax}, {bmax}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("wdtype", WDTYPES)
+def test_adapters_long_sums_lose_no_more(zb, torch, dtype, wdtype):
+    """Tensor cores cut sums off, so a chain of products of one sign loses the
+    more the longer it is.  A sum that is one chain of 24 products shows what a
+    chain loses; longer sums of the same values are rounded sums of such chains
+    and lose the same share, within a quarter for the spread and half a last
+    place for each of the additions."""
+    t, w = getattr(torch, dtype), getattr(torch, wdtype)
+    parts = {"float32": 3, "float16": 2, "bfloat16": 1}
+    wparts = 2 if wdtype == "float16" else 1
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def draw(*shape):
+        return torch.rand(*shape, generator=g, device="cuda") + 0.1
+
+    def loss(m, x, a, b):
+        ids = torch.zeros(m, dtype=torch.int32, device="cuda")
+        got = zb.add_low_rank(torch.zeros(m, b.shape[1], device="cuda"), x, a, b, ids).double()
+        want = x.double() @ a[0].double().T @ b[0].double().T
+        return float(((got - want).square().mean() / want.square().mean()).sqrt())
+
+    # A x of one block of four warps a tile, each a quarter of k in chunks of 32; B picks a rank
+    m, n = 5000, 64
+    pick = torch.eye(n, device="cuda").to(w)[None]
+    one = 4 * 32 * (12 // (parts[dtype] * wparts))
+    short, long = (loss(m, draw(m, k).to(t), draw(1, n, k).to(w), pick) for k in (one, 8 * one))
+    assert long <= 1.25 * short + 8 * 2.0**-25, (short * 2**24, long * 2**24)
+    # B h, h the elements of x as they are, over all ranks
+    one = 32 * (12 // (3 * wparts))
+    short, long = (loss(m, draw(m, r).to(t), torch.eye(r, device="cuda").to(w)[None], draw(1, n, r).to(w))
+                   for r in (one, 256))
+    assert long <= 1.25 * short + 4 * 2.0**-25, (short * 2**24, long * 2**24)
+
+
 @pytest.mark.parametrize("m", [6, 300])
 def test_adapters_leave_other_rows(zb, torch, m):
     """Rows without an adapter keep their bits, whatever they hold, and what

@@ -207,6 +207,11 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// Tensor cores cut sums off instead of rounding them, which adds up along a
+// chain of products; so a chain ends after kChainMmas of them, and chains are
+// added with rounding.
+constexpr int kChainMmas = 24;
+
 // d[j] += (rows lo, hi) x (column j of a chunk's 16-bit weights) over a chunk of
 // 32, every part with every part, the smallest products first; the same step
 // of all columns in a row, since each waits for its column's last.
@@ -340,33 +345,26 @@ __global__ void __launch_bounds__(kThreads, 2) shrink_kernel(const LowRankArgs a
             Pairs<TX> lo, hi;
             to_pairs(raw_lo, lo);
             to_pairs(raw_hi, hi);
-            // two-part weights: 4 columns' parts at a time (4096 rows of rank 64:
-            // 131 us, all 8 at once 167 us)
-            constexpr int kAtOnce = kAhead || kParts<TW> == 1 ? kN : 4;
+            // two-part weights: 2 columns' parts at a time (4096 rows of rank 64:
+            // 126 us, 4 columns at a time with their loads 140 us)
+            constexpr int kAtOnce = kAhead || kParts<TW> == 1 ? kN : 2;
             if (!kAhead) {
 #pragma unroll
-                for (int j = 0; j < kAtOnce; ++j) fetch_a(k0 + 8 * t, j);
+                for (int j = 0; j < kN; ++j) fetch_a(k0 + 8 * t, j);
             }
             fetch_x(next);
 #pragma unroll
-            for (int j0 = 0; j0 < kN; j0 += kAtOnce) {
+            for (int j0 = 0; j0 < kN; j0 += kAtOnce)
                 mma_chunk<TW, kAtOnce>(acc + j0, lo.pair, hi.pair, raw_a + j0);
-                if (j0 + kAtOnce < kN) {
-#pragma unroll
-                    for (int j = 0; j < kAtOnce; ++j) fetch_a(k0 + 8 * t, j0 + kAtOnce + j);
-                }
-            }
             if (kAhead) {
 #pragma unroll
                 for (int j = 0; j < kN; ++j) fetch_a(next, j);
             }
         };
-        // The sums so far to the warp's place in shared memory.  Tensor cores cut
-        // sums off instead of rounding them, which adds up along a chain of
-        // products; so a chain ends after 24 of them, and chains are added with
-        // rounding (4096 x 4096 x 4096 of rank 64: the sums' error 1.2e-6 in
-        // chains of 96, 3.5e-7 in chains of 24, at 79 us against 77 us).
-        constexpr int kChain = 12 / kParts<TX>;  // chunks
+        // A chain's sums to the warp's place in shared memory (4096 x 4096 x 4096
+        // of rank 64: the sums' error 1.2e-6 in chains of 96, 3.5e-7 in chains of
+        // 24, at 79 us against 77 us).
+        constexpr int kChain = kChainMmas / (2 * kParts<TX> * kParts<TW>);  // chunks
         float* place = sums + (group * 16 * kMT + 16 * mt) * width + 2 * t;
         auto put = [&](auto columns, bool add) {
             constexpr int kN = decltype(columns)::value;
@@ -450,7 +448,7 @@ template <class TW, bool kVecB, bool kVecY, int kMT>
 __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a, void* workspace, const Shape shape) {
     constexpr int kGroups = kWarps / kMT;  // warps that split a tile's columns
     __shared__ int row_of[16 * kMT];
-    extern __shared__ __align__(128) uint8_t parts[];  // [3][16 * kMT][pitch]
+    extern __shared__ __align__(128) uint8_t parts[];  // [3][16 * kMT][pitch], sums of chains
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int g = lane >> 2, t = lane & 3;
     const int mt = warp % kMT, group = warp / kMT;
@@ -560,6 +558,25 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
             }
         }
     };
+    // A chain's sums wait in shared memory, behind the parts of h, for the next
+    // one's.  Ranks of one chain need none of it.  (4096 x 4096 x 4096 of rank 256:
+    // 248 us, in one chain 246 us; sums of one sign lose 1.1e-6, in one chain
+    // 2.8e-6, with fp16 weights 5.4e-7 and 4.3e-6.)
+    constexpr int kChain = 32 * kChainMmas / (2 * 3 * kParts<TW>);  // ranks
+    float* parked = reinterpret_cast<float*>(parts + 3 * 16 * kMT * pitch) + threadIdx.x;
+    auto end_chain = [&](float(&acc)[kWarpCols / 8][4], int r0) {
+        if ((r0 + 32) % kChain != 0 && r0 + 32 < rank) return;
+        const bool add = r0 >= kChain, last = r0 + 32 >= rank;
+#pragma unroll
+        for (int i = 0; i < kWarpCols / 2; ++i) {
+            float& v = acc[i / 4][i % 4];
+            if (add) v += parked[i * kThreads];
+            if (!last) {
+                parked[i * kThreads] = v;
+                v = 0.0f;
+            }
+        }
+    };
     int c0 = first;
     const long long b_step = (long long)kStep * a.max_rank;
     if (kVecB && c0 + kWarpCols <= c_end) {
@@ -582,6 +599,7 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
                     }
                 }
                 product(acc, raw, r0);
+                if (rank > kChain) end_chain(acc, r0);
 #pragma unroll
                 for (int j = 0; j < kWarpCols / 8; ++j) raw[j][0] = next[j][0];
             }
@@ -594,6 +612,7 @@ __global__ void __launch_bounds__(kThreads, 2) expand_kernel(const LowRankArgs a
             uint4 raw[kWarpCols / 8][1];
             fetch_b(raw, b_lane, r0, c_end - c0, std::false_type{});
             product(acc, raw, r0);
+            if (rank > kChain) end_chain(acc, r0);
         }
         store(acc, c0, c_end - c0);
     }
@@ -729,7 +748,7 @@ template <class TW, int kMT>
 cudaError_t launch_expand(const LowRankArgs& a, void* ws, const Shape& shape, unsigned tiles, cudaStream_t stream) {
     const bool vb = a.max_rank % 8 == 0 && on16(a.b);
     const bool vy = a.n % 4 == 0 && on16(a.y) && a.ldy % 4 == 0;
-    const int smem = 3 * 16 * kMT * part_pitch(a.max_rank);
+    const int smem = 3 * 16 * kMT * part_pitch(a.max_rank) + (int)sizeof(float) * kThreads * kWarpCols / 2;
     const dim3 grid(tiles, (unsigned)shape.col_shares);
     if (vb && vy) return launch_grid(true, expand_kernel<TW, true, true, kMT>, grid, smem, stream, a, ws, shape);
     if (vb) return launch_grid(true, expand_kernel<TW, true, false, kMT>, grid, smem, stream, a, ws, shape);
