@@ -882,6 +882,70 @@ def test_calls_from_threads(zb, torch):
             same_bits(torch, a, b, "log probabilities")
 
 
+def test_matmul_on_another_stream(zb, torch):
+    """matmul, quantize_rows and a linear with adapters on a stream that is not
+    the current one: copies of their inputs run there, not behind the current
+    stream's work, and their outputs' memory is that stream's."""
+    st = torch.cuda.Stream()
+    lin = zb.QuantizedLinear((randn(torch, 1, 96, 80) * 0.05).cuda())
+    _, x, a, b, ids, scales, ranks = adapter_case(torch, 300, 96, 80, 3, 8, "float32", "bfloat16")
+    pool = zb.LowRankAdapters(a.cuda(), b.cuda(), scales.cuda(), ranks.cuda())
+    x, ids = x.cuda(), ids.cuda()
+    cols = x.t().contiguous().t()  # rows in a transposed order are copied
+    want = lin(x, adapters=pool, adapter_ids=ids), zb.matmul(x, lin.weight()), *zb.quantize_rows(x)
+    lin(cols, adapters=pool, adapter_ids=ids, stream=st)  # workspaces and memory at hand on both streams
+    junk = [torch.full((300, 96), math.nan, device="cuda") for _ in range(8)]
+    del junk  # what a copy on the current stream would be made in
+    torch.cuda.synchronize()
+    torch.cuda._sleep(400_000_000)  # the current stream is busy for about 0.2 s
+    got = (lin(cols, adapters=pool, adapter_ids=ids, stream=st), zb.matmul(cols, lin.weight(), stream=st),
+           *zb.quantize_rows(cols, stream=st))
+    st.synchronize()
+    with torch.cuda.stream(st):
+        host = [t.cpu() for t in got]
+    assert not torch.cuda.current_stream().query()  # nothing above waited for it
+    torch.cuda.synchronize()
+    for g, w, what in zip(host, want, ("linear with adapters", "matmul", "codes", "row scales")):
+        same_bits(torch, g, w, what)
+    # given back, the memory does not go to the current stream's next tensor
+    at = got[1].data_ptr()
+    del got, g
+    fresh = [torch.empty_like(want[1]) for _ in range(32)]
+    assert at not in [t.data_ptr() for t in fresh]
+    if torch.cuda.device_count() > 1:
+        with pytest.raises(ValueError, match="the stream is on cuda:1"):
+            zb.matmul(x, lin.weight(), stream=torch.cuda.Stream(1))
+
+
+def test_calls_of_one_step_share_a_stream(zb, torch, monkeypatch):
+    """On torch's default stream every call passes the same handle."""
+    from zyron_b200 import _lib
+
+    handles = {}
+    real = _lib.lib()
+
+    class Spy:
+        def __getattr__(self, name):
+            f = getattr(real, name)
+
+            def call(*args):
+                if name in ("zq_matmul", "zq_matmul_codes", "zq_quantize_rows", "zq_add_low_rank", "zq_rms_norm_quantize"):
+                    handles[name] = getattr(args[-1], "value", args[-1])
+                return f(*args)
+
+            return call
+
+    for module in ("zyron_b200.quantization.lib", "zyron_b200.ops.lib"):
+        monkeypatch.setattr(module, lambda: Spy())
+    lin = zb.QuantizedLinear((randn(torch, 1, 96, 80) * 0.05).cuda())
+    _, x, a, b, ids, _, _ = adapter_case(torch, 6, 96, 80, 3, 8, "float32", "bfloat16")
+    h = zb.rms_norm_quantize(x.cuda(), normed=True)
+    lin(h.normed, adapters=zb.LowRankAdapters(a.cuda(), b.cuda()), adapter_ids=ids.cuda())
+    zb.matmul_codes(*zb.quantize_rows(h.normed), lin.weight())
+    torch.cuda.synchronize()
+    assert len(handles) == 5 and len(set(handles.values())) == 1, handles
+
+
 def test_stream_argument(zb, torch):
     """A call on another stream than the current one, its inputs made there."""
     st = torch.cuda.Stream()

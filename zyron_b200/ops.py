@@ -19,34 +19,24 @@ include/zq.h.
 """
 from __future__ import annotations
 
-import contextlib
 import typing
 
 from . import _lib
 from ._lib import check, lib
-from .quantization import QuantizedMatrix
+from .quantization import QuantizedMatrix, _context
 
 if typing.TYPE_CHECKING:
     from torch import Tensor
 
-_NO_CONTEXT = contextlib.nullcontext()
-# torch's default stream has the handle 0, which the library takes for the
-# thread's own default stream.  cudaStreamLegacy names the one that torch means:
-# the same order, and torch's launches need not look at a second stream.
-_LEGACY_STREAM = 1
 torch = None  # the module, from the first call on
 _DTYPES = {}  # torch type -> ZQ_DTYPE_*
-_raw_stream = None  # device index -> raw handle of its current stream
 
 
 def _setup():
-    global torch, _raw_stream
+    global torch
     import torch as module
 
     _DTYPES.update({module.float32: 1, module.float16: 2, module.bfloat16: 3})
-    _raw_stream = getattr(module._C, "_cuda_getCurrentRawStream", None)
-    if _raw_stream is None:
-        _raw_stream = lambda index: module.cuda.current_stream(index).cuda_stream  # noqa: E731
     torch = module
 
 
@@ -71,17 +61,6 @@ def _device(first, names, *others):
         if t is not None and t.get_device() != index:
             raise _bad(f"{names.split()[i]} is on {t.device}, not on {first.device}")
     return index
-
-
-def _context(index, stream):
-    """(context manager, stream pointer): inside, the device is current and
-    allocations belong to the stream."""
-    if stream is None:
-        return (_NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)), \
-            _raw_stream(index) or _LEGACY_STREAM
-    if stream.device.index != index:
-        raise _bad(f"the stream is on {stream.device}, not on cuda:{index}")
-    return torch.cuda.stream(stream), stream.cuda_stream or _LEGACY_STREAM
 
 
 def _empty(shape, dtype, device):

@@ -14,6 +14,7 @@ through ``zq_matmul_host``).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import enum
 import threading
@@ -39,6 +40,26 @@ def _stream_ptr(stream=None):
     torch = _torch()
     s = stream if stream is not None else torch.cuda.current_stream()
     return C.c_void_p(s.cuda_stream)
+
+
+_NO_CONTEXT = contextlib.nullcontext()
+# torch's default stream has the handle 0, which the library takes for the
+# thread's own default stream.  cudaStreamLegacy names the one that torch means:
+# the same order, and torch's launches need not look at a second stream.
+_LEGACY_STREAM = 1
+
+
+def _context(index, stream):
+    """(context manager, stream handle) of a call on device `index`, on `stream`
+    (None: the device's current one): inside, the device is current and copies
+    and allocations belong to the stream that the call runs on."""
+    torch = _torch()
+    if stream is None:
+        return (_NO_CONTEXT if torch.cuda.current_device() == index else torch.cuda.device(index)), \
+            torch._C._cuda_getCurrentRawStream(index) or _LEGACY_STREAM
+    if stream.device.index != index:
+        raise _lib.ZQInvalidArgument(f"zyron_b200: the stream is on {stream.device}, not on cuda:{index}")
+    return torch.cuda.stream(stream), stream.cuda_stream or _LEGACY_STREAM
 
 
 def _payload_bytes(qtype, rows, cols):
@@ -277,29 +298,32 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
     torch = _torch()
     if input.dtype != torch.float32:
         raise _lib.ZQInvalidArgument("zyron_b200: input must be float32")
-    x = input.contiguous().reshape(-1, weights.rows())
-    m = x.shape[0]
-    if out is None:
-        out = torch.empty((m, weights.cols()), dtype=torch.float32, device=x.device)
-    s = stream if stream is not None else torch.cuda.current_stream(x.device)
-    with torch.cuda.device(x.device):
-        ws, ws_bytes = workspace(weights, m, x.device, s.cuda_stream)
-        check(lib().zq_matmul(weights.handle, C.c_void_p(x.data_ptr()), m,
-                              None if bias is None else C.c_void_p(bias.data_ptr()),
-                              C.c_void_p(out.data_ptr()), C.c_void_p(ws), ws_bytes, C.c_void_p(s.cuda_stream)))
-    return out.reshape(out_shape)
+    if input.get_device() < 0:
+        raise _lib.ZQInvalidArgument("zyron_b200: input must be on a CUDA device")
+    context, ptr = _context(input.get_device(), stream)
+    with context:
+        x = input.contiguous().reshape(-1, weights.rows())
+        m = x.shape[0]
+        if out is None:
+            out = torch.empty((m, weights.cols()), dtype=torch.float32, device=x.device)
+        ws, ws_bytes = workspace(weights, m, x.device, ptr)
+        check(lib().zq_matmul(weights.handle, x.data_ptr(), m, None if bias is None else bias.data_ptr(),
+                              out.data_ptr(), ws, ws_bytes, ptr))
+        return out.reshape(out_shape)
 
 
 def quantize_rows(x, stream=None):
     """The per-row activation quantizer alone: (codes int8 [M,K], scales fp32 [M])."""
     torch = _torch()
-    x = x.contiguous()
-    m, k = x.shape
-    q = torch.empty((m, k), dtype=torch.int8, device=x.device)
-    s = torch.empty((m,), dtype=torch.float32, device=x.device)
-    with torch.cuda.device(x.device):
-        check(lib().zq_quantize_rows(C.c_void_p(x.data_ptr()), m, k, C.c_void_p(q.data_ptr()), k,
-                                     C.c_void_p(s.data_ptr()), _stream_ptr(stream)))
+    if x.get_device() < 0:
+        raise _lib.ZQInvalidArgument("zyron_b200: input must be on a CUDA device")
+    context, ptr = _context(x.get_device(), stream)
+    with context:
+        x = x.contiguous()
+        m, k = x.shape
+        q = torch.empty((m, k), dtype=torch.int8, device=x.device)
+        s = torch.empty((m,), dtype=torch.float32, device=x.device)
+        check(lib().zq_quantize_rows(x.data_ptr(), m, k, q.data_ptr(), k, s.data_ptr(), ptr))
     return q, s
 
 
