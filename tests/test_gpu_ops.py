@@ -855,6 +855,50 @@ def test_step_in_graphs_and_streams(zb, torch, m):
                 same_bits(torch, a, b, "log probabilities")
 
 
+@pytest.mark.parametrize("m", [6, 40, 300])
+def test_captured_linears_have_scratch_of_their_own(zb, torch, monkeypatch, m):
+    """Two graphs captured on one stream, replayed at once and beside eager calls on that stream."""
+    from zyron_b200 import _lib
+
+    scratch = []
+    real = _lib.lib()
+
+    class Spy:
+        def __getattr__(self, name):
+            if name == "zq_matmul":
+                return lambda *args: scratch.append(getattr(args[5], "value", args[5])) or real.zq_matmul(*args)
+            return getattr(real, name)
+
+    monkeypatch.setattr("zyron_b200.quantization.lib", lambda: Spy())
+    lin = zb.QuantizedLinear((randn(torch, 1, 512, 384) * 0.05).cuda())
+    _, x, a, b, ids, _, _ = adapter_case(torch, m, 512, 384, 3, 8, "float32", "bfloat16")
+    pool = zb.LowRankAdapters(a.cuda(), b.cuda())
+    xs, ids = [x.cuda(), x.cuda() * 2 + 1, x.cuda() - 3], ids.cuda()
+    want = [lin(v, adapters=pool, adapter_ids=ids) for v in xs]
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        lin(xs[0])
+    graphs, outs = [], []
+    for v in xs[:2]:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=st):
+            outs.append(lin(v, adapters=pool, adapter_ids=ids))
+    others = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, other in zip(graphs, others):
+            with torch.cuda.stream(other):
+                graph.replay()
+        with torch.cuda.stream(st):
+            outs[2:] = [lin(xs[2], adapters=pool, adapter_ids=ids)]
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            same_bits(torch, got, ref, "linear")
+    eager, first, second = scratch[3], scratch[4], scratch[5]
+    assert len({eager, first, second}) == 3 and set(scratch[6:]) == {eager}
+
+
 def test_calls_from_threads(zb, torch):
     """Calls from several threads at once, each on a stream of its own."""
     import threading

@@ -258,17 +258,22 @@ _ws = _Workspaces()
 
 
 def workspace(weights, m, device, stream_key):
-    """Per-thread, per-(device, stream) cached device scratch for zq_matmul."""
+    """Device scratch for zq_matmul: (address, bytes, the tensor that holds
+    it).  Cached per thread, device and stream; a call that is being captured
+    into a graph gets scratch of its own out of the graph's memory, which no
+    other graph's replay nor a later call writes."""
     torch = _torch()
     need = lib().zq_matmul_workspace_bytes(weights.handle, m)
     key = (device, stream_key)
-    buf = _ws.bufs.get(key)
+    capturing = torch.cuda.is_current_stream_capturing()
+    buf = None if capturing else _ws.bufs.get(key)
     if buf is None or buf.numel() < need:
         buf = torch.empty(max(need, 256) + 256, dtype=torch.uint8, device=device)
-        _ws.bufs[key] = buf
+        if not capturing:
+            _ws.bufs[key] = buf
     base = buf.data_ptr()
     aligned = (base + 255) & ~255
-    return aligned, buf.numel() - (aligned - base)
+    return aligned, buf.numel() - (aligned - base), buf
 
 
 def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
@@ -306,7 +311,7 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
         m = x.shape[0]
         if out is None:
             out = torch.empty((m, weights.cols()), dtype=torch.float32, device=x.device)
-        ws, ws_bytes = workspace(weights, m, x.device, ptr)
+        ws, ws_bytes, _held = workspace(weights, m, x.device, ptr)
         check(lib().zq_matmul(weights.handle, x.data_ptr(), m, None if bias is None else bias.data_ptr(),
                               out.data_ptr(), ws, ws_bytes, ptr))
         return out.reshape(out_shape)

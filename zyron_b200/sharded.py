@@ -190,7 +190,10 @@ def sharded_matmul_gathered(x, weight_shard, peer_out: PeerOutputs, bias_shard=N
     x = x.contiguous()
     m = x.shape[0]
     s = stream if stream is not None else torch.cuda.current_stream(x.device)
-    ws, ws_bytes = workspace if workspace is not None else get_workspace(weight_shard, m, x.device, s.cuda_stream)
+    if workspace is not None:
+        ws, ws_bytes = workspace
+    else:
+        ws, ws_bytes, _held = get_workspace(weight_shard, m, x.device, s.cuda_stream)
     turn = peer_out.turn
     dst = peer_out.pointers
     ptrs = (C.c_void_p * len(dst))(*dst)
