@@ -542,6 +542,34 @@ def test_adapters_refusals_on_device(zb, torch):
     assert empty.shape == (0, 16)
 
 
+def test_linear_refusals_on_device(zb, torch):
+    """Nothing is launched for a call that is refused: out keeps what it holds."""
+    y, x, a, b, ids, _, _ = [t.cuda() for t in adapter_case(torch, 4, 32, 16, 2, 8, "float32", "bfloat16")]
+    lin = zb.QuantizedLinear(torch.ones(32, 16, device="cuda"))
+    out = torch.full((4, 16), 7.0, device="cuda")
+    for pool, bad_ids, match in (((a, b), ids.long(), "ids must be int32"), ((a, b), ids[:2], "ids must be int32"),
+                                 ((a[:, :, :31].contiguous(), b), ids, "dimension mismatch"),
+                                 ((a, b[:, :15].contiguous()), ids, "output/adapter dimension mismatch"),
+                                 ((a, b.half()), ids, "of one type"), ((a, b.cpu()), ids, "b is on cpu")):
+        with pytest.raises(ValueError, match=match):
+            lin(x, out=out, adapters=zb.LowRankAdapters(*pool), adapter_ids=bad_ids)
+    w = lin.weight()
+    for bad in (out.half(), out[:3], out.cpu(), torch.empty(4, 32, device="cuda")[:, :16], torch.empty(4, 17, device="cuda")):
+        with pytest.raises(ValueError, match="out must be contiguous float32"):
+            zb.matmul(x, w, out=bad)
+    bias = torch.zeros(16, device="cuda")
+    for bad in (bias.cpu(), bias.half(), bias[:15], torch.zeros(32, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="bias must be contiguous float32"):
+            zb.matmul(x, w, bias=bad, out=out)
+    for bad in (x.half(), x[0]):
+        with pytest.raises(ValueError, match="input must be float32"):
+            zb.quantize_rows(bad)
+    torch.cuda.synchronize()
+    assert (out == 7).all()
+    assert zb.matmul(x, w, bias=bias, out=out).data_ptr() == out.data_ptr()
+    assert zb.matmul(x.view(2, 2, 32), w, out=out).shape == (2, 2, 16)  # out by its number of elements
+
+
 # ---- log probabilities ------------------------------------------------------------
 
 def logprob_oracle(torch, x, targets, k):

@@ -112,5 +112,7 @@ def test_python_refusals(native_lib):
         zb.add_low_rank(x, x, x.bfloat16(), x.bfloat16(), x)
     with pytest.raises(ValueError, match="tensors must be on a CUDA device"):
         zb.token_logprobs(x)
+    with pytest.raises(ValueError, match="input must be on a CUDA device"):
+        zb.quantize_rows(x)
     with pytest.raises(ValueError, match="weights are empty"):
         zb.matmul_codes(x, x, zb.QuantizedMatrix())

@@ -230,11 +230,16 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
     ``ranks`` are the fields of ``LowRankAdapters``.  Rows whose id is not in
     [0, slots) are left as they are; only the first ``ranks[s]`` of an
     adapter's ranks count."""
+    return _add_low_rank(_low_rank_call(x, a, b, ids, scales, ranks, stream), y)
+
+
+def _low_rank_call(x, a, b, ids, scales, ranks, stream):
+    """The checked arguments of an adapter call but for y, which may not be there yet."""
     if torch is None:
         _setup()
     xt = _dtype(x, "x")
     wt = _dtype(a, "a")
-    index = _device(x, "y a b ids scales ranks", y, a, b, ids, scales, ranks)
+    index = _device(x, "a b ids scales ranks", a, b, ids, scales, ranks)
     if a.dim() != 3 or b.dim() != 3 or a.dtype != b.dtype:
         raise _bad("a must be [slots, max_rank, in] and b [slots, out, max_rank], of one type")
     slots, max_rank, k = a.shape
@@ -253,8 +258,16 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
         raise _bad("scales must be contiguous float32 [slots]")
     if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != (slots,) or not ranks.is_contiguous()):
         raise _bad("ranks must be contiguous int32 [slots]")
-    yr, ldy = _out_rows(y, "y", (*lead, n), torch.float32)
-    context, ptr = _context(index, stream)
+    return x, xt, a, b, wt, ids, scales, ranks, (*lead, n), index, _context(index, stream)
+
+
+def _add_low_rank(call, y):
+    x, xt, a, b, wt, ids, scales, ranks, shape, index, (context, ptr) = call
+    slots, max_rank, k = a.shape
+    n = shape[-1]
+    if y.get_device() != index:
+        raise _bad(f"y is on {y.device}, not on {x.device}")
+    yr, ldy = _out_rows(y, "y", shape, torch.float32)
     with context:
         xr, ldx = _rows(x, "x")
         if not ids.is_contiguous():

@@ -303,14 +303,24 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
     torch = _torch()
     if input.dtype != torch.float32:
         raise _lib.ZQInvalidArgument("zyron_b200: input must be float32")
-    if input.get_device() < 0:
+    index = input.get_device()
+    if index < 0:
         raise _lib.ZQInvalidArgument("zyron_b200: input must be on a CUDA device")
-    context, ptr = _context(input.get_device(), stream)
+    if weights._device != index:
+        raise _lib.ZQInvalidArgument(f"zyron_b200: the weights are on cuda:{weights._device}, not on {input.device}")
+    n = weights.cols()
+    if bias is not None and (bias.get_device() != index or bias.dtype != torch.float32 or bias.numel() != n
+                             or not bias.is_contiguous()):
+        raise _lib.ZQInvalidArgument("zyron_b200: bias must be contiguous float32 [N] on input's device")
+    if out is not None and (out.get_device() != index or out.dtype != torch.float32 or not out.is_contiguous()
+                            or out.numel() * weights.rows() != input.numel() * n):
+        raise _lib.ZQInvalidArgument("zyron_b200: out must be contiguous float32 [..., N] on input's device")
+    context, ptr = _context(index, stream)
     with context:
         x = input.contiguous().reshape(-1, weights.rows())
         m = x.shape[0]
         if out is None:
-            out = torch.empty((m, weights.cols()), dtype=torch.float32, device=x.device)
+            out = torch.empty((m, n), dtype=torch.float32, device=x.device)
         ws, ws_bytes, _held = workspace(weights, m, x.device, ptr)
         check(lib().zq_matmul(weights.handle, x.data_ptr(), m, None if bias is None else bias.data_ptr(),
                               out.data_ptr(), ws, ws_bytes, ptr))
@@ -322,6 +332,8 @@ def quantize_rows(x, stream=None):
     torch = _torch()
     if x.get_device() < 0:
         raise _lib.ZQInvalidArgument("zyron_b200: input must be on a CUDA device")
+    if x.dtype != torch.float32 or x.dim() != 2:
+        raise _lib.ZQInvalidArgument("zyron_b200: input must be float32 [M, K]")
     context, ptr = _context(x.get_device(), stream)
     with context:
         x = x.contiguous()
@@ -395,11 +407,17 @@ class QuantizedLinear:
         bias = self._b
         if isinstance(input, np.ndarray) and bias is not None:
             bias = bias.cpu().numpy()
-        y = matmul(input, self._w, bias=bias, out=out, stream=stream)
+        call = None
         if adapters is not None:
-            from .ops import add_low_rank
+            from .ops import _add_low_rank, _bad, _low_rank_call
 
-            add_low_rank(y, input, *adapters[:2], adapter_ids, *adapters[2:], stream=stream)
+            # before the projection writes `out`
+            call = _low_rank_call(input, *adapters[:2], adapter_ids, *adapters[2:], stream)
+            if call[8][-1] != self.out_features():
+                raise _bad("output/adapter dimension mismatch")
+        y = matmul(input, self._w, bias=bias, out=out, stream=stream)
+        if call is not None:
+            _add_low_rank(call, y)
         return y
 
     __call__ = forward
