@@ -215,6 +215,33 @@ def test_norm_refusals_on_device(zb, torch):
         zb.rms_norm_quantize(x, w, eps=-1.0)
 
 
+def test_norm_overlaps(zb, torch):
+    """residual_out may be x, residual, or columns beside them; any other overlap is refused."""
+    x, r, w = (t.cuda() for t in norm_case(torch, 6, 64, "float32", True))
+    want = norm_oracle(torch, x.cpu(), r.cpu(), w.cpu(), 1e-5)
+    wide = torch.zeros(6, 200, device="cuda")
+    for into in (lambda: wide[:, 64:128], lambda: wide[:, 136:]):
+        wide[:, :64], wide[:, 64:128] = x, r
+        got = zb.rms_norm_quantize(wide[:, :64], w, residual=wide[:, 64:128], residual_out=into())
+        same_bits(torch, got.codes, want[0], "codes")
+        same_bits(torch, into(), want[2], "sum")
+        same_bits(torch, wide[:, :64], x, "x")
+    flat = torch.zeros(6 * 64 + 64, device="cuda")
+    shifted = [flat[i : i + 6 * 64].view(6, 64) for i in (0, 1, 64)]
+    square = torch.zeros(64, 64, device="cuda")
+    for xx, rr, out, match in ((wide[:, :64], r, wide[:, 1:65], "overlaps x"), (x, wide[:, 64:128], wide[:, 60:124], "overlaps residual"),
+                               (shifted[0], r, shifted[1], "overlaps x"), (x, shifted[2], shifted[0], "overlaps residual"),
+                               (x, wide[1:, :64].repeat(2, 1)[:6], wide.view(12, 100)[:6, :64], None),
+                               (wide[:, :64], r, wide.view(12, 100)[:6, :64], "overlaps x")):
+        if match is None:
+            zb.rms_norm_quantize(xx, w, residual=rr, residual_out=out)
+            continue
+        with pytest.raises(ValueError, match=match):
+            zb.rms_norm_quantize(xx, w, residual=rr, residual_out=out)
+    with pytest.raises(ValueError, match="overlaps weight"):
+        zb.rms_norm_quantize(x, square[3], residual=r, residual_out=square[:6])
+
+
 # ---- matmul_codes -----------------------------------------------------------------
 
 @pytest.mark.parametrize("qtype", [1, 2])

@@ -101,6 +101,19 @@ def _out_rows(t, name, shape, dtype):
     return t, (t.stride(0) if t.shape[0] > 1 else k)
 
 
+def _apart(out, ld_out, t, ld, name):
+    """Refuses rows `out` that overlap the rows `t` otherwise than by being them."""
+    at, pitch, at_t, pitch_t = out.data_ptr(), ld_out * out.element_size(), t.data_ptr(), ld * t.element_size()
+    (m, k), width, width_t = out.shape, out.shape[1] * out.element_size(), t.shape[-1] * t.element_size()
+    if m == 0 or at == at_t and pitch == pitch_t:
+        return
+    if at + (m - 1) * pitch + width <= at_t or at_t + (t.shape[0] - 1) * pitch_t + width_t <= at:
+        return
+    # columns of one wider buffer
+    if pitch != pitch_t or not width_t <= (at - at_t) % pitch <= pitch - width:
+        raise _bad(f"residual_out overlaps {name}")
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
@@ -121,7 +134,8 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
 
     ``x`` and ``residual`` share a type (float32, float16 or bfloat16); the
     sum is rounded to it, and the norm reads the rounded sum.  The sum goes to
-    ``residual_out`` (a new tensor when None; may be ``residual`` itself).
+    ``residual_out`` (a new tensor when None; may be ``residual`` or ``x``
+    itself, and overlap neither of them otherwise).
     ``normed=True`` also returns the normed rows, e.g. for adapters.
     ``reciprocal=True`` takes the row scale as max|v| times fp32's 1/127, as
     torch computes absmax / 127.0 on a GPU, instead of the quotient: a last bit
@@ -153,6 +167,10 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
                 lds = k
             else:
                 so, lds = _out_rows(residual_out, "residual_out", shape, x.dtype)
+                _apart(so, lds, xr, ldx, "x")
+                _apart(so, lds, rr, ldr, "residual")
+                if weight is not None:
+                    _apart(so, lds, weight.view(1, k), k, "weight")
         if normed:
             n = _empty(shape, x.dtype, device)
         kp = (k + 127) // 128 * 128
