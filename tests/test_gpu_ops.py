@@ -785,6 +785,31 @@ def test_logprobs_offsets_past_32_bits(zb, torch):
     assert abs(float(got.logprobs[0, 0]) + math.log(vocab)) < tol
 
 
+# ---- devices -----------------------------------------------------------------------
+
+def test_every_operator_on_a_second_device(zb, torch):
+    """After calls on the first device, with sizes that need more shared memory
+    than a kernel may have without asking, the first device staying current."""
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    y, x, a, b, ids, scales, ranks = adapter_case(torch, 300, 264, 136, 3, 256, "float32", "bfloat16")
+    logits = randn(torch, 1, 5, 5000)
+    got = []
+    for device in ("cuda:0", "cuda:1"):
+        up = lambda *ts: [t.to(device) for t in ts]  # noqa: E731
+        yd = zb.add_low_rank(*up(y, x, a, b, ids), scales=scales.to(device), ranks=ranks.to(device))
+        n = zb.rms_norm_quantize(x.to(device), normed=True)
+        w = zb.quantize((randn(torch, 2, 264, 136) * 0.05).to(device))
+        z = zb.matmul_codes(n.codes, n.row_scale, w)
+        lp = zb.token_logprobs(logits.to(device), top_k=5)
+        got.append([yd, n.codes, n.normed, z, zb.matmul(n.normed, w), lp.entropy, lp.top_ids])
+        assert all(t.device == torch.device(device) for t in got[-1])
+    torch.cuda.synchronize(1)
+    assert torch.cuda.current_device() == 0
+    for first, second in zip(*got):
+        same_bits(torch, second, first, "second device")
+
+
 # ---- together ------------------------------------------------------------------------
 
 def make_step(zb, torch, hidden=256, vocab=1000, slots=3, rank=8):

@@ -958,12 +958,16 @@ cudaError_t launch_gemm_pair(const GemmArgs& a, cudaStream_t stream, bool pdl) {
 
 cudaError_t ensure_smem_attr_ptr(const void* kern, size_t bytes) {
     static std::mutex mu;
-    static std::unordered_map<const void*, size_t> done;
+    static std::unordered_map<const void*, size_t> done[64];  // by device, as the attribute is
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= 64) return cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     std::lock_guard<std::mutex> lk(mu);
-    auto it = done.find(kern);
-    if (it != done.end() && it->second >= bytes) return cudaSuccess;
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) done[kern] = bytes;
+    auto it = done[dev].find(kern);
+    if (it != done[dev].end() && it->second >= bytes) return cudaSuccess;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done[dev][kern] = bytes;
     return e;
 }
 

@@ -221,8 +221,8 @@ int gemm_block_n(int M, int N);
 // (device count cached per device, minus `reserved`, at least 2).
 int sm_count(int reserved = 0);
 
-// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) at most once per kernel
-// (keyed by the kernel's address) and size: host-side launch overhead matters
+// cudaFuncSetAttribute(MaxDynamicSharedMemorySize) at most once per device,
+// kernel (its address) and size: host-side launch overhead matters
 // for microsecond kernels.
 cudaError_t ensure_smem_attr_ptr(const void* kern, size_t bytes);
 template <class K>
