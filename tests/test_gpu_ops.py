@@ -769,6 +769,15 @@ def test_logprobs_refusals_on_device(zb, torch):
             zb.token_logprobs(x, **kw)
 
 
+def test_logprobs_refusals_allocate_nothing(zb, torch):
+    x = torch.zeros(4, 10, device="cuda")
+    before = torch.cuda.memory_allocated()
+    for top_k in (1 << 24, 1 << 40):
+        with pytest.raises(ValueError, match="at most 32"):
+            zb.token_logprobs(x, top_k=top_k)
+    assert torch.cuda.memory_allocated() == before
+
+
 def test_logprobs_offsets_past_32_bits(zb, torch):
     """The last rows of a buffer of more than 2^32 bytes and 2^31 elements."""
     m, vocab = 3, (1 << 30) // 3 + 12345

@@ -30,6 +30,7 @@ if typing.TYPE_CHECKING:
 
 torch = None  # the module, from the first call on
 _DTYPES = {}  # torch type -> ZQ_DTYPE_*
+_MAX_TOP = 32  # ZQ_LOGPROBS_MAX_TOP
 
 
 def _setup():
@@ -337,6 +338,8 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=True, stream=None):
             raise _bad("targets must have logits' leading dimensions, and one more at most")
     if top_k < 0:
         raise _bad("top_k must be >= 0")
+    if top_k > min(vocab, _MAX_TOP):  # before outputs of that size are allocated
+        raise _bad(f"top_k must be at most {_MAX_TOP} and at most vocab (got {top_k})")
     context, ptr = _context(index, stream)
     with context:
         rows, ld = _rows(logits, "logits")
