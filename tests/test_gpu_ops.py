@@ -470,6 +470,36 @@ def test_adapters_infinities(zb, torch):
     assert ((got.double() - want).abs() <= tol)[rest].all()
 
 
+@pytest.mark.parametrize("wdtype", WDTYPES)
+@pytest.mark.parametrize("m,rank", [(6, 8), (6, 13), (300, 40)])
+def test_adapters_infinite_weights(zb, torch, m, rank, wdtype):
+    """An infinite or NaN element of B reaches its column, one of A its
+    adapter's rows, and neither any other adapter's."""
+    y, x, a, b, ids, _, _ = adapter_case(torch, m, 64, 40, 3, rank, "float32", wdtype, "mixed", False)
+    ids[:3] = torch.arange(3, dtype=torch.int32)
+    a, b = a.abs() + 0.1, b.abs() + 0.1
+    x = x.abs() + 0.1
+    want, tol = adapter_oracle(torch, y, x, a, b, ids, None, None)
+    for bad in (math.inf, math.nan):
+        a2, b2 = a.clone(), b.clone()
+        b2[0, 7, rank - 1], b2[0, 33, 0] = bad, -bad
+        a2[1, rank - 1, 5] = bad
+        got = zb.add_low_rank(y.cuda(), x.cuda(), a2.cuda(), b2.cuda(), ids.cuda()).cpu()
+        hit = torch.zeros(m, 40, dtype=torch.bool)
+        hit[ids == 0, 7] = hit[ids == 0, 33] = True
+        hit[ids == 1] = True
+        assert not got[hit].isfinite().any()
+        assert ((got.double() - want).abs() <= tol)[~hit].all()
+
+
+def test_matmul_codes_without_rows(zb, torch):
+    w = zb.quantize(torch.ones(100, 30, device="cuda"))
+    h = zb.rms_norm_quantize(torch.ones(2, 0, 100, device="cuda"))
+    assert zb.matmul_codes(h.codes, h.row_scale, w).shape == (2, 0, 30)
+    one = zb.rms_norm_quantize(randn(torch, 1, 100).cuda(), normed=True)  # a vector
+    same_bits(torch, zb.matmul_codes(one.codes, one.row_scale, w), zb.matmul(one.normed[None], w)[0], "a vector")
+
+
 @pytest.mark.parametrize("m", [200, 600])
 def test_adapters_rows_do_not_depend_on_others(zb, torch, m):
     """A row's bits are the same twice, with the rows in another order, and
