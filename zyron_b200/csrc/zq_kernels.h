@@ -25,8 +25,9 @@ namespace zq {
 // before it has ended, and executes no launch_dependents: no kernel runs beside
 // it that could meet its lines.  The GEMV starts early and reads its activations
 // by load_l1: it lets no other start, and whatever runs beside it has brought no
-// such data to L1.  Weights, their scales, and ids, ranks and scales of adapters
-// are never the output of the library's own kernels; they may come from L1.
+// such data to L1.  Weights, biases, scales of weights, and ids, ranks and scales
+// of adapters are never the output of the library's own kernels; they may come
+// from L1.
 template <class... Params, class... Args>
 cudaError_t launch_kernel(bool early, void (*kern)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                           Args... args) {

@@ -152,9 +152,10 @@ __device__ __forceinline__ Pack<int8_t, kN> codes_of(const float (&n)[kN], float
 // The kN elements of a row from p * kN on, as far as k; zeros behind.  kAligned:
 // rows start on 16 bytes and k is a multiple of kN.  Else a lane's elements
 // come one by one, out of lines that its first access brought to L1 (such a kernel
-// neither starts early nor lets others; launch_kernel).  (Aligned
-// loads shifted into place with a neighbour's took longer: 94 us against 79 us
-// at 4000 x 4099 bf16.)
+// neither starts early nor lets others, launch_kernel; 1537 x 4099 fp32: 20.7 us,
+// with an early start and load_l2 22.4 us).  (Aligned loads shifted into place
+// with a neighbour's took longer: 94 us against 79 us at 4000 x 4099 bf16 when
+// they were tried.)
 template <bool kAligned, class T, int kN>
 __device__ __forceinline__ Pack<T, kN> load_pack(const T* row, int p, int k) {
     Pack<T, kN> v;
@@ -369,7 +370,7 @@ cudaError_t launch_type(NormArgs a, cudaStream_t stream) {
     // Elements a thread.  Many rows: 32, since what a thread does once a row
     // (two reductions, the root) then weighs least (8192 x 8192 bf16: 86 us, 16
     // a thread 125 us, 64 a thread, with fewer loads under way, 111 us; rows off
-    // the 16-byte grid, 1537 x 4099 fp32: 20 us, 16 a thread 26 us).  A row an SM
+    // the 16-byte grid, 1537 x 4099 fp32: 21 us, 16 a thread 26 us).  A row an SM
     // or fewer: 8, the shortest chains (one row of 4096 fp32: 2.7 us against
     // 3.4 us with 16).  Off the grid a warp's lanes should all have elements
     // (30000 x 100 bf16: 20 us with 8, 27 us with 16, 41 us with 32).
