@@ -226,13 +226,14 @@ zq_status zq_rms_norm_quantize(const void* x, int dtype, size_t m, size_t k, siz
  * (e.g. zq_matmul's output), x [m][k] of x_dtype with row pitch ldx; a
  * [slots][max_rank][k] and b [slots][n][max_rank] contiguous, both w_dtype
  * (ZQ_DTYPE_F16 or ZQ_DTYPE_BF16); ids int32 [m]; scales fp32 [slots] or NULL
- * (ones); ranks int32 [slots] or NULL (max_rank).  The products are exact in
- * the inputs' types and summed in fp32; A x is kept in fp32.  An infinite or
- * NaN element of x[i], or of its adapter, leaves the elements of y[i] that it
- * reaches infinite or NaN.  The addition to y takes subnormal values of y, of
- * what is added and of the sum as zeros.  A row's result depends on its own
- * inputs and on the call's sizes, not on the other rows' values or their
- * order.  max_rank <= ZQ_LOW_RANK_MAX, slots <= ZQ_LOW_RANK_MAX_SLOTS.
+ * (ones); ranks int32 [slots] or NULL (max_rank).  a and b are read as
+ * constants: no call of this library that the stream has not finished may be
+ * writing them.  The products are exact in the inputs' types and summed in
+ * fp32; A x is kept in fp32.  An infinite or NaN element of x[i], or of its
+ * adapter, leaves the elements of y[i] that it reaches infinite or NaN.  The
+ * addition to y takes subnormal values of y, of what is added and of the sum
+ * as zeros.  A row's result depends on its own inputs and on the call's sizes,
+ * not on the other rows' values or their order.  max_rank <= ZQ_LOW_RANK_MAX, slots <= ZQ_LOW_RANK_MAX_SLOTS.
  * `workspace` (256-byte aligned) must hold zq_add_low_rank_workspace_bytes
  * bytes (on the same device) and must not be shared by calls that may overlap
  * on the GPU. */

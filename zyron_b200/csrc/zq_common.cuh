@@ -332,7 +332,8 @@ __device__ __forceinline__ uint4 ld_stream_u4(const void* p) {
 #define ZQ_LOAD(NAME, OP)                                                          \
     template <class T>                                                             \
     __device__ __forceinline__ T NAME(const T* p) {                                \
-        static_assert(sizeof(T) == 16 || sizeof(T) == 4 || sizeof(T) == 2 || sizeof(T) == 8, "one load"); \
+        static_assert(sizeof(T) == 16 || sizeof(T) == 8 || sizeof(T) == 4 ||       \
+                      sizeof(T) == 2, "one load");                                 \
         T v;                                                                       \
         if constexpr (sizeof(T) == 16) {                                           \
             uint4 r;                                                               \

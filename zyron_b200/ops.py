@@ -253,7 +253,8 @@ def add_low_rank(y, x, a, b, ids, scales=None, ranks=None, stream=None):
 
 
 def _low_rank_call(x, a, b, ids, scales, ranks, stream):
-    """The checked arguments of an adapter call but for y, which may not be there yet."""
+    """The arguments of an adapter call, checked, but for y, which may not be
+    there yet; y's shape comes first."""
     if torch is None:
         _setup()
     xt = _dtype(x, "x")
@@ -277,11 +278,11 @@ def _low_rank_call(x, a, b, ids, scales, ranks, stream):
         raise _bad("scales must be contiguous float32 [slots]")
     if ranks is not None and (ranks.dtype != torch.int32 or ranks.shape != (slots,) or not ranks.is_contiguous()):
         raise _bad("ranks must be contiguous int32 [slots]")
-    return x, xt, a, b, wt, ids, scales, ranks, (*lead, n), index, _context(index, stream)
+    return (*lead, n), x, xt, a, b, wt, ids, scales, ranks, index, _context(index, stream)
 
 
 def _add_low_rank(call, y):
-    x, xt, a, b, wt, ids, scales, ranks, shape, index, (context, ptr) = call
+    shape, x, xt, a, b, wt, ids, scales, ranks, index, (context, ptr) = call
     slots, max_rank, k = a.shape
     n = shape[-1]
     if y.get_device() != index:

@@ -413,7 +413,7 @@ class QuantizedLinear:
 
             # before the projection writes `out`
             call = _low_rank_call(input, *adapters[:2], adapter_ids, *adapters[2:], stream)
-            if call[8][-1] != self.out_features():
+            if call[0][-1] != self.out_features():
                 raise _bad("output/adapter dimension mismatch")
         y = matmul(input, self._w, bias=bias, out=out, stream=stream)
         if call is not None:
