@@ -194,6 +194,28 @@ zq_status zq_dequantize_host(const zq_weight* w, float* out_host, void* stream);
 #define ZQ_DTYPE_F16 2
 #define ZQ_DTYPE_BF16 3
 
+/* zq_matmul or zq_matmul_codes with the rest of a layer in the epilogue of the
+ * same kernels:
+ *   y = round_T( act( fl(fl(acc * row_scale) * col_scale) (+ bias) ) + residual )
+ * in fp32 with one rounding to the stored type T = y_dtype.  Either x (fp32
+ * [m][rows], quantized as zq_matmul does) or q and row_scale (as
+ * zq_matmul_codes takes them) is given, the others are NULL.  bias is fp32
+ * [cols] or NULL.  Activations:
+ *   ZQ_ACT_GELU  v / (1 + exp(-2 sqrt(2/pi) (v + 0.044715 v^3))), the tanh form
+ *   ZQ_ACT_SILU  v / (1 + exp(-v))
+ *   ZQ_ACT_RELU  max(v, 0)
+ * (gelu and silu of -inf are NaN, as the formulas have it).  residual is
+ * [m][ld_residual >= cols] of y_dtype or NULL; y is [m][cols] of y_dtype and
+ * may be the residual itself (same pointer, ld_residual = cols), but overlap
+ * it in no other way.  Same workspace rule as zq_matmul. */
+#define ZQ_ACT_NONE 0
+#define ZQ_ACT_GELU 1
+#define ZQ_ACT_SILU 2
+#define ZQ_ACT_RELU 3
+zq_status zq_matmul_epilogue(const zq_weight* w, const float* x, const int8_t* q, const float* row_scale, size_t m,
+                             const float* bias, int activation, const void* residual, size_t ld_residual, void* y,
+                             int y_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Root-mean-square norm with the residual's addition, ending in the codes
  * that zq_matmul_codes multiplies.  For each of m rows of k elements:
  *   s = x + residual, rounded to `dtype`, stored to residual_out

@@ -96,6 +96,7 @@ SIGNATURES = {
     "zq_quantize_rows": (st, [vp, sz, sz, vp, sz, vp, vp]),
     "zq_weight_padded_k": (sz, [vp]),
     "zq_matmul_codes": (st, [vp, vp, vp, sz, vp, vp, vp, sz, vp]),
+    "zq_matmul_epilogue": (st, [vp, vp, vp, vp, sz, vp, C.c_int, vp, sz, vp, C.c_int, vp, sz, vp]),
     "zq_matmul": (st, [vp, vp, sz, vp, vp, vp, sz, vp]),
     "zq_matmul_noalloc": (st, [vp, vp, sz, vp, vp, vp]),
     "zq_matmul_multi": (st, [vp, vp, sz, vp, vp, C.c_int, sz, sz, vp, sz, vp]),

@@ -588,6 +588,7 @@ zq_status run_codes_out(const zq_weight* w, const int8_t* codes, const float* rs
     if (plain && !test && use_gemv(w, M)) {
         zq::GemvArgs a{w->type, w->panel, N, Kp, w->scales, codes, rs, bias, y, M};
         a.reserved_sms = reserved;
+        a.epi = out.epi;
         ZQ_CUDA(zq::launch_gemv(a, st, pdl));
         return ZQ_OK;
     }
@@ -615,6 +616,7 @@ zq_status run_codes_out(const zq_weight* w, const int8_t* codes, const float* rs
         }
         zq::SkinnyArgs a{w->type, tmap_w, &tmap_x, M, N, Kp, rs, w->scales, bias, y, counters, partials, err};
         a.reserved_sms = reserved;
+        a.epi = out.epi;
         if (test) {
             a.wait_extra = test->wait_extra;
             a.peer_limit_ns = test->limit_ns;
@@ -670,6 +672,7 @@ zq_status matmul_in_workspace_out(const zq_weight* w, const float* x, size_t m, 
         a.x = x;
         a.K = (int)w->K;
         a.reserved_sms = w->opt_reserved_sms.load(std::memory_order_relaxed);
+        a.epi = out.epi;
         ZQ_CUDA(zq::launch_gemv(a, st, true));
         return ZQ_OK;
     }
@@ -850,6 +853,47 @@ zq_status zq_matmul_codes(const zq_weight* w, const int8_t* q, const float* row_
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     uint8_t* scratch = ws + align256(m * (size_t)w->Kp) + align256(m * sizeof(float));
     return run_codes(w, q, row_scale, m, bias, y, scratch, as_stream(stream), false);
+}
+
+zq_status zq_matmul_epilogue(const zq_weight* w, const float* x, const int8_t* q, const float* row_scale, size_t m,
+                             const float* bias, int activation, const void* residual, size_t ld_residual, void* y,
+                             int y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!w) return fail(ZQ_ERR_INVALID_ARGUMENT, "ZYRON quantization: weights are empty");
+    if (activation < ZQ_ACT_NONE || activation > ZQ_ACT_RELU)
+        return fail(ZQ_ERR_INVALID_ARGUMENT, "zyron_b200: unsupported activation");
+    const size_t size = y_dtype == ZQ_DTYPE_F32 ? 4 : y_dtype == ZQ_DTYPE_F16 || y_dtype == ZQ_DTYPE_BF16 ? 2 : 0;
+    if (size == 0) return fail(ZQ_ERR_INVALID_ARGUMENT, "zyron_b200: unsupported element type");
+    if (residual && ld_residual < w->N)
+        return fail(ZQ_ERR_INVALID_ARGUMENT, "zyron_b200: a row pitch is smaller than its row");
+    if (m == 0) return ZQ_OK;
+    if ((x != nullptr) == (q != nullptr) || (q != nullptr) != (row_scale != nullptr))
+        return fail(ZQ_ERR_INVALID_ARGUMENT, "zyron_b200: either x or codes and row scales");
+    if (mul_overflows(m, w->N * size) || (residual && (mul_overflows(ld_residual, size) || mul_overflows(m, ld_residual * size))))
+        return fail(ZQ_ERR_OVERFLOW, "zyron_b200: matrix size overflow");
+    const auto off_grid = [](const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; };
+    if (off_grid(x, 4) || off_grid(row_scale, 4) || off_grid(bias, 4) || off_grid(residual, size) || off_grid(y, size))
+        return fail(ZQ_ERR_INVALID_ARGUMENT, "zyron_b200: a pointer is not aligned to its element type");
+    if (off_grid(q, 16)) return fail(ZQ_ERR_INVALID_ARGUMENT, "zyron_b200: codes must be 16-byte aligned");
+    zq_status s = validate_matmul(w, m, x ? static_cast<const void*>(x) : q, static_cast<float*>(y), workspace,
+                                  workspace_bytes);
+    if (s != ZQ_OK) return s;
+    zq::OutDesc out{};
+    out.base[0] = static_cast<float*>(y);
+    out.count = 1;
+    out.ldy = (long long)w->N;
+    out.epi.on = 1;
+    out.epi.activation = activation;
+    out.epi.dtype = y_dtype;
+    out.epi.residual = residual;
+    out.epi.ld_residual = (long long)ld_residual;
+    // 16 columns start on the 16-byte grid of every array that has them
+    const size_t grain = 16 / size;
+    out.vec = w->N % grain == 0 && !off_grid(y, 16) && !off_grid(bias, 16) &&
+              (!residual || (ld_residual % grain == 0 && !off_grid(residual, 16)));
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (x) return matmul_in_workspace_out(w, x, m, bias, out, ws, as_stream(stream));
+    uint8_t* scratch = ws + align256(m * (size_t)w->Kp) + align256(m * sizeof(float));
+    return run_codes_out(w, q, row_scale, m, bias, out, scratch, as_stream(stream), false);
 }
 
 zq_status zq_matmul_host(const zq_weight* w, const float* x_host, size_t m, const float* bias_host, float* y_host,

@@ -44,6 +44,7 @@
 // mbar_wait_bounded): on timeout the kernel records an error code, drains its
 // own in-flight copies and MMAs, frees TMEM and returns.
 #include "zq_common.cuh"
+#include "zq_epilogue.cuh"
 #include "zq_kernels.h"
 #include "zq_tcgen05.cuh"
 
@@ -295,6 +296,70 @@ __device__ __forceinline__ void store_tile_rows(uint32_t taddr, int row, bool ro
     }
 }
 
+// The plain output through the matmul's epilogue (zq_epilogue.cuh), 16 columns
+// of the thread's row at a time: the residual's words of the next 16 are on
+// their way while these are finished, and 16 instead of 32 keep the INT4
+// kernels' epilogue warps within their 72 registers.
+template <int BN>
+__device__ __forceinline__ void store_tile_rows_epi(uint32_t taddr, int row, bool row_ok, int nbase, int N, float sr,
+                                                    const float* __restrict__ col_scale,
+                                                    const float* __restrict__ bias, void* y, const Epilogue& e,
+                                                    bool vec_ok, int shift) {
+    const size_t yrow = (size_t)(row_ok ? row : 0) * (size_t)N;
+    const size_t rrow = (size_t)(row_ok ? row : 0) * (size_t)e.ld_residual;
+    const bool ahead = row_ok && vec_ok && e.residual;
+    Epi16 next;
+    if (ahead && nbase + 16 <= N) epi_load16(e, rrow + nbase, next);
+#pragma unroll 1
+    for (int c = 0; c < BN / 16; ++c) {
+        uint32_t r[16];
+        tmem_ld_32x32b_x16(taddr + c * 16, r);
+        const int n0 = nbase + c * 16;
+        const Epi16 res = next;
+        if (ahead && c + 1 < BN / 16 && n0 + 32 <= N) epi_load16(e, rrow + n0 + 16, next);
+        tmem_ld_wait();
+        if (!row_ok || n0 >= N) continue;
+        if (vec_ok && n0 + 16 <= N) {
+            const float4* cs4 = reinterpret_cast<const float4*>(col_scale + n0);
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 s = __ldg(cs4 + j);
+                v[4 * j] = zq_epilogue(acc_of(r[4 * j], shift), sr, s.x);
+                v[4 * j + 1] = zq_epilogue(acc_of(r[4 * j + 1], shift), sr, s.y);
+                v[4 * j + 2] = zq_epilogue(acc_of(r[4 * j + 2], shift), sr, s.z);
+                v[4 * j + 3] = zq_epilogue(acc_of(r[4 * j + 3], shift), sr, s.w);
+            }
+            if (bias) {
+                const float4* b4 = reinterpret_cast<const float4*>(bias + n0);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float4 b = __ldg(b4 + j);
+                    v[4 * j] += b.x;
+                    v[4 * j + 1] += b.y;
+                    v[4 * j + 2] += b.z;
+                    v[4 * j + 3] += b.w;
+                }
+            }
+            epi_activate(e.activation, v);
+            if (e.residual) epi_add16(e, res, v);
+            epi_store16(e, y, yrow + n0, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int n = n0 + j;
+                if (n < N) {
+                    float v[1] = {zq_epilogue(acc_of(r[j], shift), sr, __ldg(col_scale + n))};
+                    if (bias) v[0] += __ldg(bias + n);
+                    epi_activate(e.activation, v);
+                    if (e.residual) v[0] += epi_residual(e, rrow + n);
+                    epi_store(e, y, yrow + n, v[0]);
+                }
+            }
+        }
+    }
+}
+
 // Tile order: groups of `group_m` M-tiles; inside a group the M-tile index
 // runs fastest, then the N-tile.  The CTAs running at the same time then
 // share a few A panels (activation rows) and B panels (weight columns) in L2.
@@ -308,17 +373,20 @@ __device__ __forceinline__ void tile_coords(int t, int m_tiles, int n_tiles, int
     nt = r / gm;
 }
 
-// kGather: the output goes to several GPUs' buffers (the all-gather fused
-// into the matmul).  A separate instantiation keeps the single-destination
+// Where the output goes.  kGather: to several GPUs' buffers (the all-gather
+// fused into the matmul).  A separate instantiation keeps the single-destination
 // epilogue lean: the gather path's staging roughly doubles the epilogue
 // warps' registers and costs the plain matmul about 8 % when compiled in.
-template <int BN, int STAGES, bool kGather, bool kW4>
+// kEpilogue: one output through activation, residual and a stored type.
+enum OutKind : int { kPlain = 0, kGatherOut = 1, kEpilogueOut = 2 };
+template <int BN, int STAGES, int kOut, bool kW4>
 __global__ void __launch_bounds__(threads_for<kW4>(), 1)
     gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                    int M, int N, int Kp, const float* __restrict__ row_scale,
                    const float* __restrict__ col_scale, const float* __restrict__ bias,
                    const __grid_constant__ OutDesc out, uint32_t* __restrict__ err, int group_m, int shift) {
     using S = Smem<BN, STAGES, kW4>;
+    constexpr bool kGather = kOut == kGatherOut;
     constexpr uint32_t kTmemCols = 2 * BN;  // power of two >= 32 for BN in {64,128,256}
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = smem_align1024(smem_raw);
@@ -511,7 +579,10 @@ __global__ void __launch_bounds__(threads_for<kW4>(), 1)
             const int row = row0 + lane;
             const float sr = row < M ? load_l2(row_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
-            if constexpr (!kGather) {
+            if constexpr (kOut == kEpilogueOut) {
+                store_tile_rows_epi<BN>(taddr, row, row < M, nt * BN, N, sr, col_scale, bias, out.base[0], out.epi, vec1,
+                                        shift);
+            } else if constexpr (!kGather) {
                 store_tile_rows<BN>(taddr, row, row < M, nt * BN, N, sr, col_scale, bias, out.base[0], vec1, shift);
             } else {
                 float* stage = epi_stage + quarter * 2 * kEpiBlockFloats;  // this warp's two staging blocks
@@ -554,7 +625,9 @@ template <int BN, int STAGES, bool kW4>
 cudaError_t launch_gemm_t(const GemmArgs& a, cudaStream_t stream, bool pdl) {
     using S = Smem<BN, STAGES, kW4>;
     const bool gather = general_output(a);
-    auto kern = gather ? gemm_i8_kernel<BN, STAGES, true, kW4> : gemm_i8_kernel<BN, STAGES, false, kW4>;
+    auto kern = gather        ? gemm_i8_kernel<BN, STAGES, kGatherOut, kW4>
+                : a.out.epi.on ? gemm_i8_kernel<BN, STAGES, kEpilogueOut, kW4>
+                               : gemm_i8_kernel<BN, STAGES, kPlain, kW4>;
     const int smem = S::kTotal + (gather ? kEpiBytes : 0);
     cudaError_t e = ensure_smem_attr(kern, smem);
     if (e != cudaSuccess) return e;
@@ -668,12 +741,13 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
         : "memory");
 }
 
-template <bool kGather, bool kW4>
-__global__ void __launch_bounds__((pair_threads<kW4, kGather>()), 1)
+template <int kOut, bool kW4>
+__global__ void __launch_bounds__((pair_threads<kW4, kOut == kGatherOut>()), 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                         int M, int N, int Kp, const float* __restrict__ row_scale,
                         const float* __restrict__ col_scale, const float* __restrict__ bias,
                         const __grid_constant__ OutDesc out, uint32_t* __restrict__ err, int group_m, int shift) {
+    constexpr bool kGather = kOut == kGatherOut;
     using S = Smem2<kW4, kGather>;
     constexpr int kPS = S::kSlotsN;
     constexpr int kStages2 = S::kStages;
@@ -883,7 +957,10 @@ __global__ void __launch_bounds__((pair_threads<kW4, kGather>()), 1)
             const int row = row0 + lane;
             const float sr = row < M ? load_l2(row_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
-            if constexpr (!kGather) {
+            if constexpr (kOut == kEpilogueOut) {
+                store_tile_rows_epi<256>(taddr, row, row < M, nt * 256, N, sr, col_scale, bias, out.base[0], out.epi,
+                                         vec1, shift);
+            } else if constexpr (!kGather) {
                 store_tile_rows<256>(taddr, row, row < M, nt * 256, N, sr, col_scale, bias, out.base[0], vec1, shift);
             } else {
                 float* stage = epi_stage + quarter * 2 * kEpiBlockFloats;  // this warp's two staging blocks
@@ -919,7 +996,9 @@ __global__ void __launch_bounds__((pair_threads<kW4, kGather>()), 1)
 template <bool kW4>
 cudaError_t launch_gemm_pair(const GemmArgs& a, cudaStream_t stream, bool pdl) {
     const bool gather = general_output(a);
-    auto kern = gather ? gemm_i8_pair_kernel<true, kW4> : gemm_i8_pair_kernel<false, kW4>;
+    auto kern = gather        ? gemm_i8_pair_kernel<kGatherOut, kW4>
+                : a.out.epi.on ? gemm_i8_pair_kernel<kEpilogueOut, kW4>
+                               : gemm_i8_pair_kernel<kPlain, kW4>;
     const int smem = gather ? Smem2<kW4, true>::kTotal + kEpiBytes : Smem2<kW4, false>::kTotal;
     cudaError_t e = ensure_smem_attr(kern, smem);
     if (e != cudaSuccess) return e;

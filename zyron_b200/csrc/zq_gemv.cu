@@ -17,6 +17,7 @@
 // griddepcontrol before touching the codes.
 #include "zq_common.cuh"
 #include "zq_dot.cuh"
+#include "zq_epilogue.cuh"
 #include "zq_kernels.h"
 
 namespace zq {
@@ -29,11 +30,15 @@ constexpr int kGemvThreads = 256;
 // 16-byte loads per lane per column in flight), warp-shuffle reduction, exact
 // epilogue.
 // kUnroll: 16-byte weight chunks in flight per lane per column.
-template <int kType, int kM, int kCols, int kUnroll, bool kX16>
+// kEpi: the value goes through the matmul's epilogue (zq_epilogue.cuh) on its
+// way out, in an instantiation of its own so that the plain kernel keeps its
+// registers.
+template <int kType, int kM, int kCols, int kUnroll, bool kX16, bool kEpi>
 __device__ __forceinline__ void gemv_group(int g, const uint8_t* __restrict__ panel,
                                            int N, int Kp, size_t col_bytes, int chunks, const int8_t* __restrict__ sq,
                                            const float* __restrict__ col_scale, const float (&srow)[kM],
-                                           const float* __restrict__ bias, float* __restrict__ y, int M, int lane) {
+                                           const float* __restrict__ bias, float* __restrict__ y, int M, int lane,
+                                           const Epilogue& epi) {
     const int col0 = g * kCols;
     int acc[kCols][kM];
 #pragma unroll
@@ -82,8 +87,12 @@ __device__ __forceinline__ void gemv_group(int g, const uint8_t* __restrict__ pa
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
                 if (lane == m && m < M) {
-                    y[(size_t)m * N + col] = bias ? zq_epilogue_bias(acc[c][m], srow[m], sc, b)
-                                                  : zq_epilogue(acc[c][m], srow[m], sc);
+                    const float v = bias ? zq_epilogue_bias(acc[c][m], srow[m], sc, b)
+                                         : zq_epilogue(acc[c][m], srow[m], sc);
+                    if constexpr (kEpi)
+                        epi_finish(epi, y, N, m, col, v);
+                    else
+                        y[(size_t)m * N + col] = v;
                 }
             }
         }
@@ -151,13 +160,14 @@ __device__ __forceinline__ void quantize_row_staged(const float* __restrict__ x,
 // quantizes them itself with the standalone quantizer's arithmetic
 // (quantization.cpp:202-212: fmaxf absmax, absmax / 127 correctly rounded,
 // round half away from zero), so a decode matmul is a single launch.
-template <int kType, int kM, int kCols, int kUnroll, bool kFused, int kThreads, bool kX16>
+template <int kType, int kM, int kCols, int kUnroll, bool kFused, int kThreads, bool kX16, bool kEpi>
 __global__ void __launch_bounds__(kThreads) gemv_kernel(const uint8_t* __restrict__ panel, int N, int Kp,
                                                             const float* __restrict__ col_scale,
                                                             const int8_t* __restrict__ q,
                                                             const float* __restrict__ row_scale,
                                                             const float* __restrict__ bias, float* __restrict__ y,
-                                                            int M, const float* __restrict__ x, int K) {
+                                                            int M, const float* __restrict__ x, int K,
+                                                            const Epilogue epi) {
     extern __shared__ __align__(16) int8_t sq[];  // [kM][Kp]
     const int lane = threadIdx.x & 31;
     const int warp_global = (blockIdx.x * kThreads + threadIdx.x) >> 5;
@@ -276,8 +286,8 @@ __global__ void __launch_bounds__(kThreads) gemv_kernel(const uint8_t* __restric
     __syncthreads();
 
     for (int g = warp_global; g < groups; g += warps_total)
-        gemv_group<kType, kM, kCols, kUnroll, kX16>(g, panel, N, Kp, col_bytes, chunks, sq, col_scale, srow, bias, y, M,
-                                                    lane);
+        gemv_group<kType, kM, kCols, kUnroll, kX16, kEpi>(g, panel, N, Kp, col_bytes, chunks, sq, col_scale, srow, bias,
+                                                          y, M, lane, epi);
 }
 
 // Four chunks per lane: with at most 64 resident warps per SM, eight per
@@ -287,15 +297,15 @@ cudaError_t launch_gemv_t(const GemvArgs& a, cudaStream_t stream, bool pdl);
 
 // INT4 codes are unpacked as 16 x the code (three operations per eight
 // codes instead of nine) whenever the dot then fits in int32.
-template <int kType, int kM, int kCols, int kUnroll, bool kFused, bool kX16>
-cudaError_t launch_gemv_x(const GemvArgs& a, cudaStream_t stream, bool pdl) {
+template <int kType, int kM, int kCols, int kUnroll, bool kFused, bool kX16, bool kEpi>
+cudaError_t launch_gemv_e(const GemvArgs& a, cudaStream_t stream, bool pdl) {
     // The fused variant runs 512-thread blocks, so each SM reads and
     // quantizes the activation rows half as often as with 256 (512 keeps the
     // register budget of the 256-thread variants: no spills, same occupancy).
     constexpr int kThreads = kFused ? 512 : kGemvThreads;
     // codes [kM][Kp]; the fused one-row kernel also stages the fp32 row
     const size_t smem = (size_t)kM * a.Kp + (kFused && kM == 1 && kType == kInt8 ? 4 * (size_t)a.Kp : 0);
-    auto kern = gemv_kernel<kType, kM, kCols, kUnroll, kFused, kThreads, kX16>;
+    auto kern = gemv_kernel<kType, kM, kCols, kUnroll, kFused, kThreads, kX16, kEpi>;
     cudaError_t e = ensure_smem_attr(kern, smem);
     if (e != cudaSuccess) return e;
     const int sms = sm_count(a.reserved_sms);
@@ -338,7 +348,13 @@ cudaError_t launch_gemv_x(const GemvArgs& a, cudaStream_t stream, bool pdl) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kern, a.panel, a.N, a.Kp, a.col_scale, a.q, a.row_scale, a.bias, a.y,
-                              a.M, a.x, a.K);
+                              a.M, a.x, a.K, a.epi);
+}
+
+template <int kType, int kM, int kCols, int kUnroll, bool kFused, bool kX16>
+cudaError_t launch_gemv_x(const GemvArgs& a, cudaStream_t stream, bool pdl) {
+    return a.epi.on ? launch_gemv_e<kType, kM, kCols, kUnroll, kFused, kX16, true>(a, stream, pdl)
+                    : launch_gemv_e<kType, kM, kCols, kUnroll, kFused, kX16, false>(a, stream, pdl);
 }
 
 template <int kType, int kM, int kCols, int kUnroll, bool kFused>

@@ -62,6 +62,17 @@ inline int padded_k(int type, int K) {
     return (K + 127) / 128 * 128;
 }
 
+// What a plain matmul does with a finished value before it is stored
+// (zq_matmul_epilogue; zq_epilogue.cuh has the arithmetic).  Off: the value is
+// stored as it is, in fp32, by kernels that have none of this compiled in.
+struct Epilogue {
+    int on = 0;
+    int activation = 0;              // ZQ_ACT_*
+    int dtype = ZQ_DTYPE_F32;        // ZQ_DTYPE_* of the residual and of the output
+    const void* residual = nullptr;  // [M][ld_residual] or null
+    long long ld_residual = 0;
+};
+
 struct GemvArgs {
     int type;
     const uint8_t* panel;
@@ -76,6 +87,7 @@ struct GemvArgs {
     const float* x = nullptr; // fp32 activations [M][K], quantized inside the kernel (M <= 4)
     int K = 0;
     int reserved_sms = 0;     // SMs left out of the grid
+    Epilogue epi = {};
 };
 
 // Where the GEMM epilogue writes: element (row, col) of the matmul goes to
@@ -94,6 +106,9 @@ struct OutDesc {
     // blocks with TMA through them.
     int tma;
     CUtensorMap map[kMaxOutputs];
+    // One plain output only: base[0] then points to elements of epi.dtype, and
+    // vec allows 16-byte accesses of the residual too.
+    Epilogue epi;
 };
 
 struct GemmArgs {
@@ -149,6 +164,7 @@ struct SkinnyArgs {
     int wait_extra = 0;
     uint64_t peer_limit_ns = 0;
     int reserved_sms = 0;  // SMs left out of the grid
+    Epilogue epi = {};
 };
 // Weight columns per decode tile and the tiles of N columns.
 int skinny_block_n();

@@ -61,6 +61,7 @@
 // Warps: 0 TMA producer; 1 TMEM allocator + MMA issuer; 2-5 epilogue;
 // 6.. (INT4 only) unpack, two per stage.  Every mbarrier wait is bounded.
 #include "zq_common.cuh"
+#include "zq_epilogue.cuh"
 #include "zq_kernels.h"
 #include "zq_tcgen05.cuh"
 
@@ -243,13 +244,14 @@ __device__ __forceinline__ bool wait_count_bounded(const int* p, int target, uin
     }
 }
 
-template <int kType>
+// kEpi: finished values go through the matmul's epilogue (zq_epilogue.cuh).
+template <int kType, bool kEpi>
 __global__ void __launch_bounds__(SkCfg<kType>::kThreads, 1)
     skinny_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x, int M,
                   int N, int KG, long long T, const float* __restrict__ row_scale,
                   const float* __restrict__ col_scale, const float* __restrict__ bias, float* __restrict__ y,
                   int* __restrict__ counters, int* __restrict__ partials, uint32_t* __restrict__ err,
-                  int wait_extra, unsigned long long peer_limit_ns, int x16) {
+                  int wait_extra, unsigned long long peer_limit_ns, int x16, const Epilogue epi) {
     using C = SkCfg<kType>;
     constexpr int S = C::kStages;
     constexpr uint32_t kTmemCols = 2 * kSkChains * kSkRows;  // two buffers of four 16-column accumulators
@@ -516,7 +518,25 @@ __global__ void __launch_bounds__(SkCfg<kType>::kThreads, 1)
             const int n = (int)(b * kSkBlockN) + col_local;
             if (owner_lane && n < N) {
                 const float sc = __ldg(col_scale + n);
-                if (bias) {
+                if constexpr (kEpi) {
+                    float v[kSkRows];
+                    const float bv = bias ? __ldcg(bias + n) : 0.0f;
+#pragma unroll
+                    for (int m = 0; m < kSkRows; ++m)
+                        v[m] = bias ? zq_epilogue_bias((int32_t)r[m], sr[m], sc, bv) : zq_epilogue((int32_t)r[m], sr[m], sc);
+                    epi_activate(epi.activation, v);
+                    if (epi.residual) {
+                        float res[kSkRows];  // every row's load before the first sum
+#pragma unroll
+                        for (int m = 0; m < kSkRows; ++m)
+                            res[m] = m < M ? epi_residual(epi, (size_t)m * (size_t)epi.ld_residual + n) : 0.0f;
+#pragma unroll
+                        for (int m = 0; m < kSkRows; ++m) v[m] += res[m];
+                    }
+#pragma unroll
+                    for (int m = 0; m < kSkRows; ++m)
+                        if (m < M) epi_store(epi, y, (size_t)m * N + n, v[m]);
+                } else if (bias) {
                     const float bv = __ldcg(bias + n);
 #pragma unroll
                     for (int m = 0; m < kSkRows; ++m)
@@ -588,9 +608,9 @@ __global__ void zero_words_kernel(int* __restrict__ p, int n) {
     for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) p[i] = 0;
 }
 
-template <int kType>
+template <int kType, bool kEpi>
 cudaError_t launch_skinny_t(const SkinnyArgs& a, cudaStream_t stream, bool pdl) {
-    auto kern = skinny_kernel<kType>;
+    auto kern = skinny_kernel<kType, kEpi>;
     constexpr int smem = sk_smem_bytes<kType>();
     cudaError_t e = ensure_smem_attr(kern, smem);
     if (e != cudaSuccess) return e;
@@ -613,7 +633,7 @@ cudaError_t launch_skinny_t(const SkinnyArgs& a, cudaStream_t stream, bool pdl) 
     return cudaLaunchKernelEx(&cfg, kern, *a.tmap_w, *a.tmap_x, a.M, a.N, KG, T, a.row_scale, a.col_scale, a.bias,
                               a.y, a.counters, a.partials, a.err, a.wait_extra,
                               (unsigned long long)(a.peer_limit_ns ? a.peer_limit_ns : 4000000000ull),
-                              (kType == kInt4 && int4_x16_fits(a.Kp)) ? 1 : 0);
+                              (kType == kInt4 && int4_x16_fits(a.Kp)) ? 1 : 0, a.epi);
 }
 
 }  // namespace
@@ -642,7 +662,11 @@ cudaError_t launch_zero_words(int* p, int n, cudaStream_t stream) {
 
 cudaError_t launch_skinny(const SkinnyArgs& a, cudaStream_t stream, bool pdl) {
     if (a.M < 1 || a.M > kSkinnyMaxRows) return cudaErrorInvalidValue;
-    return a.type == kInt8 ? launch_skinny_t<kInt8>(a, stream, pdl) : launch_skinny_t<kInt4>(a, stream, pdl);
+    if (a.epi.on)
+        return a.type == kInt8 ? launch_skinny_t<kInt8, true>(a, stream, pdl)
+                               : launch_skinny_t<kInt4, true>(a, stream, pdl);
+    return a.type == kInt8 ? launch_skinny_t<kInt8, false>(a, stream, pdl)
+                           : launch_skinny_t<kInt4, false>(a, stream, pdl);
 }
 
 }  // namespace zq

@@ -102,7 +102,7 @@ def _out_rows(t, name, shape, dtype):
     return t, (t.stride(0) if t.shape[0] > 1 else k)
 
 
-def _apart(out, ld_out, t, ld, name):
+def _apart(out, ld_out, t, ld, name, what="residual_out"):
     """Refuses rows `out` that overlap the rows `t` otherwise than by being them."""
     at, pitch, at_t, pitch_t = out.data_ptr(), ld_out * out.element_size(), t.data_ptr(), ld * t.element_size()
     (m, k), width, width_t = out.shape, out.shape[1] * out.element_size(), t.shape[-1] * t.element_size()
@@ -112,7 +112,7 @@ def _apart(out, ld_out, t, ld, name):
         return
     # columns of one wider buffer
     if pitch != pitch_t or not width_t <= (at - at_t) % pitch <= pitch - width:
-        raise _bad(f"residual_out overlaps {name}")
+        raise _bad(f"{what} overlaps {name}")
 
 
 def _ptr(t):
@@ -186,11 +186,58 @@ def rms_norm_quantize(x, weight=None, residual=None, eps=1e-5, residual_out=None
     return NormQuantized(codes, scale, residual_out, n)
 
 
-def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None, stream=None):
+_ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2, "relu": 3}  # ZQ_ACT_*
+
+
+def _epilogue(shape, index, activation, residual, dtype, out):
+    """The checked epilogue of a matmul with an output of `shape` on device
+    `index`, as the function that makes the call (with that device and the
+    call's stream current)."""
+    if torch is None:
+        _setup()
+    if activation not in _ACTIVATIONS:
+        raise _bad("activation must be None, 'gelu', 'silu' or 'relu'")
+    if dtype is None:
+        dtype = torch.float32 if residual is None else residual.dtype
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise _bad("dtype must be float32, float16 or bfloat16")
+    shape = torch.Size(shape)
+    if residual is not None:
+        if residual.get_device() != index:
+            raise _bad(f"residual is on {residual.device}, not on cuda:{index}")
+        if residual.shape != shape or residual.dtype != dtype:
+            raise _bad(f"residual must have shape {tuple(shape)} and type {dtype}")
+    n = shape[-1]
+    if out is not None:
+        if out.get_device() != index:
+            raise _bad(f"out is on {out.device}, not on cuda:{index}")
+        if out.shape != shape or out.dtype != dtype or not out.is_contiguous():
+            raise _bad(f"out must be contiguous, of shape {tuple(shape)} and type {dtype}")
+
+    def call(weights, x, codes, scale, bias, ws, ws_bytes, stream):
+        y, res, ld = out, None, 0
+        if residual is not None:
+            res, ld = _rows(residual, "residual")
+            if out is not None:
+                _apart(out.view(-1, n), n, res, ld, "residual", "out")
+        if y is None:
+            y = _empty(shape, dtype, f"cuda:{index}")
+        m = y.numel() // n
+        check(lib().zq_matmul_epilogue(weights.handle, _ptr(x), _ptr(codes), _ptr(scale), m, _ptr(bias),
+                                       _ACTIVATIONS[activation], _ptr(res), ld, y.data_ptr(), code, ws, ws_bytes, stream))
+        return y
+
+    return call
+
+
+def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None, stream=None, activation=None,
+                 residual=None, dtype=None):
     """``matmul`` on activations that are quantized already: ``codes`` int8
     [..., K] and ``row_scale`` fp32 [...], as ``rms_norm_quantize`` or
     ``quantize_rows`` leave them.  Codes whose rows are not 128-aligned, as
-    those of ``rms_norm_quantize`` are, are copied first."""
+    those of ``rms_norm_quantize`` are, are copied first.  ``activation``,
+    ``residual`` and ``dtype`` are those of ``matmul``."""
     if torch is None:
         _setup()
     if weights is None or weights.empty():
@@ -207,7 +254,10 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
     n = weights.cols()
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
         raise _bad("bias must be contiguous float32 of the output's last dimension")
-    if out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (*lead, n) or not out.is_contiguous()):
+    epilogue = None
+    if activation is not None or residual is not None or dtype is not None:
+        epilogue = _epilogue((*lead, n), index, activation, residual, dtype, out)
+    elif out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (*lead, n) or not out.is_contiguous()):
         raise _bad("out must be contiguous float32 [..., N]")
     context, ptr = _context(index, stream)
     with context:
@@ -220,11 +270,13 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
             padded[:, :k] = q
             q = padded
         scale = row_scale.contiguous()
-        if out is None:
+        if out is None and epilogue is None:
             out = _empty((*lead, n), torch.float32, q.device)
         need = lib().zq_matmul_workspace_bytes(weights.handle, m)
         ws = _empty((need + 256,), torch.uint8, q.device)
         base = (ws.data_ptr() + 255) & ~255
+        if epilogue is not None:
+            return epilogue(weights, None, q, scale, bias, base, need, ptr)
         check(lib().zq_matmul_codes(weights.handle, q.data_ptr(), scale.data_ptr(), m, _ptr(bias), out.data_ptr(),
                                     base, need, ptr))
     return out

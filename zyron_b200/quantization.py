@@ -276,11 +276,19 @@ def workspace(weights, m, device, stream_key):
     return aligned, buf.numel() - (aligned - base), buf
 
 
-def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
+def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None, activation=None, residual=None,
+           dtype=None):
     """quantization::matmul (quantization.cpp:177-238); with ``bias`` it is
     QuantizedLinear::forward (quantized_linear.cpp:33-50).
 
     torch CUDA input -> torch CUDA output; numpy input -> numpy output.
+
+    The rest of a layer runs in the same kernel (``zq_matmul_epilogue``; torch
+    CUDA input only): ``activation`` ("gelu" in its tanh form, "silu" or
+    "relu") of the product with its bias, then ``residual`` (the output's shape
+    and type) added, all in fp32, then one rounding to ``dtype`` (float32,
+    float16 or bfloat16; by default the residual's type, or float32).  ``out``
+    may be the residual itself, and overlap it in no other way.
     """
     ndim = input.ndim if isinstance(input, np.ndarray) else input.dim()
     if ndim < 2:
@@ -291,7 +299,10 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
         raise _lib.ZQInvalidArgument("ZYRON quantization: input/weight dimension mismatch")
     out_shape = tuple(input.shape[:-1]) + (weights.cols(),)
 
+    fused = activation is not None or residual is not None or dtype is not None
     if isinstance(input, np.ndarray):
+        if fused:
+            raise _lib.ZQInvalidArgument("zyron_b200: activation, residual and dtype need a CUDA tensor as input")
         x = np.ascontiguousarray(input, dtype=np.float32).reshape(-1, weights.rows())
         y = np.empty((x.shape[0], weights.cols()), dtype=np.float32)
         b = None if bias is None else np.ascontiguousarray(bias, dtype=np.float32)
@@ -312,6 +323,15 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None):
     if bias is not None and (bias.get_device() != index or bias.dtype != torch.float32 or bias.numel() != n
                              or not bias.is_contiguous()):
         raise _lib.ZQInvalidArgument("zyron_b200: bias must be contiguous float32 [N] on input's device")
+    if fused:
+        from .ops import _epilogue
+
+        epilogue = _epilogue(out_shape, index, activation, residual, dtype, out)
+        context, ptr = _context(index, stream)
+        with context:
+            x = input.contiguous()
+            ws, ws_bytes, _held = workspace(weights, x.numel() // weights.rows(), x.device, ptr)
+            return epilogue(weights, x, None, None, bias, ws, ws_bytes, ptr)
     if out is not None and (out.get_device() != index or out.dtype != torch.float32 or not out.is_contiguous()
                             or out.numel() * weights.rows() != input.numel() * n):
         raise _lib.ZQInvalidArgument("zyron_b200: out must be contiguous float32 [..., N] on input's device")
@@ -391,12 +411,19 @@ class QuantizedLinear:
     def bias(self):
         return self._b
 
-    def forward(self, input, out=None, stream=None, adapters=None, adapter_ids=None):
+    def forward(self, input, out=None, stream=None, adapters=None, adapter_ids=None, activation=None, residual=None,
+                dtype=None):
         """``adapters`` (ops.LowRankAdapters of this projection) with
         ``adapter_ids`` (int32, input's leading dimensions) adds each row's
-        low-rank adapter onto the output; torch CUDA input only."""
+        low-rank adapter onto the output; torch CUDA input only.
+        ``activation``, ``residual`` and ``dtype`` are ``matmul``'s; adapters
+        are added to the projection itself, so they go with none of them but
+        a float32 residual."""
         if (adapters is None) != (adapter_ids is None):
             raise _lib.ZQInvalidArgument("zyron_b200: adapters and adapter_ids go together")
+        if adapters is not None and (activation is not None or dtype not in (None, _torch().float32)
+                                     or residual is not None and residual.dtype != _torch().float32):
+            raise _lib.ZQInvalidArgument("zyron_b200: adapters are added to a float32 output without an activation")
         if adapters is not None and isinstance(input, np.ndarray):
             raise _lib.ZQInvalidArgument("zyron_b200: adapters need a CUDA tensor as input")
         ndim = input.ndim if isinstance(input, np.ndarray) else input.dim()
@@ -415,7 +442,8 @@ class QuantizedLinear:
             call = _low_rank_call(input, *adapters[:2], adapter_ids, *adapters[2:], stream)
             if call[0][-1] != self.out_features():
                 raise _bad("output/adapter dimension mismatch")
-        y = matmul(input, self._w, bias=bias, out=out, stream=stream)
+        y = matmul(input, self._w, bias=bias, out=out, stream=stream, activation=activation, residual=residual,
+                   dtype=dtype)
         if call is not None:
             _add_low_rank(call, y)
         return y
