@@ -286,6 +286,79 @@ zq_status zq_token_logprobs(const void* logits, int dtype, size_t m, size_t voca
                             size_t n_targets, size_t top_k, float* logprobs, float* entropy, float* top_logprobs,
                             int64_t* top_ids, void* stream);
 
+/* A batch of requests over a paged key/value cache, as zq_append_kv and
+ * zq_paged_attention take it.  The rows of a call are the new tokens of all
+ * requests, one request after the other: request b owns the rows
+ * [starts[b], starts[b + 1]) of `rows` (starts is int32 [requests + 1], not
+ * decreasing; NULL: one row each, rows = requests).  Rows that no request owns
+ * are neither read for a result nor written.  lengths (int32 [requests]) counts
+ * each request's own cached tokens, its new ones included, but not a shared
+ * prefix; the i-th of its n new tokens stands at position lengths[b] - n + i.
+ * pages (int32 [requests][ld_pages], max_pages of each row used) names the
+ * cache page of each `page` tokens.  The caches are [cache_pages][kv_heads]
+ * [page][dim] of ZQ_DTYPE_F16 or ZQ_DTYPE_BF16, a page's block contiguous,
+ * pages ld_k_page and ld_v_page elements apart; the two may interleave, but not
+ * overlap.  dim <= ZQ_PAGED_MAX_DIM and page are multiples of 8.
+ *
+ * starts, lengths and pages are read on the device when the call runs, so a
+ * captured call follows what they hold at its replay.  Values that the call's
+ * sizes do not allow are clamped or left out, never followed: starts and
+ * lengths to [0, rows] and [0, max_pages * page]; a token on a page outside
+ * [0, cache_pages) is not stored, and not seen. */
+typedef struct zq_paged_batch {
+    const int32_t* starts;
+    const int32_t* lengths;
+    const int32_t* pages;
+    size_t ld_pages, max_pages;
+    size_t requests, rows;
+    size_t page, cache_pages, kv_heads, dim;
+    size_t ld_k_page, ld_v_page;
+    int cache_dtype;
+} zq_paged_batch;
+#define ZQ_PAGED_MAX_DIM 128
+
+/* New tokens' keys and values into the cache, their queries and keys rotated by
+ * position: with angle = (position + offset) * inv_freq[p], p < rotated / 2,
+ *   (a, b) -> (a cos - b sin, a sin + b cos)
+ * over the elements (2p, 2p + 1) of a head where `interleaved` (as the
+ * reference's apply_rope, src/model/quantized_language_model.cpp:347-384), else
+ * (p, p + rotated / 2); elements from `rotated` on pass as they are.  Angles are
+ * formed in 64 bits, the rest in fp32, rounded once to the cache's type.
+ * q [rows][heads][dim] and k, v [rows][kv_heads][dim] are of `dtype`, each
+ * row's heads contiguous, ldq, ldk and ldv elements from row to row (the three
+ * may lie in one buffer); q_out [rows][heads][dim] is of the cache's type,
+ * contiguous.  q and q_out may both be NULL.  inv_freq is fp64 [rotated / 2] or
+ * NULL (rotated 0); `offset` is what stands before a request's own tokens, e.g.
+ * a shared prefix.  A request's tokens before its position 0 (more rows than
+ * its length) are not stored.  Where two tokens of a call name the same place
+ * of the cache, either may end up there.  Outputs must not overlap inputs. */
+zq_status zq_append_kv(const zq_paged_batch* batch, const void* q, size_t ldq, const void* k, size_t ldk,
+                       const void* v, size_t ldv, int dtype, size_t heads, void* k_cache, void* v_cache, void* q_out,
+                       const double* inv_freq, size_t rotated, int interleaved, int64_t offset, void* stream);
+
+/* Attention of the new tokens over the cache:
+ *   out = sum_j exp(s_j - max s) v_j / sum_j exp(s_j - max s),  s_j = scale * q . k_j
+ * over the tokens of the shared prefix -- prefix_length tokens on prefix_pages
+ * (int32 [ceil(prefix_length / page)]), computed once for all rows -- and the
+ * request's own: all of them, or with `causal` those up to the row's own
+ * position.  heads is a multiple of kv_heads; query heads
+ * [h * heads / kv_heads, ...) read kv head h; at most ZQ_ATTENTION_MAX_GROUP of
+ * them.  q and out are [rows][heads][dim] of the cache's type, ldq and ld_out
+ * elements from row to row, q 16-byte aligned with ldq a multiple of 8, out
+ * 8-byte aligned with ld_out a multiple of 4; out must not overlap q.  Scores,
+ * weights, sums and outputs are fp32, rounded once to out.
+ * A row that sees no token is zero.  What a row does not see does not reach it,
+ * infinities and NaN included; tokens behind a request's length are not read.
+ * `workspace` (256-byte aligned) must hold zq_paged_attention_workspace_bytes
+ * bytes and must not be shared by calls that may overlap on the GPU; 0 bytes
+ * means that the sizes are refused. */
+#define ZQ_ATTENTION_MAX_GROUP 128
+size_t zq_paged_attention_workspace_bytes(const zq_paged_batch* batch, size_t heads, size_t prefix_length);
+zq_status zq_paged_attention(const zq_paged_batch* batch, const void* q, size_t ldq, size_t heads,
+                             const void* k_cache, const void* v_cache, const int32_t* prefix_pages,
+                             size_t prefix_length, int causal, float scale, void* out, size_t ld_out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- column-sharded matmul over NCCL ------------------------------------ */
 
 /* Columns [*begin, *end) of rank `rank` when n_cols columns are split over

@@ -116,6 +116,9 @@ SIGNATURES = {
     "zq_add_low_rank_workspace_bytes": (sz, [sz, sz, sz, sz, sz]),
     "zq_add_low_rank": (st, [vp, sz, vp, C.c_int, sz, sz, sz, sz, vp, vp, C.c_int, sz, sz, vp, vp, vp, vp, sz, vp]),
     "zq_token_logprobs": (st, [vp, C.c_int, sz, sz, sz, vp, sz, sz, vp, vp, vp, vp, vp]),
+    "zq_append_kv": (st, [vp, vp, sz, vp, sz, vp, sz, C.c_int, sz, vp, vp, vp, vp, sz, C.c_int, C.c_int64, vp]),
+    "zq_paged_attention_workspace_bytes": (sz, [vp, sz, sz]),
+    "zq_paged_attention": (st, [vp, vp, sz, sz, vp, vp, vp, sz, C.c_int, C.c_float, vp, sz, vp, sz, vp]),
     "zq_ipc_export": (st, [vp, vp]),
     "zq_ipc_import": (st, [vp, C.POINTER(vp)]),
     "zq_ipc_close": (st, [vp]),
@@ -131,6 +134,14 @@ SIGNATURES = {
     "zq_sampler_destroy": (st, [vp]),
     "zq_sample_next": (st, [vp, vp, sz, vp, sz, vp, C.POINTER(C.c_int64)]),
 }
+
+
+class PagedBatchC(C.Structure):
+    """zq_paged_batch (include/zq.h)."""
+
+    _fields_ = [("starts", vp), ("lengths", vp), ("pages", vp), ("ld_pages", sz), ("max_pages", sz), ("requests", sz),
+                ("rows", sz), ("page", sz), ("cache_pages", sz), ("kv_heads", sz), ("dim", sz), ("ld_k_page", sz),
+                ("ld_v_page", sz), ("cache_dtype", C.c_int)]
 
 
 class GenerationConfigC(C.Structure):

@@ -1,0 +1,608 @@
+// zq_attention.cu -- attention of new tokens over a paged cache, a prefix that
+// all requests share computed once for all of them (zq_paged_attention).
+//
+//   s_j = scale * q . k_j,   o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m)
+//
+// over the prefix's keys and the request's own, of which a causal row at
+// position t sees those up to t.  One pass over the keys with a running maximum
+// m, sum and output in fp32, in base 2.
+//
+// Split.  A request's rows of one kv head -- its new tokens times the heads of
+// the group, which all read the same keys -- make an item (in tiles of kRows
+// rows); the shared prefix is one more request whose rows are all the call's
+// rows.  Items are cut into units of 64 keys, and every block takes an equal run
+// of units, whatever the lengths are: it finds its run by a scan over the
+// requests' lengths, so the plan lives on the device and a captured call follows
+// the lengths of its replay.  A block's run covers whole items and at most two
+// parts of items, whose sums it leaves in a slot of its own; a second kernel
+// joins the parts of each item that a border cuts.  With a prefix, own and
+// prefix results stay in fp32 with their maxima and sums, and a third joins the
+// two.
+//
+// Bound: a decode batch reads its cache once, memory bandwidth.  A warp streams
+// its own 16 keys of a unit through a ring of cp.async stages, so that no
+// barrier stands between the memory and the products; q stays in registers; the
+// products are mma.sync, which at 16 rows take 4 of the 22 cycles a key's bytes
+// take an SM.  exp(s - m) enters the second product as a sum of two 16-bit
+// parts, so that it is not rounded to the cache's type.
+#include "zq_attention.cuh"
+
+namespace zq {
+
+namespace {
+
+using namespace attn;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kSlice = 16;              // keys of a warp's stage
+constexpr int kUnit = kSlice * kWarps;  // keys of a unit
+constexpr int kStages = 3;
+constexpr int kBlocksPerSm = 2;
+
+template <int kD>
+constexpr int kStageBytes = kSlice * kD * 2 * 2;  // keys, then values
+// The ring of every warp, reused for the warps' sums; q.
+template <int kD, int kMT>
+constexpr int kSmemBytes = kWarps * kStages * kStageBytes<kD> + 16 * kMT * kD * 2;
+
+// Where warp w leaves its sums: the start of its ring.
+template <int kD>
+__device__ __forceinline__ float* warp_sums(uint8_t* smem, int w) {
+    return reinterpret_cast<float*>(smem + w * kStages * kStageBytes<kD>);
+}
+
+// 16-byte chunk `c` of row `r` of a row-major tile of kD 16-bit elements, chunks
+// XOR-swizzled by row so that eight rows of a column of chunks lie in different banks.
+template <int kD>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return (uint32_t)(r * kD * 2 + ((c ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {
+    const int n = live ? 16 : 0;  // 0: the chunk is filled with zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <class T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (sizeof(T) == 2 && kIsHalf<T>)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// ---- the plan ------------------------------------------------------------------
+
+// Units of one request: tiles of rows x kv heads x units of keys.  At least one
+// unit of keys, so that rows that see none are written too.
+template <int kRows>
+struct Plan {
+    const AttentionArgs& a;
+    int group;        // heads of a kv head
+    int prefix_rows;  // rows of the call that have the prefix, 0: not in this plan
+
+    __device__ __forceinline__ int tiles(int rows) const { return (int)(((long long)rows * group + kRows - 1) / kRows); }
+    __device__ __forceinline__ int units(int keys) const { return keys > 0 ? (keys - 1) / kUnit + 1 : 1; }
+    __device__ __forceinline__ long long cost(const Request& r) const {
+        return (long long)tiles(r.rows) * a.batch.kv_heads * units(r.length);
+    }
+    __device__ __forceinline__ Request get(int b) const {
+        if (b >= 0) return load_request(a.batch, b);
+        return Request{0, prefix_rows, a.prefix_length};  // the prefix: request -1
+    }
+};
+
+struct Found {
+    long long total;  // units of the call
+    long long before; // units before request b
+    int b;
+};
+
+// The request that holds unit (total * num / den), by a scan of the whole block.
+// Every thread gets the result; `scratch` is kThreads / 32 + 4 words of 64 bits.
+template <int kRows>
+__device__ Found find_unit(const Plan<kRows>& plan, long long num, long long den, long long* scratch) {
+    const int n = plan.a.batch.requests;
+    const int each = (n + kThreads - 1) / kThreads;
+    const int first = threadIdx.x * each, last = min(first + each, n);
+    long long mine = 0;
+    for (int b = first; b < last; ++b) mine += plan.cost(plan.get(b));
+    const long long head = plan.prefix_rows ? plan.cost(plan.get(-1)) : 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    long long total = head, before = head + sum - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += scratch[w];
+        total += scratch[w];
+    }
+    const long long unit = total * num / den;
+    if (threadIdx.x == 0) {
+        scratch[kWarps] = 0;
+        scratch[kWarps + 1] = unit < head ? -1 : n;
+    }
+    __syncthreads();
+    if (unit >= before && unit < before + mine) {
+        int b = first;
+        long long c = plan.cost(plan.get(b));
+        while (unit >= before + c) {
+            before += c;
+            c = plan.cost(plan.get(++b));
+        }
+        scratch[kWarps] = before;
+        scratch[kWarps + 1] = b;
+    }
+    __syncthreads();
+    const Found f{total, scratch[kWarps], (int)scratch[kWarps + 1]};
+    __syncthreads();
+    return f;
+}
+
+// ---- the kernel -----------------------------------------------------------------
+
+// kMT: 16-row tiles of an item's kRows = 16 kMT rows.
+template <class T, int kD, int kMT>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const AttentionArgs a, const Workspace ws) {
+    constexpr int kRows = 16 * kMT;
+    constexpr int kChunks = kD / 8;  // 16-byte chunks of a row
+    static_assert(kStages * kStageBytes<kD> >= kRows * (kD + 2) * 4, "a warp's sums fit in its ring");
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ long long scratch[kWarps + 4];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* ring = smem + warp * kStages * kStageBytes<kD>;
+    const uint32_t ring_u = smem_u32(ring);
+    uint8_t* q_tile = smem + kWarps * kStages * kStageBytes<kD>;
+    const uint32_t q_u = smem_u32(q_tile);
+    const PagedBatch& p = a.batch;
+    const int group = a.heads / p.kv_heads, dim = p.dim;
+
+    pdl_wait_primary();
+    pdl_launch_dependents();
+    Plan<kRows> plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
+    const Found at = find_unit(plan, blockIdx.x, gridDim.x, scratch);
+    const long long u0 = at.total * blockIdx.x / gridDim.x, u1 = at.total * (blockIdx.x + 1) / gridDim.x;
+    if (u0 >= u1) return;
+    int b = at.b;
+    long long before = at.before;
+    Request r = plan.get(b);
+
+    for (long long u = u0; u < u1;) {
+        // The item of unit u, and the units of it that are this block's.
+        long long cost = plan.cost(r);
+        while (u >= before + cost) {
+            before += cost;
+            r = plan.get(++b);
+            cost = plan.cost(r);
+        }
+        const int units = plan.units(r.length), tiles = plan.tiles(r.rows);
+        const long long item = (u - before) / units;
+        const int c0 = (int)((u - before) - item * units);
+        const int c1 = (int)min((long long)units, c0 + (u1 - u));
+        const int head0 = (int)(item / tiles), tile = (int)(item % tiles);
+        const bool prefix = b < 0;
+        const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)b * p.ld_pages;
+        const int row0 = tile * kRows, item_rows = min(kRows, r.rows * group - row0);
+
+        // q of the item: row i is token i / group, head i % group of the kv head's.
+        for (int i = threadIdx.x; i < kRows * kChunks; i += kThreads) {
+            const int row = i / kChunks, c = i % kChunks;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (row < item_rows && c * 8 < dim) {
+                const int token = (row0 + row) / group, head = (row0 + row) % group;
+                v = load_l2(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
+                                                           (long long)(r.first + token) * a.ldq +
+                                                           (long long)(head0 * group + head) * dim + c * 8));
+            }
+            *reinterpret_cast<uint4*>(q_tile + chunk_at<kD>(row, c)) = v;
+        }
+
+        // Keys [0, limit) are seen by the thread's rows g and g + 8 of each tile.
+        int limit[kMT][2], low = r.length;
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = row0 + mt * 16 + e * 8 + (lane >> 2);
+                int n = r.length;
+                if (!prefix && a.causal) n = min(n, max(r.length - r.rows + row / group + 1, 0));
+                limit[mt][e] = n;
+                low = min(low, n);
+            }
+        low = __reduce_min_sync(0xffffffffu, low);
+
+        // Slice i of the warp: keys (c0 + i) * 64 + warp * 16 ... in two halves of
+        // eight, each inside one page.  A lane keeps the pages of half a slice;
+        // a batch of 16 slices is looked up at a time.
+        const int key0 = c0 * kUnit + warp * kSlice;
+        const int slices = key0 < r.length ? min(c1 - c0, (r.length - key0 - 1) / kUnit + 1) : 0;
+        int found = -1, offset = 0;
+        uint32_t missing = 0;  // two bits a stage: a half on no page of the cache
+        const T* kc = static_cast<const T*>(a.k_cache) + (long long)head0 * p.page * dim;
+        const T* vc = static_cast<const T*>(a.v_cache) + (long long)head0 * p.page * dim;
+        const auto issue = [&](int i) {
+            if (i < slices) {
+                if ((i & 15) == 0) {
+                    const int key = key0 + (i + (lane >> 1)) * kUnit + (lane & 1) * 8;
+                    found = -1;
+                    if (key < r.length) {
+                        const int index = key / p.page;
+                        offset = (key - index * p.page) * dim;
+                        const int id = load_l2(table + index);
+                        found = id >= 0 && id < p.cache_pages ? id : -1;
+                    }
+                }
+                const int stage = i % kStages;
+                const uint32_t dst = ring_u + stage * kStageBytes<kD>;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int from = (i & 15) * 2 + half;
+                    const int page = __shfl_sync(0xffffffffu, found, from);
+                    const int off = __shfl_sync(0xffffffffu, offset, from);
+                    const int keys = r.length - (key0 + i * kUnit + half * 8);  // valid keys of this half
+                    missing &= ~(1u << (2 * stage + half));
+                    if (page < 0 && keys > 0) missing |= 1u << (2 * stage + half);
+                    const T* ks = kc + page * p.ld_k_page + off;
+                    const T* vs = vc + page * p.ld_v_page + off;
+#pragma unroll
+                    for (int j = 0; j < 8 * kChunks / 32; ++j) {
+                        const int row = (j * 32 + lane) / kChunks, c = (j * 32 + lane) % kChunks;
+                        const bool live = page >= 0 && row < keys && c * 8 < dim;
+                        const uint32_t to = chunk_at<kD>(half * 8 + row, c);
+                        cp_async16(dst + to, live ? ks + row * dim + c * 8 : a.k_cache, live);
+                        cp_async16(dst + kSlice * kD * 2 + to, live ? vs + row * dim + c * 8 : a.v_cache, live);
+                    }
+                }
+            }
+            cp_async_commit();
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) issue(i);
+        __syncthreads();  // q is there
+
+        // One tile's q stays in registers; two tiles' would not fit beside their sums.
+        const auto load_q = [&](int mt, int k, uint32_t (&f)[4]) {
+            ldmatrix4(q_u + chunk_at<kD>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), f);
+        };
+        uint32_t qf[kMT == 1 ? kD / 16 : 1][4];
+        if constexpr (kMT == 1) {
+#pragma unroll
+            for (int k = 0; k < kD / 16; ++k) load_q(0, k, qf[k]);
+        }
+        float o[kMT][kD / 8][4], top[kMT][2], sum[kMT][2];
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt) {
+#pragma unroll
+            for (int n = 0; n < kD / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
+            top[mt][0] = top[mt][1] = -INFINITY;
+            sum[mt][0] = sum[mt][1] = 0.0f;
+        }
+
+        for (int i = 0; i < slices; ++i) {
+            issue(i + kStages - 1);
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            const int stage = i % kStages, key = key0 + i * kUnit;
+            const uint32_t k_u = ring_u + stage * kStageBytes<kD>, v_u = k_u + kSlice * kD * 2;
+            float s[kMT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kD / 16; ++k) {
+                uint32_t f[4];
+                // lanes 0-7 / 8-15: keys 0-7, low / high half of 16 elements; 16-31: keys 8-15
+                ldmatrix4(k_u + chunk_at<kD>((lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)), f);
+#pragma unroll
+                for (int mt = 0; mt < kMT; ++mt) {
+                    if constexpr (kMT > 1) load_q(mt, k, qf[0]);
+                    mma16816<T>(s[mt][0], qf[kMT == 1 ? k : 0], f[0], f[1]);
+                    mma16816<T>(s[mt][1], qf[kMT == 1 ? k : 0], f[2], f[3]);
+                }
+            }
+            const uint32_t gone = (missing >> (2 * stage)) & 3u;
+            const bool masked = key + kSlice > low || gone;
+            uint32_t hi[kMT][4], lo[kMT][4];
+            float pr[kMT][2][4];
+#pragma unroll
+            for (int mt = 0; mt < kMT; ++mt) {
+                float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float t = s[mt][n][e] * a.scale_log2;
+                        if (masked) {
+                            const int j = key + n * 8 + (lane & 3) * 2 + (e & 1);
+                            if (j >= limit[mt][e >> 1] || ((gone >> n) & 1)) t = -INFINITY;
+                        }
+                        s[mt][n][e] = t;
+                        most[e >> 1] = fmaxf(most[e >> 1], t);
+                    }
+                float ref[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 1));
+                    most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 2));
+                    const float now = fmaxf(top[mt][e], most[e]);
+                    ref[e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: every weight is 0
+                    const float keep = exp2_approx(top[mt][e] - ref[e]);
+                    top[mt][e] = now;
+                    if (keep != 1.0f) {
+                        sum[mt][e] *= keep;
+#pragma unroll
+                        for (int n = 0; n < kD / 8; ++n) {
+                            o[mt][n][2 * e] *= keep;
+                            o[mt][n][2 * e + 1] *= keep;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        pr[mt][n][e] = exp2_approx(s[mt][n][e] - ref[e >> 1]);
+                        sum[mt][e >> 1] += pr[mt][n][e];
+                    }
+                // the accumulators' layout is that of the second product's left operand
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        split_pair<T>(pr[mt][n][2 * e], pr[mt][n][2 * e + 1], hi[mt][2 * n + e], lo[mt][2 * n + e]);
+            }
+            if (masked && wild_values<T, kD>(v_u, lane)) {
+                // A value that some rows must not see is no number: 0 times it would
+                // reach them through the product.  Each row takes its own keys' alone.
+#pragma unroll 1
+                for (int kk = 0; kk < kSlice; ++kk) {
+                    const int n = kk >> 3, from = (lane & ~3) | ((kk & 7) >> 1);
+#pragma unroll
+                    for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float w0 = n ? pr[mt][1][2 * e] : pr[mt][0][2 * e];
+                            const float w1 = n ? pr[mt][1][2 * e + 1] : pr[mt][0][2 * e + 1];
+                            const float w = __shfl_sync(0xffffffffu, kk & 1 ? w1 : w0, from);
+                            if (key + kk < limit[mt][e] && !((gone >> n) & 1)) {
+#pragma unroll
+                                for (int d = 0; d < kD / 8; ++d) {
+                                    const T* v = reinterpret_cast<const T*>(
+                                        ring + (v_u - ring_u) + chunk_at<kD>(kk, d) + (lane & 3) * 4);
+                                    o[mt][d][2 * e] += w * to_float(v[0]);
+                                    o[mt][d][2 * e + 1] += w * to_float(v[1]);
+                                }
+                            }
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < kD / 16; ++d) {
+                    uint32_t f[4];
+                    // lanes 0-15: keys 0-15 of elements 0-7; 16-31: of elements 8-15
+                    ldmatrix4_trans(v_u + chunk_at<kD>(lane & 15, 2 * d + (lane >> 4)), f);
+#pragma unroll
+                    for (int mt = 0; mt < kMT; ++mt) {
+                        mma16816<T>(o[mt][2 * d], hi[mt], f[0], f[1]);
+                        mma16816<T>(o[mt][2 * d + 1], hi[mt], f[2], f[3]);
+                        mma16816<T>(o[mt][2 * d], lo[mt], f[0], f[1]);
+                        mma16816<T>(o[mt][2 * d + 1], lo[mt], f[2], f[3]);
+                    }
+                }
+            }
+            __syncwarp();  // the stage may be written again
+        }
+        cp_async_wait<0>();
+        __syncwarp();
+
+        // The warps' sums meet in shared memory: [row][dim], then the row's maximum and sum.
+        float* mine = reinterpret_cast<float*>(ring);
+        float* stats = mine + kRows * kD;
+#pragma unroll
+        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int row = mt * 16 + e * 8 + (lane >> 2);
+#pragma unroll
+                for (int n = 0; n < kD / 8; ++n)
+                    *reinterpret_cast<float2*>(mine + row * kD + n * 8 + (lane & 3) * 2) =
+                        make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
+                float t = sum[mt][e];
+                t += __shfl_xor_sync(0xffffffffu, t, 1);
+                t += __shfl_xor_sync(0xffffffffu, t, 2);
+                if ((lane & 3) == 0) {
+                    stats[2 * row] = top[mt][e];
+                    stats[2 * row + 1] = t;
+                }
+            }
+        __syncthreads();
+        const bool whole = c0 == 0 && c1 == units;
+        const int slot = u == u0 ? 0 : 1;
+        for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
+            const int row = i / (kD / 4), d = i % (kD / 4) * 4;
+            float most = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w)
+                most = fmaxf(most, warp_sums<kD>(smem, w)[kRows * kD + 2 * row]);
+            const float ref = most == -INFINITY ? 0.0f : most;
+            float total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float* ow = warp_sums<kD>(smem, w);
+                const float keep = exp2_approx(ow[kRows * kD + 2 * row] - ref);
+                total += ow[kRows * kD + 2 * row + 1] * keep;
+                const float4 x = *reinterpret_cast<const float4*>(ow + row * kD + d);
+                v[0] += x.x * keep;
+                v[1] += x.y * keep;
+                v[2] += x.z * keep;
+                v[3] += x.w * keep;
+            }
+            if (d >= dim) continue;
+            const int token = (row0 + row) / group, head = head0 * group + (row0 + row) % group;
+            if (!whole)
+                put_part(ws, ((long long)blockIdx.x * 2 + slot) * kRows + row, kD, d, v, most, total);
+            else
+                put_row<T>(a, ws, prefix, r.first + token, head, d, v, most, total);
+        }
+        __syncthreads();  // the sums are read: the rings and q may be written again
+        u += c1 - c0;
+    }
+}
+
+// Joins the parts of the item that border blockIdx.x + 1 cuts, if it is the
+// first border inside it.
+template <class T, int kD, int kMT>
+__global__ void __launch_bounds__(kThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int blocks) {
+    constexpr int kRows = 16 * kMT;
+    __shared__ long long scratch[kWarps + 4];
+    const PagedBatch& p = a.batch;
+    const int group = a.heads / p.kv_heads;
+    const int g = blockIdx.x + 1;
+    // The plan's inputs are older than the kernel before this one, which has
+    // waited for their writers.
+    Plan<kRows> plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
+    const Found at = find_unit(plan, g, blocks, scratch);
+    pdl_launch_dependents();
+    pdl_wait_primary();  // before any return: who waits for this kernel counts on the one before it too
+    const long long u = at.total * g / blocks;
+    if (u >= at.total) return;
+    const Request r = plan.get(at.b);
+    const int units = plan.units(r.length), tiles = plan.tiles(r.rows);
+    const long long item = (u - at.before) / units;
+    const long long start = at.before + item * units, end = start + units;
+    if (u == start || at.total * (g - 1) / blocks > start) return;
+    const int head0 = (int)(item / tiles), tile = (int)(item % tiles);
+    const int row0 = tile * kRows, item_rows = min(kRows, r.rows * group - row0);
+    // Block h's part lies in its first slot, but for the block in whose run the
+    // item begins behind another's units.
+    const int first = at.total * (g - 1) / blocks == start ? 0 : 1;
+    for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
+        const int row = i / (kD / 4), d = i % (kD / 4) * 4;
+        if (d >= p.dim) continue;
+        Joined j;
+        for (int h = g - 1; h < blocks && at.total * h / blocks < end; ++h) {
+            if (at.total * h / blocks == at.total * (h + 1) / blocks) continue;  // a block without units
+            j.add(ws, ((long long)h * 2 + (h == g - 1 ? first : 0)) * kRows + row, kD, d);
+        }
+        const int token = (row0 + row) / group, head = head0 * group + (row0 + row) % group;
+        put_row<T>(a, ws, at.b < 0, r.first + token, head, d, j.v, j.most, j.total);
+    }
+}
+
+// Joins the own and the prefix result of every row that a request owns.
+template <class T>
+__global__ void __launch_bounds__(256) join_prefix_kernel(const AttentionArgs a, const Workspace ws) {
+    const PagedBatch& p = a.batch;
+    const int t = blockIdx.x;
+    const bool owned = request_of_row(p, t) >= 0;
+    pdl_launch_dependents();
+    pdl_wait_primary();
+    if (!owned) return;
+    const int each = p.dim / 4;
+    for (int i = threadIdx.x; i < a.heads * each; i += 256) {
+        const int head = i / each, d = i % each * 4;
+        const long long row = (long long)t * a.heads + head;
+        Joined j;
+        j.add_row(ws.row_stats[0], ws.row_sums[0], row, p.dim, d);
+        j.add_row(ws.row_stats[1], ws.row_sums[1], row, p.dim, d);
+        put_out<T>(a, t, head, d, j.v, j.total);
+    }
+}
+
+template <class T, int kD, int kMT>
+cudaError_t launch_t(const AttentionArgs& a, Workspace ws, cudaStream_t stream) {
+    constexpr int smem = kSmemBytes<kD, kMT>;
+    cudaError_t e = ensure_smem_attr(attend_kernel<T, kD, kMT>, smem);
+    if (e != cudaSuccess) return e;
+    const int blocks = kBlocksPerSm * sm_count();
+    e = launch_pdl_kernel(attend_kernel<T, kD, kMT>, dim3(blocks), dim3(kThreads), smem, stream, a, ws);
+    if (e != cudaSuccess) return e;
+    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(blocks - 1), dim3(kThreads), 0, stream, a, ws, blocks);
+    if (e != cudaSuccess || a.prefix_length == 0) return e;
+    return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);
+}
+
+template <class T>
+cudaError_t launch_d(const AttentionArgs& a, Workspace ws, cudaStream_t stream) {
+    // 16-row tiles where no item has more rows
+    const int group = a.heads / a.batch.kv_heads;
+    const bool one = a.batch.starts || a.prefix_length > 0 ? (long long)a.batch.rows * group <= 16 : group <= 16;
+    if (a.batch.dim <= 64)
+        return one ? launch_t<T, 64, 1>(a, ws, stream) : launch_t<T, 64, 2>(a, ws, stream);
+    return one ? launch_t<T, 128, 1>(a, ws, stream) : launch_t<T, 128, 2>(a, ws, stream);
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// Lays the workspace out; base null: its size alone.
+Workspace layout(const AttentionArgs& a, uint8_t* base, size_t* bytes) {
+    Workspace ws{};
+    size_t at = 0;
+    const auto take = [&](size_t n) {
+        float* p = base ? reinterpret_cast<float*>(base + at) : nullptr;
+        at += align256(n * sizeof(float));
+        return p;
+    };
+    const size_t parts = (size_t)kBlocksPerSm * sm_count() * 2 * 32;
+    const size_t width = a.batch.dim <= 64 ? 64 : 128;
+    ws.part_sums = take(parts * width);
+    ws.part_stats = take(parts * 2);
+    if (a.prefix_length > 0) {
+        const size_t rows = (size_t)a.batch.rows * a.heads;
+        for (int k = 0; k < 2; ++k) {
+            ws.row_sums[k] = take(rows * a.batch.dim);
+            ws.row_stats[k] = take(rows * 2);
+        }
+    }
+    *bytes = at;
+    return ws;
+}
+
+}  // namespace
+
+size_t attention_workspace_bytes(const AttentionArgs& a) {
+    size_t n = 0;
+    layout(a, nullptr, &n);
+    return n;
+}
+
+cudaError_t launch_paged_attention(const AttentionArgs& a, int dtype, void* workspace, cudaStream_t stream) {
+    size_t n = 0;
+    const Workspace ws = layout(a, static_cast<uint8_t*>(workspace), &n);
+    return dtype == ZQ_DTYPE_F16 ? launch_d<__half>(a, ws, stream) : launch_d<__nv_bfloat16>(a, ws, stream);
+}
+
+}  // namespace zq

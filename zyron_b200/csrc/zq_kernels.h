@@ -232,6 +232,60 @@ struct LowRankArgs {
 size_t low_rank_workspace_bytes(const LowRankArgs& a);  // m > 0
 cudaError_t launch_add_low_rank(const LowRankArgs& a, int x_dtype, int w_dtype, void* workspace, cudaStream_t stream);
 
+// A batch of requests over a paged cache (zq_append_kv, zq_paged_attention;
+// zq_paged.cuh has how it is read).  The caches are [cache_pages][kv_heads][page][dim]
+// of a 16-bit type; pitches in elements.
+struct PagedBatch {
+    const int32_t* starts;   // [requests + 1], null: one row each
+    const int32_t* lengths;  // [requests]
+    const int32_t* pages;    // [requests][ld_pages], max_pages used
+    long long ld_pages;
+    int requests;
+    int rows;       // rows of the whole call
+    int max_pages;
+    int page;       // tokens a page
+    int cache_pages;
+    int kv_heads;
+    int dim;
+    long long ld_k_page, ld_v_page;  // from page to page of the caches
+};
+
+// zq_append_kv (zq_append.cu).
+struct AppendArgs {
+    PagedBatch batch;
+    const void* q;  // [rows][heads][dim], null: keys and values only
+    const void* k;  // [rows][kv_heads][dim]
+    const void* v;
+    long long ldq, ldk, ldv;  // from row to row
+    void* k_cache;
+    void* v_cache;
+    void* q_out;  // [rows][heads][dim], the cache's type
+    const double* inv_freq;  // [rotated / 2], null: no rotation
+    int heads;
+    int rotated;
+    int interleaved;
+    long long offset;
+};
+cudaError_t launch_append_kv(const AppendArgs& a, int dtype, int cache_dtype, cudaStream_t stream);
+
+// zq_paged_attention (zq_attention.cu and zq_attention_sm100.cu).
+struct AttentionArgs {
+    PagedBatch batch;
+    const void* q;  // [rows][heads][dim]
+    long long ldq;
+    const void* k_cache;
+    const void* v_cache;
+    void* out;      // [rows][heads][dim]
+    long long ld_out;
+    const int32_t* prefix_pages;
+    int prefix_length;
+    int heads;
+    int causal;
+    float scale_log2;  // scale x log2(e)
+};
+size_t attention_workspace_bytes(const AttentionArgs& a);
+cudaError_t launch_paged_attention(const AttentionArgs& a, int dtype, void* workspace, cudaStream_t stream);
+
 int gemm_block_n(int M, int N);
 
 // Multiprocessors of the current device available to the persistent kernels

@@ -1,6 +1,6 @@
 // zq_ops.cu -- C ABI of the operators around the quantized matmul
-// (zq_rms_norm_quantize, zq_add_low_rank, zq_token_logprobs): argument checks
-// and launches.
+// (zq_rms_norm_quantize, zq_add_low_rank, zq_token_logprobs, zq_append_kv,
+// zq_paged_attention): argument checks and launches.
 #include "zq.h"
 #include "zq_internal.h"
 #include "zq_kernels.h"
@@ -30,6 +30,59 @@ bool aligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) %
 // Rows of `pitch` elements of `size` bytes whose byte offsets fit in 63 bits.
 bool offsets_fit(size_t rows, size_t pitch, size_t size) {
     return pitch <= kIntMax * 64 && (rows == 0 || pitch <= (std::numeric_limits<size_t>::max() >> 1) / size / rows);
+}
+
+// The sizes of a batch over a paged cache, checked; its pointers are not.
+zq_status check_batch(const zq_paged_batch* b, zq::PagedBatch* out) {
+    if (!b) return invalid("zyron_b200: null pointer");
+    if (b->cache_dtype != ZQ_DTYPE_F16 && b->cache_dtype != ZQ_DTYPE_BF16)
+        return invalid("zyron_b200: the cache must be fp16 or bf16");
+    if (b->dim == 0 || b->dim % 8 != 0 || b->dim > ZQ_PAGED_MAX_DIM)
+        return invalid("zyron_b200: dim must be a multiple of 8 and at most 128");
+    if (b->page == 0 || b->page % 8 != 0 || b->page > (1u << 20))
+        return invalid("zyron_b200: page must be a multiple of 8 and at most 2^20");
+    if (b->kv_heads == 0 || b->kv_heads > 65535) return invalid("zyron_b200: kv_heads must be in [1, 65535]");
+    if (b->ld_pages < b->max_pages) return invalid("zyron_b200: a row pitch is smaller than its row");
+    if (!b->starts && b->rows != b->requests) return invalid("zyron_b200: without starts every request has one row");
+    if (b->rows > kIntMax / 512 || b->requests > kIntMax - 4096 || b->max_pages > kIntMax || b->cache_pages > kIntMax)
+        return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: dimension too large");
+    const size_t block = b->kv_heads * b->page * b->dim;  // < 2^44
+    if (b->cache_pages > 0 && (b->ld_k_page < block || b->ld_v_page < block))
+        return invalid("zyron_b200: a page pitch is smaller than its page");
+    if (!offsets_fit(b->cache_pages, b->ld_k_page, 2) || !offsets_fit(b->cache_pages, b->ld_v_page, 2) ||
+        !offsets_fit(b->requests, b->ld_pages, 4) || b->ld_k_page > kIntMax * 64 || b->ld_v_page > kIntMax * 64)
+        return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: matrix size overflow");
+    out->starts = b->starts;
+    out->lengths = b->lengths;
+    out->pages = b->pages;
+    out->ld_pages = (long long)b->ld_pages;
+    out->requests = (int)b->requests;
+    out->rows = (int)b->rows;
+    out->max_pages = (int)b->max_pages;
+    out->page = (int)b->page;
+    out->cache_pages = (int)b->cache_pages;
+    out->kv_heads = (int)b->kv_heads;
+    out->dim = (int)b->dim;
+    out->ld_k_page = (long long)b->ld_k_page;
+    out->ld_v_page = (long long)b->ld_v_page;
+    return ZQ_OK;
+}
+
+// The batch's own pointers and those of the caches (16-byte accesses where the
+// kernels make them).
+zq_status check_batch_pointers(const zq_paged_batch* b, const void* k_cache, const void* v_cache) {
+    if (!b->lengths || (b->max_pages && !b->pages) || (b->cache_pages && (!k_cache || !v_cache)))
+        return invalid("zyron_b200: null pointer");
+    if (!aligned(b->starts, 4) || !aligned(b->lengths, 4) || !aligned(b->pages, 4))
+        return invalid("zyron_b200: a pointer is not aligned to its element type");
+    return ZQ_OK;
+}
+
+zq_status check_heads(size_t heads, size_t kv_heads) {
+    if (heads == 0 || heads % kv_heads != 0) return invalid("zyron_b200: heads must be a multiple of kv_heads");
+    if (heads / kv_heads > ZQ_ATTENTION_MAX_GROUP)
+        return invalid("zyron_b200: at most 128 query heads a kv head");
+    return ZQ_OK;
 }
 
 }  // namespace
@@ -181,6 +234,103 @@ zq_status zq_token_logprobs(const void* logits, int dtype, size_t m, size_t voca
     r.top_ids = top_ids;
     const cudaError_t e = zq::launch_token_logprobs(r, dtype, as_stream(stream));
     return e == cudaSuccess ? ZQ_OK : zq::cuda_error(e, "token_logprobs");
+}
+
+zq_status zq_append_kv(const zq_paged_batch* batch, const void* q, size_t ldq, const void* k, size_t ldk,
+                       const void* v, size_t ldv, int dtype, size_t heads, void* k_cache, void* v_cache, void* q_out,
+                       const double* inv_freq, size_t rotated, int interleaved, int64_t offset, void* stream) {
+    zq::AppendArgs a{};
+    zq_status s = check_batch(batch, &a.batch);
+    if (s != ZQ_OK) return s;
+    const size_t size = dtype_bytes(dtype);
+    if (size == 0) return invalid("zyron_b200: unsupported element type");
+    if ((q == nullptr) != (q_out == nullptr)) return invalid("zyron_b200: q and q_out go together");
+    if (q && (s = check_heads(heads, batch->kv_heads)) != ZQ_OK) return s;
+    if (rotated % 2 != 0 || rotated > batch->dim) return invalid("zyron_b200: rotated must be even and at most dim");
+    if ((rotated != 0) != (inv_freq != nullptr)) return invalid("zyron_b200: rotated and inv_freq go together");
+    if (offset < 0 || offset > (int64_t)1 << 40) return invalid("zyron_b200: offset must be in [0, 2^40]");
+    if ((q && ldq < heads * batch->dim) || ldk < batch->kv_heads * batch->dim || ldv < batch->kv_heads * batch->dim)
+        return invalid("zyron_b200: a row pitch is smaller than its row");
+    if (batch->rows == 0 || batch->requests == 0) return ZQ_OK;
+    if (!k || !v) return invalid("zyron_b200: null pointer");
+    if ((s = check_batch_pointers(batch, k_cache, v_cache)) != ZQ_OK) return s;
+    if (!offsets_fit(batch->rows, ldq, size) || !offsets_fit(batch->rows, ldk, size) ||
+        !offsets_fit(batch->rows, ldv, size))
+        return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: matrix size overflow");
+    if (!aligned(q, size) || !aligned(k, size) || !aligned(v, size) || !aligned(q_out, 2) || !aligned(k_cache, 2) ||
+        !aligned(v_cache, 2) || !aligned(inv_freq, 8))
+        return invalid("zyron_b200: a pointer is not aligned to its element type");
+    a.q = q;
+    a.k = k;
+    a.v = v;
+    a.ldq = (long long)ldq;
+    a.ldk = (long long)ldk;
+    a.ldv = (long long)ldv;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.q_out = q_out;
+    a.inv_freq = inv_freq;
+    a.heads = (int)heads;
+    a.rotated = (int)rotated;
+    a.interleaved = interleaved != 0;
+    a.offset = offset;
+    const cudaError_t e = zq::launch_append_kv(a, dtype, batch->cache_dtype, as_stream(stream));
+    return e == cudaSuccess ? ZQ_OK : zq::cuda_error(e, "append_kv");
+}
+
+size_t zq_paged_attention_workspace_bytes(const zq_paged_batch* batch, size_t heads, size_t prefix_length) {
+    zq::AttentionArgs a{};
+    if (check_batch(batch, &a.batch) != ZQ_OK || check_heads(heads, batch->kv_heads) != ZQ_OK ||
+        prefix_length > kIntMax - 4096)
+        return 0;
+    a.heads = (int)heads;
+    a.prefix_length = (int)prefix_length;
+    return zq::attention_workspace_bytes(a);
+}
+
+zq_status zq_paged_attention(const zq_paged_batch* batch, const void* q, size_t ldq, size_t heads,
+                             const void* k_cache, const void* v_cache, const int32_t* prefix_pages,
+                             size_t prefix_length, int causal, float scale, void* out, size_t ld_out,
+                             void* workspace, size_t workspace_bytes, void* stream) {
+    zq::AttentionArgs a{};
+    zq_status s = check_batch(batch, &a.batch);
+    if (s != ZQ_OK) return s;
+    if ((s = check_heads(heads, batch->kv_heads)) != ZQ_OK) return s;
+    if (!std::isfinite(scale)) return invalid("zyron_b200: scale must be finite");
+    if (ldq < heads * batch->dim || ld_out < heads * batch->dim)
+        return invalid("zyron_b200: a row pitch is smaller than its row");
+    if (ldq % 8 != 0 || ld_out % 4 != 0) return invalid("zyron_b200: ldq must be a multiple of 8, ld_out of 4");
+    if (batch->ld_k_page % 8 != 0 || batch->ld_v_page % 8 != 0)
+        return invalid("zyron_b200: page pitches must be multiples of 8");
+    if (prefix_length > kIntMax - 4096) return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: dimension too large");
+    if (batch->rows == 0 || batch->requests == 0) return ZQ_OK;
+    if (!q || !out || (prefix_length && !prefix_pages)) return invalid("zyron_b200: null pointer");
+    if ((s = check_batch_pointers(batch, k_cache, v_cache)) != ZQ_OK) return s;
+    if (!offsets_fit(batch->rows, ldq, 2) || !offsets_fit(batch->rows, ld_out, 2))
+        return zq::set_error(ZQ_ERR_OVERFLOW, "zyron_b200: matrix size overflow");
+    if (!aligned(q, 16) || !aligned(k_cache, 16) || !aligned(v_cache, 16) || !aligned(out, 8) ||
+        !aligned(prefix_pages, 4))
+        return invalid("zyron_b200: q and the caches must be 16-byte aligned, out 8-byte");
+    a.q = q;
+    a.ldq = (long long)ldq;
+    a.k_cache = k_cache;
+    a.v_cache = v_cache;
+    a.out = out;
+    a.ld_out = (long long)ld_out;
+    a.prefix_pages = prefix_pages;
+    a.prefix_length = (int)prefix_length;
+    a.heads = (int)heads;
+    a.causal = causal != 0;
+    a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    const size_t need = zq::attention_workspace_bytes(a);
+    if (!workspace || workspace_bytes < need) {
+        char buf[128];
+        std::snprintf(buf, sizeof buf, "zyron_b200: workspace too small (%zu < %zu bytes)", workspace_bytes, need);
+        return invalid(buf);
+    }
+    if (!aligned(workspace, 256)) return invalid("zyron_b200: workspace must be 256-byte aligned");
+    const cudaError_t e = zq::launch_paged_attention(a, batch->cache_dtype, workspace, as_stream(stream));
+    return e == cudaSuccess ? ZQ_OK : zq::cuda_error(e, "paged_attention");
 }
 
 }  // extern "C"

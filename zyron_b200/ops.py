@@ -10,6 +10,9 @@
   them as ``adapters``.
 * ``token_logprobs``: log probabilities of given tokens, the entropy and the
   most likely alternatives over a head's logits (``zq_token_logprobs``).
+* ``append_kv`` and ``paged_attention``: the paged key/value cache of a batch,
+  its new tokens rotated and stored, and attention over it with a prefix that
+  the requests share (``zq_append_kv``, ``zq_paged_attention``).
 
 All take and return torch CUDA tensors, run on ``stream`` (default: the
 device's current stream) without synchronising, allocate their outputs and
@@ -19,6 +22,7 @@ include/zq.h.
 """
 from __future__ import annotations
 
+import ctypes as C
 import typing
 
 from . import _lib
@@ -102,11 +106,12 @@ def _out_rows(t, name, shape, dtype):
     return t, (t.stride(0) if t.shape[0] > 1 else k)
 
 
-def _apart(out, ld_out, t, ld, name, what="residual_out"):
-    """Refuses rows `out` that overlap the rows `t` otherwise than by being them."""
+def _apart(out, ld_out, t, ld, name, what="residual_out", same=True):
+    """Refuses rows `out` that overlap the rows `t`, otherwise than by being
+    them where `same` allows that."""
     at, pitch, at_t, pitch_t = out.data_ptr(), ld_out * out.element_size(), t.data_ptr(), ld * t.element_size()
     (m, k), width, width_t = out.shape, out.shape[1] * out.element_size(), t.shape[-1] * t.element_size()
-    if m == 0 or at == at_t and pitch == pitch_t:
+    if m == 0 or same and at == at_t and pitch == pitch_t:
         return
     if at + (m - 1) * pitch + width <= at_t or at_t + (t.shape[0] - 1) * pitch_t + width_t <= at:
         return
@@ -410,3 +415,164 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=True, stream=None):
         check(lib().zq_token_logprobs(rows.data_ptr(), dtype, rows.shape[0], vocab, ld, _ptr(targets), n, top_k,
                                       _ptr(lp), _ptr(ent), _ptr(top_lp), _ptr(top_ids), ptr))
     return TokenLogprobs(lp, ent, top_lp, top_ids)
+
+
+def _heads(t, name, rows, dim, dtype=None):
+    """A [rows, heads, dim] tensor with contiguous heads: (tensor, row pitch)."""
+    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim:
+        raise _bad(f"{name} must be [rows, heads, dim] with dim {dim}, and {rows} rows")
+    if dtype is not None and t.dtype != dtype:
+        raise _bad(f"{name} must be {dtype}")
+    width = t.shape[1] * dim
+    if t.is_contiguous():
+        return t, width
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim) or (rows > 1 and t.stride(0) < width):
+        return t.contiguous(), width
+    return t, (t.stride(0) if rows > 1 else width)
+
+
+def _paged_batch(rows, k_cache, v_cache, pages, lengths, starts):
+    """The checked batch of a call over a paged cache."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+        raise _bad("k_cache and v_cache must be [pages, kv_heads, page, dim], of one shape and type")
+    cache_pages, kv_heads, page, dim = k_cache.shape
+    code = _DTYPES.get(k_cache.dtype)
+    if code is None or code == 1:
+        raise _bad("the cache must be float16 or bfloat16")
+    block = kv_heads * page * dim
+    pitch = []
+    for t in (k_cache, v_cache):
+        ok = t.is_contiguous() or (t.stride(3) == 1 and t.stride(2) == dim and
+                                   (kv_heads == 1 or t.stride(1) == page * dim) and
+                                   (cache_pages <= 1 or t.stride(0) >= block))
+        if not ok:
+            raise _bad("each page's [kv_heads, page, dim] must be contiguous in the caches")
+        pitch.append(t.stride(0) if cache_pages > 1 else block)
+    at = (v_cache.data_ptr() - k_cache.data_ptr()) // k_cache.element_size()
+    if cache_pages and -((cache_pages - 1) * pitch[1] + block) < at < (cache_pages - 1) * pitch[0] + block:
+        # interleaved page by page, or one inside the other
+        if pitch[0] != pitch[1] or not block <= at % pitch[0] <= pitch[0] - block:
+            raise _bad("k_cache and v_cache overlap")
+    if pages.dim() != 2 or pages.dtype != torch.int32 or lengths.dtype != torch.int32 or lengths.dim() != 1:
+        raise _bad("pages must be int32 [requests, max_pages] and lengths int32 [requests]")
+    requests, max_pages = pages.shape
+    if lengths.shape[0] != requests or not lengths.is_contiguous():
+        raise _bad("lengths must be contiguous int32 [requests], as many as rows of pages")
+    if max_pages > 1 and pages.stride(1) != 1 or requests > 1 and pages.stride(0) < max_pages:
+        raise _bad("pages must have contiguous rows that do not overlap")
+    if starts is None:
+        if requests != rows:
+            raise _bad(f"without starts every request has one row: {requests} requests, {rows} rows")
+    elif starts.dtype != torch.int32 or starts.shape != (requests + 1,) or not starts.is_contiguous():
+        raise _bad("starts must be contiguous int32 [requests + 1]")
+    return _lib.PagedBatchC(_ptr(starts), lengths.data_ptr(), pages.data_ptr(),
+                            pages.stride(0) if requests > 1 else max_pages, max_pages, requests, rows, page, cache_pages,
+                            kv_heads, dim, pitch[0], pitch[1], code)
+
+
+def append_kv(q, k, v, k_cache, v_cache, pages, lengths, starts=None, inv_freq=None, interleaved=True, offset=0,
+              stream=None):
+    """Stores new tokens' keys and values in a paged cache and rotates queries
+    and keys by position on the way; returns the rotated queries in the cache's
+    type (``None`` where ``q`` is).
+
+    ``q`` [rows, heads, dim], ``k`` and ``v`` [rows, kv_heads, dim] share a type
+    (float32, float16 or bfloat16) and may be columns of one projection's
+    output; the caches are float16 or bfloat16 [pages, kv_heads, page, dim].
+    The rows are the requests' new tokens one request after the other, request
+    b's from ``starts[b]`` to ``starts[b + 1]`` (None: one row each);
+    ``lengths[b]`` counts its cached tokens, the new ones included, and
+    ``pages[b]`` (int32 [requests, max_pages]) names the pages that hold them.
+    All three are read on the device when the call runs.
+
+    ``inv_freq`` (float64 [rotated / 2], None: no rotation) holds the angle of
+    each pair per position, ``interleaved`` says whether pairs are neighbours
+    or half a rotation apart, and ``offset`` is the position of a request's
+    first own token, such as a shared prefix's length.  Tokens whose page is
+    outside the cache are not stored; rows that no request owns are neither
+    stored nor written in the result."""
+    if torch is None:
+        _setup()
+    dtype = _dtype(k, "k")
+    index = _device(k, "q v k_cache v_cache pages lengths starts inv_freq", q, v, k_cache, v_cache, pages, lengths, starts,
+                    inv_freq)
+    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype:
+        raise _bad("k and v must be [rows, kv_heads, dim], of one shape and type")
+    rows = k.shape[0]
+    batch = _paged_batch(rows, k_cache, v_cache, pages, lengths, starts)
+    if k.shape[1] != k_cache.shape[1]:
+        raise _bad("k and v must have the caches' kv_heads")
+    dim = k_cache.shape[3]
+    rotated = 0
+    if inv_freq is not None:
+        if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
+            raise _bad("inv_freq must be contiguous float64 [rotated / 2]")
+        rotated = 2 * inv_freq.shape[0]
+    context, ptr = _context(index, stream)
+    with context:
+        k, ldk = _heads(k, "k", rows, dim)
+        v, ldv = _heads(v, "v", rows, dim)
+        out, heads, ldq = None, 0, 0
+        if q is not None:
+            q, ldq = _heads(q, "q", rows, dim, k.dtype)
+            heads = q.shape[1]
+            out = torch.empty_strided((rows, heads, dim), (heads * dim, dim, 1), dtype=k_cache.dtype, device=k.device)
+        check(lib().zq_append_kv(C.byref(batch), _ptr(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, dtype, heads,
+                                 k_cache.data_ptr(), v_cache.data_ptr(), _ptr(out), inv_freq.data_ptr() if rotated else None,
+                                 rotated, interleaved, offset, ptr))
+    return out
+
+
+def paged_attention(q, k_cache, v_cache, pages, lengths, starts=None, prefix_pages=None, prefix_length=0, causal=True,
+                    scale=None, out=None, stream=None):
+    """Attention of new tokens ``q`` [rows, heads, dim] (the cache's type) over
+    a paged cache, as ``append_kv`` leaves it and with its ``pages``,
+    ``lengths`` and ``starts``; returns [rows, heads, dim].
+
+    Every row sees the ``prefix_length`` tokens of a prefix that all requests
+    share (on ``prefix_pages``, int32), which is computed once for all of them,
+    and its request's own tokens, with ``causal`` those up to its own
+    position.  ``scale`` is 1 / sqrt(dim) by default.  A row that sees no token
+    is zero; rows that no request owns are left as ``out`` has them."""
+    if torch is None:
+        _setup()
+    index = _device(q, "k_cache v_cache pages lengths starts prefix_pages out", k_cache, v_cache, pages, lengths, starts,
+                    prefix_pages, out)
+    if q.dim() != 3:
+        raise _bad("q must be [rows, heads, dim]")
+    rows, heads = q.shape[:2]
+    batch = _paged_batch(rows, k_cache, v_cache, pages, lengths, starts)
+    page, dim = k_cache.shape[2:]
+    if prefix_length < 0:
+        raise _bad("prefix_length must be >= 0")
+    if prefix_length:
+        if prefix_pages is None or prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or \
+                not prefix_pages.is_contiguous() or prefix_pages.shape[0] * page < prefix_length:
+            raise _bad("prefix_pages must be contiguous int32 and hold prefix_length tokens")
+    if scale is None:
+        scale = dim**-0.5 if dim else 1.0
+    if heads == 0 or heads % k_cache.shape[1]:
+        raise _bad("heads must be a multiple of kv_heads")
+    context, ptr = _context(index, stream)
+    with context:
+        q, ldq = _heads(q, "q", rows, dim, k_cache.dtype)
+        if q.data_ptr() % 16 or ldq % 8:
+            q, ldq = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device).copy_(q), heads * dim
+        if out is None:
+            out = torch.empty_strided((rows, heads, dim), (heads * dim, dim, 1), dtype=q.dtype, device=q.device)
+            ld_out = heads * dim
+        else:
+            if out.shape != q.shape or out.dtype != q.dtype:
+                raise _bad(f"out must have shape {tuple(q.shape)} and type {q.dtype}")
+            if out.stride(2) != 1 or (heads > 1 and out.stride(1) != dim) or (rows > 1 and out.stride(0) < heads * dim):
+                raise _bad("out must have contiguous rows that do not overlap")
+            ld_out = out.stride(0) if rows > 1 else heads * dim
+            if rows:
+                _apart(out.flatten(1), ld_out, q.flatten(1), ldq, "q", "out", same=False)
+        need = lib().zq_paged_attention_workspace_bytes(C.byref(batch), heads, prefix_length)
+        ws = _empty((need + 256,), torch.uint8, q.device)
+        base = (ws.data_ptr() + 255) & ~255
+        check(lib().zq_paged_attention(C.byref(batch), q.data_ptr(), ldq, heads, k_cache.data_ptr(), v_cache.data_ptr(),
+                                       _ptr(prefix_pages) if prefix_length else None, prefix_length, causal, scale,
+                                       out.data_ptr(), ld_out, base, need, ptr))
+    return out
