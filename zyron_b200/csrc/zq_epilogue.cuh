@@ -18,12 +18,24 @@
 
 namespace zq {
 
-__device__ __forceinline__ float epi_gelu(float v) {
-    // -2 sqrt(2/pi) and -2 sqrt(2/pi) 0.044715
-    const float t = v * fmaf(-0.07135481627f, v * v, -1.59576912161f);
-    return __fdividef(v, 1.0f + expf(t));
+// float(acc) * s_row * s_col, each product rounded, a NaN being any NaN.
+__device__ __forceinline__ float epi_value(int32_t acc, float s_row, float s_col) {
+    return __fmul_rn(__fmul_rn(__int2float_rn(acc), s_row), s_col);
 }
-__device__ __forceinline__ float epi_silu(float v) { return __fdividef(v, 1.0f + expf(-v)); }
+
+// v / (1 + 2^t): the base-2 exponential and the reciprocal of the special
+// function unit (2^-22.5 and 2^-23 off), each one instruction.
+__device__ __forceinline__ float epi_logistic(float v, float t) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+    return v * r;
+}
+__device__ __forceinline__ float epi_gelu(float v) {
+    // log2(e) times -2 sqrt(2/pi) 0.044715 and -2 sqrt(2/pi)
+    return epi_logistic(v, v * fmaf(-0.10294324f, v * v, -2.3022082f));
+}
+__device__ __forceinline__ float epi_silu(float v) { return epi_logistic(v, v * -1.4426950f); }
 __device__ __forceinline__ float epi_relu(float v) { return v < 0.0f ? 0.0f : v; }  // NaN stays
 
 template <int N>
@@ -61,6 +73,109 @@ __device__ __forceinline__ void epi_finish(const Epilogue& e, void* y, int n, in
     epi_activate(e.activation, v);
     if (e.residual) v[0] += epi_residual(e, (size_t)row * (size_t)e.ld_residual + (size_t)col);
     epi_store(e, y, (size_t)row * (size_t)n + (size_t)col, v[0]);
+}
+
+// A warp's block of 32 rows x 16 columns whose rows lie on no grid: turned
+// around in shared memory, so that 16 lanes take one row's columns and their
+// accesses merge (333 x 2050 x 1003 with an fp32 residual took 36 us row by
+// lane).  `stage` is the warp's own 32 x kEpiPitch16 floats.
+constexpr int kEpiPitch16 = 17;
+__device__ __forceinline__ void epi_finish_block(const Epilogue& e, void* y, int n, int row0, int rows, int col0,
+                                                 const float (&v)[16], float* stage) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();  // the block before has been read
+#pragma unroll
+    for (int j = 0; j < 16; ++j) stage[lane * kEpiPitch16 + j] = v[j];
+    __syncwarp();
+    const int col = col0 + (lane & 15), sub = lane >> 4;
+    if (col >= n) return;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float r[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = half * 16 + i * 2 + sub;
+            r[i] = e.residual && row < rows ? epi_residual(e, (size_t)(row0 + row) * (size_t)e.ld_residual + col) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int row = half * 16 + i * 2 + sub;
+            if (row < rows)
+                epi_store(e, y, (size_t)(row0 + row) * (size_t)n + col, stage[row * kEpiPitch16 + (lane & 15)] + r[i]);
+        }
+    }
+}
+
+// The same on the 16-byte grid, 16 bytes a lane: four lanes a row of fp32, two of
+// 16 bits, so that the residual's sectors are read once.  Row by lane, every
+// 16-byte access of a warp touches 32 rows, and half of each sector that it
+// brings is asked for again: 4096 x 4096 x 11008 with an fp32 residual took
+// 321 us.  `stage` is 32 x kEpiPitchWide floats.
+constexpr int kEpiPitchWide = 20;
+struct EpiWide {
+    uint4 w[4];
+};
+__device__ __forceinline__ void epi_load_wide(const Epilogue& e, int row0, int rows, int col0, EpiWide& r) {
+    const int lane = threadIdx.x & 31;
+    const bool full = e.dtype == ZQ_DTYPE_F32;
+    const int sub = full ? lane >> 2 : lane >> 1, each = full ? 8 : 16;
+    const int col = col0 + (full ? 4 * (lane & 3) : 8 * (lane & 1));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * each + sub;
+        if ((full || i < 2) && row < rows)
+            r.w[i] = load_l2(reinterpret_cast<const uint4*>(
+                static_cast<const uint8_t*>(e.residual) +
+                ((size_t)(row0 + row) * (size_t)e.ld_residual + (size_t)col) * (full ? 4 : 2)));
+    }
+}
+template <class T>
+__device__ __forceinline__ void epi_put_halves(const Epilogue& e, void* y, int n, int row0, int rows, int col0,
+                                               const EpiWide& r, const float* stage) {
+    const int lane = threadIdx.x & 31, col = 8 * (lane & 1);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int row = i * 16 + (lane >> 1);
+        if (row >= rows) continue;
+        const float4 a = *reinterpret_cast<const float4*>(stage + row * kEpiPitchWide + col);
+        const float4 b = *reinterpret_cast<const float4*>(stage + row * kEpiPitchWide + col + 4);
+        float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        Pack<T, 8> p;
+        if (e.residual) {
+            memcpy(&p, &r.w[i], 16);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += to_float(p.e[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p.e[j] = from_float<T>(v[j]);
+        *reinterpret_cast<Pack<T, 8>*>(static_cast<T*>(y) + (size_t)(row0 + row) * (size_t)n + col0 + col) = p;
+    }
+}
+__device__ __forceinline__ void epi_finish_wide(const Epilogue& e, void* y, int n, int row0, int rows, int col0,
+                                                const float (&v)[16], const EpiWide& r, float* stage) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();  // the block before has been read
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4*>(stage + lane * kEpiPitchWide + 4 * j) =
+            make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    __syncwarp();
+    if (e.dtype == ZQ_DTYPE_F16) return epi_put_halves<__half>(e, y, n, row0, rows, col0, r, stage);
+    if (e.dtype == ZQ_DTYPE_BF16) return epi_put_halves<__nv_bfloat16>(e, y, n, row0, rows, col0, r, stage);
+    const int col = 4 * (lane & 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2);
+        if (row >= rows) continue;
+        float4 o = *reinterpret_cast<const float4*>(stage + row * kEpiPitchWide + col);
+        if (e.residual) {
+            o.x += __uint_as_float(r.w[i].x);
+            o.y += __uint_as_float(r.w[i].y);
+            o.z += __uint_as_float(r.w[i].z);
+            o.w += __uint_as_float(r.w[i].w);
+        }
+        *reinterpret_cast<float4*>(static_cast<float*>(y) + (size_t)(row0 + row) * (size_t)n + col0 + col) = o;
+    }
 }
 
 // 16 consecutive elements of a row on the 16-byte grid: raw residual words

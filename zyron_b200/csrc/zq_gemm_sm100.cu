@@ -61,22 +61,39 @@ namespace {
 constexpr int kBM = 128;
 constexpr int kBK = 128;  // bytes == int8 codes per k-block (one 128 B swizzle row)
 constexpr int kUmmaK = 32;
-constexpr int kThreads = 192;
-constexpr int kEpilogueThreads = 128;
 constexpr int kUnpackThreads = 512;  // warps 6..21 of an INT4-weight kernel (two per slot: 0.95x)
 constexpr int kUnpackWarps = kUnpackThreads / 32;
 constexpr int kSlots = 4;              // packed + unpacked B tiles of an INT4-weight kernel
 constexpr int kSlotWarps = kUnpackWarps / kSlots;  // unpack warps per slot
+// Where the output goes.  kGatherOut: to several GPUs' buffers (the all-gather
+// fused into the matmul).  A separate instantiation keeps the single-destination
+// epilogue lean: the gather path's staging roughly doubles the epilogue
+// warps' registers and costs the plain matmul about 8 % when compiled in.
+// kEpilogueOut: one output through activation, residual and a stored type.
+enum OutKind : int { kPlain = 0, kGatherOut = 1, kEpilogueOut = 2 };
+// Epilogue warps: one per TMEM lane quarter, or (kEpilogueOut of INT8 weights) two
+// that halve the columns between them.  A single warp's chain of loads, products
+// and stores was what short k took its time from: 4096 x 4096 x 11008 to bf16
+// with bias and gelu 199 us.  The INT4 kernels have no registers for four more.
+template <int kOut, bool kW4>
+constexpr int kEpiWarps = kOut == kEpilogueOut && !kW4 ? 8 : 4;
+template <int kOut, bool kW4>
+constexpr int threads_for() { return 64 + 32 * kEpiWarps<kOut, kW4> + (kW4 ? kUnpackThreads : 0); }
+// kEpilogueOut: a staging block a warp (INT4: for rows off the 16-byte grid alone).
 template <bool kW4>
-constexpr int threads_for() { return kW4 ? kThreads + kUnpackThreads : kThreads; }
+constexpr int kEpiStageFloats = 32 * (kW4 ? kEpiPitch16 : kEpiPitchWide);
+template <int kOut, bool kW4>
+constexpr int kEpiStageBytes = kOut == kEpilogueOut ? kEpiWarps<kOut, kW4> * kEpiStageFloats<kW4> * 4 : 0;
 // The 2-SM kernel's INT4 slots: four unpack warps each; the gathering kernel
 // keeps four slots beside its epilogue staging, the plain one takes one more
 // (8192 x 8192 x 16384: 2273 TOPS against 2057 with four).
 constexpr int kPairSlotsGather = 4, kPairSlotsPlain = 5;
 template <bool kW4, bool kGather>
 constexpr int pair_slots() { return kW4 ? (kGather ? kPairSlotsGather : kPairSlotsPlain) : kSlots; }
-template <bool kW4, bool kGather>
-constexpr int pair_threads() { return kW4 ? kThreads + 32 * kSlotWarps * pair_slots<kW4, kGather>() : kThreads; }
+template <bool kW4, int kOut>
+constexpr int pair_threads() {
+    return 64 + 32 * kEpiWarps<kOut, kW4> + (kW4 ? 32 * kSlotWarps * pair_slots<kW4, kOut == kGatherOut>() : 0);
+}
 
 // An accumulator word: the int32 dot, or (INT4 weights unpacked as 16 x the
 // code, see unpack_stage) 16 x the dot, shifted back exactly.
@@ -264,21 +281,29 @@ __device__ __forceinline__ void store_tile_rows(uint32_t taddr, int row, bool ro
         if (vec_ok && n0 + 32 <= N) {
             const float4* b4 = bias ? reinterpret_cast<const float4*>(bias + n0) : nullptr;
             float4* dst = reinterpret_cast<float4*>(yrow + n0);
+            // Products and sums without the reference's NaN rules, 32 at a time
+            // with no branch between them (a branch an operation kept them one
+            // behind the other: 4096 x 4096 x 11008 took 203 us); where one is a
+            // NaN, the four it lies in are formed again by the rules.
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const float4 s = __ldg(cs4 + j);
-                float4 o;
+                float4 o = make_float4(epi_value(acc_of(r[4 * j + 0], shift), sr, s.x),
+                                       epi_value(acc_of(r[4 * j + 1], shift), sr, s.y),
+                                       epi_value(acc_of(r[4 * j + 2], shift), sr, s.z),
+                                       epi_value(acc_of(r[4 * j + 3], shift), sr, s.w));
+                float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (b4) {
-                    const float4 b = __ldg(b4 + j);
-                    o.x = zq_epilogue_bias(acc_of(r[4 * j + 0], shift), sr, s.x, b.x);
-                    o.y = zq_epilogue_bias(acc_of(r[4 * j + 1], shift), sr, s.y, b.y);
-                    o.z = zq_epilogue_bias(acc_of(r[4 * j + 2], shift), sr, s.z, b.z);
-                    o.w = zq_epilogue_bias(acc_of(r[4 * j + 3], shift), sr, s.w, b.w);
-                } else {
-                    o.x = zq_epilogue(acc_of(r[4 * j + 0], shift), sr, s.x);
-                    o.y = zq_epilogue(acc_of(r[4 * j + 1], shift), sr, s.y);
-                    o.z = zq_epilogue(acc_of(r[4 * j + 2], shift), sr, s.z);
-                    o.w = zq_epilogue(acc_of(r[4 * j + 3], shift), sr, s.w);
+                    b = __ldg(b4 + j);
+                    o = make_float4(__fadd_rn(o.x, b.x), __fadd_rn(o.y, b.y), __fadd_rn(o.z, b.z), __fadd_rn(o.w, b.w));
+                }
+                if (isnan(o.x) | isnan(o.y) | isnan(o.z) | isnan(o.w)) {
+                    const int32_t a0 = acc_of(r[4 * j + 0], shift), a1 = acc_of(r[4 * j + 1], shift),
+                                  a2 = acc_of(r[4 * j + 2], shift), a3 = acc_of(r[4 * j + 3], shift);
+                    o = b4 ? make_float4(zq_epilogue_bias(a0, sr, s.x, b.x), zq_epilogue_bias(a1, sr, s.y, b.y),
+                                         zq_epilogue_bias(a2, sr, s.z, b.z), zq_epilogue_bias(a3, sr, s.w, b.w))
+                           : make_float4(zq_epilogue(a0, sr, s.x), zq_epilogue(a1, sr, s.y), zq_epilogue(a2, sr, s.z),
+                                         zq_epilogue(a3, sr, s.w));
                 }
                 dst[j] = o;
             }
@@ -297,65 +322,73 @@ __device__ __forceinline__ void store_tile_rows(uint32_t taddr, int row, bool ro
 }
 
 // The plain output through the matmul's epilogue (zq_epilogue.cuh), 16 columns
-// of the thread's row at a time: the residual's words of the next 16 are on
-// their way while these are finished, and 16 instead of 32 keep the INT4
-// kernels' epilogue warps within their 72 registers.
-template <int BN>
-__device__ __forceinline__ void store_tile_rows_epi(uint32_t taddr, int row, bool row_ok, int nbase, int N, float sr,
+// of the thread's row at a time: columns [0, kCols) of the tile from nbase on.
+// kAhead: the residual's words, the scales and the biases are on their way while
+// the accumulators come, and rows are turned around in shared memory; without
+// (INT4 kernels have neither the registers nor the shared memory) words are
+// loaded where they are used, and a thread stores its own row.
+template <int kCols, bool kAhead>
+__device__ __forceinline__ void store_tile_rows_epi(uint32_t taddr, int row, int M, int nbase, int N, float sr,
                                                     const float* __restrict__ col_scale,
                                                     const float* __restrict__ bias, void* y, const Epilogue& e,
-                                                    bool vec_ok, int shift) {
+                                                    bool vec_ok, int shift, float* stage) {
+    const bool row_ok = row < M;
+    const int lane = threadIdx.x & 31;
     const size_t yrow = (size_t)(row_ok ? row : 0) * (size_t)N;
     const size_t rrow = (size_t)(row_ok ? row : 0) * (size_t)e.ld_residual;
-    const bool ahead = row_ok && vec_ok && e.residual;
-    Epi16 next;
-    if (ahead && nbase + 16 <= N) epi_load16(e, rrow + nbase, next);
+    const int row0 = row - lane;
+    const bool wide_res = vec_ok && e.residual;
+    // 16 values of a row vector of the columns, zeros behind the last
+    const auto load16 = [&](const float* p, int n0, float (&to)[16]) {
+        if (vec_ok && n0 + 16 <= N) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 t = __ldg(reinterpret_cast<const float4*>(p + n0) + j);
+                to[4 * j] = t.x, to[4 * j + 1] = t.y, to[4 * j + 2] = t.z, to[4 * j + 3] = t.w;
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) to[j] = n0 + j < N ? __ldg(p + n0 + j) : 0.0f;
+        }
+    };
+    EpiWide next;
+    if (kAhead && wide_res && nbase + 16 <= N) epi_load_wide(e, row0, M - row0, nbase, next);
 #pragma unroll 1
-    for (int c = 0; c < BN / 16; ++c) {
+    for (int c = 0; c < kCols / 16; ++c) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(taddr + c * 16, r);
         const int n0 = nbase + c * 16;
-        const Epi16 res = next;
-        if (ahead && c + 1 < BN / 16 && n0 + 32 <= N) epi_load16(e, rrow + n0 + 16, next);
+        float s[16], b[16];
+        EpiWide res;
+        if constexpr (kAhead) {
+            load16(col_scale, n0, s);
+            if (bias) load16(bias, n0, b);
+            res = next;
+            if (wide_res && c + 1 < kCols / 16 && n0 + 32 <= N) epi_load_wide(e, row0, M - row0, n0 + 16, next);
+        }
         tmem_ld_wait();
-        if (!row_ok || n0 >= N) continue;
-        if (vec_ok && n0 + 16 <= N) {
-            const float4* cs4 = reinterpret_cast<const float4*>(col_scale + n0);
-            float v[16];
+        if (n0 >= N) break;
+        if constexpr (!kAhead) load16(col_scale, n0, s);
+        float v[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 s = __ldg(cs4 + j);
-                v[4 * j] = zq_epilogue(acc_of(r[4 * j], shift), sr, s.x);
-                v[4 * j + 1] = zq_epilogue(acc_of(r[4 * j + 1], shift), sr, s.y);
-                v[4 * j + 2] = zq_epilogue(acc_of(r[4 * j + 2], shift), sr, s.z);
-                v[4 * j + 3] = zq_epilogue(acc_of(r[4 * j + 3], shift), sr, s.w);
-            }
-            if (bias) {
-                const float4* b4 = reinterpret_cast<const float4*>(bias + n0);
+        for (int j = 0; j < 16; ++j) v[j] = epi_value(acc_of(r[j], shift), sr, s[j]);
+        if (bias) {
+            if constexpr (!kAhead) load16(bias, n0, b);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float4 b = __ldg(b4 + j);
-                    v[4 * j] += b.x;
-                    v[4 * j + 1] += b.y;
-                    v[4 * j + 2] += b.z;
-                    v[4 * j + 3] += b.w;
-                }
+            for (int j = 0; j < 16; ++j) v[j] += b[j];
+        }
+        epi_activate(e.activation, v);
+        if (!vec_ok || n0 + 16 > N) {
+            epi_finish_block(e, y, N, row0, M - row0, n0, v, stage);
+        } else if constexpr (kAhead) {
+            epi_finish_wide(e, y, N, row0, M - row0, n0, v, res, stage);
+        } else if (row_ok) {
+            if (e.residual) {
+                Epi16 w;
+                epi_load16(e, rrow + n0, w);
+                epi_add16(e, w, v);
             }
-            epi_activate(e.activation, v);
-            if (e.residual) epi_add16(e, res, v);
             epi_store16(e, y, yrow + n0, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int n = n0 + j;
-                if (n < N) {
-                    float v[1] = {zq_epilogue(acc_of(r[j], shift), sr, __ldg(col_scale + n))};
-                    if (bias) v[0] += __ldg(bias + n);
-                    epi_activate(e.activation, v);
-                    if (e.residual) v[0] += epi_residual(e, rrow + n);
-                    epi_store(e, y, yrow + n, v[0]);
-                }
-            }
         }
     }
 }
@@ -373,14 +406,8 @@ __device__ __forceinline__ void tile_coords(int t, int m_tiles, int n_tiles, int
     nt = r / gm;
 }
 
-// Where the output goes.  kGather: to several GPUs' buffers (the all-gather
-// fused into the matmul).  A separate instantiation keeps the single-destination
-// epilogue lean: the gather path's staging roughly doubles the epilogue
-// warps' registers and costs the plain matmul about 8 % when compiled in.
-// kEpilogue: one output through activation, residual and a stored type.
-enum OutKind : int { kPlain = 0, kGatherOut = 1, kEpilogueOut = 2 };
 template <int BN, int STAGES, int kOut, bool kW4>
-__global__ void __launch_bounds__(threads_for<kW4>(), 1)
+__global__ void __launch_bounds__((threads_for<kOut, kW4>()), 1)
     gemm_i8_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                    int M, int N, int Kp, const float* __restrict__ row_scale,
                    const float* __restrict__ col_scale, const float* __restrict__ bias,
@@ -428,7 +455,7 @@ __global__ void __launch_bounds__(threads_for<kW4>(), 1)
             }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
-            mbar_init(&tempty[a], kEpilogueThreads);
+            mbar_init(&tempty[a], 32 * kEpiWarps<kOut, kW4>);
         }
         mbar_init(mma_done, 1);
         fence_mbar_init();
@@ -580,8 +607,11 @@ __global__ void __launch_bounds__(threads_for<kW4>(), 1)
             const float sr = row < M ? load_l2(row_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * BN);
             if constexpr (kOut == kEpilogueOut) {
-                store_tile_rows_epi<BN>(taddr, row, row < M, nt * BN, N, sr, col_scale, bias, out.base[0], out.epi, vec1,
-                                        shift);
+                constexpr int kSplit = kEpiWarps<kOut, kW4> / 4, kCols = BN / kSplit;
+                const int part = (warp - 2) / 4;
+                store_tile_rows_epi<kCols, !kW4>(taddr + part * kCols, row, M, nt * BN + part * kCols, N, sr, col_scale, bias,
+                                           out.base[0], out.epi, vec1, shift,
+                                           epi_stage + (warp - 2) * kEpiStageFloats<kW4>);
             } else if constexpr (!kGather) {
                 store_tile_rows<BN>(taddr, row, row < M, nt * BN, N, sr, col_scale, bias, out.base[0], vec1, shift);
             } else {
@@ -628,7 +658,8 @@ cudaError_t launch_gemm_t(const GemmArgs& a, cudaStream_t stream, bool pdl) {
     auto kern = gather        ? gemm_i8_kernel<BN, STAGES, kGatherOut, kW4>
                 : a.out.epi.on ? gemm_i8_kernel<BN, STAGES, kEpilogueOut, kW4>
                                : gemm_i8_kernel<BN, STAGES, kPlain, kW4>;
-    const int smem = S::kTotal + (gather ? kEpiBytes : 0);
+    static_assert(S::kTotal + kEpiStageBytes<kEpilogueOut, kW4> <= 227 * 1024, "shared memory of the epilogue kernel");
+    const int smem = S::kTotal + (gather ? kEpiBytes : a.out.epi.on ? kEpiStageBytes<kEpilogueOut, kW4> : 0);
     cudaError_t e = ensure_smem_attr(kern, smem);
     if (e != cudaSuccess) return e;
     const int sms = sm_count(a.reserved_sms);
@@ -637,7 +668,7 @@ cudaError_t launch_gemm_t(const GemmArgs& a, cudaStream_t stream, bool pdl) {
 
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(threads_for<kW4>());
+    cfg.blockDim = dim3(a.out.epi.on && !gather ? threads_for<kEpilogueOut, kW4>() : threads_for<kPlain, kW4>());
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -742,7 +773,7 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar) {
 }
 
 template <int kOut, bool kW4>
-__global__ void __launch_bounds__((pair_threads<kW4, kOut == kGatherOut>()), 1)
+__global__ void __launch_bounds__((pair_threads<kW4, kOut>()), 1)
     gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
                         int M, int N, int Kp, const float* __restrict__ row_scale,
                         const float* __restrict__ col_scale, const float* __restrict__ bias,
@@ -797,7 +828,7 @@ __global__ void __launch_bounds__((pair_threads<kW4, kOut == kGatherOut>()), 1)
             }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&tfull[a], 1);
-            mbar_init(&tempty[a], 2 * kEpilogueThreads);  // both CTAs' epilogue threads
+            mbar_init(&tempty[a], 2 * 32 * kEpiWarps<kOut, kW4>);  // both CTAs' epilogue threads
         }
         mbar_init(mma_done, 1);
         fence_mbar_init();
@@ -958,8 +989,11 @@ __global__ void __launch_bounds__((pair_threads<kW4, kOut == kGatherOut>()), 1)
             const float sr = row < M ? load_l2(row_scale + row) : 0.0f;
             const uint32_t taddr = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(acc * 256);
             if constexpr (kOut == kEpilogueOut) {
-                store_tile_rows_epi<256>(taddr, row, row < M, nt * 256, N, sr, col_scale, bias, out.base[0], out.epi,
-                                         vec1, shift);
+                constexpr int kSplit = kEpiWarps<kOut, kW4> / 4, kCols = 256 / kSplit;
+                const int part = (warp - 2) / 4;
+                store_tile_rows_epi<kCols, !kW4>(taddr + part * kCols, row, M, nt * 256 + part * kCols, N, sr, col_scale, bias,
+                                           out.base[0], out.epi, vec1, shift,
+                                           epi_stage + (warp - 2) * kEpiStageFloats<kW4>);
             } else if constexpr (!kGather) {
                 store_tile_rows<256>(taddr, row, row < M, nt * 256, N, sr, col_scale, bias, out.base[0], vec1, shift);
             } else {
@@ -999,7 +1033,10 @@ cudaError_t launch_gemm_pair(const GemmArgs& a, cudaStream_t stream, bool pdl) {
     auto kern = gather        ? gemm_i8_pair_kernel<kGatherOut, kW4>
                 : a.out.epi.on ? gemm_i8_pair_kernel<kEpilogueOut, kW4>
                                : gemm_i8_pair_kernel<kPlain, kW4>;
-    const int smem = gather ? Smem2<kW4, true>::kTotal + kEpiBytes : Smem2<kW4, false>::kTotal;
+    static_assert(Smem2<kW4, false>::kTotal + kEpiStageBytes<kEpilogueOut, kW4> <= 227 * 1024,
+                  "shared memory of the epilogue kernel");
+    const int smem = gather ? Smem2<kW4, true>::kTotal + kEpiBytes
+                            : Smem2<kW4, false>::kTotal + (a.out.epi.on ? kEpiStageBytes<kEpilogueOut, kW4> : 0);
     cudaError_t e = ensure_smem_attr(kern, smem);
     if (e != cudaSuccess) return e;
     const int sms = sm_count(a.reserved_sms);
@@ -1009,7 +1046,9 @@ cudaError_t launch_gemm_pair(const GemmArgs& a, cudaStream_t stream, bool pdl) {
     if (clusters > tiles) clusters = tiles;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(2 * clusters);
-    cfg.blockDim = dim3(gather ? pair_threads<kW4, true>() : pair_threads<kW4, false>());
+    cfg.blockDim = dim3(gather        ? pair_threads<kW4, kGatherOut>()
+                        : a.out.epi.on ? pair_threads<kW4, kEpilogueOut>()
+                                       : pair_threads<kW4, kPlain>());
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];

@@ -17,13 +17,14 @@
 #include "zq_kernels.h"
 
 #include <cstdint>
+#include <type_traits>
 
 namespace zq {
 
 // ---------------------------------------------------------------------------
-// Per-row dynamic activation quantizer (quantization.cpp:202-212).
-// One warp per row: pass 1 reduces |x| with fmaxf (NaN skipped, like
-// std::max), pass 2 writes codes; the [K, Kp) tail is zero-filled.
+// Per-row dynamic activation quantizer (quantization.cpp:202-212): the largest
+// |x| by fmaxf (NaN skipped, like std::max), then the codes; the [K, Kp) tail is
+// zero-filled.
 // ---------------------------------------------------------------------------
 // Block 0 also clears `zero[0, n_zero)` (see launch_quantize_rows).
 __device__ __forceinline__ void clear_words(int* zero, int n_zero) {
@@ -31,51 +32,64 @@ __device__ __forceinline__ void clear_words(int* zero, int n_zero) {
         for (int i = threadIdx.x; i < n_zero; i += blockDim.x) zero[i] = 0;
 }
 
-// Reads x twice, the second time from L1 where the row fits: neither starts
-// early nor lets others (launch_kernel).
-template <bool kVec>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const float* __restrict__ x, int M, int K,
-                                                            int Kp, int8_t* __restrict__ q,
-                                                            float* __restrict__ row_scale, int* zero, int n_zero) {
-    clear_words(zero, n_zero);
-    const int warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;
-    const int lane = threadIdx.x & 31;
-    if (warp >= M) return;
-    const float* xr = x + (size_t)warp * K;
-    int8_t* qr = q + (size_t)warp * Kp;
+__device__ __forceinline__ uint32_t code_word(const float4& v, float s, float rcp) {
+    return (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.x, s, rcp, 127) |
+           ((uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.y, s, rcp, 127) << 8) |
+           ((uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.z, s, rcp, 127) << 16) |
+           ((uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.w, s, rcp, 127) << 24);
+}
 
+// Rows longer than a group of warps holds below, or off the 16-byte grid (kVec
+// false: element by element): a block of kT threads a row, the first 32
+// elements of each thread in registers, the rest read again.  One warp a row
+// took 44 us for 12 rows of 11008.
+template <int kT, bool kVec>
+__global__ void __launch_bounds__(kT) quantize_long_rows_kernel(const float* __restrict__ x, int K, int Kp,
+                                                                int8_t* __restrict__ q, float* __restrict__ row_scale,
+                                                                int* zero, int n_zero) {
+    pdl_launch_dependents();
+    pdl_wait_primary();  // x may come from, and q / counters be read by, the kernels before
+    clear_words(zero, n_zero);
+    using V = typename std::conditional<kVec, float4, float>::type;
+    constexpr int kHeld = 128 / (int)sizeof(V);
+    __shared__ float part[kT / 32];
+    const int t = threadIdx.x;
+    const V* xr = reinterpret_cast<const V*>(x + (size_t)blockIdx.x * K);
+    int8_t* qr = q + (size_t)blockIdx.x * Kp;
+    const int n = kVec ? K >> 2 : K;
+    const auto largest = [](const V& v, float m) {
+        if constexpr (kVec)
+            return fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+        else
+            return fmaxf(m, fabsf(v));
+    };
+    V v[kHeld];
     float m = 0.0f;
-    if (kVec) {
-        const float4* x4 = reinterpret_cast<const float4*>(xr);
-        for (int i = lane; i < (K >> 2); i += 32) {
-            const float4 v = __ldg(x4 + i);
-            m = fmaxf(m, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
-        }
-    } else {
-        for (int i = lane; i < K; i += 32) m = fmaxf(m, fabsf(__ldg(xr + i)));
-    }
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) v[i] = t + i * kT < n ? load_l2(xr + t + i * kT) : V{};
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) m = largest(v[i], m);
+    for (uint32_t i = t + kHeld * kT; i < (uint32_t)n; i += kT) m = largest(load_l2(xr + i), m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((t & 31) == 0) part[t >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kT / 32; ++w) m = fmaxf(m, part[w]);
     const float s = zq_scale_from_absmax(m, 127.0f);
-    if (lane == 0) row_scale[warp] = s;
+    if (t == 0) row_scale[blockIdx.x] = s;
     const float rcp = zq_quant_rcp(s);
-
-    if (kVec) {
-        const float4* x4 = reinterpret_cast<const float4*>(xr);
-        uint32_t* q4 = reinterpret_cast<uint32_t*>(qr);
-        for (int i = lane; i < (K >> 2); i += 32) {
-            const float4 v = __ldg(x4 + i);
-            const uint32_t b0 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.x, s, rcp, 127);
-            const uint32_t b1 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.y, s, rcp, 127);
-            const uint32_t b2 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.z, s, rcp, 127);
-            const uint32_t b3 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v.w, s, rcp, 127);
-            q4[i] = b0 | (b1 << 8) | (b2 << 16) | (b3 << 24);
-        }
-        for (int i = (K >> 2) + lane; i < (Kp >> 2); i += 32) q4[i] = 0u;
-    } else {
-        for (int i = lane; i < K; i += 32) qr[i] = (int8_t)zq_quantize_value_rcp(__ldg(xr + i), s, rcp, 127);
-        for (int i = K + lane; i < Kp; i += 32) qr[i] = 0;
-    }
+    const auto put = [&](uint32_t i, const V& e) {
+        if constexpr (kVec)
+            reinterpret_cast<uint32_t*>(qr)[i] = code_word(e, s, rcp);
+        else
+            qr[i] = (int8_t)zq_quantize_value_rcp(e, s, rcp, 127);
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+        if (t + i * kT < n) put(t + i * kT, v[i]);
+    for (uint32_t i = t + kHeld * kT; i < (uint32_t)n; i += kT) put(i, load_l2(xr + i));
+    for (uint32_t i = (uint32_t)K + t; i < (uint32_t)Kp; i += kT) qr[i] = 0;
 }
 
 // Register-resident variant: a row is held by kWarpsPerRow warps, each lane
@@ -127,11 +141,7 @@ __global__ void __launch_bounds__(256) quantize_rows_reg_kernel(const float* __r
     for (int i = 0; i < kVec; ++i) {
         const int idx = t + i * kT;
         if (idx < k4) {
-            const uint32_t b0 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v[i].x, s, rcp, 127);
-            const uint32_t b1 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v[i].y, s, rcp, 127);
-            const uint32_t b2 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v[i].z, s, rcp, 127);
-            const uint32_t b3 = (uint32_t)(uint8_t)(int8_t)zq_quantize_value_rcp(v[i].w, s, rcp, 127);
-            q4[idx] = b0 | (b1 << 8) | (b2 << 16) | (b3 << 24);
+            q4[idx] = code_word(v[i], s, rcp);
         }
     }
     for (int i = k4 + t; i < (Kp >> 2); i += kT) q4[i] = 0u;
@@ -159,15 +169,15 @@ cudaError_t launch_quantize_rows(const float* x, int M, int K, int Kp, int8_t* q
                                               Kp, q, row_scale, zero, n_zero);
         }
     }
-    const int rows_per_block = 8;
-    const dim3 grid((M + rows_per_block - 1) / rows_per_block);
-    const bool vec = (K % 4 == 0) && (Kp % 4 == 0) && ((reinterpret_cast<uintptr_t>(x) & 15u) == 0) &&
-                     ((reinterpret_cast<uintptr_t>(q) & 3u) == 0);
-    if (vec)
-        return launch_kernel(false, quantize_rows_kernel<true>, grid, dim3(256), 0, stream, x, M, K, Kp, q, row_scale,
-                             zero, n_zero);
-    return launch_kernel(false, quantize_rows_kernel<false>, grid, dim3(256), 0, stream, x, M, K, Kp, q, row_scale,
-                         zero, n_zero);
+    const auto launch = [&](auto kern, int threads) {
+        return launch_pdl_kernel(kern, dim3(M), dim3(threads), 0, stream, x, K, Kp, q, row_scale, zero, n_zero);
+    };
+    if (K <= 8192) return launch(quantize_long_rows_kernel<256, false>, 256);
+    if (K <= 16384)
+        return aligned ? launch(quantize_long_rows_kernel<512, true>, 512)
+                       : launch(quantize_long_rows_kernel<512, false>, 512);
+    return aligned ? launch(quantize_long_rows_kernel<1024, true>, 1024)
+                   : launch(quantize_long_rows_kernel<1024, false>, 1024);
 }
 
 // ---------------------------------------------------------------------------
