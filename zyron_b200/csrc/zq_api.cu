@@ -709,6 +709,21 @@ zq_status set_error(zq_status s, const char* msg) { return fail(s, msg); }
 
 zq_status device_error_word(uint32_t** out) { return device_error_ptr(out); }
 
+zq_status encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                       const uint64_t* pitches, const uint32_t* box) {
+    zq_status s = get_encoder();
+    if (s != ZQ_OK) return s;
+    cuuint64_t d[5], p[4];
+    cuuint32_t b[5], one[5];
+    for (int i = 0; i < rank; ++i) d[i] = dims[i], b[i] = box[i], one[i] = 1u;
+    for (int i = 0; i + 1 < rank; ++i) p[i] = pitches[i];
+    const CUresult r = g_encode(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, p, b, one,
+                                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(ZQ_ERR_CUDA, "zyron_b200: cuTensorMapEncodeTiled failed");
+    return ZQ_OK;
+}
+
 zq_status parse_zyq(const void* bytes, size_t len, ZyqRecord* rec) {
     const uint8_t* p = static_cast<const uint8_t*>(bytes);
     size_t off = 0;

@@ -8,23 +8,23 @@
 // m, sum and output in fp32, in base 2.
 //
 // Split.  A request's rows of one kv head -- its new tokens times the heads of
-// the group, which all read the same keys -- make an item (in tiles of kRows
-// rows); the shared prefix is one more request whose rows are all the call's
-// rows.  Items are cut into units of 64 keys, and every block takes an equal run
-// of units, whatever the lengths are: it finds its run by a scan over the
-// requests' lengths, so the plan lives on the device and a captured call follows
-// the lengths of its replay.  A block's run covers whole items and at most two
-// parts of items, whose sums it leaves in a slot of its own; a second kernel
-// joins the parts of each item that a border cuts.  With a prefix, own and
-// prefix results stay in fp32 with their maxima and sums, and a third joins the
-// two.
+// the group, which all read the same keys -- make an item (more than 256 rows:
+// several); the shared prefix is one more request whose rows are all the call's
+// rows.  Every block takes an equal run of the items' key tiles, whatever the
+// lengths are: it finds its run by a scan over the requests, so the plan lives on
+// the device and a captured call follows the lengths of its replay.  A run covers
+// whole items and at most two parts of items, whose sums it leaves in a slot of
+// its own; a second kernel joins the parts of each item that a border cuts.  With
+// a prefix, own and prefix results stay in fp32 with their maxima and sums, and a
+// third joins the two.
 //
-// Bound: a decode batch reads its cache once, memory bandwidth.  A warp streams
-// its own 16 keys of a unit through a ring of cp.async stages, so that no
-// barrier stands between the memory and the products; q stays in registers; the
-// products are mma.sync, which at 16 rows take 4 of the 22 cycles a key's bytes
-// take an SM.  exp(s - m) enters the second product as a sum of two 16-bit
-// parts, so that it is not rounded to the cache's type.
+// Items of many rows are matrix products for tcgen05 (zq_attention_sm100.cu).
+// This file has the kernel of few rows -- single tokens, drafts: a decode batch
+// reads its cache once, memory bandwidth.  A warp streams its own 16 keys of 64
+// through a ring of cp.async stages, so that no barrier stands between the memory
+// and the products; the products are mma.sync, which at 16 rows take 4 of the 22
+// cycles that a key's bytes take an SM.  exp(s - m) enters the second product as
+// a sum of two 16-bit parts, so that it is not rounded to the cache's type.
 #include "zq_attention.cuh"
 
 namespace zq {
@@ -37,8 +37,10 @@ constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kSlice = 16;              // keys of a warp's stage
 constexpr int kUnit = kSlice * kWarps;  // keys of a unit
+static_assert(kUnit == FewPlan::kKeys, "a unit is one round of the warps");
 constexpr int kStages = 3;
 constexpr int kBlocksPerSm = 2;
+constexpr int kJoinThreads = 256;
 
 template <int kD>
 constexpr int kStageBytes = kSlice * kD * 2 * 2;  // keys, then values
@@ -93,90 +95,16 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ---- the plan ------------------------------------------------------------------
-
-// Units of one request: tiles of rows x kv heads x units of keys.  At least one
-// unit of keys, so that rows that see none are written too.
-template <int kRows>
-struct Plan {
-    const AttentionArgs& a;
-    int group;        // heads of a kv head
-    int prefix_rows;  // rows of the call that have the prefix, 0: not in this plan
-
-    __device__ __forceinline__ int tiles(int rows) const { return (int)(((long long)rows * group + kRows - 1) / kRows); }
-    __device__ __forceinline__ int units(int keys) const { return keys > 0 ? (keys - 1) / kUnit + 1 : 1; }
-    __device__ __forceinline__ long long cost(const Request& r) const {
-        return (long long)tiles(r.rows) * a.batch.kv_heads * units(r.length);
-    }
-    __device__ __forceinline__ Request get(int b) const {
-        if (b >= 0) return load_request(a.batch, b);
-        return Request{0, prefix_rows, a.prefix_length};  // the prefix: request -1
-    }
-};
-
-struct Found {
-    long long total;  // units of the call
-    long long before; // units before request b
-    int b;
-};
-
-// The request that holds unit (total * num / den), by a scan of the whole block.
-// Every thread gets the result; `scratch` is kThreads / 32 + 4 words of 64 bits.
-template <int kRows>
-__device__ Found find_unit(const Plan<kRows>& plan, long long num, long long den, long long* scratch) {
-    const int n = plan.a.batch.requests;
-    const int each = (n + kThreads - 1) / kThreads;
-    const int first = threadIdx.x * each, last = min(first + each, n);
-    long long mine = 0;
-    for (int b = first; b < last; ++b) mine += plan.cost(plan.get(b));
-    const long long head = plan.prefix_rows ? plan.cost(plan.get(-1)) : 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long sum = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += v;
-    }
-    if (lane == 31) scratch[warp] = sum;
-    __syncthreads();
-    long long total = head, before = head + sum - mine;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += scratch[w];
-        total += scratch[w];
-    }
-    const long long unit = total * num / den;
-    if (threadIdx.x == 0) {
-        scratch[kWarps] = 0;
-        scratch[kWarps + 1] = unit < head ? -1 : n;
-    }
-    __syncthreads();
-    if (unit >= before && unit < before + mine) {
-        int b = first;
-        long long c = plan.cost(plan.get(b));
-        while (unit >= before + c) {
-            before += c;
-            c = plan.cost(plan.get(++b));
-        }
-        scratch[kWarps] = before;
-        scratch[kWarps + 1] = b;
-    }
-    __syncthreads();
-    const Found f{total, scratch[kWarps], (int)scratch[kWarps + 1]};
-    __syncthreads();
-    return f;
-}
-
 // ---- the kernel -----------------------------------------------------------------
 
 // kMT: 16-row tiles of an item's kRows = 16 kMT rows.
 template <class T, int kD, int kMT>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const AttentionArgs a, const Workspace ws) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(const AttentionArgs a, const Workspace ws) {
     constexpr int kRows = 16 * kMT;
     constexpr int kChunks = kD / 8;  // 16-byte chunks of a row
     static_assert(kStages * kStageBytes<kD> >= kRows * (kD + 2) * 4, "a warp's sums fit in its ring");
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long scratch[kWarps + 4];
+    __shared__ long long scratch[kWarps + 2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* ring = smem + warp * kStages * kStageBytes<kD>;
     const uint32_t ring_u = smem_u32(ring);
@@ -187,37 +115,21 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const At
 
     pdl_wait_primary();
     pdl_launch_dependents();
-    Plan<kRows> plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
-    const Found at = find_unit(plan, blockIdx.x, gridDim.x, scratch);
-    const long long u0 = at.total * blockIdx.x / gridDim.x, u1 = at.total * (blockIdx.x + 1) / gridDim.x;
-    if (u0 >= u1) return;
-    int b = at.b;
-    long long before = at.before;
-    Request r = plan.get(b);
+    const FewPlan plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
+    Cursor<FewPlan> way(plan, find_block<kThreads>(plan, blockIdx.x, gridDim.x, scratch), blockIdx.x);
 
-    for (long long u = u0; u < u1;) {
-        // The item of unit u, and the units of it that are this block's.
-        long long cost = plan.cost(r);
-        while (u >= before + cost) {
-            before += cost;
-            r = plan.get(++b);
-            cost = plan.cost(r);
-        }
-        const int units = plan.units(r.length), tiles = plan.tiles(r.rows);
-        const long long item = (u - before) / units;
-        const int c0 = (int)((u - before) - item * units);
-        const int c1 = (int)min((long long)units, c0 + (u1 - u));
-        const int head0 = (int)(item / tiles), tile = (int)(item % tiles);
-        const bool prefix = b < 0;
-        const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)b * p.ld_pages;
-        const int row0 = tile * kRows, item_rows = min(kRows, r.rows * group - row0);
+    while (way.next()) {
+        const Request r = way.it.r;
+        const int c0 = way.first_tile, c1 = way.end_tile, head0 = way.it.head, item_rows = r.rows * group;
+        const bool prefix = way.it.b < 0;
+        const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)way.it.b * p.ld_pages;
 
         // q of the item: row i is token i / group, head i % group of the kv head's.
         for (int i = threadIdx.x; i < kRows * kChunks; i += kThreads) {
             const int row = i / kChunks, c = i % kChunks;
             uint4 v = make_uint4(0, 0, 0, 0);
             if (row < item_rows && c * 8 < dim) {
-                const int token = (row0 + row) / group, head = (row0 + row) % group;
+                const int token = row / group, head = row % group;
                 v = load_l2(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
                                                            (long long)(r.first + token) * a.ldq +
                                                            (long long)(head0 * group + head) * dim + c * 8));
@@ -231,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const At
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int row = row0 + mt * 16 + e * 8 + (lane >> 2);
+                const int row = mt * 16 + e * 8 + (lane >> 2);
                 int n = r.length;
                 if (!prefix && a.causal) n = min(n, max(r.length - r.rows + row / group + 1, 0));
                 limit[mt][e] = n;
@@ -449,8 +361,6 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const At
                 }
             }
         __syncthreads();
-        const bool whole = c0 == 0 && c1 == units;
-        const int slot = u == u0 ? 0 : 1;
         for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
             const int row = i / (kD / 4), d = i % (kD / 4) * 4;
             float most = -INFINITY;
@@ -471,54 +381,36 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_kernel(const At
                 v[3] += x.w * keep;
             }
             if (d >= dim) continue;
-            const int token = (row0 + row) / group, head = head0 * group + (row0 + row) % group;
-            if (!whole)
-                put_part(ws, ((long long)blockIdx.x * 2 + slot) * kRows + row, kD, d, v, most, total);
+            const int token = row / group, head = head0 * group + row % group;
+            if (!way.whole)
+                put_part(ws.part_sums[0], ws.part_stats[0], ((long long)blockIdx.x * 2 + way.slot) * kRows + row, kD, d, v,
+                         most, total);
             else
                 put_row<T>(a, ws, prefix, r.first + token, head, d, v, most, total);
         }
         __syncthreads();  // the sums are read: the rings and q may be written again
-        u += c1 - c0;
     }
 }
 
-// Joins the parts of the item that border blockIdx.x + 1 cuts, if it is the
-// first border inside it.
+// Joins the items that borders of the kernel of few rows (the first few_blocks - 1
+// blocks) and of the other kernel cut.
 template <class T, int kD, int kMT>
-__global__ void __launch_bounds__(kThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int blocks) {
-    constexpr int kRows = 16 * kMT;
-    __shared__ long long scratch[kWarps + 4];
+__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_blocks,
+                                                                 int many_blocks) {
+    __shared__ long long scratch[kJoinThreads / 32 + 2];
     const PagedBatch& p = a.batch;
-    const int group = a.heads / p.kv_heads;
-    const int g = blockIdx.x + 1;
-    // The plan's inputs are older than the kernel before this one, which has
+    const int group = a.heads / p.kv_heads, borders = max(few_blocks - 1, 0);
+    // The plans' inputs are older than the kernel before this one, which has
     // waited for their writers.
-    Plan<kRows> plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
-    const Found at = find_unit(plan, g, blocks, scratch);
-    pdl_launch_dependents();
-    pdl_wait_primary();  // before any return: who waits for this kernel counts on the one before it too
-    const long long u = at.total * g / blocks;
-    if (u >= at.total) return;
-    const Request r = plan.get(at.b);
-    const int units = plan.units(r.length), tiles = plan.tiles(r.rows);
-    const long long item = (u - at.before) / units;
-    const long long start = at.before + item * units, end = start + units;
-    if (u == start || at.total * (g - 1) / blocks > start) return;
-    const int head0 = (int)(item / tiles), tile = (int)(item % tiles);
-    const int row0 = tile * kRows, item_rows = min(kRows, r.rows * group - row0);
-    // Block h's part lies in its first slot, but for the block in whose run the
-    // item begins behind another's units.
-    const int first = at.total * (g - 1) / blocks == start ? 0 : 1;
-    for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
-        const int row = i / (kD / 4), d = i % (kD / 4) * 4;
-        if (d >= p.dim) continue;
-        Joined j;
-        for (int h = g - 1; h < blocks && at.total * h / blocks < end; ++h) {
-            if (at.total * h / blocks == at.total * (h + 1) / blocks) continue;  // a block without units
-            j.add(ws, ((long long)h * 2 + (h == g - 1 ? first : 0)) * kRows + row, kD, d);
-        }
-        const int token = (row0 + row) / group, head = head0 * group + (row0 + row) % group;
-        put_row<T>(a, ws, at.b < 0, r.first + token, head, d, j.v, j.most, j.total);
+    const int prefix_rows = a.prefix_length > 0 ? live_rows(p) : 0;
+    if ((int)blockIdx.x < borders) {
+        const FewPlan plan{a, group, prefix_rows};
+        join_item<T, 16 * kMT, kD, kJoinThreads>(plan, ws, 0, blockIdx.x + 1, few_blocks, 16 * kMT, scratch);
+    } else {
+        const int tokens = kManyRows / 2 / group * 2;
+        const ManyPlan plan{a, group, prefix_rows, tokens};
+        join_item<T, kManyRows, kD, kJoinThreads>(plan, ws, 1, blockIdx.x - borders + 1, many_blocks, tokens * group,
+                                                  scratch);
     }
 }
 
@@ -536,39 +428,64 @@ __global__ void __launch_bounds__(256) join_prefix_kernel(const AttentionArgs a,
         const int head = i / each, d = i % each * 4;
         const long long row = (long long)t * a.heads + head;
         Joined j;
-        j.add_row(ws.row_stats[0], ws.row_sums[0], row, p.dim, d);
-        j.add_row(ws.row_stats[1], ws.row_sums[1], row, p.dim, d);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            j.add(load_l2(reinterpret_cast<const float2*>(ws.row_stats[k]) + row),
+                  load_l2(reinterpret_cast<const float4*>(ws.row_sums[k] + row * p.dim + d)));
         put_out<T>(a, t, head, d, j.v, j.total);
     }
 }
 
+// How a call is launched, from its sizes alone.
+struct Shape {
+    int few_rows;     // 16 or 32: the rows of the kernel of few rows; 0: it has none
+    int few_blocks;
+    int many_blocks;  // 0: no item can have more than few_rows
+    int width;
+};
+Shape shape_of(const AttentionArgs& a) {
+    Shape s{};
+    const int group = a.heads / a.batch.kv_heads;
+    const long long all = (long long)a.batch.rows * group;
+    // the most rows of a kv head that an item may have
+    const long long most = a.batch.starts || a.prefix_length > 0 ? all : group;
+    if (group <= 32) s.few_rows = most <= 16 || (!a.batch.starts && group <= 16) ? 16 : 32;
+    s.few_blocks = s.few_rows ? kBlocksPerSm * sm_count() : 0;
+    s.many_blocks = most > s.few_rows ? sm_count() : 0;
+    s.width = a.batch.dim <= 64 ? 64 : 128;
+    return s;
+}
+
 template <class T, int kD, int kMT>
-cudaError_t launch_t(const AttentionArgs& a, Workspace ws, cudaStream_t stream) {
-    constexpr int smem = kSmemBytes<kD, kMT>;
-    cudaError_t e = ensure_smem_attr(attend_kernel<T, kD, kMT>, smem);
+cudaError_t launch_t(const AttentionArgs& a, int dtype, const Shape& s, const Workspace& ws, cudaStream_t stream) {
+    cudaError_t e = cudaSuccess;
+    if (s.many_blocks) e = launch_attend_many(a, dtype, ws, s.many_blocks, stream);
     if (e != cudaSuccess) return e;
-    const int blocks = kBlocksPerSm * sm_count();
-    e = launch_pdl_kernel(attend_kernel<T, kD, kMT>, dim3(blocks), dim3(kThreads), smem, stream, a, ws);
-    if (e != cudaSuccess) return e;
-    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(blocks - 1), dim3(kThreads), 0, stream, a, ws, blocks);
+    if (s.few_blocks) {
+        constexpr int smem = kSmemBytes<kD, kMT>;
+        e = ensure_smem_attr(attend_few_kernel<T, kD, kMT>, smem);
+        if (e != cudaSuccess) return e;
+        e = launch_pdl_kernel(attend_few_kernel<T, kD, kMT>, dim3(s.few_blocks), dim3(kThreads), smem, stream, a, ws);
+        if (e != cudaSuccess) return e;
+    }
+    const int borders = (s.few_blocks ? s.few_blocks - 1 : 0) + (s.many_blocks ? s.many_blocks - 1 : 0);
+    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(borders), dim3(kJoinThreads), 0, stream, a, ws,
+                          s.few_blocks, s.many_blocks);
     if (e != cudaSuccess || a.prefix_length == 0) return e;
     return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);
 }
 
 template <class T>
-cudaError_t launch_d(const AttentionArgs& a, Workspace ws, cudaStream_t stream) {
-    // 16-row tiles where no item has more rows
-    const int group = a.heads / a.batch.kv_heads;
-    const bool one = a.batch.starts || a.prefix_length > 0 ? (long long)a.batch.rows * group <= 16 : group <= 16;
-    if (a.batch.dim <= 64)
-        return one ? launch_t<T, 64, 1>(a, ws, stream) : launch_t<T, 64, 2>(a, ws, stream);
-    return one ? launch_t<T, 128, 1>(a, ws, stream) : launch_t<T, 128, 2>(a, ws, stream);
+cudaError_t launch_d(const AttentionArgs& a, int dtype, const Shape& s, const Workspace& ws, cudaStream_t stream) {
+    if (s.width == 64)
+        return s.few_rows == 32 ? launch_t<T, 64, 2>(a, dtype, s, ws, stream) : launch_t<T, 64, 1>(a, dtype, s, ws, stream);
+    return s.few_rows == 32 ? launch_t<T, 128, 2>(a, dtype, s, ws, stream) : launch_t<T, 128, 1>(a, dtype, s, ws, stream);
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
 // Lays the workspace out; base null: its size alone.
-Workspace layout(const AttentionArgs& a, uint8_t* base, size_t* bytes) {
+Workspace layout(const AttentionArgs& a, const Shape& s, uint8_t* base, size_t* bytes) {
     Workspace ws{};
     size_t at = 0;
     const auto take = [&](size_t n) {
@@ -576,10 +493,11 @@ Workspace layout(const AttentionArgs& a, uint8_t* base, size_t* bytes) {
         at += align256(n * sizeof(float));
         return p;
     };
-    const size_t parts = (size_t)kBlocksPerSm * sm_count() * 2 * 32;
-    const size_t width = a.batch.dim <= 64 ? 64 : 128;
-    ws.part_sums = take(parts * width);
-    ws.part_stats = take(parts * 2);
+    const size_t parts[2] = {(size_t)s.few_blocks * 2 * s.few_rows, (size_t)s.many_blocks * 2 * kManyRows};
+    for (int k = 0; k < 2; ++k) {
+        ws.part_sums[k] = take(parts[k] * s.width);
+        ws.part_stats[k] = take(parts[k] * 2);
+    }
     if (a.prefix_length > 0) {
         const size_t rows = (size_t)a.batch.rows * a.heads;
         for (int k = 0; k < 2; ++k) {
@@ -595,14 +513,18 @@ Workspace layout(const AttentionArgs& a, uint8_t* base, size_t* bytes) {
 
 size_t attention_workspace_bytes(const AttentionArgs& a) {
     size_t n = 0;
-    layout(a, nullptr, &n);
+    layout(a, shape_of(a), nullptr, &n);
     return n;
 }
 
-cudaError_t launch_paged_attention(const AttentionArgs& a, int dtype, void* workspace, cudaStream_t stream) {
+cudaError_t launch_paged_attention(const AttentionArgs& args, int dtype, void* workspace, cudaStream_t stream) {
+    AttentionArgs a = args;
+    const Shape s = shape_of(a);
+    a.few_rows = s.few_rows;
     size_t n = 0;
-    const Workspace ws = layout(a, static_cast<uint8_t*>(workspace), &n);
-    return dtype == ZQ_DTYPE_F16 ? launch_d<__half>(a, ws, stream) : launch_d<__nv_bfloat16>(a, ws, stream);
+    const Workspace ws = layout(a, s, static_cast<uint8_t*>(workspace), &n);
+    return dtype == ZQ_DTYPE_F16 ? launch_d<__half>(a, dtype, s, ws, stream)
+                                 : launch_d<__nv_bfloat16>(a, dtype, s, ws, stream);
 }
 
 }  // namespace zq

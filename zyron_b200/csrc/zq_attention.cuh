@@ -11,10 +11,10 @@ namespace attn {
 // Sums are kept as the unscaled output row, with the maximum (base 2) that its
 // weights are relative to and their sum.
 struct Workspace {
-    float* part_sums;    // parts of cut items: [block][2][rows of a tile][width]
-    float* part_stats;   // [block][2][rows of a tile][2]
-    float* row_sums[2];  // with a prefix: own and prefix sums of every row, [rows][heads][dim]
-    float* row_stats[2]; // [rows][heads][2]
+    float* part_sums[2];   // parts of cut items of the kernel of few rows and of the other: [block][2][rows][width]
+    float* part_stats[2];  // [block][2][rows][2]
+    float* row_sums[2];    // with a prefix: own and prefix sums of every row, [rows][heads][dim]
+    float* row_stats[2];   // [rows][heads][2]
 };
 
 template <class T>
@@ -66,14 +66,202 @@ __device__ __forceinline__ int live_rows(const PagedBatch& p) {
     return min(max(load_l2(p.starts + p.requests), 0), p.rows);
 }
 
-// Four elements of a part.
-__device__ __forceinline__ void put_part(const Workspace& ws, long long row, int width, int d, const float (&v)[4],
-                                         float most, float total) {
-    *reinterpret_cast<float4*>(ws.part_sums + row * width + d) = make_float4(v[0], v[1], v[2], v[3]);
-    if (d == 0) {
-        ws.part_stats[2 * row] = most;
-        ws.part_stats[2 * row + 1] = total;
+// ---- plans ----------------------------------------------------------------------
+//
+// A plan deals the call's work out to the blocks of one kernel.  Work is counted
+// in units; every block takes `share` consecutive ones.  Items (a tile of a
+// request's rows of one kv head) follow one another, and a place inside an item
+// stands for a border between its key tiles (cut()).
+struct Item {
+    Request r;
+    int b;           // request, -1: the prefix
+    int head;        // kv head
+    int tile;        // tile of rows
+    long long start, end;  // units
+    int key_tiles;
+};
+
+// Requests of at most a.few_rows rows of a kv head: one item a head, units of 64
+// keys, at least one, so that rows that see no key are written too.
+struct FewPlan {
+    static constexpr int kKeys = 64;
+    const AttentionArgs& a;
+    int group, prefix_rows;
+
+    __device__ __forceinline__ Request get(int b) const {
+        return b >= 0 ? load_request(a.batch, b) : Request{0, prefix_rows, a.prefix_length};
     }
+    __device__ __forceinline__ int key_tiles(const Request& r) const { return r.length > 0 ? (r.length - 1) / kKeys + 1 : 1; }
+    __device__ __forceinline__ long long cost(const Request& r) const {
+        return r.rows > 0 && (long long)r.rows * group <= a.few_rows ? (long long)a.batch.kv_heads * key_tiles(r) : 0;
+    }
+    __device__ __forceinline__ Item item(int b, const Request& r, long long before, long long unit) const {
+        const int n = key_tiles(r);
+        const int head = (int)((unit - before) / n);
+        const long long start = before + (long long)head * n;
+        return Item{r, b, head, 0, start, start + n, n};
+    }
+    __device__ __forceinline__ int cut(const Item& it, long long unit) const {
+        return (int)(min(max(unit, it.start), it.end) - it.start);
+    }
+};
+
+// The other requests: tiles of `tokens` tokens, units of a key.  A causal tile
+// sees the more keys the later it comes, so tile t counts base + step t units
+// (one key tile's worth more than its keys: what an item costs besides), and a
+// border is the key tile that lies as far along.
+struct ManyPlan {
+    static constexpr int kKeys = 128;
+    const AttentionArgs& a;
+    int group, prefix_rows;
+    int tokens;
+
+    __device__ __forceinline__ Request get(int b) const {
+        return b >= 0 ? load_request(a.batch, b) : Request{0, prefix_rows, a.prefix_length};
+    }
+    __device__ __forceinline__ bool causal(int b) const { return b >= 0 && a.causal; }
+    __device__ __forceinline__ int tiles(const Request& r) const { return (r.rows + tokens - 1) / tokens; }
+    __device__ __forceinline__ long long base(int b, const Request& r) const {
+        return (causal(b) ? (long long)max(r.length - r.rows, 0) + tokens : r.length) + kKeys;
+    }
+    __device__ __forceinline__ long long until(long long base, long long step, long long tile) const {
+        return tile * base + step * (tile * (tile - 1) / 2);
+    }
+    __device__ __forceinline__ long long cost_of(int b, const Request& r) const {
+        if ((long long)r.rows * group <= a.few_rows || r.rows <= 0) return 0;
+        return a.batch.kv_heads * until(base(b, r), causal(b) ? tokens : 0, tiles(r));
+    }
+    __device__ __forceinline__ Item item(int b, const Request& r, long long before, long long unit) const {
+        const long long base_ = base(b, r), step = causal(b) ? tokens : 0;
+        const int n = tiles(r);
+        const long long each = until(base_, step, n);
+        const int head = (int)((unit - before) / each);
+        const long long at = unit - before - head * each;
+        int lo = 0, hi = n;  // the last tile that starts at or before `at`
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (until(base_, step, mid) <= at)
+                lo = mid;
+            else
+                hi = mid;
+        }
+        const long long start = before + head * each + until(base_, step, lo);
+        int keys = r.length;
+        if (causal(b)) keys = min(keys, max(r.length - r.rows + (int)min((long long)r.rows, (lo + 1LL) * tokens), 0));
+        return Item{r, b, head, lo, start, start + base_ + step * lo, keys > 0 ? (keys - 1) / kKeys + 1 : 1};
+    }
+    __device__ __forceinline__ int cut(const Item& it, long long unit) const {
+        return (int)((min(max(unit, it.start), it.end) - it.start) * it.key_tiles / (it.end - it.start));
+    }
+};
+__device__ __forceinline__ long long cost_of(const FewPlan& plan, int, const Request& r) { return plan.cost(r); }
+__device__ __forceinline__ long long cost_of(const ManyPlan& plan, int b, const Request& r) { return plan.cost_of(b, r); }
+
+struct Found {
+    long long share;   // units a block
+    long long total;   // units of the call
+    long long before;  // units before request b
+    int b;             // the request that holds the block's first unit
+};
+
+// Block `g` of `blocks`: its share and where it begins, by a scan of the whole
+// block (kThreads threads) over the requests.  `scratch` is kThreads / 32 + 2
+// words of 64 bits.
+template <int kThreads, class Plan>
+__device__ Found find_block(const Plan& plan, long long g, int blocks, long long* scratch) {
+    constexpr int kWarps = kThreads / 32;
+    const int n = plan.a.batch.requests;
+    const int each = (n + kThreads - 1) / kThreads;
+    const int first = min(threadIdx.x * each, (unsigned)n), last = min(first + each, n);
+    long long mine = 0;
+    for (int b = first; b < last; ++b) mine += cost_of(plan, b, plan.get(b));
+    const long long head = plan.prefix_rows ? cost_of(plan, -1, plan.get(-1)) : 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    long long total = head, before = head + sum - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += scratch[w];
+        total += scratch[w];
+    }
+    const long long share = (total + blocks - 1) / blocks;
+    const long long unit = g * share;
+    if (unit < head) {
+        if (threadIdx.x == 0) scratch[kWarps] = 0, scratch[kWarps + 1] = -1;
+    } else if (unit >= before && unit < before + mine) {
+        int b = first;
+        long long c = cost_of(plan, b, plan.get(b));
+        while (unit >= before + c) {
+            before += c;
+            ++b;
+            c = cost_of(plan, b, plan.get(b));
+        }
+        scratch[kWarps] = before;
+        scratch[kWarps + 1] = b;
+    }
+    __syncthreads();
+    return Found{share, total, scratch[kWarps], (int)scratch[kWarps + 1]};  // before and b: if unit < total
+}
+
+// A block's way through its items.
+template <class Plan>
+struct Cursor {
+    const Plan& plan;
+    long long unit, last;  // the block's units
+    long long before, cost;
+    int b;
+    Request r;
+    // the current part
+    Item it;
+    int first_tile, end_tile;
+    bool whole;
+    int slot;
+
+    __device__ __forceinline__ Cursor(const Plan& p, const Found& f, long long g)
+        : plan(p), unit(g * f.share), last(min(f.total, (g + 1) * f.share)), before(f.before), b(f.b), begin(unit) {
+        if (unit < last) {
+            r = plan.get(b);
+            cost = cost_of(plan, b, r);
+        }
+    }
+    // The next part with key tiles of its own; false at the end.
+    __device__ __forceinline__ bool next() {
+        while (unit < last) {
+            while (unit >= before + cost) {
+                before += cost;
+                r = plan.get(++b);
+                cost = cost_of(plan, b, r);
+            }
+            it = plan.item(b, r, before, unit);
+            const long long to = min(it.end, last);
+            first_tile = plan.cut(it, unit);
+            end_tile = plan.cut(it, to);
+            unit = to;
+            if (first_tile < end_tile) {
+                whole = first_tile == 0 && end_tile == it.key_tiles;
+                slot = it.start <= begin ? 0 : 1;
+                return true;
+            }
+        }
+        return false;
+    }
+
+  private:
+    long long begin;
+};
+
+// Four elements of a part.
+__device__ __forceinline__ void put_part(float* sums, float* stats, long long row, int width, int d, const float (&v)[4],
+                                         float most, float total) {
+    *reinterpret_cast<float4*>(sums + row * width + d) = make_float4(v[0], v[1], v[2], v[3]);
+    if (d == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(most, total);
 }
 
 // Four elements of a row's output.  A row that sees no key is zero.
@@ -103,27 +291,76 @@ __device__ __forceinline__ void put_row(const AttentionArgs& a, const Workspace&
     }
 }
 
-// Sums of several parts of the same keys' row, in a fixed order.
+// Sums of several parts of a row, in a fixed order.
 struct Joined {
     float most = -INFINITY, total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 
-    __device__ __forceinline__ void add_row(const float* stats, const float* sums, long long row, int width, int d) {
-        const float m = load_l2(stats + 2 * row), l = load_l2(stats + 2 * row + 1);
-        const float4 x = load_l2(reinterpret_cast<const float4*>(sums + row * width + d));
-        const float now = fmaxf(most, m);
+    __device__ __forceinline__ void add(const float2& stats, const float4& x) {
+        const float now = fmaxf(most, stats.x);
         const float ref = now == -INFINITY ? 0.0f : now;
-        const float keep = exp2_approx(most - ref), weight = exp2_approx(m - ref);
+        const float keep = exp2_approx(most - ref), weight = exp2_approx(stats.x - ref);
         most = now;
-        total = total * keep + l * weight;
+        total = total * keep + stats.y * weight;
         v[0] = v[0] * keep + x.x * weight;
         v[1] = v[1] * keep + x.y * weight;
         v[2] = v[2] * keep + x.z * weight;
         v[3] = v[3] * keep + x.w * weight;
     }
-    __device__ __forceinline__ void add(const Workspace& ws, long long row, int width, int d) {
-        add_row(ws.part_stats, ws.part_sums, row, width, d);
-    }
 };
+
+// Joins the parts of the item that border g (block g's first unit) cuts, if it is
+// the first border inside it.  kRows, kWidth: a part's; tile_rows of them used.
+template <class T, int kRows, int kWidth, int kThreads, class Plan>
+__device__ void join_item(const Plan& plan, const Workspace& ws, int kind, int g, int blocks, int tile_rows,
+                          long long* scratch) {
+    const AttentionArgs& a = plan.a;
+    const PagedBatch& p = a.batch;
+    const Found at = find_block<kThreads>(plan, g, blocks, scratch);
+    pdl_launch_dependents();
+    pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
+    const long long u = g * at.share;
+    if (u >= at.total) return;
+    const Item it = plan.item(at.b, plan.get(at.b), at.before, u);
+    if (u == it.start || (g - 1) * at.share > it.start) return;
+    // Blocks h0 .. h1 hold parts of it; those without key tiles wrote none, and an
+    // item that one block holds alone is finished.
+    const int h0 = g - 1, h1 = (int)((it.end - 1) / at.share);
+    const auto has = [&](int h) { return plan.cut(it, h * at.share) < plan.cut(it, (h + 1) * at.share); };
+    int parts = 0;
+    for (int h = h0; h <= h1 && parts < 2; ++h) parts += has(h);
+    if (parts < 2) return;
+    const int first_slot = h0 * at.share >= it.start ? 0 : 1;
+    const int row0 = it.tile * tile_rows;
+    const int rows = (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - row0);
+    for (int i = threadIdx.x; i < rows * (kWidth / 4); i += kThreads) {
+        const int row = i / (kWidth / 4), d = i % (kWidth / 4) * 4;
+        if (d >= p.dim) continue;
+        Joined j;
+        for (int h = h0; h <= h1; h += 8) {
+            float2 stats[8];
+            float4 sums[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {  // eight parts' loads under way at once
+                stats[k] = make_float2(-INFINITY, 0.0f);
+                sums[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (h + k <= h1 && has(h + k)) {
+                    const long long at_row = ((long long)(h + k) * 2 + (h + k == h0 ? first_slot : 0)) * kRows + row;
+                    stats[k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + at_row);
+                    sums[k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind] + at_row * kWidth + d));
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) j.add(stats[k], sums[k]);
+        }
+        const int token = (row0 + row) / plan.group, head = it.head * plan.group + (row0 + row) % plan.group;
+        put_row<T>(a, ws, it.b < 0, it.r.first + token, head, d, j.v, j.most, j.total);
+    }
+}
+
+// The kernel of the requests with more than a.few_rows rows a kv head
+// (zq_attention_sm100.cu).
+constexpr int kManyRows = 256;  // rows of an item: two tiles of 128
+cudaError_t launch_attend_many(const AttentionArgs& a, int dtype, const Workspace& ws, int blocks, cudaStream_t stream);
 
 }  // namespace attn
 }  // namespace zq

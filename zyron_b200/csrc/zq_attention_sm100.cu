@@ -1,0 +1,624 @@
+// zq_attention_sm100.cu -- attention items of many rows on 5th-generation tensor
+// cores: prompts, long drafts, and the shared prefix of a batch, whose rows are
+// all the batch's (zq_paged_attention; zq_attention.cu has the formulas and how
+// work is split).
+//
+// A persistent block takes 256 rows of a kv head as two tiles of 128 (new tokens
+// times the heads of the group) and walks their key tiles of 128:
+//   warp 9       TMA: q once an item, then key and value tiles alternately through
+//                a ring of shared-memory slots, a box for each run of tokens in a
+//                page; tokens that do not exist are boxes outside the tensor, which
+//                arrive as zeros.
+//   warp 8       issues the MMAs: S_i = Q_i K^T into TMEM, O_i += P_i V with P_i read
+//                from TMEM, the two tiles by turns, so that the tensor cores work on
+//                one while the other is in its softmax.  V is the MN-major operand:
+//                rows of the same boxes as K's, nothing is transposed.
+//   warps 0-7    a warpgroup a tile, a thread a row: scores from TMEM, running
+//                maximum, exp2, P back to TMEM over its own scores, 16 bits each.
+// A row's reference is raised, and its output in TMEM rescaled, only when its
+// maximum has grown by more than 2^8 since: weights up to 2^8 lose nothing in the
+// sums' 32 bits.  P is rounded to the cache's type for the second product, half a
+// step of each weight.
+//
+// Bound: 4 dim operations a (row, key) on the tensor cores against one exponential,
+// of which the special function unit makes 16 a cycle and SM: at dim 128 both take
+// 2048 cycles for 256 rows x 128 keys.
+//
+// A value that is no number must not reach rows that do not see it, and 0 times it
+// would.  Tiles that a causal border cuts are searched for one; if there is, the
+// warpgroup adds its own weighted values by itself and the MMA is left out.
+#include "zq_attention.cuh"
+#include "zq_internal.h"
+#include "zq_tcgen05.cuh"
+
+#include <numeric>
+
+namespace zq {
+
+namespace {
+
+using namespace attn;
+
+constexpr int kManyThreads = 320;
+constexpr int kTile = 128;             // rows of a q tile, keys of a key tile
+constexpr int kHalfBytes = kTile * 128;  // 128 rows x 64 elements, 128-byte swizzled
+constexpr int kBadRing = 8;
+
+template <int kD>
+struct Smem {
+    static constexpr int kHalves = kD / 64;
+    static constexpr int kTileBytes = kHalves * kHalfBytes;
+    static constexpr int kSlots = kD == 128 ? 4 : 8;
+    static constexpr int kRing = 2 * kTileBytes;  // after the two q tiles
+    static constexpr int kBars = kRing + kSlots * kTileBytes;
+    static constexpr int kTotal = 1024 + kBars + 256;
+};
+
+// Instruction descriptor of tcgen05.mma.kind::f16: A and B both fp16 or both bf16,
+// A K-major, fp32 accumulators.
+template <class T>
+__host__ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
+    const uint32_t type = kIsHalf<T> ? 0u : 1u;
+    return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+           ((uint32_t)(kTile >> 4) << 24);
+}
+
+// MN-major operand with 128-byte swizzle: 64 elements of the N dimension by 8 of K
+// are 1024 bytes; the next 8 of K follow (SBO), the next 64 of N a tile half on (LBO).
+__device__ __forceinline__ uint64_t make_mn_desc(uint32_t saddr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((saddr >> 4) & 0x3FFFu);
+    d |= (uint64_t)(kHalfBytes >> 4) << 16;
+    d |= (uint64_t)(1024u >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// A from TMEM: two elements a column.
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_t* bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+        "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t tmem_ld_32x32b_x1(uint32_t taddr) {
+    uint32_t r;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+    return r;
+}
+
+// Whether any thread of a warpgroup (barrier 1 or 2, 128 threads) says so.
+template <int kBarrier>
+__device__ __forceinline__ bool any_at(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "barrier.cta.red.or.pred p, %2, 128, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v), "n"(kBarrier)
+        : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ bool group_any(int wg, bool v) { return wg == 0 ? any_at<1>(v) : any_at<2>(v); }
+
+template <class T>
+__device__ __forceinline__ uint32_t pack_pair(float x, float y) {
+    Pack<T, 2> p{{from_float<T>(x), from_float<T>(y)}};
+    uint32_t r;
+    memcpy(&r, &p, 4);
+    return r;
+}
+
+// Address of 16-byte chunk c of row r of a tile in shared memory.
+__device__ __forceinline__ const uint8_t* tile_chunk(const uint8_t* tile, int r, int c) {
+    return tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+
+// Rows from `valid` to the end of their box hold what the page holds behind a
+// request's last token: zeros instead, since 0 times a NaN there would count.
+// Both warpgroups write the same zeros.
+template <int kD>
+__device__ __forceinline__ void clear_tail(uint8_t* v_tile, int valid, int box, int t) {
+    const int end = min((valid + box - 1) / box * box, kTile);
+    for (int i = t; i < (end - valid) * (kD / 8); i += 128) {
+        const int r = valid + i / (kD / 8), c = i % (kD / 8);
+        *reinterpret_cast<uint4*>(const_cast<uint8_t*>(tile_chunk(v_tile, r, c))) = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+
+// Whether rows [from, to) of a value tile hold an infinity or NaN (this thread's share).
+template <class T, int kD>
+__device__ __forceinline__ bool wild_rows(const uint8_t* v_tile, int from, int to, int t) {
+    constexpr uint32_t kOnes = kIsHalf<T> ? 0x7C007C00u : 0x7F807F80u;
+    bool wild = false;
+    for (int i = t; i < (to - from) * (kD / 8); i += 128) {
+        const uint4 w = *reinterpret_cast<const uint4*>(tile_chunk(v_tile, from + i / (kD / 8), i % (kD / 8)));
+        const uint32_t e[4] = {w.x & kOnes, w.y & kOnes, w.z & kOnes, w.w & kOnes};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            wild |= (e[j] & 0xFFFF0000u) == (kOnes & 0xFFFF0000u) || (e[j] & 0xFFFFu) == (kOnes & 0xFFFFu);
+    }
+    return wild;
+}
+
+// O += P V of one tile by the warpgroup itself, every row with the keys that it
+// sees alone (`seen` of them from the tile's start, less those of `bad` eighths).
+template <class T, int kD>
+__device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, const uint8_t* v_tile, int seen, uint32_t bad,
+                                            bool first) {
+    tmem_st_wait();  // P is there
+#pragma unroll 1
+    for (int c = 0; c < kD / 32; ++c) {
+        uint32_t o[32];
+        if (first) {
+#pragma unroll
+            for (int d = 0; d < 32; ++d) o[d] = 0u;
+        } else {
+            tmem_ld_32x32b_x32(o_addr + c * 32, o);
+            tmem_ld_wait();
+        }
+#pragma unroll 1
+        for (int k = 0; k < kTile; ++k) {
+            const uint32_t pair = tmem_ld_32x32b_x1(p_addr + k / 2);
+            tmem_ld_wait();
+            Pack<T, 2> p;
+            memcpy(&p, &pair, 4);
+            if (k >= seen || ((bad >> (k >> 3)) & 1)) continue;
+            const float w = to_float(k & 1 ? p.e[1] : p.e[0]);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                Pack<T, 8> v;
+                memcpy(&v, tile_chunk(v_tile, k, c * 4 + q), 16);
+#pragma unroll
+                for (int d = 0; d < 8; ++d)
+                    o[8 * q + d] = __float_as_uint(fmaf(w, to_float(v.e[d]), __uint_as_float(o[8 * q + d])));
+            }
+        }
+        tmem_st_32x32b_x32(o_addr + c * 32, o);
+        tmem_st_wait();
+    }
+}
+
+struct Shape {
+    int group, tile_tokens;  // tokens of a 128-row tile
+    int box;                 // tokens of a page box
+    int cache_end;           // a page outside the cache
+};
+
+template <class T, int kD>
+__global__ void __launch_bounds__(kManyThreads, 1)
+    attend_many_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
+                       const __grid_constant__ CUtensorMap tmap_v, const AttentionArgs a, const Workspace ws,
+                       const Shape shape, uint32_t* __restrict__ err) {
+    using S = Smem<kD>;
+    constexpr int kSlots = S::kSlots;
+    constexpr uint32_t kTmemCols = 512;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    __shared__ long long scratch[kManyThreads / 32 + 2];
+    uint8_t* smem = smem_align1024(smem_raw);
+    uint8_t* ring = smem + S::kRing;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
+    uint64_t* q_full = bars;
+    uint64_t* q_empty = bars + 1;
+    uint64_t* s_full = bars + 2;   // by tile: scores are there (MMA)
+    uint64_t* p_ready = bars + 4;  // by tile: weights are there (its warpgroup)
+    uint64_t* o_done = bars + 6;   // by tile: the item's last product is done (MMA)
+    uint64_t* mma_done = bars + 8;
+    uint64_t* kv_full = bars + 9;
+    uint64_t* kv_empty = kv_full + kSlots;
+    uint32_t* bad_ring = reinterpret_cast<uint32_t*>(kv_empty + kSlots);  // eighths of a key tile on no page
+    volatile uint32_t* own = bad_ring + kBadRing;                         // by tile: its warpgroup added the values
+    uint32_t* tmem_slot = bad_ring + kBadRing + 2;
+    static_assert((9 + 2 * 8) * 8 + (kBadRing + 3) * 4 <= 256, "barriers");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const PagedBatch& p = a.batch;
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        mbar_init(q_empty, 1);
+        mbar_init(mma_done, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_ready[i], 128);
+            mbar_init(&o_done[i], 1);
+        }
+        for (int i = 0; i < kSlots; ++i) {
+            mbar_init(&kv_full[i], 1);
+            mbar_init(&kv_empty[i], 1);
+        }
+        fence_mbar_init();
+        tma_prefetch_desc(&tmap_q);
+        tma_prefetch_desc(&tmap_k);
+        tma_prefetch_desc(&tmap_v);
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(kTmemCols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_wait_primary();
+    pdl_launch_dependents();
+
+    const ManyPlan plan{a, shape.group, a.prefix_length > 0 ? live_rows(p) : 0, 2 * shape.tile_tokens};
+    Cursor<ManyPlan> way(plan, find_block<kManyThreads>(plan, blockIdx.x, gridDim.x, scratch), blockIdx.x);
+    // Tiles of the item that hold rows.
+    const auto q_tiles = [&] { return way.it.r.rows - way.it.tile * 2 * shape.tile_tokens > shape.tile_tokens ? 2 : 1; };
+    // Tile n of this block (counted over its parts): keys in slot (2 n) % kSlots, values in the next.
+    const auto slot_of = [](int seq) { return seq % kSlots; };
+    const auto phase_of = [](int seq) { return (uint32_t)(seq / kSlots) & 1u; };
+
+    if (warp == 9) {
+        const uint32_t q_bytes = (uint32_t)(128 * shape.group * shape.tile_tokens);
+        const int boxes = kTile / shape.box;  // of a half tile; at most 16
+        int n = 0;
+        uint32_t part = 0;
+        bool ok = true, q_issued = false;
+        while (ok && way.next()) {
+            const Request r = way.it.r;
+            const bool prefix = way.it.b < 0;
+            const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)way.it.b * p.ld_pages;
+            const int tiles = q_tiles(), head = way.it.head;
+            if (!mbar_wait_bounded(q_empty, (part & 1) ^ 1u, err, kDevErrTimeoutProducer)) break;
+            if (lane == 0) mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * S::kHalves) * q_bytes);
+            __syncwarp();
+            if (lane < tiles * S::kHalves) {
+                const int i = lane / S::kHalves, half = lane % S::kHalves;
+                tma_load_3d(smem + i * S::kTileBytes + half * kHalfBytes, &tmap_q, q_full, half * 64, head * shape.group,
+                            r.first + (way.it.tile * 2 + i) * shape.tile_tokens);
+            }
+            q_issued = true;
+            ++part;
+            for (int j = way.first_tile; j < way.end_tile; ++j, ++n) {
+                // Lane i looks box i's page up.
+                const int key = j * kTile + lane * shape.box;
+                int id = shape.cache_end, row = 0;
+                bool bad = false;
+                if (lane < boxes && key < r.length) {
+                    const int index = key / p.page;
+                    row = key - index * p.page;
+                    const int v = load_l2(table + index);
+                    bad = v < 0 || v >= p.cache_pages;
+                    if (!bad) id = v;
+                }
+                const uint32_t eighths = bad ? ((1u << (shape.box / 8)) - 1u) << (lane * (shape.box / 8)) : 0u;
+                const uint32_t missing = __reduce_or_sync(0xffffffffu, eighths);
+                if (lane == 0) bad_ring[n % kBadRing] = missing;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int seq = 2 * n + kv, slot = slot_of(seq);
+                    if (!mbar_wait_bounded(&kv_empty[slot], phase_of(seq) ^ 1u, err, kDevErrTimeoutProducer)) {
+                        ok = false;
+                        break;
+                    }
+                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], S::kTileBytes);
+                    __syncwarp();
+                    const int box = lane / S::kHalves, half = lane % S::kHalves;
+                    const int page = __shfl_sync(0xffffffffu, id, box), at = __shfl_sync(0xffffffffu, row, box);
+                    if (box < boxes)
+                        tma_load_4d(ring + slot * S::kTileBytes + half * kHalfBytes + box * shape.box * 128,
+                                    kv ? &tmap_v : &tmap_k, &kv_full[slot], half * 64, at, head, page);
+                }
+                if (!ok) break;
+            }
+        }
+        // Every copy lands before the block can exit.
+        if (q_issued) mbar_drain_bounded(q_full, (part - 1) & 1u, err, kDevErrTimeoutDrain);
+        for (int seq = max(0, 2 * n - kSlots); seq < 2 * n; ++seq)
+            mbar_drain_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutDrain);
+    } else if (warp == 8) {
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
+            const uint32_t q_u = smem_u32(smem), ring_u = smem_u32(ring);
+            const auto scores = [&](int i, int slot) {
+                const uint32_t qa = q_u + i * S::kTileBytes, kb = ring_u + slot * S::kTileBytes;
+#pragma unroll
+                for (int k = 0; k < kD / 16; ++k) {
+                    const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
+                    umma_f16(tmem + i * kTile, make_sw128_desc(qa + at), make_sw128_desc(kb + at), idesc_s, k > 0);
+                }
+                umma_commit(&s_full[i]);
+            };
+            int n = 0;
+            uint32_t part = 0, weights[2] = {0, 0};
+            bool ok = true;
+            const auto wait_kv = [&](int seq) {
+                if (!mbar_wait_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutMma)) ok = false;
+                tmem_fence_after();
+            };
+            while (ok && way.next()) {
+                const int tiles = q_tiles();
+                if (!mbar_wait_bounded(q_full, part & 1, err, kDevErrTimeoutMma)) break;
+                ++part;
+                wait_kv(2 * n);
+                if (!ok) break;
+                for (int i = 0; i < tiles; ++i) scores(i, slot_of(2 * n));
+                umma_commit(&kv_empty[slot_of(2 * n)]);
+                for (int j = way.first_tile; j < way.end_tile && ok; ++j, ++n) {
+                    const bool more = j + 1 < way.end_tile;
+                    for (int i = 0; i < tiles && ok; ++i) {
+                        if (!mbar_wait_bounded(&p_ready[i], weights[i] & 1, err, kDevErrTimeoutMma)) {
+                            ok = false;
+                            break;
+                        }
+                        ++weights[i];
+                        if (i == 0) wait_kv(2 * n + 1);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        if (!own[i]) {
+                            const uint32_t vb = ring_u + slot_of(2 * n + 1) * S::kTileBytes;
+#pragma unroll
+                            for (int k = 0; k < kTile / 16; ++k)
+                                umma_f16_ts(tmem + 2 * kTile + i * kD, tmem + i * kTile + k * 8, make_mn_desc(vb + k * 2048),
+                                            idesc_o, j > way.first_tile || k > 0);
+                        }
+                        if (i == tiles - 1) umma_commit(&kv_empty[slot_of(2 * n + 1)]);
+                        if (more) {
+                            if (i == 0) wait_kv(2 * n + 2);
+                            if (!ok) break;
+                            scores(i, slot_of(2 * n + 2));
+                            if (i == tiles - 1) umma_commit(&kv_empty[slot_of(2 * n + 2)]);
+                        } else {
+                            umma_commit(&o_done[i]);
+                            if (i == tiles - 1) umma_commit(q_empty);
+                        }
+                    }
+                }
+            }
+            // All MMAs issued by this thread complete before TMEM is freed.
+            umma_commit(mma_done);
+            mbar_drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
+        }
+    } else {
+        const int wg = warp >> 2, t = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + wg * kTile, o_addr = tmem + lanes + 2 * kTile + wg * kD;
+        const float scale = a.scale_log2;
+        int n = 0;
+        uint32_t seen_scores = 0, parts = 0;
+        bool ok = true;
+        while (ok && way.next()) {
+            if (wg >= q_tiles()) {
+                n += way.end_tile - way.first_tile;
+                continue;
+            }
+            const Request r = way.it.r;
+            const bool prefix = way.it.b < 0, causal = !prefix && a.causal;
+            const int token0 = (way.it.tile * 2 + wg) * shape.tile_tokens;  // of the tile, in the request
+            const int token = token0 + t / shape.group, in_group = t % shape.group;
+            const bool row_ok = t < shape.tile_tokens * shape.group && token < r.rows;
+            const auto limit_of = [&](int tok) {
+                return causal ? min(max(r.length - r.rows + tok + 1, 0), r.length) : r.length;
+            };
+            const int limit = limit_of(row_ok ? token : r.rows - 1), low = limit_of(token0);
+            float ref = -INFINITY, sum = 0.0f;
+            for (int j = way.first_tile; j < way.end_tile; ++j, ++n) {
+                const int key0 = j * kTile;
+                if (!mbar_wait_bounded(&s_full[wg], seen_scores & 1, err, kDevErrTimeoutEpilogue)) {
+                    ok = false;
+                    break;
+                }
+                ++seen_scores;
+                tmem_fence_after();
+                const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
+                tmem_ld_wait();
+                const bool masked = key0 + kTile > low || bad;
+                float mul = scale;
+                if (masked) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const int key = c * 32 + k;
+                            const bool out = key >= limit - key0 || ((bad >> (key >> 3)) & 1);
+                            s[c][k] = __float_as_uint(out ? -INFINITY : __uint_as_float(s[c][k]) * scale);
+                        }
+                    mul = 1.0f;
+                }
+                float most[4];
+                if (mul >= 0.0f) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        most[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                        for (int k = 1; k < 32; ++k) most[c] = fmaxf(most[c], __uint_as_float(s[c][k]));
+                    }
+                    most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        most[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+                        for (int k = 1; k < 32; ++k) most[c] = fminf(most[c], __uint_as_float(s[c][k]));
+                    }
+                    most[0] = fminf(fminf(most[0], most[1]), fminf(most[2], most[3]));
+                }
+                const float top = most[0] * mul;
+                const bool grown = top > ref + 8.0f;  // from -inf: by anything
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float now = grown ? top : ref;
+                    const float keep = grown ? exp2_approx(ref - now) : 1.0f;
+                    ref = now;
+                    sum *= keep;
+                    if (j > way.first_tile) {
+                        // The products before these scores are complete with them.
+#pragma unroll 1
+                        for (int c = 0; c < kD / 32; ++c) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(o_addr + c * 32, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                            tmem_st_32x32b_x32(o_addr + c * 32, o);
+                        }
+                    }
+                }
+                const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
+                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float x = exp2_approx(fmaf(__uint_as_float(s[c][2 * k]), mul, from));
+                        const float y = exp2_approx(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, from));
+                        part[k & 3] += x + y;
+                        w[k] = pack_pair<T>(x, y);
+                    }
+                    tmem_st_32x32b_x16(s_addr + c * 16, w);
+                }
+                sum += (part[0] + part[1]) + (part[2] + part[3]);
+                bool wild = false;
+                if (masked) {
+                    const int valid = min(kTile, r.length - key0), from_key = max(low - key0, 0);
+                    if (valid % shape.box != 0 || from_key < valid) {
+                        uint8_t* v_tile = ring + slot_of(2 * n + 1) * S::kTileBytes;
+                        if (!mbar_wait_bounded(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1), err,
+                                               kDevErrTimeoutEpilogue)) {
+                            ok = false;
+                            break;
+                        }
+                        if (valid > 0 && valid % shape.box != 0) clear_tail<kD>(v_tile, valid, shape.box, t);
+                        if (from_key < valid) {
+                            wild = group_any(wg, wild_rows<T, kD>(v_tile, from_key, valid, t));
+                            if (wild) add_own_values<T, kD>(o_addr, s_addr, v_tile, limit - key0, bad, j == way.first_tile);
+                        }
+                    }
+                }
+                if (t == 0) own[wg] = wild;
+                tmem_st_wait();
+                tmem_fence_before();
+                mbar_arrive(&p_ready[wg]);
+            }
+            if (!ok) break;
+            if (!mbar_wait_bounded(&o_done[wg], parts & 1, err, kDevErrTimeoutEpilogue)) break;
+            ++parts;
+            tmem_fence_after();
+            const int row = wg * shape.tile_tokens * shape.group + t;  // of the item
+#pragma unroll 1
+            for (int c = 0; c < kD / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld_32x32b_x32(o_addr + c * 32, o);
+                tmem_ld_wait();
+                if (!row_ok) continue;
+#pragma unroll
+                for (int k = 0; k < 32; k += 4) {
+                    const int d = c * 32 + k;
+                    if (d >= p.dim) break;
+                    const float v[4] = {__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
+                                        __uint_as_float(o[k + 3])};
+                    if (way.whole)
+                        put_row<T>(a, ws, prefix, r.first + token, way.it.head * shape.group + in_group, d, v, ref, sum);
+                    else
+                        put_part(ws.part_sums[1], ws.part_stats[1],
+                                 ((long long)blockIdx.x * 2 + way.slot) * kManyRows + row, kD, d, v, ref, sum);
+                }
+            }
+            tmem_fence_before();  // O has been read before the next weights are announced
+        }
+    }
+    tmem_fence_before();
+    __syncthreads();
+    tmem_fence_after();
+    if (warp == 8)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <class T, int kD>
+cudaError_t launch_many_t(const AttentionArgs& a, const Workspace& ws, int blocks, cudaStream_t stream) {
+    const PagedBatch& p = a.batch;
+    Shape s{};
+    s.group = a.heads / p.kv_heads;
+    s.tile_tokens = kTile / s.group;
+    s.box = (int)std::gcd((long long)p.page, (long long)kTile);
+    // A cache without pages: a view of one that no box asks for.
+    const int pages = p.cache_pages > 0 ? p.cache_pages : 1;
+    s.cache_end = pages;
+    uint32_t* err = nullptr;
+    if (device_error_word(&err) != ZQ_OK) return cudaErrorUnknown;
+    const CUtensorMapDataType type =
+        kIsHalf<T> ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    CUtensorMap q, k, v;
+    const uint64_t q_dims[3] = {(uint64_t)p.dim, (uint64_t)a.heads, (uint64_t)p.rows};
+    const uint64_t q_pitch[2] = {(uint64_t)p.dim * 2, (uint64_t)a.ldq * 2};
+    const uint32_t q_box[3] = {64, (uint32_t)s.group, (uint32_t)s.tile_tokens};
+    const uint64_t c_dims[4] = {(uint64_t)p.dim, (uint64_t)p.page, (uint64_t)p.kv_heads, (uint64_t)pages};
+    const uint32_t c_box[4] = {64, (uint32_t)s.box, 1, 1};
+    uint64_t c_pitch[3] = {(uint64_t)p.dim * 2, (uint64_t)p.page * p.dim * 2, (uint64_t)p.ld_k_page * 2};
+    if (encode_tiled(&q, type, 3, a.q, q_dims, q_pitch, q_box) != ZQ_OK) return cudaErrorInvalidValue;
+    if (encode_tiled(&k, type, 4, p.cache_pages > 0 ? a.k_cache : a.q, c_dims, c_pitch, c_box) != ZQ_OK)
+        return cudaErrorInvalidValue;
+    c_pitch[2] = (uint64_t)p.ld_v_page * 2;
+    if (encode_tiled(&v, type, 4, p.cache_pages > 0 ? a.v_cache : a.q, c_dims, c_pitch, c_box) != ZQ_OK)
+        return cudaErrorInvalidValue;
+    const auto kern = attend_many_kernel<T, kD>;
+    const cudaError_t e = ensure_smem_attr(kern, Smem<kD>::kTotal);
+    if (e != cudaSuccess) return e;
+    return launch_pdl_kernel(kern, dim3(blocks), dim3(kManyThreads), Smem<kD>::kTotal, stream, q, k, v, a, ws, s, err);
+}
+
+}  // namespace
+
+namespace attn {
+
+cudaError_t launch_attend_many(const AttentionArgs& a, int dtype, const Workspace& ws, int blocks, cudaStream_t stream) {
+    if (dtype == ZQ_DTYPE_F16)
+        return a.batch.dim <= 64 ? launch_many_t<__half, 64>(a, ws, blocks, stream)
+                                 : launch_many_t<__half, 128>(a, ws, blocks, stream);
+    return a.batch.dim <= 64 ? launch_many_t<__nv_bfloat16, 64>(a, ws, blocks, stream)
+                             : launch_many_t<__nv_bfloat16, 128>(a, ws, blocks, stream);
+}
+
+}  // namespace attn
+}  // namespace zq

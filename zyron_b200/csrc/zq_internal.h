@@ -64,6 +64,12 @@ zq_status concat_cols(zq_weight* const* parts, int n, void* stream, zq_weight** 
 // Records a CUDA failure as the calling thread's last error.
 zq_status cuda_error(cudaError_t e, const char* what);
 
+// Tensor map of `rank` dimensions of 16-bit elements (innermost first, pitches in
+// bytes from the second on), boxes of 64 elements by box[1 ..] with the 128-byte
+// swizzle, zeros outside.
+zq_status encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+                       const uint64_t* pitches, const uint32_t* box);
+
 // The current device's error word, where bounded device waits record a
 // timeout (read and cleared by zq_device_error).
 zq_status device_error_word(uint32_t** out);

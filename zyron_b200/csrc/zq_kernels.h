@@ -282,6 +282,9 @@ struct AttentionArgs {
     int heads;
     int causal;
     float scale_log2;  // scale x log2(e)
+    // filled in by the launcher: requests of at most so many rows (new tokens x
+    // heads of a kv head) go to the kernel of few rows
+    int few_rows = 0;
 };
 size_t attention_workspace_bytes(const AttentionArgs& a);
 cudaError_t launch_paged_attention(const AttentionArgs& a, int dtype, void* workspace, cudaStream_t stream);
