@@ -393,11 +393,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
 }
 
 // Joins the items that borders of the kernel of few rows (the first few_blocks - 1
-// blocks) and of the other kernel cut.
+// blocks) and of the other kernel (eight blocks a border, 32 rows each) cut.
 template <class T, int kD, int kMT>
 __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_blocks,
                                                                  int many_blocks) {
     __shared__ long long scratch[kJoinThreads / 32 + 2];
+    extern __shared__ int parts[];
     const PagedBatch& p = a.batch;
     const int group = a.heads / p.kv_heads, borders = max(few_blocks - 1, 0);
     // The plans' inputs are older than the kernel before this one, which has
@@ -405,12 +406,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const Attentio
     const int prefix_rows = a.prefix_length > 0 ? live_rows(p) : 0;
     if ((int)blockIdx.x < borders) {
         const FewPlan plan{a, group, prefix_rows};
-        join_item<T, 16 * kMT, kD, kJoinThreads>(plan, ws, 0, blockIdx.x + 1, few_blocks, 16 * kMT, scratch);
+        join_item<T, 16 * kMT, kD, kJoinThreads>(plan, ws, 0, blockIdx.x + 1, few_blocks, 16 * kMT, 0, scratch,
+                                                   parts);
     } else {
         const int tokens = kManyRows / 2 / group * 2;
         const ManyPlan plan{a, group, prefix_rows, tokens};
-        join_item<T, kManyRows, kD, kJoinThreads>(plan, ws, 1, blockIdx.x - borders + 1, many_blocks, tokens * group,
-                                                  scratch);
+        const int k = blockIdx.x - borders;
+        constexpr int kSlices = kManyRows / kSliceRows;
+        join_item<T, kManyRows, kD, kJoinThreads>(plan, ws, 1, k / kSlices + 1, many_blocks, tokens * group,
+                                                  k % kSlices * kSliceRows, scratch, parts);
     }
 }
 
@@ -468,8 +472,10 @@ cudaError_t launch_t(const AttentionArgs& a, int dtype, const Shape& s, const Wo
         e = launch_pdl_kernel(attend_few_kernel<T, kD, kMT>, dim3(s.few_blocks), dim3(kThreads), smem, stream, a, ws);
         if (e != cudaSuccess) return e;
     }
-    const int borders = (s.few_blocks ? s.few_blocks - 1 : 0) + (s.many_blocks ? s.many_blocks - 1 : 0);
-    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(borders), dim3(kJoinThreads), 0, stream, a, ws,
+    const int joins = (s.few_blocks ? s.few_blocks - 1 : 0) +
+                      (s.many_blocks ? (s.many_blocks - 1) * (kManyRows / kSliceRows) : 0);
+    const size_t parts = sizeof(int) * (size_t)(s.few_blocks > s.many_blocks ? s.few_blocks : s.many_blocks);
+    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(joins), dim3(kJoinThreads), parts, stream, a, ws,
                           s.few_blocks, s.many_blocks);
     if (e != cudaSuccess || a.prefix_length == 0) return e;
     return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);

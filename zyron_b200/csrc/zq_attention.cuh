@@ -309,42 +309,60 @@ struct Joined {
 };
 
 // Joins the parts of the item that border g (block g's first unit) cuts, if it is
-// the first border inside it.  kRows, kWidth: a part's; tile_rows of them used.
+// the first border inside it: rows [from, from + kSliceRows) of it.  kRows, kWidth:
+// a part's; tile_rows of them used.  `parts` holds the numbers of `blocks` parts.
+constexpr int kSliceRows = 32;
 template <class T, int kRows, int kWidth, int kThreads, class Plan>
-__device__ void join_item(const Plan& plan, const Workspace& ws, int kind, int g, int blocks, int tile_rows,
-                          long long* scratch) {
+__device__ void join_item(const Plan& plan, const Workspace& ws, int kind, int g, int blocks, int tile_rows, int from,
+                          long long* scratch, int* parts) {
     const AttentionArgs& a = plan.a;
     const PagedBatch& p = a.batch;
     const Found at = find_block<kThreads>(plan, g, blocks, scratch);
     pdl_launch_dependents();
-    pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
     const long long u = g * at.share;
-    if (u >= at.total) return;
-    const Item it = plan.item(at.b, plan.get(at.b), at.before, u);
-    if (u == it.start || (g - 1) * at.share > it.start) return;
-    // Blocks h0 .. h1 hold parts of it; those without key tiles wrote none, and an
-    // item that one block holds alone is finished.
-    const int h0 = g - 1, h1 = (int)((it.end - 1) / at.share);
-    const auto has = [&](int h) { return plan.cut(it, h * at.share) < plan.cut(it, (h + 1) * at.share); };
-    int parts = 0;
-    for (int h = h0; h <= h1 && parts < 2; ++h) parts += has(h);
-    if (parts < 2) return;
-    const int first_slot = h0 * at.share >= it.start ? 0 : 1;
+    Item it{};
+    bool mine = u < at.total;
+    if (mine) {
+        it = plan.item(at.b, plan.get(at.b), at.before, u);
+        mine = u > it.start && (g - 1) * at.share <= it.start;
+    }
     const int row0 = it.tile * tile_rows;
-    const int rows = (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - row0);
-    for (int i = threadIdx.x; i < rows * (kWidth / 4); i += kThreads) {
-        const int row = i / (kWidth / 4), d = i % (kWidth / 4) * 4;
+    const int rows = mine ? (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - row0) : 0;
+    pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
+    if (from >= rows) return;
+    // Blocks g - 1 .. hold parts of it; those without key tiles wrote none, and an
+    // item that one block holds alone is finished.
+    __shared__ int count;
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x, h1 = (int)((it.end - 1) / at.share);
+        int n = 0;
+        for (int h0 = g - 1; h0 <= h1; h0 += 32) {
+            const int h = h0 + lane;
+            const bool has = h <= h1 && plan.cut(it, h * at.share) < plan.cut(it, (h + 1) * at.share);
+            const unsigned m = __ballot_sync(0xffffffffu, has);
+            // the first block's part may lie in its second slot
+            if (has) parts[n + __popc(m & ((1u << lane) - 1u))] = 2 * h + (h == g - 1 && h * at.share < it.start ? 1 : 0);
+            n += __popc(m);
+        }
+        if (lane == 0) count = n;
+    }
+    __syncthreads();
+    const int n = count;
+    if (n < 2) return;
+    const int last = min(rows, from + kSliceRows);
+    for (int i = threadIdx.x; i < (last - from) * (kWidth / 4); i += kThreads) {
+        const int row = from + i / (kWidth / 4), d = i % (kWidth / 4) * 4;
         if (d >= p.dim) continue;
         Joined j;
-        for (int h = h0; h <= h1; h += 8) {
+        for (int k0 = 0; k0 < n; k0 += 8) {
             float2 stats[8];
             float4 sums[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {  // eight parts' loads under way at once
                 stats[k] = make_float2(-INFINITY, 0.0f);
                 sums[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (h + k <= h1 && has(h + k)) {
-                    const long long at_row = ((long long)(h + k) * 2 + (h + k == h0 ? first_slot : 0)) * kRows + row;
+                if (k0 + k < n) {
+                    const long long at_row = (long long)parts[k0 + k] * kRows + row;
                     stats[k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + at_row);
                     sums[k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind] + at_row * kWidth + d));
                 }

@@ -449,42 +449,41 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 ++seen_scores;
                 tmem_fence_after();
                 const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
-                uint32_t s[4][32];
+                // The scores are read twice, 32 a time, for the maximum and for the
+                // weights: a row of 128 does not fit beside the rest of the thread's
+                // registers.  Where some are masked (or the scale turns the order
+                // around), the first pass leaves them scaled and masked.
+                const bool masked = key0 + kTile > low || bad, rewrite = masked || scale < 0.0f;
+                float mul = scale, most = -INFINITY;
+                {
+                    uint32_t s[2][32];
+                    tmem_ld_32x32b_x32(s_addr, s[0]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
-                tmem_ld_wait();
-                const bool masked = key0 + kTile > low || bad;
-                float mul = scale;
-                if (masked) {
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_ld_wait();
+                        uint32_t(&x)[32] = s[c & 1];
+                        if (c < 3) tmem_ld_32x32b_x32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
+                        if (rewrite) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const int key = c * 32 + k;
-                            const bool out = key >= limit - key0 || ((bad >> (key >> 3)) & 1);
-                            s[c][k] = __float_as_uint(out ? -INFINITY : __uint_as_float(s[c][k]) * scale);
+                            for (int k = 0; k < 32; ++k) {
+                                const int key = c * 32 + k;
+                                const bool out = key >= limit - key0 || ((bad >> (key >> 3)) & 1);
+                                x[k] = __float_as_uint(out ? -INFINITY : __uint_as_float(x[k]) * scale);
+                            }
+                            tmem_st_32x32b_x32(s_addr + c * 32, x);
                         }
-                    mul = 1.0f;
-                }
-                float most[4];
-                if (mul >= 0.0f) {
+                        float m[4];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        most[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-                        for (int k = 1; k < 32; ++k) most[c] = fmaxf(most[c], __uint_as_float(s[c][k]));
+                        for (int k = 0; k < 32; ++k)
+                            m[k & 3] = k < 4 ? __uint_as_float(x[k]) : fmaxf(m[k & 3], __uint_as_float(x[k]));
+                        most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
                     }
-                    most[0] = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        most[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-                        for (int k = 1; k < 32; ++k) most[c] = fminf(most[c], __uint_as_float(s[c][k]));
+                    if (rewrite) {
+                        tmem_st_wait();
+                        mul = 1.0f;
                     }
-                    most[0] = fminf(fminf(most[0], most[1]), fminf(most[2], most[3]));
                 }
-                const float top = most[0] * mul;
+                const float top = most * mul;
                 const bool grown = top > ref + 8.0f;  // from -inf: by anything
                 if (__any_sync(0xffffffffu, grown)) {
                     const float now = grown ? top : ref;
@@ -506,17 +505,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
                 float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                {
+                    uint32_t s[2][32];
+                    tmem_ld_32x32b_x32(s_addr, s[0]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t w[16];
+                    for (int c = 0; c < 4; ++c) {
+                        tmem_ld_wait();
+                        const uint32_t(&x)[32] = s[c & 1];
+                        if (c < 3) tmem_ld_32x32b_x32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
+                        uint32_t w[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float x = exp2_approx(fmaf(__uint_as_float(s[c][2 * k]), mul, from));
-                        const float y = exp2_approx(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, from));
-                        part[k & 3] += x + y;
-                        w[k] = pack_pair<T>(x, y);
+                        for (int k = 0; k < 16; ++k) {
+                            const float u = exp2_approx(fmaf(__uint_as_float(x[2 * k]), mul, from));
+                            const float v = exp2_approx(fmaf(__uint_as_float(x[2 * k + 1]), mul, from));
+                            part[k & 3] += u + v;
+                            w[k] = pack_pair<T>(u, v);
+                        }
+                        tmem_st_32x32b_x16(s_addr + c * 16, w);
                     }
-                    tmem_st_32x32b_x16(s_addr + c * 16, w);
                 }
                 sum += (part[0] + part[1]) + (part[2] + part[3]);
                 bool wild = false;
