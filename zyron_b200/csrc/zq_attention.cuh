@@ -101,6 +101,18 @@ struct FewPlan {
         const long long start = before + (long long)head * n;
         return Item{r, b, head, 0, start, start + n, n};
     }
+    // The first item of a request that has some, and the one behind an item of the
+    // same request.
+    __device__ __forceinline__ Item first(int b, const Request& r, long long unit) const {
+        const int n = key_tiles(r);
+        return Item{r, b, 0, 0, unit, unit + n, n};
+    }
+    __device__ __forceinline__ bool advance(Item& it) const {
+        if (++it.head == a.batch.kv_heads) return false;
+        it.start = it.end;
+        it.end += it.key_tiles;
+        return true;
+    }
     __device__ __forceinline__ int cut(const Item& it, long long unit) const {
         return (int)(min(max(unit, it.start), it.end) - it.start);
     }
@@ -146,9 +158,27 @@ struct ManyPlan {
                 hi = mid;
         }
         const long long start = before + head * each + until(base_, step, lo);
+        return Item{r, b, head, lo, start, start + base_ + step * lo, key_tiles(b, r, lo)};
+    }
+    __device__ __forceinline__ int key_tiles(int b, const Request& r, int tile) const {
         int keys = r.length;
-        if (causal(b)) keys = min(keys, max(r.length - r.rows + (int)min((long long)r.rows, (lo + 1LL) * tokens), 0));
-        return Item{r, b, head, lo, start, start + base_ + step * lo, keys > 0 ? (keys - 1) / kKeys + 1 : 1};
+        if (causal(b)) keys = min(keys, max(r.length - r.rows + (int)min((long long)r.rows, (tile + 1LL) * tokens), 0));
+        return keys > 0 ? (keys - 1) / kKeys + 1 : 1;
+    }
+    __device__ __forceinline__ Item first(int b, const Request& r, long long unit) const {
+        return Item{r, b, 0, 0, unit, unit + base(b, r), key_tiles(b, r, 0)};
+    }
+    __device__ __forceinline__ bool advance(Item& it) const {
+        if ((it.tile + 1LL) * tokens < it.r.rows) {
+            ++it.tile;
+        } else {
+            if (++it.head == a.batch.kv_heads) return false;
+            it.tile = 0;
+        }
+        it.start = it.end;
+        it.end += base(it.b, it.r) + (causal(it.b) ? (long long)tokens * it.tile : 0);
+        it.key_tiles = key_tiles(it.b, it.r, it.tile);
+        return true;
     }
     __device__ __forceinline__ int cut(const Item& it, long long unit) const {
         return (int)((min(max(unit, it.start), it.end) - it.start) * it.key_tiles / (it.end - it.start));
@@ -210,14 +240,13 @@ __device__ Found find_block(const Plan& plan, long long g, int blocks, long long
     return Found{share, total, scratch[kWarps], (int)scratch[kWarps + 1]};  // before and b: if unit < total
 }
 
-// A block's way through its items.
+// A block's way through its items: found once, then step by step, without a
+// division but at the borders that cut an item (a search and 64-bit divisions an
+// item took 12 us a part).
 template <class Plan>
 struct Cursor {
     const Plan& plan;
     long long unit, last;  // the block's units
-    long long before, cost;
-    int b;
-    Request r;
     // the current part
     Item it;
     int first_tile, end_tile;
@@ -225,24 +254,22 @@ struct Cursor {
     int slot;
 
     __device__ __forceinline__ Cursor(const Plan& p, const Found& f, long long g)
-        : plan(p), unit(g * f.share), last(min(f.total, (g + 1) * f.share)), before(f.before), b(f.b), begin(unit) {
-        if (unit < last) {
-            r = plan.get(b);
-            cost = cost_of(plan, b, r);
-        }
+        : plan(p), unit(g * f.share), last(min(f.total, (g + 1) * f.share)), begin(unit) {
+        if (unit < last) it = plan.item(f.b, plan.get(f.b), f.before, unit);
     }
     // The next part with key tiles of its own; false at the end.
     __device__ __forceinline__ bool next() {
         while (unit < last) {
-            while (unit >= before + cost) {
-                before += cost;
-                r = plan.get(++b);
-                cost = cost_of(plan, b, r);
+            if (unit >= it.end && !plan.advance(it)) {
+                int b = it.b;
+                Request r;
+                do r = plan.get(++b);
+                while (cost_of(plan, b, r) == 0);
+                it = plan.first(b, r, unit);
             }
-            it = plan.item(b, r, before, unit);
             const long long to = min(it.end, last);
-            first_tile = plan.cut(it, unit);
-            end_tile = plan.cut(it, to);
+            first_tile = unit == it.start ? 0 : plan.cut(it, unit);
+            end_tile = to == it.end ? it.key_tiles : plan.cut(it, to);
             unit = to;
             if (first_tile < end_tile) {
                 whole = first_tile == 0 && end_tile == it.key_tiles;

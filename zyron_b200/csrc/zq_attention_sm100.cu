@@ -43,6 +43,17 @@ constexpr int kManyThreads = 320;
 constexpr int kTile = 128;             // rows of a q tile, keys of a key tile
 constexpr int kHalfBytes = kTile * 128;  // 128 rows x 64 elements, 128-byte swizzled
 constexpr int kBadRing = 8;
+constexpr int kPartRing = 4;
+
+// What the producer tells the other warps of a part.  It is at most two parts ahead
+// of the warpgroups (q has one place), so a ring of four is never overrun.
+struct Part {
+    int first, rows, length;  // of the request
+    int token0, head;         // first token of the item, kv head
+    int first_tile, end_tile;
+    int flags;                // kEnd, kPrefix, kWhole, kSecondSlot
+};
+enum : int { kEnd = 1, kPrefix = 2, kWhole = 4, kSecondSlot = 8 };
 
 template <int kD>
 struct Smem {
@@ -51,7 +62,7 @@ struct Smem {
     static constexpr int kSlots = kD == 128 ? 4 : 8;
     static constexpr int kRing = 2 * kTileBytes;  // after the two q tiles
     static constexpr int kBars = kRing + kSlots * kTileBytes;
-    static constexpr int kTotal = 1024 + kBars + 256;
+    static constexpr int kTotal = 1024 + kBars + 512;
 };
 
 // Instruction descriptor of tcgen05.mma.kind::f16: A and B both fp16 or both bf16,
@@ -253,7 +264,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     uint32_t* bad_ring = reinterpret_cast<uint32_t*>(kv_empty + kSlots);  // eighths of a key tile on no page
     volatile uint32_t* own = bad_ring + kBadRing;                         // by tile: its warpgroup added the values
     uint32_t* tmem_slot = bad_ring + kBadRing + 2;
-    static_assert((9 + 2 * 8) * 8 + (kBadRing + 3) * 4 <= 256, "barriers");
+    uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 4);
+    Part* parts = reinterpret_cast<Part*>(part_full + kPartRing);
+    static_assert((9 + 2 * 8 + kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedBatch& p = a.batch;
 
@@ -266,6 +279,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             mbar_init(&p_ready[i], 128);
             mbar_init(&o_done[i], 1);
         }
+        for (int i = 0; i < kPartRing; ++i) mbar_init(&part_full[i], 1);
         for (int i = 0; i < kSlots; ++i) {
             mbar_init(&kv_full[i], 1);
             mbar_init(&kv_empty[i], 1);
@@ -289,9 +303,15 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     pdl_launch_dependents();
 
     const ManyPlan plan{a, shape.group, a.prefix_length > 0 ? live_rows(p) : 0, 2 * shape.tile_tokens};
-    Cursor<ManyPlan> way(plan, find_block<kManyThreads>(plan, blockIdx.x, gridDim.x, scratch), blockIdx.x);
+    const Found found = find_block<kManyThreads>(plan, blockIdx.x, gridDim.x, scratch);
     // Tiles of the item that hold rows.
-    const auto q_tiles = [&] { return way.it.r.rows - way.it.tile * 2 * shape.tile_tokens > shape.tile_tokens ? 2 : 1; };
+    const auto q_tiles = [&](const Part& q) { return q.rows - q.token0 > shape.tile_tokens ? 2 : 1; };
+    // The block's part number `i`; false: the producer gave up.
+    const auto part_at = [&](uint32_t i, Part& q) {
+        if (!mbar_wait_bounded(&part_full[i % kPartRing], (i / kPartRing) & 1, err, kDevErrTimeoutMma)) return false;
+        q = parts[i % kPartRing];
+        return true;
+    };
     // Tile n of this block (counted over its parts): keys in slot (2 n) % kSlots, values in the next.
     const auto slot_of = [](int seq) { return seq % kSlots; };
     const auto phase_of = [](int seq) { return (uint32_t)(seq / kSlots) & 1u; };
@@ -302,22 +322,32 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         int n = 0;
         uint32_t part = 0;
         bool ok = true, q_issued = false;
-        while (ok && way.next()) {
+        Cursor<ManyPlan> way(plan, found, blockIdx.x);
+        while (ok) {
+            const bool more = way.next();
             const Request r = way.it.r;
             const bool prefix = way.it.b < 0;
+            const int head = way.it.head;
+            const Part q{r.first, r.rows, r.length, way.it.tile * 2 * shape.tile_tokens, head, way.first_tile, way.end_tile,
+                         more ? (prefix ? kPrefix : 0) | (way.whole ? kWhole : 0) | (way.slot ? kSecondSlot : 0) : kEnd};
+            if (lane == 0) {
+                parts[part % kPartRing] = q;
+                mbar_arrive(&part_full[part % kPartRing]);
+            }
+            if (!more) break;
             const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)way.it.b * p.ld_pages;
-            const int tiles = q_tiles(), head = way.it.head;
+            const int tiles = q_tiles(q);
             if (!mbar_wait_bounded(q_empty, (part & 1) ^ 1u, err, kDevErrTimeoutProducer)) break;
             if (lane == 0) mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * S::kHalves) * q_bytes);
             __syncwarp();
             if (lane < tiles * S::kHalves) {
                 const int i = lane / S::kHalves, half = lane % S::kHalves;
                 tma_load_3d(smem + i * S::kTileBytes + half * kHalfBytes, &tmap_q, q_full, half * 64, head * shape.group,
-                            r.first + (way.it.tile * 2 + i) * shape.tile_tokens);
+                            r.first + q.token0 + i * shape.tile_tokens);
             }
             q_issued = true;
             ++part;
-            for (int j = way.first_tile; j < way.end_tile; ++j, ++n) {
+            for (int j = q.first_tile; j < q.end_tile; ++j, ++n) {
                 // Lane i looks box i's page up.
                 const int key = j * kTile + lane * shape.box;
                 int id = shape.cache_end, row = 0;
@@ -374,16 +404,17 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 if (!mbar_wait_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutMma)) ok = false;
                 tmem_fence_after();
             };
-            while (ok && way.next()) {
-                const int tiles = q_tiles();
+            Part q;
+            while (ok && part_at(part, q) && !(q.flags & kEnd)) {
+                const int tiles = q_tiles(q);
                 if (!mbar_wait_bounded(q_full, part & 1, err, kDevErrTimeoutMma)) break;
                 ++part;
                 wait_kv(2 * n);
                 if (!ok) break;
                 for (int i = 0; i < tiles; ++i) scores(i, slot_of(2 * n));
                 umma_commit(&kv_empty[slot_of(2 * n)]);
-                for (int j = way.first_tile; j < way.end_tile && ok; ++j, ++n) {
-                    const bool more = j + 1 < way.end_tile;
+                for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++n) {
+                    const bool more = j + 1 < q.end_tile;
                     for (int i = 0; i < tiles && ok; ++i) {
                         if (!mbar_wait_bounded(&p_ready[i], weights[i] & 1, err, kDevErrTimeoutMma)) {
                             ok = false;
@@ -398,7 +429,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
 #pragma unroll
                             for (int k = 0; k < kTile / 16; ++k)
                                 umma_f16_ts(tmem + 2 * kTile + i * kD, tmem + i * kTile + k * 8, make_mn_desc(vb + k * 2048),
-                                            idesc_o, j > way.first_tile || k > 0);
+                                            idesc_o, j > q.first_tile || k > 0);
                         }
                         if (i == tiles - 1) umma_commit(&kv_empty[slot_of(2 * n + 1)]);
                         if (more) {
@@ -423,16 +454,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t s_addr = tmem + lanes + wg * kTile, o_addr = tmem + lanes + 2 * kTile + wg * kD;
         const float scale = a.scale_log2;
         int n = 0;
-        uint32_t seen_scores = 0, parts = 0;
+        uint32_t seen_scores = 0, done = 0, part = 0;
         bool ok = true;
-        while (ok && way.next()) {
-            if (wg >= q_tiles()) {
-                n += way.end_tile - way.first_tile;
+        Part r;
+        while (ok && part_at(part++, r) && !(r.flags & kEnd)) {
+            if (wg >= q_tiles(r)) {
+                n += r.end_tile - r.first_tile;
                 continue;
             }
-            const Request r = way.it.r;
-            const bool prefix = way.it.b < 0, causal = !prefix && a.causal;
-            const int token0 = (way.it.tile * 2 + wg) * shape.tile_tokens;  // of the tile, in the request
+            const bool prefix = r.flags & kPrefix, causal = !prefix && a.causal;
+            const int token0 = r.token0 + wg * shape.tile_tokens;  // of the tile, in the request
             const int token = token0 + t / shape.group, in_group = t % shape.group;
             const bool row_ok = t < shape.tile_tokens * shape.group && token < r.rows;
             const auto limit_of = [&](int tok) {
@@ -440,7 +471,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             };
             const int limit = limit_of(row_ok ? token : r.rows - 1), low = limit_of(token0);
             float ref = -INFINITY, sum = 0.0f;
-            for (int j = way.first_tile; j < way.end_tile; ++j, ++n) {
+            for (int j = r.first_tile; j < r.end_tile; ++j, ++n) {
                 const int key0 = j * kTile;
                 if (!mbar_wait_bounded(&s_full[wg], seen_scores & 1, err, kDevErrTimeoutEpilogue)) {
                     ok = false;
@@ -490,7 +521,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const float keep = grown ? exp2_approx(ref - now) : 1.0f;
                     ref = now;
                     sum *= keep;
-                    if (j > way.first_tile) {
+                    if (j > r.first_tile) {
                         // The products before these scores are complete with them.
 #pragma unroll 1
                         for (int c = 0; c < kD / 32; ++c) {
@@ -538,7 +569,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                         if (valid > 0 && valid % shape.box != 0) clear_tail<kD>(v_tile, valid, shape.box, t);
                         if (from_key < valid) {
                             wild = group_any(wg, wild_rows<T, kD>(v_tile, from_key, valid, t));
-                            if (wild) add_own_values<T, kD>(o_addr, s_addr, v_tile, limit - key0, bad, j == way.first_tile);
+                            if (wild) add_own_values<T, kD>(o_addr, s_addr, v_tile, limit - key0, bad, j == r.first_tile);
                         }
                     }
                 }
@@ -548,8 +579,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 mbar_arrive(&p_ready[wg]);
             }
             if (!ok) break;
-            if (!mbar_wait_bounded(&o_done[wg], parts & 1, err, kDevErrTimeoutEpilogue)) break;
-            ++parts;
+            if (!mbar_wait_bounded(&o_done[wg], done & 1, err, kDevErrTimeoutEpilogue)) break;
+            ++done;
             tmem_fence_after();
             const int row = wg * shape.tile_tokens * shape.group + t;  // of the item
 #pragma unroll 1
@@ -564,11 +595,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     if (d >= p.dim) break;
                     const float v[4] = {__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
                                         __uint_as_float(o[k + 3])};
-                    if (way.whole)
-                        put_row<T>(a, ws, prefix, r.first + token, way.it.head * shape.group + in_group, d, v, ref, sum);
+                    if (r.flags & kWhole)
+                        put_row<T>(a, ws, prefix, r.first + token, r.head * shape.group + in_group, d, v, ref, sum);
                     else
                         put_part(ws.part_sums[1], ws.part_stats[1],
-                                 ((long long)blockIdx.x * 2 + way.slot) * kManyRows + row, kD, d, v, ref, sum);
+                                 ((long long)blockIdx.x * 2 + (r.flags & kSecondSlot ? 1 : 0)) * kManyRows + row, kD, d, v, ref, sum);
                 }
             }
             tmem_fence_before();  // O has been read before the next weights are announced
