@@ -116,7 +116,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
     pdl_wait_primary();
     pdl_launch_dependents();
     const FewPlan plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
-    Cursor<FewPlan> way(plan, find_block<kThreads>(plan, blockIdx.x, gridDim.x, scratch), blockIdx.x);
+    const Found found = find_block<kThreads>(plan, blockIdx.x, gridDim.x, scratch);
+    Cursor<FewPlan> way(plan, found, blockIdx.x);
+    if (threadIdx.x == 0) ws.cuts[0][blockIdx.x] = way.cut(found.share, blockIdx.x, kRows);
 
     while (way.next()) {
         const Request r = way.it.r;
@@ -395,27 +397,17 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
 // Joins the items that borders of the kernel of few rows (the first few_blocks - 1
 // blocks) and of the other kernel (eight blocks a border, 32 rows each) cut.
 template <class T, int kD, int kMT>
-__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_blocks,
-                                                                 int many_blocks) {
-    __shared__ long long scratch[kJoinThreads / 32 + 2];
+__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_blocks) {
     extern __shared__ int parts[];
-    const PagedBatch& p = a.batch;
-    const int group = a.heads / p.kv_heads, borders = max(few_blocks - 1, 0);
-    // The plans' inputs are older than the kernel before this one, which has
-    // waited for their writers.
-    const int prefix_rows = a.prefix_length > 0 ? live_rows(p) : 0;
-    if ((int)blockIdx.x < borders) {
-        const FewPlan plan{a, group, prefix_rows};
-        join_item<T, 16 * kMT, kD, kJoinThreads>(plan, ws, 0, blockIdx.x + 1, few_blocks, 16 * kMT, 0, scratch,
-                                                   parts);
-    } else {
-        const int tokens = kManyRows / 2 / group * 2;
-        const ManyPlan plan{a, group, prefix_rows, tokens};
-        const int k = blockIdx.x - borders;
-        constexpr int kSlices = kManyRows / kSliceRows;
-        join_item<T, kManyRows, kD, kJoinThreads>(plan, ws, 1, k / kSlices + 1, many_blocks, tokens * group,
-                                                  k % kSlices * kSliceRows, scratch, parts);
-    }
+    pdl_launch_dependents();
+    pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
+    const int borders = max(few_blocks - 1, 0), k = (int)blockIdx.x - borders;
+    constexpr int kSlices = kManyRows / kSliceRows;
+    if (k < 0)
+        join_item<T, FewPlan, 16 * kMT, kD, false, kJoinThreads>(a, ws, 0, blockIdx.x + 1, 0, parts);
+    else
+        join_item<T, ManyPlan, kManyRows, kD, true, kJoinThreads>(a, ws, 1, k / kSlices + 1, k % kSlices * kSliceRows,
+                                                                  parts);
 }
 
 // Joins the own and the prefix result of every row that a request owns.
@@ -476,7 +468,7 @@ cudaError_t launch_t(const AttentionArgs& a, int dtype, const Shape& s, const Wo
                       (s.many_blocks ? (s.many_blocks - 1) * (kManyRows / kSliceRows) : 0);
     const size_t parts = sizeof(int) * (size_t)(s.few_blocks > s.many_blocks ? s.few_blocks : s.many_blocks);
     e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(joins), dim3(kJoinThreads), parts, stream, a, ws,
-                          s.few_blocks, s.many_blocks);
+                          s.few_blocks);
     if (e != cudaSuccess || a.prefix_length == 0) return e;
     return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);
 }
@@ -503,6 +495,7 @@ Workspace layout(const AttentionArgs& a, const Shape& s, uint8_t* base, size_t* 
     for (int k = 0; k < 2; ++k) {
         ws.part_sums[k] = take(parts[k] * s.width);
         ws.part_stats[k] = take(parts[k] * 2);
+        ws.cuts[k] = reinterpret_cast<Cut*>(take((size_t)(k ? s.many_blocks : s.few_blocks) * (sizeof(Cut) / sizeof(float))));
     }
     if (a.prefix_length > 0) {
         const size_t rows = (size_t)a.batch.rows * a.heads;

@@ -10,9 +10,14 @@ namespace attn {
 
 // Sums are kept as the unscaled output row, with the maximum (base 2) that its
 // weights are relative to and their sum.
+struct Cut;
 struct Workspace {
-    float* part_sums[2];   // parts of cut items of the kernel of few rows and of the other: [block][2][rows][width]
-    float* part_stats[2];  // [block][2][rows][2]
+    // Of the kernel of few rows and of the other: parts of cut items, [block][2][rows][width]
+    // and [block][2][width / 4][rows][4] (a thread a row there), their statistics
+    // [block][2][rows][2], and by block the item that its first unit cuts.
+    float* part_sums[2];
+    float* part_stats[2];
+    Cut* cuts[2];
     float* row_sums[2];    // with a prefix: own and prefix sums of every row, [rows][heads][dim]
     float* row_stats[2];   // [rows][heads][2]
 };
@@ -113,8 +118,8 @@ struct FewPlan {
         it.end += it.key_tiles;
         return true;
     }
-    __device__ __forceinline__ int cut(const Item& it, long long unit) const {
-        return (int)(min(max(unit, it.start), it.end) - it.start);
+    __device__ static __forceinline__ int cut(long long start, long long end, int, long long unit) {
+        return (int)(min(max(unit, start), end) - start);
     }
 };
 
@@ -180,12 +185,22 @@ struct ManyPlan {
         it.key_tiles = key_tiles(it.b, it.r, it.tile);
         return true;
     }
-    __device__ __forceinline__ int cut(const Item& it, long long unit) const {
-        return (int)((min(max(unit, it.start), it.end) - it.start) * it.key_tiles / (it.end - it.start));
+    __device__ static __forceinline__ int cut(long long start, long long end, int key_tiles, long long unit) {
+        return (int)((min(max(unit, start), end) - start) * key_tiles / (end - start));
     }
 };
 __device__ __forceinline__ long long cost_of(const FewPlan& plan, int, const Request& r) { return plan.cost(r); }
 __device__ __forceinline__ long long cost_of(const ManyPlan& plan, int b, const Request& r) { return plan.cost_of(b, r); }
+
+// What the join needs to know of an item that the border in front of a block's
+// first unit cuts; rows 0: none, or an earlier border cuts it too.
+struct alignas(16) Cut {
+    long long start, end, share;
+    int rows;       // of the item
+    int first_row;  // of the request
+    int row0;       // the item's first, among the request's rows of the kv head
+    int head, key_tiles, prefix;
+};
 
 struct Found {
     long long share;   // units a block
@@ -268,8 +283,8 @@ struct Cursor {
                 it = plan.first(b, r, unit);
             }
             const long long to = min(it.end, last);
-            first_tile = unit == it.start ? 0 : plan.cut(it, unit);
-            end_tile = to == it.end ? it.key_tiles : plan.cut(it, to);
+            first_tile = unit == it.start ? 0 : Plan::cut(it.start, it.end, it.key_tiles, unit);
+            end_tile = to == it.end ? it.key_tiles : Plan::cut(it.start, it.end, it.key_tiles, to);
             unit = to;
             if (first_tile < end_tile) {
                 whole = first_tile == 0 && end_tile == it.key_tiles;
@@ -278,6 +293,16 @@ struct Cursor {
             }
         }
         return false;
+    }
+
+    // The cut that block g's own first border makes (before the first next()).
+    __device__ __forceinline__ Cut cut(long long share, long long g, int tile_rows) const {
+        Cut c{};
+        if (unit < last && it.start < unit && it.start >= (g - 1) * share) {
+            c = Cut{it.start, it.end, share, 0, it.r.first, it.tile * tile_rows, it.head, it.key_tiles, it.b < 0};
+            c.rows = (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - c.row0);
+        }
+        return c;
     }
 
   private:
@@ -335,40 +360,35 @@ struct Joined {
     }
 };
 
-// Joins the parts of the item that border g (block g's first unit) cuts, if it is
-// the first border inside it: rows [from, from + kSliceRows) of it.  kRows, kWidth:
-// a part's; tile_rows of them used.  `parts` holds the numbers of `blocks` parts.
+// Joins the parts of the item that border g (in front of block g's first unit)
+// cuts: rows [from, from + kSliceRows) of it.  kRows, kWidth: a part's; kByRow: its
+// rows lie side by side (the kernel of many rows).  `parts` has room for the
+// numbers of all parts.
 constexpr int kSliceRows = 32;
-template <class T, int kRows, int kWidth, int kThreads, class Plan>
-__device__ void join_item(const Plan& plan, const Workspace& ws, int kind, int g, int blocks, int tile_rows, int from,
-                          long long* scratch, int* parts) {
-    const AttentionArgs& a = plan.a;
+template <class T, class Plan, int kRows, int kWidth, bool kByRow, int kThreads>
+__device__ void join_item(const AttentionArgs& a, const Workspace& ws, int kind, int g, int from, int* parts) {
     const PagedBatch& p = a.batch;
-    const Found at = find_block<kThreads>(plan, g, blocks, scratch);
-    pdl_launch_dependents();
-    const long long u = g * at.share;
-    Item it{};
-    bool mine = u < at.total;
-    if (mine) {
-        it = plan.item(at.b, plan.get(at.b), at.before, u);
-        mine = u > it.start && (g - 1) * at.share <= it.start;
+    const int group = a.heads / p.kv_heads;
+    Cut c;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(Cut) / 16); ++i) {
+        const uint4 w = load_l2(reinterpret_cast<const uint4*>(ws.cuts[kind] + g) + i);
+        memcpy(reinterpret_cast<char*>(&c) + 16 * i, &w, 16);
     }
-    const int row0 = it.tile * tile_rows;
-    const int rows = mine ? (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - row0) : 0;
-    pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
-    if (from >= rows) return;
+    if (from >= c.rows) return;
     // Blocks g - 1 .. hold parts of it; those without key tiles wrote none, and an
     // item that one block holds alone is finished.
     __shared__ int count;
     if (threadIdx.x < 32) {
-        const int lane = threadIdx.x, h1 = (int)((it.end - 1) / at.share);
+        const int lane = threadIdx.x, h1 = (int)((c.end - 1) / c.share);
         int n = 0;
         for (int h0 = g - 1; h0 <= h1; h0 += 32) {
             const int h = h0 + lane;
-            const bool has = h <= h1 && plan.cut(it, h * at.share) < plan.cut(it, (h + 1) * at.share);
+            const bool has = h <= h1 && Plan::cut(c.start, c.end, c.key_tiles, h * c.share) <
+                                            Plan::cut(c.start, c.end, c.key_tiles, (h + 1) * c.share);
             const unsigned m = __ballot_sync(0xffffffffu, has);
             // the first block's part may lie in its second slot
-            if (has) parts[n + __popc(m & ((1u << lane) - 1u))] = 2 * h + (h == g - 1 && h * at.share < it.start ? 1 : 0);
+            if (has) parts[n + __popc(m & ((1u << lane) - 1u))] = 2 * h + (h == g - 1 && h * c.share < c.start ? 1 : 0);
             n += __popc(m);
         }
         if (lane == 0) count = n;
@@ -376,29 +396,32 @@ __device__ void join_item(const Plan& plan, const Workspace& ws, int kind, int g
     __syncthreads();
     const int n = count;
     if (n < 2) return;
-    const int last = min(rows, from + kSliceRows);
-    for (int i = threadIdx.x; i < (last - from) * (kWidth / 4); i += kThreads) {
-        const int row = from + i / (kWidth / 4), d = i % (kWidth / 4) * 4;
-        if (d >= p.dim) continue;
+    const int rows = min(c.rows - from, kSliceRows);
+    for (int i = threadIdx.x; i < kSliceRows * (kWidth / 4); i += kThreads) {
+        const int in = kByRow ? i % kSliceRows : i / (kWidth / 4);
+        const int d = (kByRow ? i / kSliceRows : i % (kWidth / 4)) * 4, row = from + in;
+        if (d >= p.dim || in >= rows) continue;
         Joined j;
-        for (int k0 = 0; k0 < n; k0 += 8) {
-            float2 stats[8];
-            float4 sums[8];
+        for (int k0 = 0; k0 < n; k0 += 4) {
+            float2 stats[4];
+            float4 sums[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {  // eight parts' loads under way at once
+            for (int k = 0; k < 4; ++k) {  // four parts' loads under way at once
                 stats[k] = make_float2(-INFINITY, 0.0f);
                 sums[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (k0 + k < n) {
-                    const long long at_row = (long long)parts[k0 + k] * kRows + row;
-                    stats[k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + at_row);
-                    sums[k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind] + at_row * kWidth + d));
+                    const long long part = parts[k0 + k];
+                    const long long at = kByRow ? (part * (kWidth / 4) + d / 4) * kRows + row
+                                                : (part * kRows + row) * (kWidth / 4) + d / 4;
+                    stats[k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + part * kRows + row);
+                    sums[k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind]) + at);
                 }
             }
 #pragma unroll
-            for (int k = 0; k < 8; ++k) j.add(stats[k], sums[k]);
+            for (int k = 0; k < 4; ++k) j.add(stats[k], sums[k]);
         }
-        const int token = (row0 + row) / plan.group, head = it.head * plan.group + (row0 + row) % plan.group;
-        put_row<T>(a, ws, it.b < 0, it.r.first + token, head, d, j.v, j.most, j.total);
+        const int token = (c.row0 + row) / group, head = c.head * group + (c.row0 + row) % group;
+        put_row<T>(a, ws, c.prefix, c.first_row + token, head, d, j.v, j.most, j.total);
     }
 }
 

@@ -10,11 +10,14 @@
 //                page; tokens that do not exist are boxes outside the tensor, which
 //                arrive as zeros.
 //   warp 8       issues the MMAs: S_i = Q_i K^T into TMEM, O_i += P_i V with P_i read
-//                from TMEM, the two tiles by turns, so that the tensor cores work on
-//                one while the other is in its softmax.  V is the MN-major operand:
-//                rows of the same boxes as K's, nothing is transposed.
+//                from TMEM, for the two tiles by turns and 64 keys at a time.  V is the
+//                MN-major operand: rows of the same boxes as K's, nothing is transposed.
 //   warps 0-7    a warpgroup a tile, a thread a row: scores from TMEM, running
 //                maximum, exp2, P back to TMEM over its own scores, 16 bits each.
+// A tile's scores have two places of 64 keys, so the next are there when a
+// warpgroup has its weights of the last ready: with one place of 128, each
+// waited for P V and Q K^T in turn, 4500 cycles for 256 rows x 128 keys where the
+// softmax itself takes 2250.
 // A row's reference is raised, and its output in TMEM rescaled, only when its
 // maximum has grown by more than 2^8 since: weights up to 2^8 lose nothing in the
 // sums' 32 bits.  P is rounded to the cache's type for the second product, half a
@@ -41,6 +44,7 @@ using namespace attn;
 
 constexpr int kManyThreads = 320;
 constexpr int kTile = 128;             // rows of a q tile, keys of a key tile
+constexpr int kStep = 64;              // keys of a step, half a key tile
 constexpr int kHalfBytes = kTile * 128;  // 128 rows x 64 elements, 128-byte swizzled
 constexpr int kBadRing = 8;
 constexpr int kPartRing = 4;
@@ -168,16 +172,14 @@ __device__ __forceinline__ const uint8_t* tile_chunk(const uint8_t* tile, int r,
     return tile + (c >> 3) * kHalfBytes + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// Rows from `valid` to the end of their box hold what the page holds behind a
-// request's last token: zeros instead, since 0 times a NaN there would count.
-// Both warpgroups write the same zeros.
+// Rows [from, to) of a value tile that hold what a page holds behind a request's
+// last token: zeros instead, since 0 times a NaN there would count.  Both
+// warpgroups write the same zeros.
 template <int kD>
-__device__ __forceinline__ void clear_tail(uint8_t* v_tile, int valid, int box, int t) {
-    const int end = min((valid + box - 1) / box * box, kTile);
-    for (int i = t; i < (end - valid) * (kD / 8); i += 128) {
-        const int r = valid + i / (kD / 8), c = i % (kD / 8);
-        *reinterpret_cast<uint4*>(const_cast<uint8_t*>(tile_chunk(v_tile, r, c))) = make_uint4(0, 0, 0, 0);
-    }
+__device__ __forceinline__ void clear_rows(uint8_t* v_tile, int from, int to, int t) {
+    for (int i = t; i < (to - from) * (kD / 8); i += 128)
+        *reinterpret_cast<uint4*>(const_cast<uint8_t*>(tile_chunk(v_tile, from + i / (kD / 8), i % (kD / 8)))) =
+            make_uint4(0, 0, 0, 0);
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
@@ -196,11 +198,12 @@ __device__ __forceinline__ bool wild_rows(const uint8_t* v_tile, int from, int t
     return wild;
 }
 
-// O += P V of one tile by the warpgroup itself, every row with the keys that it
-// sees alone (`seen` of them from the tile's start, less those of `bad` eighths).
+// O += P V of one step by the warpgroup itself, every row with the keys that it
+// sees alone (`seen` of them from the step's first, less those of `bad` eighths of
+// the key tile); `row0` is the step's first row in the value tile.
 template <class T, int kD>
-__device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, const uint8_t* v_tile, int seen, uint32_t bad,
-                                            bool first) {
+__device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, const uint8_t* v_tile, int row0, int seen,
+                                            uint32_t bad, bool first) {
     tmem_st_wait();  // P is there
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {
@@ -213,20 +216,22 @@ __device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, co
             tmem_ld_wait();
         }
 #pragma unroll 1
-        for (int k = 0; k < kTile; ++k) {
+        for (int k = 0; k < kStep; ++k) {
             const uint32_t pair = tmem_ld_32x32b_x1(p_addr + k / 2);
             tmem_ld_wait();
             Pack<T, 2> p;
             memcpy(&p, &pair, 4);
-            if (k >= seen || ((bad >> (k >> 3)) & 1)) continue;
+            const bool sees = k < seen && !((bad >> ((row0 + k) >> 3)) & 1);
             const float w = to_float(k & 1 ? p.e[1] : p.e[0]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 Pack<T, 8> v;
-                memcpy(&v, tile_chunk(v_tile, k, c * 4 + q), 16);
+                memcpy(&v, tile_chunk(v_tile, row0 + k, c * 4 + q), 16);
 #pragma unroll
-                for (int d = 0; d < 8; ++d)
-                    o[8 * q + d] = __float_as_uint(fmaf(w, to_float(v.e[d]), __uint_as_float(o[8 * q + d])));
+                for (int d = 0; d < 8; ++d) {
+                    const float sum = fmaf(w, to_float(v.e[d]), __uint_as_float(o[8 * q + d]));
+                    if (sees) o[8 * q + d] = __float_as_uint(sum);
+                }
             }
         }
         tmem_st_32x32b_x32(o_addr + c * 32, o);
@@ -238,6 +243,7 @@ struct Shape {
     int group, tile_tokens;  // tokens of a 128-row tile
     int box;                 // tokens of a page box
     int cache_end;           // a page outside the cache
+    int wide_out;            // out takes 16-byte stores
 };
 
 template <class T, int kD>
@@ -255,18 +261,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     uint64_t* q_full = bars;
     uint64_t* q_empty = bars + 1;
-    uint64_t* s_full = bars + 2;   // by tile: scores are there (MMA)
-    uint64_t* p_ready = bars + 4;  // by tile: weights are there (its warpgroup)
-    uint64_t* o_done = bars + 6;   // by tile: the item's last product is done (MMA)
-    uint64_t* mma_done = bars + 8;
-    uint64_t* kv_full = bars + 9;
+    // by tile and half, a phase a key tile
+    uint64_t* s_full = bars + 2;    // scores are there (MMA)
+    uint64_t* p_ready = bars + 6;   // weights are there (the tile's warpgroup)
+    uint64_t* o_done = bars + 10;   // the product with the values is done (MMA)
+    uint64_t* mma_done = bars + 14;
+    uint64_t* kv_full = bars + 15;
     uint64_t* kv_empty = kv_full + kSlots;
     uint32_t* bad_ring = reinterpret_cast<uint32_t*>(kv_empty + kSlots);  // eighths of a key tile on no page
-    volatile uint32_t* own = bad_ring + kBadRing;                         // by tile: its warpgroup added the values
-    uint32_t* tmem_slot = bad_ring + kBadRing + 2;
-    uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 4);
+    volatile uint32_t* own = bad_ring + kBadRing;  // by tile and half: its warpgroup added the values
+    uint32_t* tmem_slot = bad_ring + kBadRing + 4;
+    uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 6);
     Part* parts = reinterpret_cast<Part*>(part_full + kPartRing);
-    static_assert((9 + 2 * 8 + kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
+    static_assert((15 + 2 * 8 + kPartRing) * 8 + (kBadRing + 6) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedBatch& p = a.batch;
 
@@ -274,7 +281,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(mma_done, 1);
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 128);
             mbar_init(&o_done[i], 1);
@@ -323,6 +330,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         uint32_t part = 0;
         bool ok = true, q_issued = false;
         Cursor<ManyPlan> way(plan, found, blockIdx.x);
+        if (lane == 0) ws.cuts[1][blockIdx.x] = way.cut(found.share, blockIdx.x, plan.tokens * shape.group);
         while (ok) {
             const bool more = way.next();
             const Request r = way.it.r;
@@ -386,19 +394,20 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             mbar_drain_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutDrain);
     } else if (warp == 8) {
         if (lane == 0) {
-            constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
+            constexpr uint32_t idesc_s = idesc_f16<T>(kStep, false), idesc_o = idesc_f16<T>(kD, true);
             const uint32_t q_u = smem_u32(smem), ring_u = smem_u32(ring);
-            const auto scores = [&](int i, int slot) {
-                const uint32_t qa = q_u + i * S::kTileBytes, kb = ring_u + slot * S::kTileBytes;
+            const auto scores = [&](int i, int half, int slot) {
+                const uint32_t qa = q_u + i * S::kTileBytes, kb = ring_u + slot * S::kTileBytes + half * kStep * 128;
 #pragma unroll
                 for (int k = 0; k < kD / 16; ++k) {
                     const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    umma_f16(tmem + i * kTile, make_sw128_desc(qa + at), make_sw128_desc(kb + at), idesc_s, k > 0);
+                    umma_f16(tmem + i * kTile + half * kStep, make_sw128_desc(qa + at), make_sw128_desc(kb + at), idesc_s,
+                             k > 0);
                 }
-                umma_commit(&s_full[i]);
+                umma_commit(&s_full[2 * i + half]);
             };
             int n = 0;
-            uint32_t part = 0, weights[2] = {0, 0};
+            uint32_t part = 0, weights[2] = {0, 0};  // key tiles whose weights have been taken, by tile
             bool ok = true;
             const auto wait_kv = [&](int seq) {
                 if (!mbar_wait_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutMma)) ok = false;
@@ -411,37 +420,37 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 ++part;
                 wait_kv(2 * n);
                 if (!ok) break;
-                for (int i = 0; i < tiles; ++i) scores(i, slot_of(2 * n));
+                for (int half = 0; half < 2; ++half)
+                    for (int i = 0; i < tiles; ++i) scores(i, half, slot_of(2 * n));
                 umma_commit(&kv_empty[slot_of(2 * n)]);
                 for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++n) {
                     const bool more = j + 1 < q.end_tile;
-                    for (int i = 0; i < tiles && ok; ++i) {
-                        if (!mbar_wait_bounded(&p_ready[i], weights[i] & 1, err, kDevErrTimeoutMma)) {
-                            ok = false;
-                            break;
-                        }
-                        ++weights[i];
-                        if (i == 0) wait_kv(2 * n + 1);
-                        if (!ok) break;
-                        tmem_fence_after();
-                        if (!own[i]) {
-                            const uint32_t vb = ring_u + slot_of(2 * n + 1) * S::kTileBytes;
-#pragma unroll
-                            for (int k = 0; k < kTile / 16; ++k)
-                                umma_f16_ts(tmem + 2 * kTile + i * kD, tmem + i * kTile + k * 8, make_mn_desc(vb + k * 2048),
-                                            idesc_o, j > q.first_tile || k > 0);
-                        }
-                        if (i == tiles - 1) umma_commit(&kv_empty[slot_of(2 * n + 1)]);
-                        if (more) {
-                            if (i == 0) wait_kv(2 * n + 2);
+                    for (int half = 0; half < 2 && ok; ++half) {
+                        for (int i = 0; i < tiles; ++i) {
+                            const int at = 2 * i + half;
+                            if (!mbar_wait_bounded(&p_ready[at], weights[i] & 1, err, kDevErrTimeoutMma)) ok = false;
+                            if (at == 0) wait_kv(2 * n + 1);
                             if (!ok) break;
-                            scores(i, slot_of(2 * n + 2));
-                            if (i == tiles - 1) umma_commit(&kv_empty[slot_of(2 * n + 2)]);
-                        } else {
-                            umma_commit(&o_done[i]);
-                            if (i == tiles - 1) umma_commit(q_empty);
+                            tmem_fence_after();
+                            if (!own[at]) {
+                                const uint32_t vb = ring_u + slot_of(2 * n + 1) * S::kTileBytes + half * kStep * 128;
+#pragma unroll
+                                for (int k = 0; k < kStep / 16; ++k)
+                                    umma_f16_ts(tmem + 2 * kTile + i * kD, tmem + i * kTile + half * kStep + k * 8,
+                                                make_mn_desc(vb + k * 2048), idesc_o, j > q.first_tile || half > 0 || k > 0);
+                            }
+                            umma_commit(&o_done[at]);
+                            if (more) {
+                                if (at == 0) wait_kv(2 * n + 2);
+                                if (!ok) break;
+                                scores(i, half, slot_of(2 * n + 2));
+                            }
                         }
                     }
+                    if (!ok) break;
+                    for (int i = 0; i < tiles; ++i) ++weights[i];
+                    umma_commit(&kv_empty[slot_of(2 * n + 1)]);
+                    umma_commit(more ? &kv_empty[slot_of(2 * n + 2)] : q_empty);
                 }
             }
             // All MMAs issued by this thread complete before TMEM is freed.
@@ -451,10 +460,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     } else {
         const int wg = warp >> 2, t = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_addr = tmem + lanes + wg * kTile, o_addr = tmem + lanes + 2 * kTile + wg * kD;
+        const uint32_t o_addr = tmem + lanes + 2 * kTile + wg * kD;
         const float scale = a.scale_log2;
         int n = 0;
-        uint32_t seen_scores = 0, done = 0, part = 0;
+        uint32_t tiles_done = 0, part = 0;
         bool ok = true;
         Part r;
         while (ok && part_at(part++, r) && !(r.flags & kEnd)) {
@@ -462,7 +471,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 n += r.end_tile - r.first_tile;
                 continue;
             }
-            const bool prefix = r.flags & kPrefix, causal = !prefix && a.causal;
+            const bool causal = !(r.flags & kPrefix) && a.causal;
             const int token0 = r.token0 + wg * shape.tile_tokens;  // of the tile, in the request
             const int token = token0 + t / shape.group, in_group = t % shape.group;
             const bool row_ok = t < shape.tile_tokens * shape.group && token < r.rows;
@@ -471,136 +480,172 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             };
             const int limit = limit_of(row_ok ? token : r.rows - 1), low = limit_of(token0);
             float ref = -INFINITY, sum = 0.0f;
-            for (int j = r.first_tile; j < r.end_tile; ++j, ++n) {
-                const int key0 = j * kTile;
-                if (!mbar_wait_bounded(&s_full[wg], seen_scores & 1, err, kDevErrTimeoutEpilogue)) {
-                    ok = false;
-                    break;
-                }
-                ++seen_scores;
-                tmem_fence_after();
-                const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
-                // The scores are read twice, 32 a time, for the maximum and for the
-                // weights: a row of 128 does not fit beside the rest of the thread's
-                // registers.  Where some are masked (or the scale turns the order
-                // around), the first pass leaves them scaled and masked.
-                const bool masked = key0 + kTile > low || bad, rewrite = masked || scale < 0.0f;
-                float mul = scale, most = -INFINITY;
-                {
+            for (int j = r.first_tile; j < r.end_tile && ok; ++j, ++n, ++tiles_done) {
+#pragma unroll 1
+                for (int half = 0; half < 2; ++half) {
+                    const int at = 2 * wg + half, key0 = j * kTile + half * kStep;
+                    const uint32_t s_addr = tmem + lanes + wg * kTile + half * kStep;
+                    if (!mbar_wait_bounded(&s_full[at], tiles_done & 1, err, kDevErrTimeoutEpilogue)) {
+                        ok = false;
+                        break;
+                    }
+                    tmem_fence_after();
+                    const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
                     uint32_t s[2][32];
                     tmem_ld_32x32b_x32(s_addr, s[0]);
+                    tmem_ld_32x32b_x32(s_addr + 32, s[1]);
+                    tmem_ld_wait();
+                    // Masked scores are scaled first; so are all where the scale turns
+                    // the order around.
+                    const bool masked = key0 + kStep > low || bad;
+                    float mul = scale;
+                    if (masked || scale < 0.0f) {
+                        const uint32_t gone = bad >> (half * (kStep / 8));
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld_wait();
-                        uint32_t(&x)[32] = s[c & 1];
-                        if (c < 3) tmem_ld_32x32b_x32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
-                        if (rewrite) {
+                        for (int c = 0; c < 2; ++c)
 #pragma unroll
                             for (int k = 0; k < 32; ++k) {
                                 const int key = c * 32 + k;
-                                const bool out = key >= limit - key0 || ((bad >> (key >> 3)) & 1);
-                                x[k] = __float_as_uint(out ? -INFINITY : __uint_as_float(x[k]) * scale);
+                                const bool out = key >= limit - key0 || ((gone >> (key >> 3)) & 1);
+                                s[c][k] = __float_as_uint(out ? -INFINITY : __uint_as_float(s[c][k]) * scale);
                             }
-                            tmem_st_32x32b_x32(s_addr + c * 32, x);
-                        }
-                        float m[4];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k)
-                            m[k & 3] = k < 4 ? __uint_as_float(x[k]) : fmaxf(m[k & 3], __uint_as_float(x[k]));
-                        most = fmaxf(most, fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-                    }
-                    if (rewrite) {
-                        tmem_st_wait();
                         mul = 1.0f;
                     }
-                }
-                const float top = most * mul;
-                const bool grown = top > ref + 8.0f;  // from -inf: by anything
-                if (__any_sync(0xffffffffu, grown)) {
-                    const float now = grown ? top : ref;
-                    const float keep = grown ? exp2_approx(ref - now) : 1.0f;
-                    ref = now;
-                    sum *= keep;
-                    if (j > r.first_tile) {
-                        // The products before these scores are complete with them.
-#pragma unroll 1
-                        for (int c = 0; c < kD / 32; ++c) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(o_addr + c * 32, o);
-                            tmem_ld_wait();
+                    float m[4];
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                            tmem_st_32x32b_x32(o_addr + c * 32, o);
+                    for (int k = 0; k < 32; ++k) {
+                        const float x = fmaxf(__uint_as_float(s[0][k]), __uint_as_float(s[1][k]));
+                        m[k & 3] = k < 4 ? x : fmaxf(m[k & 3], x);
+                    }
+                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
+                    const bool grown = top > ref + 8.0f;  // from -inf: by anything
+                    if (__any_sync(0xffffffffu, grown)) {
+                        const float now = grown ? top : ref;
+                        const float keep = grown ? exp2_approx(ref - now) : 1.0f;
+                        ref = now;
+                        sum *= keep;
+                        if (j > r.first_tile || half > 0) {
+                            // The product of the step before must be in O.
+                            const uint32_t phase = half ? tiles_done : tiles_done - 1;
+                            if (!mbar_wait_bounded(&o_done[at ^ 1], phase & 1, err, kDevErrTimeoutEpilogue)) {
+                                ok = false;
+                                break;
+                            }
+                            tmem_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < kD / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_ld_32x32b_x32(o_addr + c * 32, o);
+                                tmem_ld_wait();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                                tmem_st_32x32b_x32(o_addr + c * 32, o);
+                            }
                         }
                     }
-                }
-                const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
-                float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                {
-                    uint32_t s[2][32];
-                    tmem_ld_32x32b_x32(s_addr, s[0]);
+                    const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
+                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        tmem_ld_wait();
-                        const uint32_t(&x)[32] = s[c & 1];
-                        if (c < 3) tmem_ld_32x32b_x32(s_addr + (c + 1) * 32, s[(c + 1) & 1]);
+                    for (int c = 0; c < 2; ++c) {
                         uint32_t w[16];
 #pragma unroll
                         for (int k = 0; k < 16; ++k) {
-                            const float u = exp2_approx(fmaf(__uint_as_float(x[2 * k]), mul, from));
-                            const float v = exp2_approx(fmaf(__uint_as_float(x[2 * k + 1]), mul, from));
-                            part[k & 3] += u + v;
+                            const float u = exp2_approx(fmaf(__uint_as_float(s[c][2 * k]), mul, from));
+                            const float v = exp2_approx(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, from));
+                            acc[k & 3] += u + v;
                             w[k] = pack_pair<T>(u, v);
                         }
                         tmem_st_32x32b_x16(s_addr + c * 16, w);
                     }
-                }
-                sum += (part[0] + part[1]) + (part[2] + part[3]);
-                bool wild = false;
-                if (masked) {
-                    const int valid = min(kTile, r.length - key0), from_key = max(low - key0, 0);
-                    if (valid % shape.box != 0 || from_key < valid) {
-                        uint8_t* v_tile = ring + slot_of(2 * n + 1) * S::kTileBytes;
-                        if (!mbar_wait_bounded(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1), err,
-                                               kDevErrTimeoutEpilogue)) {
-                            ok = false;
-                            break;
-                        }
-                        if (valid > 0 && valid % shape.box != 0) clear_tail<kD>(v_tile, valid, shape.box, t);
-                        if (from_key < valid) {
-                            wild = group_any(wg, wild_rows<T, kD>(v_tile, from_key, valid, t));
-                            if (wild) add_own_values<T, kD>(o_addr, s_addr, v_tile, limit - key0, bad, j == r.first_tile);
+                    sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                    bool wild = false;
+                    if (masked) {
+                        // Rows of this step in the value tile: those behind the
+                        // request's last token in its box, those that some row does not see.
+                        const int valid = min(kTile, r.length - j * kTile), row0 = half * kStep, row1 = row0 + kStep;
+                        const int clear0 = max(valid, row0);
+                        const int clear1 = min((valid + shape.box - 1) / shape.box * shape.box, row1);
+                        const int from_row = max(low - j * kTile, row0), to_row = min(valid, row1);
+                        if (clear0 < clear1 || from_row < to_row) {
+                            uint8_t* v_tile = ring + slot_of(2 * n + 1) * S::kTileBytes;
+                            if (!mbar_wait_bounded(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1), err,
+                                                   kDevErrTimeoutEpilogue)) {
+                                ok = false;
+                                break;
+                            }
+                            if (clear0 < clear1) clear_rows<kD>(v_tile, clear0, clear1, t);
+                            if (from_row < to_row) {
+                                wild = group_any(wg, wild_rows<T, kD>(v_tile, from_row, to_row, t));
+                                if (wild) {
+                                    const bool first = j == r.first_tile && half == 0;
+                                    // The products before must be in O.
+                                    if (!first && !mbar_wait_bounded(&o_done[at ^ 1], (half ? tiles_done : tiles_done - 1) & 1,
+                                                                     err, kDevErrTimeoutEpilogue)) {
+                                        ok = false;
+                                        break;
+                                    }
+                                    tmem_fence_after();
+                                    add_own_values<T, kD>(o_addr, s_addr, v_tile, row0, limit - key0, bad, first);
+                                }
+                            }
                         }
                     }
+                    if (t == 0) own[at] = wild;
+                    tmem_st_wait();
+                    tmem_fence_before();
+                    mbar_arrive(&p_ready[at]);
                 }
-                if (t == 0) own[wg] = wild;
-                tmem_st_wait();
-                tmem_fence_before();
-                mbar_arrive(&p_ready[wg]);
             }
             if (!ok) break;
-            if (!mbar_wait_bounded(&o_done[wg], done & 1, err, kDevErrTimeoutEpilogue)) break;
-            ++done;
+            if (!mbar_wait_bounded(&o_done[2 * wg + 1], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) break;
             tmem_fence_after();
             const int row = wg * shape.tile_tokens * shape.group + t;  // of the item
+            const bool whole = r.flags & kWhole, final = whole && a.prefix_length == 0;
+            const int head = r.head * shape.group + in_group;
+            const float norm = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that sees no key is zero
+            const long long part_at_row = (long long)blockIdx.x * 2 + (r.flags & kSecondSlot ? 1 : 0);
+            if (!whole && row_ok)
+                *reinterpret_cast<float2*>(ws.part_stats[1] + 2 * (part_at_row * kManyRows + row)) = make_float2(ref, sum);
+            T* out_row = static_cast<T*>(a.out) + (long long)(r.first + token) * a.ld_out + (long long)head * p.dim;
 #pragma unroll 1
             for (int c = 0; c < kD / 32; ++c) {
                 uint32_t o[32];
                 tmem_ld_32x32b_x32(o_addr + c * 32, o);
                 tmem_ld_wait();
-                if (!row_ok) continue;
+                if (row_ok) {
 #pragma unroll
-                for (int k = 0; k < 32; k += 4) {
-                    const int d = c * 32 + k;
-                    if (d >= p.dim) break;
-                    const float v[4] = {__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
-                                        __uint_as_float(o[k + 3])};
-                    if (r.flags & kWhole)
-                        put_row<T>(a, ws, prefix, r.first + token, r.head * shape.group + in_group, d, v, ref, sum);
-                    else
-                        put_part(ws.part_sums[1], ws.part_stats[1],
-                                 ((long long)blockIdx.x * 2 + (r.flags & kSecondSlot ? 1 : 0)) * kManyRows + row, kD, d, v, ref, sum);
+                    for (int k = 0; k < 32; k += 8) {
+                        const int d = c * 32 + k;
+                        if (d < p.dim) {
+                            if (final) {
+                                Pack<T, 8> w;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e)
+                                    w.e[e] = from_float<T>(sum == 0.0f ? 0.0f : __uint_as_float(o[k + e]) * norm);
+                                if (shape.wide_out) {
+                                    *reinterpret_cast<Pack<T, 8>*>(out_row + d) = w;
+                                } else {
+                                    const uint2* h = reinterpret_cast<const uint2*>(&w);
+                                    reinterpret_cast<uint2*>(out_row + d)[0] = h[0];
+                                    reinterpret_cast<uint2*>(out_row + d)[1] = h[1];
+                                }
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; e += 4) {
+                                    const float v[4] = {__uint_as_float(o[k + e]), __uint_as_float(o[k + e + 1]),
+                                                        __uint_as_float(o[k + e + 2]), __uint_as_float(o[k + e + 3])};
+                                    if (whole)
+                                        put_row<T>(a, ws, r.flags & kPrefix, r.first + token, head, d + e, v, ref, sum);
+                                    else
+                                        *reinterpret_cast<float4*>(
+                                            ws.part_sums[1] + 4 * ((part_at_row * (kD / 4) + (d + e) / 4) * kManyRows + row)) =
+                                            make_float4(v[0], v[1], v[2], v[3]);
+                                }
+                            }
+                        }
+                    }
                 }
+                __syncwarp();
             }
             tmem_fence_before();  // O has been read before the next weights are announced
         }
@@ -622,6 +667,7 @@ cudaError_t launch_many_t(const AttentionArgs& a, const Workspace& ws, int block
     // A cache without pages: a view of one that no box asks for.
     const int pages = p.cache_pages > 0 ? p.cache_pages : 1;
     s.cache_end = pages;
+    s.wide_out = a.ld_out % 8 == 0 && reinterpret_cast<uintptr_t>(a.out) % 16 == 0;
     uint32_t* err = nullptr;
     if (device_error_word(&err) != ZQ_OK) return cudaErrorUnknown;
     const CUtensorMapDataType type =
