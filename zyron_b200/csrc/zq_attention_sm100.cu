@@ -10,14 +10,16 @@
 //                page; tokens that do not exist are boxes outside the tensor, which
 //                arrive as zeros.
 //   warp 8       issues the MMAs: S_i = Q_i K^T into TMEM, O_i += P_i V with P_i read
-//                from TMEM, for the two tiles by turns and 64 keys at a time.  V is the
-//                MN-major operand: rows of the same boxes as K's, nothing is transposed.
-//   warps 0-7    a warpgroup a tile, a thread a row: scores from TMEM, running
-//                maximum, exp2, P back to TMEM over its own scores, 16 bits each.
-// A tile's scores have two places of 64 keys, so the next are there when a
-// warpgroup has its weights of the last ready: with one place of 128, each
-// waited for P V and Q K^T in turn, 4500 cycles for 256 rows x 128 keys where the
-// softmax itself takes 2250.
+//                from TMEM, for the two tiles by turns.  V is the MN-major operand:
+//                rows of the same boxes as K's, nothing is transposed.
+//   warps 0-7    a warpgroup a tile, a thread a row: scores from TMEM into registers,
+//                running maximum, exp2, P back to TMEM, 16 bits each.
+// TMEM holds the two outputs, the two P and one S, which both tiles use by turns:
+// a warpgroup takes its scores into registers at once, so the next product starts
+// while it works, and finds its next scores there when it is done.  With a place of
+// its own for each tile's scores, P over them, a warpgroup waited for P V and Q K^T
+// in turn: 4500 cycles for 256 rows x 128 keys (5700 in steps of 64 keys, since an
+// MMA of 64 columns takes as long as one of 128), where the softmax takes 2250.
 // A row's reference is raised, and its output in TMEM rescaled, only when its
 // maximum has grown by more than 2^8 since: weights up to 2^8 lose nothing in the
 // sums' 32 bits.  P is rounded to the cache's type for the second product, half a
@@ -44,7 +46,8 @@ using namespace attn;
 
 constexpr int kManyThreads = 320;
 constexpr int kTile = 128;             // rows of a q tile, keys of a key tile
-constexpr int kStep = 64;              // keys of a step, half a key tile
+// TMEM columns: the scores of whichever tile, P (two keys a column), O.
+constexpr int kScoreCol = 0, kWeightCol = 128, kOutCol = 256;
 constexpr int kHalfBytes = kTile * 128;  // 128 rows x 64 elements, 128-byte swizzled
 constexpr int kBadRing = 8;
 constexpr int kPartRing = 4;
@@ -117,13 +120,15 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* tmap, uint64_
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
     asm volatile(
@@ -198,12 +203,11 @@ __device__ __forceinline__ bool wild_rows(const uint8_t* v_tile, int from, int t
     return wild;
 }
 
-// O += P V of one step by the warpgroup itself, every row with the keys that it
-// sees alone (`seen` of them from the step's first, less those of `bad` eighths of
-// the key tile); `row0` is the step's first row in the value tile.
+// O += P V of one key tile by the warpgroup itself, every row with the keys that it
+// sees alone (`seen` of them, less those of `bad` eighths).
 template <class T, int kD>
-__device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, const uint8_t* v_tile, int row0, int seen,
-                                            uint32_t bad, bool first) {
+__device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, const uint8_t* v_tile, int seen, uint32_t bad,
+                                            bool first) {
     tmem_st_wait();  // P is there
 #pragma unroll 1
     for (int c = 0; c < kD / 32; ++c) {
@@ -216,17 +220,17 @@ __device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, co
             tmem_ld_wait();
         }
 #pragma unroll 1
-        for (int k = 0; k < kStep; ++k) {
+        for (int k = 0; k < kTile; ++k) {
             const uint32_t pair = tmem_ld_32x32b_x1(p_addr + k / 2);
             tmem_ld_wait();
             Pack<T, 2> p;
             memcpy(&p, &pair, 4);
-            const bool sees = k < seen && !((bad >> ((row0 + k) >> 3)) & 1);
+            const bool sees = k < seen && !((bad >> (k >> 3)) & 1);
             const float w = to_float(k & 1 ? p.e[1] : p.e[0]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 Pack<T, 8> v;
-                memcpy(&v, tile_chunk(v_tile, row0 + k, c * 4 + q), 16);
+                memcpy(&v, tile_chunk(v_tile, k, c * 4 + q), 16);
 #pragma unroll
                 for (int d = 0; d < 8; ++d) {
                     const float sum = fmaf(w, to_float(v.e[d]), __uint_as_float(o[8 * q + d]));
@@ -261,19 +265,20 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kBars);
     uint64_t* q_full = bars;
     uint64_t* q_empty = bars + 1;
-    // by tile and half, a phase a key tile
-    uint64_t* s_full = bars + 2;    // scores are there (MMA)
-    uint64_t* p_ready = bars + 6;   // weights are there (the tile's warpgroup)
-    uint64_t* o_done = bars + 10;   // the product with the values is done (MMA)
-    uint64_t* mma_done = bars + 14;
-    uint64_t* kv_full = bars + 15;
+    // by tile, a phase a key tile
+    uint64_t* s_full = bars + 2;   // scores are there (MMA)
+    uint64_t* p_ready = bars + 4;  // weights are there (the tile's warpgroup)
+    uint64_t* o_done = bars + 6;   // the product with the values is done (MMA)
+    uint64_t* s_free = bars + 8;   // the scores have been taken (whichever warpgroup's they are)
+    uint64_t* mma_done = bars + 9;
+    uint64_t* kv_full = bars + 10;
     uint64_t* kv_empty = kv_full + kSlots;
     uint32_t* bad_ring = reinterpret_cast<uint32_t*>(kv_empty + kSlots);  // eighths of a key tile on no page
-    volatile uint32_t* own = bad_ring + kBadRing;  // by tile and half: its warpgroup added the values
-    uint32_t* tmem_slot = bad_ring + kBadRing + 4;
-    uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 6);
+    volatile uint32_t* own = bad_ring + kBadRing;  // by tile: its warpgroup added the values
+    uint32_t* tmem_slot = bad_ring + kBadRing + 2;
+    uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 4);
     Part* parts = reinterpret_cast<Part*>(part_full + kPartRing);
-    static_assert((15 + 2 * 8 + kPartRing) * 8 + (kBadRing + 6) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
+    static_assert((10 + 2 * 8 + kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedBatch& p = a.batch;
 
@@ -281,7 +286,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
         mbar_init(mma_done, 1);
-        for (int i = 0; i < 4; ++i) {
+        mbar_init(s_free, 128);
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 128);
             mbar_init(&o_done[i], 1);
@@ -394,64 +400,60 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             mbar_drain_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutDrain);
     } else if (warp == 8) {
         if (lane == 0) {
-            constexpr uint32_t idesc_s = idesc_f16<T>(kStep, false), idesc_o = idesc_f16<T>(kD, true);
+            constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
             const uint32_t q_u = smem_u32(smem), ring_u = smem_u32(ring);
-            const auto scores = [&](int i, int half, int slot) {
-                const uint32_t qa = q_u + i * S::kTileBytes, kb = ring_u + slot * S::kTileBytes + half * kStep * 128;
+            int n = 0;
+            uint32_t part = 0, taken = 0, weights[2] = {0, 0};
+            bool ok = true;
+            const auto wait_for = [&](uint64_t* bar, uint32_t phase) {
+                ok = ok && mbar_wait_bounded(bar, phase & 1, err, kDevErrTimeoutMma);
+                tmem_fence_after();
+                return ok;
+            };
+            // S = Q_i K^T of key tile `tile`, once the scores before have been taken.
+            const auto scores = [&](int i, int tile) {
+                if (taken > 0 && !wait_for(s_free, taken - 1)) return;
+                ++taken;
+                const uint32_t qa = q_u + i * S::kTileBytes, kb = ring_u + slot_of(2 * tile) * S::kTileBytes;
 #pragma unroll
                 for (int k = 0; k < kD / 16; ++k) {
                     const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    umma_f16(tmem + i * kTile + half * kStep, make_sw128_desc(qa + at), make_sw128_desc(kb + at), idesc_s,
-                             k > 0);
+                    umma_f16(tmem + kScoreCol, make_sw128_desc(qa + at), make_sw128_desc(kb + at), idesc_s, k > 0);
                 }
-                umma_commit(&s_full[2 * i + half]);
+                umma_commit(&s_full[i]);
             };
-            int n = 0;
-            uint32_t part = 0, weights[2] = {0, 0};  // key tiles whose weights have been taken, by tile
-            bool ok = true;
-            const auto wait_kv = [&](int seq) {
-                if (!mbar_wait_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutMma)) ok = false;
-                tmem_fence_after();
+            // O_i += P_i V of key tile `tile`.
+            const auto values = [&](int i, int tile, bool first) {
+                if (!wait_for(&p_ready[i], weights[i]++)) return;
+                if (!own[i]) {
+                    const uint32_t vb = ring_u + slot_of(2 * tile + 1) * S::kTileBytes;
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k)
+                        umma_f16_ts(tmem + kOutCol + i * kD, tmem + kWeightCol + i * (kTile / 2) + k * 8,
+                                    make_mn_desc(vb + k * 2048), idesc_o, !first || k > 0);
+                }
+                umma_commit(&o_done[i]);
             };
             Part q;
             while (ok && part_at(part, q) && !(q.flags & kEnd)) {
                 const int tiles = q_tiles(q);
-                if (!mbar_wait_bounded(q_full, part & 1, err, kDevErrTimeoutMma)) break;
-                ++part;
-                wait_kv(2 * n);
-                if (!ok) break;
-                for (int half = 0; half < 2; ++half)
-                    for (int i = 0; i < tiles; ++i) scores(i, half, slot_of(2 * n));
-                umma_commit(&kv_empty[slot_of(2 * n)]);
+                if (!wait_for(q_full, part++)) break;
                 for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++n) {
-                    const bool more = j + 1 < q.end_tile;
-                    for (int half = 0; half < 2 && ok; ++half) {
-                        for (int i = 0; i < tiles; ++i) {
-                            const int at = 2 * i + half;
-                            if (!mbar_wait_bounded(&p_ready[at], weights[i] & 1, err, kDevErrTimeoutMma)) ok = false;
-                            if (at == 0) wait_kv(2 * n + 1);
-                            if (!ok) break;
-                            tmem_fence_after();
-                            if (!own[at]) {
-                                const uint32_t vb = ring_u + slot_of(2 * n + 1) * S::kTileBytes + half * kStep * 128;
-#pragma unroll
-                                for (int k = 0; k < kStep / 16; ++k)
-                                    umma_f16_ts(tmem + 2 * kTile + i * kD, tmem + i * kTile + half * kStep + k * 8,
-                                                make_mn_desc(vb + k * 2048), idesc_o, j > q.first_tile || half > 0 || k > 0);
-                            }
-                            umma_commit(&o_done[at]);
-                            if (more) {
-                                if (at == 0) wait_kv(2 * n + 2);
-                                if (!ok) break;
-                                scores(i, half, slot_of(2 * n + 2));
-                            }
-                        }
+                    const bool first = j == q.first_tile;
+                    if (!wait_for(&kv_full[slot_of(2 * n)], phase_of(2 * n))) break;
+                    for (int i = 0; i < tiles && ok; ++i) {
+                        scores(i, n);
+                        if (!first && ok) values(i, n - 1, j - 1 == q.first_tile);
                     }
                     if (!ok) break;
-                    for (int i = 0; i < tiles; ++i) ++weights[i];
-                    umma_commit(&kv_empty[slot_of(2 * n + 1)]);
-                    umma_commit(more ? &kv_empty[slot_of(2 * n + 2)] : q_empty);
+                    umma_commit(&kv_empty[slot_of(2 * n)]);
+                    if (!first) umma_commit(&kv_empty[slot_of(2 * n - 1)]);
+                    if (!wait_for(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1))) break;
                 }
+                if (!ok) break;
+                umma_commit(q_empty);
+                for (int i = 0; i < tiles && ok; ++i) values(i, n - 1, q.end_tile - 1 == q.first_tile);
+                if (ok) umma_commit(&kv_empty[slot_of(2 * n - 1)]);
             }
             // All MMAs issued by this thread complete before TMEM is freed.
             umma_commit(mma_done);
@@ -460,7 +462,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     } else {
         const int wg = warp >> 2, t = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t o_addr = tmem + lanes + 2 * kTile + wg * kD;
+        const uint32_t s_addr = tmem + lanes + kScoreCol, p_addr = tmem + lanes + kWeightCol + wg * (kTile / 2),
+                       o_addr = tmem + lanes + kOutCol + wg * kD;
         const float scale = a.scale_log2;
         int n = 0;
         uint32_t tiles_done = 0, part = 0;
@@ -480,124 +483,116 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             };
             const int limit = limit_of(row_ok ? token : r.rows - 1), low = limit_of(token0);
             float ref = -INFINITY, sum = 0.0f;
-            for (int j = r.first_tile; j < r.end_tile && ok; ++j, ++n, ++tiles_done) {
-#pragma unroll 1
-                for (int half = 0; half < 2; ++half) {
-                    const int at = 2 * wg + half, key0 = j * kTile + half * kStep;
-                    const uint32_t s_addr = tmem + lanes + wg * kTile + half * kStep;
-                    if (!mbar_wait_bounded(&s_full[at], tiles_done & 1, err, kDevErrTimeoutEpilogue)) {
-                        ok = false;
-                        break;
-                    }
-                    tmem_fence_after();
-                    const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
-                    uint32_t s[2][32];
-                    tmem_ld_32x32b_x32(s_addr, s[0]);
-                    tmem_ld_32x32b_x32(s_addr + 32, s[1]);
-                    tmem_ld_wait();
-                    // Masked scores are scaled first; so are all where the scale turns
-                    // the order around.
-                    const bool masked = key0 + kStep > low || bad;
-                    float mul = scale;
-                    if (masked || scale < 0.0f) {
-                        const uint32_t gone = bad >> (half * (kStep / 8));
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-#pragma unroll
-                            for (int k = 0; k < 32; ++k) {
-                                const int key = c * 32 + k;
-                                const bool out = key >= limit - key0 || ((gone >> (key >> 3)) & 1);
-                                s[c][k] = __float_as_uint(out ? -INFINITY : __uint_as_float(s[c][k]) * scale);
-                            }
-                        mul = 1.0f;
-                    }
-                    float m[4];
-#pragma unroll
-                    for (int k = 0; k < 32; ++k) {
-                        const float x = fmaxf(__uint_as_float(s[0][k]), __uint_as_float(s[1][k]));
-                        m[k & 3] = k < 4 ? x : fmaxf(m[k & 3], x);
-                    }
-                    const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
-                    const bool grown = top > ref + 8.0f;  // from -inf: by anything
-                    if (__any_sync(0xffffffffu, grown)) {
-                        const float now = grown ? top : ref;
-                        const float keep = grown ? exp2_approx(ref - now) : 1.0f;
-                        ref = now;
-                        sum *= keep;
-                        if (j > r.first_tile || half > 0) {
-                            // The product of the step before must be in O.
-                            const uint32_t phase = half ? tiles_done : tiles_done - 1;
-                            if (!mbar_wait_bounded(&o_done[at ^ 1], phase & 1, err, kDevErrTimeoutEpilogue)) {
-                                ok = false;
-                                break;
-                            }
-                            tmem_fence_after();
-#pragma unroll 1
-                            for (int c = 0; c < kD / 32; ++c) {
-                                uint32_t o[32];
-                                tmem_ld_32x32b_x32(o_addr + c * 32, o);
-                                tmem_ld_wait();
-#pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                                tmem_st_32x32b_x32(o_addr + c * 32, o);
-                            }
-                        }
-                    }
-                    const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) {
-                            const float u = exp2_approx(fmaf(__uint_as_float(s[c][2 * k]), mul, from));
-                            const float v = exp2_approx(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, from));
-                            acc[k & 3] += u + v;
-                            w[k] = pack_pair<T>(u, v);
-                        }
-                        tmem_st_32x32b_x16(s_addr + c * 16, w);
-                    }
-                    sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-                    bool wild = false;
-                    if (masked) {
-                        // Rows of this step in the value tile: those behind the
-                        // request's last token in its box, those that some row does not see.
-                        const int valid = min(kTile, r.length - j * kTile), row0 = half * kStep, row1 = row0 + kStep;
-                        const int clear0 = max(valid, row0);
-                        const int clear1 = min((valid + shape.box - 1) / shape.box * shape.box, row1);
-                        const int from_row = max(low - j * kTile, row0), to_row = min(valid, row1);
-                        if (clear0 < clear1 || from_row < to_row) {
-                            uint8_t* v_tile = ring + slot_of(2 * n + 1) * S::kTileBytes;
-                            if (!mbar_wait_bounded(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1), err,
-                                                   kDevErrTimeoutEpilogue)) {
-                                ok = false;
-                                break;
-                            }
-                            if (clear0 < clear1) clear_rows<kD>(v_tile, clear0, clear1, t);
-                            if (from_row < to_row) {
-                                wild = group_any(wg, wild_rows<T, kD>(v_tile, from_row, to_row, t));
-                                if (wild) {
-                                    const bool first = j == r.first_tile && half == 0;
-                                    // The products before must be in O.
-                                    if (!first && !mbar_wait_bounded(&o_done[at ^ 1], (half ? tiles_done : tiles_done - 1) & 1,
-                                                                     err, kDevErrTimeoutEpilogue)) {
-                                        ok = false;
-                                        break;
-                                    }
-                                    tmem_fence_after();
-                                    add_own_values<T, kD>(o_addr, s_addr, v_tile, row0, limit - key0, bad, first);
-                                }
-                            }
-                        }
-                    }
-                    if (t == 0) own[at] = wild;
-                    tmem_st_wait();
-                    tmem_fence_before();
-                    mbar_arrive(&p_ready[at]);
+            for (int j = r.first_tile; j < r.end_tile; ++j, ++n, ++tiles_done) {
+                const int key0 = j * kTile;
+                const bool first = j == r.first_tile;
+                if (!mbar_wait_bounded(&s_full[wg], tiles_done & 1, err, kDevErrTimeoutEpilogue)) {
+                    ok = false;
+                    break;
                 }
+                tmem_fence_after();
+                const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
+                uint32_t s[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
+                tmem_ld_wait();
+                tmem_fence_before();
+                mbar_arrive(s_free);
+                // Masked scores are scaled first; so are all where the scale turns the
+                // order around.
+                const bool masked = key0 + kTile > low || bad;
+                float mul = scale;
+                if (masked || scale < 0.0f) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const int key = c * 32 + k;
+                            const bool out = key >= limit - key0 || ((bad >> (key >> 3)) & 1);
+                            s[c][k] = __float_as_uint(out ? -INFINITY : __uint_as_float(s[c][k]) * scale);
+                        }
+                    mul = 1.0f;
+                }
+                float m[4];
+#pragma unroll
+                for (int k = 0; k < 64; ++k) {
+                    const float x = fmaxf(__uint_as_float(s[k / 32][k % 32]), __uint_as_float(s[2 + k / 32][k % 32]));
+                    m[k & 3] = k < 4 ? x : fmaxf(m[k & 3], x);
+                }
+                const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
+                const bool grown = top > ref + 8.0f;  // from -inf: by anything
+                const bool rescale = __any_sync(0xffffffffu, grown);
+                if (rescale) {
+                    const float now = grown ? top : ref;
+                    const float keep = grown ? exp2_approx(ref - now) : 1.0f;
+                    ref = now;
+                    sum *= keep;
+                    if (!first) {
+                        // The product of the key tile before must be in O.
+                        if (!mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
+                            ok = false;
+                            break;
+                        }
+                        tmem_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < kD / 8; ++c) {
+                            uint32_t o[8];
+                            tmem_ld_32x32b_x8(o_addr + c * 8, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                            tmem_st_32x32b_x8(o_addr + c * 8, o);
+                        }
+                    }
+                }
+                const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float u = exp2_approx(fmaf(__uint_as_float(s[c][2 * k]), mul, from));
+                        const float v = exp2_approx(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, from));
+                        acc[k & 3] += u + v;
+                        s[c / 2][(c & 1) * 16 + k] = pack_pair<T>(u, v);  // over scores that have been used
+                    }
+                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                // The product that reads the weights before must be done.
+                if (!first && !rescale &&
+                    !mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
+                    ok = false;
+                    break;
+                }
+                tmem_fence_after();
+                tmem_st_32x32b_x32(p_addr, s[0]);
+                tmem_st_32x32b_x32(p_addr + 32, s[1]);
+                bool wild = false;
+                if (masked) {
+                    // Rows of the value tile: those behind the request's last token in
+                    // its box, and those that some row does not see.
+                    const int valid = min(kTile, r.length - key0), from_row = max(low - key0, 0);
+                    const int clear_to = (valid + shape.box - 1) / shape.box * shape.box;
+                    if (valid < clear_to || from_row < valid) {
+                        uint8_t* v_tile = ring + slot_of(2 * n + 1) * S::kTileBytes;
+                        if (!mbar_wait_bounded(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1), err,
+                                               kDevErrTimeoutEpilogue)) {
+                            ok = false;
+                            break;
+                        }
+                        if (valid < clear_to) clear_rows<kD>(v_tile, valid, clear_to, t);
+                        if (from_row < valid) {
+                            wild = group_any(wg, wild_rows<T, kD>(v_tile, from_row, valid, t));
+                            if (wild) add_own_values<T, kD>(o_addr, p_addr, v_tile, limit - key0, bad, first);
+                        }
+                    }
+                }
+                if (t == 0) own[wg] = wild;
+                tmem_st_wait();
+                tmem_fence_before();
+                mbar_arrive(&p_ready[wg]);
             }
             if (!ok) break;
-            if (!mbar_wait_bounded(&o_done[2 * wg + 1], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) break;
+            if (!mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) break;
             tmem_fence_after();
             const int row = wg * shape.tile_tokens * shape.group + t;  // of the item
             const bool whole = r.flags & kWhole, final = whole && a.prefix_length == 0;
