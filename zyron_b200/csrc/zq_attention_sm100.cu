@@ -5,10 +5,10 @@
 //
 // A persistent block takes 256 rows of a kv head as two tiles of 128 (new tokens
 // times the heads of the group) and walks their key tiles of 128:
-//   warp 9       TMA: q once an item, then key and value tiles alternately through
-//                a ring of shared-memory slots, a box for each run of tokens in a
-//                page; tokens that do not exist are boxes outside the tensor, which
-//                arrive as zeros.
+//   warp 9       TMA: q once an item, then groups of a key tile and the value tile
+//                before it through a ring in shared memory, a box for each run of
+//                tokens in a page; tokens that do not exist are boxes outside the
+//                tensor, which arrive as zeros.
 //   warp 8       issues the MMAs: S_i = Q_i K^T into TMEM, O_i += P_i V with P_i read
 //                from TMEM, for the two tiles by turns.  V is the MN-major operand:
 //                rows of the same boxes as K's, nothing is transposed.
@@ -66,9 +66,10 @@ template <int kD>
 struct Smem {
     static constexpr int kHalves = kD / 64;
     static constexpr int kTileBytes = kHalves * kHalfBytes;
-    static constexpr int kSlots = kD == 128 ? 4 : 8;
+    static constexpr int kGroupBytes = 2 * kTileBytes;  // keys, then values
+    static constexpr int kGroups = kD == 128 ? 2 : 4;
     static constexpr int kRing = 2 * kTileBytes;  // after the two q tiles
-    static constexpr int kBars = kRing + kSlots * kTileBytes;
+    static constexpr int kBars = kRing + kGroups * kGroupBytes;
     static constexpr int kTotal = 1024 + kBars + 512;
 };
 
@@ -256,7 +257,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                        const __grid_constant__ CUtensorMap tmap_v, const AttentionArgs a, const Workspace ws,
                        const Shape shape, uint32_t* __restrict__ err) {
     using S = Smem<kD>;
-    constexpr int kSlots = S::kSlots;
+    constexpr int kGroups = S::kGroups;
     constexpr uint32_t kTmemCols = 512;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ long long scratch[kManyThreads / 32 + 2];
@@ -272,13 +273,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     uint64_t* s_free = bars + 8;   // the scores have been taken (whichever warpgroup's they are)
     uint64_t* mma_done = bars + 9;
     uint64_t* kv_full = bars + 10;
-    uint64_t* kv_empty = kv_full + kSlots;
-    uint32_t* bad_ring = reinterpret_cast<uint32_t*>(kv_empty + kSlots);  // eighths of a key tile on no page
+    uint64_t* kv_empty = kv_full + kGroups;
+    uint32_t* bad_ring = reinterpret_cast<uint32_t*>(kv_empty + kGroups);  // eighths of a key tile on no page
     volatile uint32_t* own = bad_ring + kBadRing;  // by tile: its warpgroup added the values
     uint32_t* tmem_slot = bad_ring + kBadRing + 2;
     uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 4);
     Part* parts = reinterpret_cast<Part*>(part_full + kPartRing);
-    static_assert((10 + 2 * 8 + kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
+    static_assert((10 + 2 * 4 + kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedBatch& p = a.batch;
 
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             mbar_init(&o_done[i], 1);
         }
         for (int i = 0; i < kPartRing; ++i) mbar_init(&part_full[i], 1);
-        for (int i = 0; i < kSlots; ++i) {
+        for (int i = 0; i < kGroups; ++i) {
             mbar_init(&kv_full[i], 1);
             mbar_init(&kv_empty[i], 1);
         }
@@ -325,14 +326,16 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         q = parts[i % kPartRing];
         return true;
     };
-    // Tile n of this block (counted over its parts): keys in slot (2 n) % kSlots, values in the next.
-    const auto slot_of = [](int seq) { return seq % kSlots; };
-    const auto phase_of = [](int seq) { return (uint32_t)(seq / kSlots) & 1u; };
+    // A part of T key tiles has T + 1 groups: keys of tile k in group k, values in
+    // the next; groups are counted over the block's parts.
+    const auto keys_of = [&](int g) { return ring + g % kGroups * S::kGroupBytes; };
+    const auto values_of = [&](int g) { return keys_of(g) + S::kTileBytes; };
+    const auto phase_of = [](int g) { return (uint32_t)(g / kGroups) & 1u; };
 
     if (warp == 9) {
         const uint32_t q_bytes = (uint32_t)(128 * shape.group * shape.tile_tokens);
         const int boxes = kTile / shape.box;  // of a half tile; at most 16
-        int n = 0;
+        int n = 0, g = 0;
         uint32_t part = 0;
         bool ok = true, q_issued = false;
         Cursor<ManyPlan> way(plan, found, blockIdx.x);
@@ -361,48 +364,55 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
             q_issued = true;
             ++part;
-            for (int j = q.first_tile; j < q.end_tile; ++j, ++n) {
-                // Lane i looks box i's page up.
-                const int key = j * kTile + lane * shape.box;
-                int id = shape.cache_end, row = 0;
-                bool bad = false;
-                if (lane < boxes && key < r.length) {
-                    const int index = key / p.page;
-                    row = key - index * p.page;
-                    const int v = load_l2(table + index);
-                    bad = v < 0 || v >= p.cache_pages;
-                    if (!bad) id = v;
-                }
-                const uint32_t eighths = bad ? ((1u << (shape.box / 8)) - 1u) << (lane * (shape.box / 8)) : 0u;
-                const uint32_t missing = __reduce_or_sync(0xffffffffu, eighths);
-                if (lane == 0) bad_ring[n % kBadRing] = missing;
-#pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const int seq = 2 * n + kv, slot = slot_of(seq);
-                    if (!mbar_wait_bounded(&kv_empty[slot], phase_of(seq) ^ 1u, err, kDevErrTimeoutProducer)) {
-                        ok = false;
-                        break;
+            int id = 0, row = 0, id_before = 0, row_before = 0;
+            for (int j = q.first_tile; j <= q.end_tile; ++j, ++g) {
+                const bool keys = j < q.end_tile, values = j > q.first_tile;
+                id_before = id;
+                row_before = row;
+                if (keys) {
+                    // Lane i looks box i's page up.
+                    const int key = j * kTile + lane * shape.box;
+                    id = shape.cache_end;
+                    row = 0;
+                    bool bad = false;
+                    if (lane < boxes && key < r.length) {
+                        const int index = key / p.page;
+                        row = key - index * p.page;
+                        const int v = load_l2(table + index);
+                        bad = v < 0 || v >= p.cache_pages;
+                        if (!bad) id = v;
                     }
-                    if (lane == 0) mbar_arrive_expect_tx(&kv_full[slot], S::kTileBytes);
-                    __syncwarp();
-                    const int box = lane / S::kHalves, half = lane % S::kHalves;
-                    const int page = __shfl_sync(0xffffffffu, id, box), at = __shfl_sync(0xffffffffu, row, box);
-                    if (box < boxes)
-                        tma_load_4d(ring + slot * S::kTileBytes + half * kHalfBytes + box * shape.box * 128,
-                                    kv ? &tmap_v : &tmap_k, &kv_full[slot], half * 64, at, head, page);
+                    const uint32_t eighths = bad ? ((1u << (shape.box / 8)) - 1u) << (lane * (shape.box / 8)) : 0u;
+                    const uint32_t missing = __reduce_or_sync(0xffffffffu, eighths);
+                    if (lane == 0) bad_ring[n % kBadRing] = missing;
+                    ++n;
                 }
-                if (!ok) break;
+                uint64_t* full = &kv_full[g % kGroups];
+                if (!mbar_wait_bounded(&kv_empty[g % kGroups], phase_of(g) ^ 1u, err, kDevErrTimeoutProducer)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_arrive_expect_tx(full, (uint32_t)((int)keys + (int)values) * S::kTileBytes);
+                __syncwarp();
+                const int box = lane / S::kHalves, half = lane % S::kHalves;
+                const int at = half * kHalfBytes + box * shape.box * 128;
+                const int k_page = __shfl_sync(0xffffffffu, id, box), k_row = __shfl_sync(0xffffffffu, row, box);
+                const int v_page = __shfl_sync(0xffffffffu, id_before, box), v_row = __shfl_sync(0xffffffffu, row_before, box);
+                if (box < boxes) {
+                    if (keys) tma_load_4d(keys_of(g) + at, &tmap_k, full, half * 64, k_row, head, k_page);
+                    if (values) tma_load_4d(values_of(g) + at, &tmap_v, full, half * 64, v_row, head, v_page);
+                }
             }
         }
         // Every copy lands before the block can exit.
         if (q_issued) mbar_drain_bounded(q_full, (part - 1) & 1u, err, kDevErrTimeoutDrain);
-        for (int seq = max(0, 2 * n - kSlots); seq < 2 * n; ++seq)
-            mbar_drain_bounded(&kv_full[slot_of(seq)], phase_of(seq), err, kDevErrTimeoutDrain);
+        for (int i = max(0, g - kGroups); i < g; ++i)
+            mbar_drain_bounded(&kv_full[i % kGroups], phase_of(i), err, kDevErrTimeoutDrain);
     } else if (warp == 8) {
         if (lane == 0) {
             constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
-            const uint32_t q_u = smem_u32(smem), ring_u = smem_u32(ring);
-            int n = 0;
+            const uint32_t q_u = smem_u32(smem);
+            int g = 0;
             uint32_t part = 0, taken = 0, weights[2] = {0, 0};
             bool ok = true;
             const auto wait_for = [&](uint64_t* bar, uint32_t phase) {
@@ -410,11 +420,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 tmem_fence_after();
                 return ok;
             };
-            // S = Q_i K^T of key tile `tile`, once the scores before have been taken.
-            const auto scores = [&](int i, int tile) {
+            // S = Q_i K^T of group g's keys, once the scores before have been taken.
+            const auto scores = [&](int i) {
                 if (taken > 0 && !wait_for(s_free, taken - 1)) return;
                 ++taken;
-                const uint32_t qa = q_u + i * S::kTileBytes, kb = ring_u + slot_of(2 * tile) * S::kTileBytes;
+                const uint32_t qa = q_u + i * S::kTileBytes, kb = smem_u32(keys_of(g));
 #pragma unroll
                 for (int k = 0; k < kD / 16; ++k) {
                     const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
@@ -422,11 +432,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 umma_commit(&s_full[i]);
             };
-            // O_i += P_i V of key tile `tile`.
-            const auto values = [&](int i, int tile, bool first) {
+            // O_i += P_i V of group g's values.
+            const auto values = [&](int i, bool first) {
                 if (!wait_for(&p_ready[i], weights[i]++)) return;
                 if (!own[i]) {
-                    const uint32_t vb = ring_u + slot_of(2 * tile + 1) * S::kTileBytes;
+                    const uint32_t vb = smem_u32(values_of(g));
 #pragma unroll
                     for (int k = 0; k < kTile / 16; ++k)
                         umma_f16_ts(tmem + kOutCol + i * kD, tmem + kWeightCol + i * (kTile / 2) + k * 8,
@@ -437,23 +447,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             Part q;
             while (ok && part_at(part, q) && !(q.flags & kEnd)) {
                 const int tiles = q_tiles(q);
-                if (!wait_for(q_full, part++)) break;
-                for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++n) {
-                    const bool first = j == q.first_tile;
-                    if (!wait_for(&kv_full[slot_of(2 * n)], phase_of(2 * n))) break;
+                if (!wait_for(q_full, part++) || !wait_for(&kv_full[g % kGroups], phase_of(g))) break;
+                for (int j = q.first_tile; j <= q.end_tile && ok; ++j, ++g) {
                     for (int i = 0; i < tiles && ok; ++i) {
-                        scores(i, n);
-                        if (!first && ok) values(i, n - 1, j - 1 == q.first_tile);
+                        if (j < q.end_tile) scores(i);
+                        // The next group is waited for while products are under way.
+                        if (ok && i == tiles - 1 && j < q.end_tile) {
+                            if (j + 1 == q.end_tile) umma_commit(q_empty);
+                            wait_for(&kv_full[(g + 1) % kGroups], phase_of(g + 1));
+                        }
+                        if (ok && j > q.first_tile) values(i, j - 1 == q.first_tile);
                     }
-                    if (!ok) break;
-                    umma_commit(&kv_empty[slot_of(2 * n)]);
-                    if (!first) umma_commit(&kv_empty[slot_of(2 * n - 1)]);
-                    if (!wait_for(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1))) break;
+                    if (ok) umma_commit(&kv_empty[g % kGroups]);
                 }
-                if (!ok) break;
-                umma_commit(q_empty);
-                for (int i = 0; i < tiles && ok; ++i) values(i, n - 1, q.end_tile - 1 == q.first_tile);
-                if (ok) umma_commit(&kv_empty[slot_of(2 * n - 1)]);
             }
             // All MMAs issued by this thread complete before TMEM is freed.
             umma_commit(mma_done);
@@ -465,13 +471,14 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         const uint32_t s_addr = tmem + lanes + kScoreCol, p_addr = tmem + lanes + kWeightCol + wg * (kTile / 2),
                        o_addr = tmem + lanes + kOutCol + wg * kD;
         const float scale = a.scale_log2;
-        int n = 0;
+        int n = 0, g = 0;
         uint32_t tiles_done = 0, part = 0;
         bool ok = true;
         Part r;
-        while (ok && part_at(part++, r) && !(r.flags & kEnd)) {
+        for (; ok && part_at(part++, r) && !(r.flags & kEnd); ++g) {
             if (wg >= q_tiles(r)) {
                 n += r.end_tile - r.first_tile;
+                g += r.end_tile - r.first_tile;
                 continue;
             }
             const bool causal = !(r.flags & kPrefix) && a.causal;
@@ -483,7 +490,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             };
             const int limit = limit_of(row_ok ? token : r.rows - 1), low = limit_of(token0);
             float ref = -INFINITY, sum = 0.0f;
-            for (int j = r.first_tile; j < r.end_tile; ++j, ++n, ++tiles_done) {
+            for (int j = r.first_tile; j < r.end_tile; ++j, ++n, ++g, ++tiles_done) {
                 const int key0 = j * kTile;
                 const bool first = j == r.first_tile;
                 if (!mbar_wait_bounded(&s_full[wg], tiles_done & 1, err, kDevErrTimeoutEpilogue)) {
@@ -520,20 +527,21 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     m[k & 3] = k < 4 ? x : fmaxf(m[k & 3], x);
                 }
                 const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
+                // The product of the key tile before is in O, and has read its weights.
+                if (!first) {
+                    if (!mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
+                        ok = false;
+                        break;
+                    }
+                    tmem_fence_after();
+                }
                 const bool grown = top > ref + 8.0f;  // from -inf: by anything
-                const bool rescale = __any_sync(0xffffffffu, grown);
-                if (rescale) {
+                if (__any_sync(0xffffffffu, grown)) {
                     const float now = grown ? top : ref;
                     const float keep = grown ? exp2_approx(ref - now) : 1.0f;
                     ref = now;
                     sum *= keep;
                     if (!first) {
-                        // The product of the key tile before must be in O.
-                        if (!mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
-                            ok = false;
-                            break;
-                        }
-                        tmem_fence_after();
 #pragma unroll 1
                         for (int c = 0; c < kD / 8; ++c) {
                             uint32_t o[8];
@@ -548,24 +556,19 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
+                for (int c = 0; c < 8; ++c) {
+                    uint32_t w[8];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float u = exp2_approx(fmaf(__uint_as_float(s[c][2 * k]), mul, from));
-                        const float v = exp2_approx(fmaf(__uint_as_float(s[c][2 * k + 1]), mul, from));
+                    for (int k = 0; k < 8; ++k) {
+                        const int at = (c & 1) * 16 + 2 * k;
+                        const float u = exp2_approx(fmaf(__uint_as_float(s[c / 2][at]), mul, from));
+                        const float v = exp2_approx(fmaf(__uint_as_float(s[c / 2][at + 1]), mul, from));
                         acc[k & 3] += u + v;
-                        s[c / 2][(c & 1) * 16 + k] = pack_pair<T>(u, v);  // over scores that have been used
+                        w[k] = pack_pair<T>(u, v);
                     }
-                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
-                // The product that reads the weights before must be done.
-                if (!first && !rescale &&
-                    !mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
-                    ok = false;
-                    break;
+                    tmem_st_32x32b_x8(p_addr + c * 8, w);
                 }
-                tmem_fence_after();
-                tmem_st_32x32b_x32(p_addr, s[0]);
-                tmem_st_32x32b_x32(p_addr + 32, s[1]);
+                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
                 bool wild = false;
                 if (masked) {
                     // Rows of the value tile: those behind the request's last token in
@@ -573,9 +576,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const int valid = min(kTile, r.length - key0), from_row = max(low - key0, 0);
                     const int clear_to = (valid + shape.box - 1) / shape.box * shape.box;
                     if (valid < clear_to || from_row < valid) {
-                        uint8_t* v_tile = ring + slot_of(2 * n + 1) * S::kTileBytes;
-                        if (!mbar_wait_bounded(&kv_full[slot_of(2 * n + 1)], phase_of(2 * n + 1), err,
-                                               kDevErrTimeoutEpilogue)) {
+                        uint8_t* v_tile = values_of(g + 1);
+                        if (!mbar_wait_bounded(&kv_full[(g + 1) % kGroups], phase_of(g + 1), err, kDevErrTimeoutEpilogue)) {
                             ok = false;
                             break;
                         }
