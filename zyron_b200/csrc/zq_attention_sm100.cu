@@ -94,22 +94,36 @@ __device__ __forceinline__ uint64_t make_mn_desc(uint32_t saddr) {
     return d;
 }
 
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// Issued by the one thread with `leads`.  The warp stays together around it, so that
+// descriptors are formed in uniform registers, where the instruction wants them: in
+// a branch of one lane they are moved there one by one, 100 cycles an MMA of 64.
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                         uint32_t accumulate, bool leads) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"((uint32_t)leads)
         : "memory");
 }
 // A from TMEM: two elements a column.
 __device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                            uint32_t accumulate) {
+                                            uint32_t accumulate, bool leads) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, e;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "setp.ne.b32 e, %5, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"((uint32_t)leads)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_if(uint64_t* bar, bool leads) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\t"
+        "setp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"((uint32_t)leads)
         : "memory");
 }
 
@@ -409,62 +423,64 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = max(0, g - kGroups); i < g; ++i)
             mbar_drain_bounded(&kv_full[i % kGroups], phase_of(i), err, kDevErrTimeoutDrain);
     } else if (warp == 8) {
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
-            const uint32_t q_u = smem_u32(smem);
-            int g = 0;
-            uint32_t part = 0, taken = 0, weights[2] = {0, 0};
-            bool ok = true;
-            const auto wait_for = [&](uint64_t* bar, uint32_t phase) {
-                ok = ok && mbar_wait_bounded(bar, phase & 1, err, kDevErrTimeoutMma);
-                tmem_fence_after();
-                return ok;
-            };
-            // S = Q_i K^T of group g's keys, once the scores before have been taken.
-            const auto scores = [&](int i) {
-                if (taken > 0 && !wait_for(s_free, taken - 1)) return;
-                ++taken;
-                const uint32_t qa = q_u + i * S::kTileBytes, kb = smem_u32(keys_of(g));
+        constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
+        const bool leads = lane == 0;
+        const uint64_t q_desc = make_sw128_desc(smem_u32(smem)), k_desc = make_sw128_desc(smem_u32(ring)),
+                       v_desc = make_mn_desc(smem_u32(ring) + S::kTileBytes);
+        int g = 0;
+        uint32_t part = 0, taken = 0, weights[2] = {0, 0};
+        bool ok = true;
+        const auto wait_for = [&](uint64_t* bar, uint32_t phase) {
+            ok = ok && mbar_wait_bounded(bar, phase & 1, err, kDevErrTimeoutMma);
+            tmem_fence_after();
+            return ok;
+        };
+        // S = Q_i K^T of group g's keys, once the scores before have been taken.
+        const auto scores = [&](int i) {
+            if (taken > 0 && !wait_for(s_free, taken - 1)) return;
+            ++taken;
+            const uint64_t qa = q_desc + (uint32_t)(i * S::kTileBytes >> 4),
+                           kb = k_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
 #pragma unroll
-                for (int k = 0; k < kD / 16; ++k) {
-                    const uint32_t at = (k >> 2) * kHalfBytes + (k & 3) * 32;
-                    umma_f16(tmem + kScoreCol, make_sw128_desc(qa + at), make_sw128_desc(kb + at), idesc_s, k > 0);
-                }
-                umma_commit(&s_full[i]);
-            };
-            // O_i += P_i V of group g's values.
-            const auto values = [&](int i, bool first) {
-                if (!wait_for(&p_ready[i], weights[i]++)) return;
-                if (!own[i]) {
-                    const uint32_t vb = smem_u32(values_of(g));
-#pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k)
-                        umma_f16_ts(tmem + kOutCol + i * kD, tmem + kWeightCol + i * (kTile / 2) + k * 8,
-                                    make_mn_desc(vb + k * 2048), idesc_o, !first || k > 0);
-                }
-                umma_commit(&o_done[i]);
-            };
-            Part q;
-            while (ok && part_at(part, q) && !(q.flags & kEnd)) {
-                const int tiles = q_tiles(q);
-                if (!wait_for(q_full, part++) || !wait_for(&kv_full[g % kGroups], phase_of(g))) break;
-                for (int j = q.first_tile; j <= q.end_tile && ok; ++j, ++g) {
-                    for (int i = 0; i < tiles && ok; ++i) {
-                        if (j < q.end_tile) scores(i);
-                        // The next group is waited for while products are under way.
-                        if (ok && i == tiles - 1 && j < q.end_tile) {
-                            if (j + 1 == q.end_tile) umma_commit(q_empty);
-                            wait_for(&kv_full[(g + 1) % kGroups], phase_of(g + 1));
-                        }
-                        if (ok && j > q.first_tile) values(i, j - 1 == q.first_tile);
-                    }
-                    if (ok) umma_commit(&kv_empty[g % kGroups]);
-                }
+            for (int k = 0; k < kD / 16; ++k) {
+                constexpr int kHalf = kHalfBytes >> 4;
+                umma_f16(tmem + kScoreCol, qa + ((k >> 2) * kHalf + (k & 3) * 2), kb + ((k >> 2) * kHalf + (k & 3) * 2),
+                         idesc_s, k > 0, leads);
             }
-            // All MMAs issued by this thread complete before TMEM is freed.
-            umma_commit(mma_done);
-            mbar_drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
+            umma_commit_if(&s_full[i], leads);
+        };
+        // O_i += P_i V of group g's values.
+        const auto values = [&](int i, bool first) {
+            if (!wait_for(&p_ready[i], weights[i]++)) return;
+            if (!own[i]) {
+                const uint64_t vb = v_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
+#pragma unroll
+                for (int k = 0; k < kTile / 16; ++k)
+                    umma_f16_ts(tmem + kOutCol + i * kD, tmem + kWeightCol + i * (kTile / 2) + k * 8, vb + k * (2048 >> 4),
+                                idesc_o, !first || k > 0, leads);
+            }
+            umma_commit_if(&o_done[i], leads);
+        };
+        Part q;
+        while (ok && part_at(part, q) && !(q.flags & kEnd)) {
+            const int tiles = q_tiles(q);
+            if (!wait_for(q_full, part++) || !wait_for(&kv_full[g % kGroups], phase_of(g))) break;
+            for (int j = q.first_tile; j <= q.end_tile && ok; ++j, ++g) {
+                for (int i = 0; i < tiles && ok; ++i) {
+                    if (j < q.end_tile) scores(i);
+                    // The next group is waited for while products are under way.
+                    if (ok && i == tiles - 1 && j < q.end_tile) {
+                        if (j + 1 == q.end_tile) umma_commit_if(q_empty, leads);
+                        wait_for(&kv_full[(g + 1) % kGroups], phase_of(g + 1));
+                    }
+                    if (ok && j > q.first_tile) values(i, j - 1 == q.first_tile);
+                }
+                if (ok) umma_commit_if(&kv_empty[g % kGroups], leads);
+            }
         }
+        // All MMAs issued by this warp complete before TMEM is freed.
+        umma_commit_if(mma_done, leads);
+        mbar_drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
     } else {
         const int wg = warp >> 2, t = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
