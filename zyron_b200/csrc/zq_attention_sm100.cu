@@ -179,6 +179,28 @@ __device__ __forceinline__ bool any_at(bool v) {
 }
 __device__ __forceinline__ bool group_any(int wg, bool v) { return wg == 0 ? any_at<1>(v) : any_at<2>(v); }
 
+// Two fp32 values an instruction.
+__device__ __forceinline__ uint64_t pack_f32(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f32(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 template <class T>
 __device__ __forceinline__ uint32_t pack_pair(float x, float y) {
     Pack<T, 2> p{{from_float<T>(x), from_float<T>(y)}};
@@ -256,6 +278,17 @@ __device__ __noinline__ void add_own_values(uint32_t o_addr, uint32_t p_addr, co
         tmem_st_32x32b_x32(o_addr + c * 32, o);
         tmem_st_wait();
     }
+}
+
+// The waits with their long way out of line: the code of the loops stays small.
+__device__ __noinline__ bool wait_long(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t code) {
+    return mbar_wait_bounded(bar, parity, err, code);
+}
+__device__ __forceinline__ bool wait_bounded(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t code) {
+    return mbar_try_wait(bar, parity) || wait_long(bar, parity, err, code);
+}
+__device__ __noinline__ void drain_bounded(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t code) {
+    mbar_drain_bounded(bar, parity, err, code);
 }
 
 struct Shape {
@@ -336,7 +369,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const auto q_tiles = [&](const Part& q) { return q.rows - q.token0 > shape.tile_tokens ? 2 : 1; };
     // The block's part number `i`; false: the producer gave up.
     const auto part_at = [&](uint32_t i, Part& q) {
-        if (!mbar_wait_bounded(&part_full[i % kPartRing], (i / kPartRing) & 1, err, kDevErrTimeoutMma)) return false;
+        if (!wait_bounded(&part_full[i % kPartRing], (i / kPartRing) & 1, err, kDevErrTimeoutMma)) return false;
         q = parts[i % kPartRing];
         return true;
     };
@@ -368,7 +401,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             if (!more) break;
             const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)way.it.b * p.ld_pages;
             const int tiles = q_tiles(q);
-            if (!mbar_wait_bounded(q_empty, (part & 1) ^ 1u, err, kDevErrTimeoutProducer)) break;
+            if (!wait_bounded(q_empty, (part & 1) ^ 1u, err, kDevErrTimeoutProducer)) break;
             if (lane == 0) mbar_arrive_expect_tx(q_full, (uint32_t)(tiles * S::kHalves) * q_bytes);
             __syncwarp();
             if (lane < tiles * S::kHalves) {
@@ -402,7 +435,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     ++n;
                 }
                 uint64_t* full = &kv_full[g % kGroups];
-                if (!mbar_wait_bounded(&kv_empty[g % kGroups], phase_of(g) ^ 1u, err, kDevErrTimeoutProducer)) {
+                if (!wait_bounded(&kv_empty[g % kGroups], phase_of(g) ^ 1u, err, kDevErrTimeoutProducer)) {
                     ok = false;
                     break;
                 }
@@ -419,9 +452,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             }
         }
         // Every copy lands before the block can exit.
-        if (q_issued) mbar_drain_bounded(q_full, (part - 1) & 1u, err, kDevErrTimeoutDrain);
+        if (q_issued) drain_bounded(q_full, (part - 1) & 1u, err, kDevErrTimeoutDrain);
         for (int i = max(0, g - kGroups); i < g; ++i)
-            mbar_drain_bounded(&kv_full[i % kGroups], phase_of(i), err, kDevErrTimeoutDrain);
+            drain_bounded(&kv_full[i % kGroups], phase_of(i), err, kDevErrTimeoutDrain);
     } else if (warp == 8) {
         constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
         const bool leads = lane == 0;
@@ -431,7 +464,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         uint32_t part = 0, taken = 0, weights[2] = {0, 0};
         bool ok = true;
         const auto wait_for = [&](uint64_t* bar, uint32_t phase) {
-            ok = ok && mbar_wait_bounded(bar, phase & 1, err, kDevErrTimeoutMma);
+            ok = ok && wait_bounded(bar, phase & 1, err, kDevErrTimeoutMma);
             tmem_fence_after();
             return ok;
         };
@@ -480,7 +513,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         }
         // All MMAs issued by this warp complete before TMEM is freed.
         umma_commit_if(mma_done, leads);
-        mbar_drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
+        drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
     } else {
         const int wg = warp >> 2, t = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -509,33 +542,41 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             for (int j = r.first_tile; j < r.end_tile; ++j, ++n, ++g, ++tiles_done) {
                 const int key0 = j * kTile;
                 const bool first = j == r.first_tile;
-                if (!mbar_wait_bounded(&s_full[wg], tiles_done & 1, err, kDevErrTimeoutEpilogue)) {
+                if (!wait_bounded(&s_full[wg], tiles_done & 1, err, kDevErrTimeoutEpilogue)) {
                     ok = false;
                     break;
                 }
                 tmem_fence_after();
                 const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
+                // Masked scores are scaled and masked in their place first, in a loop of
+                // its own (unrolled beside the rest, the code of all warps no longer
+                // stays in the instruction cache, and the MMA warp's steps take 100 to
+                // 200 cycles each); so are all where the scale turns the order around.
+                const bool masked = key0 + kTile > low || bad;
+                float mul = scale;
+                if (masked || scale < 0.0f) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        tmem_ld_32x32b_x32(s_addr + c * 32, x);
+                        tmem_ld_wait();
+                        const int seen = limit - key0 - c * 32;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) {
+                            const bool out = k >= seen || ((bad >> (c * 4 + (k >> 3))) & 1);
+                            x[k] = __float_as_uint(out ? -INFINITY : __uint_as_float(x[k]) * scale);
+                        }
+                        tmem_st_32x32b_x32(s_addr + c * 32, x);
+                    }
+                    tmem_st_wait();
+                    mul = 1.0f;
+                }
                 uint32_t s[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
                 tmem_ld_wait();
                 tmem_fence_before();
                 mbar_arrive(s_free);
-                // Masked scores are scaled first; so are all where the scale turns the
-                // order around.
-                const bool masked = key0 + kTile > low || bad;
-                float mul = scale;
-                if (masked || scale < 0.0f) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const int key = c * 32 + k;
-                            const bool out = key >= limit - key0 || ((bad >> (key >> 3)) & 1);
-                            s[c][k] = __float_as_uint(out ? -INFINITY : __uint_as_float(s[c][k]) * scale);
-                        }
-                    mul = 1.0f;
-                }
                 float m[4];
 #pragma unroll
                 for (int k = 0; k < 64; ++k) {
@@ -545,7 +586,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
                 // The product of the key tile before is in O, and has read its weights.
                 if (!first) {
-                    if (!mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
+                    if (!wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
                         ok = false;
                         break;
                     }
@@ -570,21 +611,24 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                 }
                 const float from = ref == -INFINITY ? 0.0f : -ref;  // nothing seen yet: every weight is 0
-                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint64_t mul2 = pack_f32(mul, mul), from2 = pack_f32(from, from);
+                uint64_t acc[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     uint32_t w[8];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
                         const int at = (c & 1) * 16 + 2 * k;
-                        const float u = exp2_approx(fmaf(__uint_as_float(s[c / 2][at]), mul, from));
-                        const float v = exp2_approx(fmaf(__uint_as_float(s[c / 2][at + 1]), mul, from));
-                        acc[k & 3] += u + v;
+                        const float2 x = unpack_f32(
+                            fma_f32x2(pack_f32(__uint_as_float(s[c / 2][at]), __uint_as_float(s[c / 2][at + 1])), mul2, from2));
+                        const float u = exp2_approx(x.x), v = exp2_approx(x.y);
+                        acc[k & 1] = add_f32x2(acc[k & 1], pack_f32(u, v));
                         w[k] = pack_pair<T>(u, v);
                     }
                     tmem_st_32x32b_x8(p_addr + c * 8, w);
                 }
-                sum += (acc[0] + acc[1]) + (acc[2] + acc[3]);
+                const float2 both = unpack_f32(add_f32x2(acc[0], acc[1]));
+                sum += both.x + both.y;
                 bool wild = false;
                 if (masked) {
                     // Rows of the value tile: those behind the request's last token in
@@ -593,7 +637,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     const int clear_to = (valid + shape.box - 1) / shape.box * shape.box;
                     if (valid < clear_to || from_row < valid) {
                         uint8_t* v_tile = values_of(g + 1);
-                        if (!mbar_wait_bounded(&kv_full[(g + 1) % kGroups], phase_of(g + 1), err, kDevErrTimeoutEpilogue)) {
+                        if (!wait_bounded(&kv_full[(g + 1) % kGroups], phase_of(g + 1), err, kDevErrTimeoutEpilogue)) {
                             ok = false;
                             break;
                         }
@@ -610,7 +654,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 mbar_arrive(&p_ready[wg]);
             }
             if (!ok) break;
-            if (!mbar_wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) break;
+            if (!wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) break;
             tmem_fence_after();
             const int row = wg * shape.tile_tokens * shape.group + t;  // of the item
             const bool whole = r.flags & kWhole, final = whole && a.prefix_length == 0;
