@@ -9,9 +9,12 @@
 //                before it through a ring in shared memory, a box for each run of
 //                tokens in a page; tokens that do not exist are boxes outside the
 //                tensor, which arrive as zeros.
-//   warp 8       issues the MMAs: S_i = Q_i K^T into TMEM, O_i += P_i V with P_i read
-//                from TMEM, for the two tiles by turns.  V is the MN-major operand:
-//                rows of the same boxes as K's, nothing is transposed.
+//   warp 8       issues S_i = Q_i K^T into TMEM, for the two tiles by turns.
+//   warp 10      issues O_i += P_i V with P_i read from TMEM.  V is the MN-major
+//                operand: rows of the same boxes as K's, nothing is transposed.
+//                (A thread takes about 50 cycles to issue an MMA of 64 and as long
+//                as eight for a wait and a commit, so one warp for both kept the
+//                tensor cores at half their rate.)
 //   warps 0-7    a warpgroup a tile, a thread a row: scores from TMEM into registers,
 //                running maximum, exp2, P back to TMEM, 16 bits each.
 // TMEM holds the two outputs, the two P and one S, which both tiles use by turns:
@@ -44,7 +47,7 @@ namespace {
 
 using namespace attn;
 
-constexpr int kManyThreads = 320;
+constexpr int kManyThreads = 352;
 constexpr int kTile = 128;             // rows of a q tile, keys of a key tile
 // TMEM columns: the scores of whichever tile, P (two keys a column), O.
 constexpr int kScoreCol = 0, kWeightCol = 128, kOutCol = 256;
@@ -333,7 +336,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     if (threadIdx.x == 0) {
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
-        mbar_init(mma_done, 1);
+        mbar_init(mma_done, 2);
         mbar_init(s_free, 128);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = 0; i < kPartRing; ++i) mbar_init(&part_full[i], 1);
         for (int i = 0; i < kGroups; ++i) {
             mbar_init(&kv_full[i], 1);
-            mbar_init(&kv_empty[i], 1);
+            mbar_init(&kv_empty[i], 2);  // both issuing warps
         }
         fence_mbar_init();
         tma_prefetch_desc(&tmap_q);
@@ -456,62 +459,72 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = max(0, g - kGroups); i < g; ++i)
             drain_bounded(&kv_full[i % kGroups], phase_of(i), err, kDevErrTimeoutDrain);
     } else if (warp == 8) {
-        constexpr uint32_t idesc_s = idesc_f16<T>(kTile, false), idesc_o = idesc_f16<T>(kD, true);
+        // S = Q_i K^T of each group's keys, once the scores before have been taken.
+        constexpr uint32_t idesc = idesc_f16<T>(kTile, false);
+        constexpr int kHalf = kHalfBytes >> 4;
         const bool leads = lane == 0;
-        const uint64_t q_desc = make_sw128_desc(smem_u32(smem)), k_desc = make_sw128_desc(smem_u32(ring)),
-                       v_desc = make_mn_desc(smem_u32(ring) + S::kTileBytes);
+        const uint64_t q_desc = make_sw128_desc(smem_u32(smem)), k_desc = make_sw128_desc(smem_u32(ring));
         int g = 0;
-        uint32_t part = 0, taken = 0, weights[2] = {0, 0};
+        uint32_t part = 0, taken = 0;
         bool ok = true;
-        const auto wait_for = [&](uint64_t* bar, uint32_t phase) {
-            ok = ok && wait_bounded(bar, phase & 1, err, kDevErrTimeoutMma);
-            tmem_fence_after();
-            return ok;
-        };
-        // S = Q_i K^T of group g's keys, once the scores before have been taken.
-        const auto scores = [&](int i) {
-            if (taken > 0 && !wait_for(s_free, taken - 1)) return;
-            ++taken;
-            const uint64_t qa = q_desc + (uint32_t)(i * S::kTileBytes >> 4),
-                           kb = k_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
-#pragma unroll
-            for (int k = 0; k < kD / 16; ++k) {
-                constexpr int kHalf = kHalfBytes >> 4;
-                umma_f16(tmem + kScoreCol, qa + ((k >> 2) * kHalf + (k & 3) * 2), kb + ((k >> 2) * kHalf + (k & 3) * 2),
-                         idesc_s, k > 0, leads);
-            }
-            umma_commit_if(&s_full[i], leads);
-        };
-        // O_i += P_i V of group g's values.
-        const auto values = [&](int i, bool first) {
-            if (!wait_for(&p_ready[i], weights[i]++)) return;
-            if (!own[i]) {
-                const uint64_t vb = v_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
-#pragma unroll
-                for (int k = 0; k < kTile / 16; ++k)
-                    umma_f16_ts(tmem + kOutCol + i * kD, tmem + kWeightCol + i * (kTile / 2) + k * 8, vb + k * (2048 >> 4),
-                                idesc_o, !first || k > 0, leads);
-            }
-            umma_commit_if(&o_done[i], leads);
-        };
         Part q;
         while (ok && part_at(part, q) && !(q.flags & kEnd)) {
             const int tiles = q_tiles(q);
-            if (!wait_for(q_full, part++) || !wait_for(&kv_full[g % kGroups], phase_of(g))) break;
-            for (int j = q.first_tile; j <= q.end_tile && ok; ++j, ++g) {
+            ok = wait_bounded(q_full, part++ & 1, err, kDevErrTimeoutMma);
+            for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++g) {
+                ok = wait_bounded(&kv_full[g % kGroups], phase_of(g), err, kDevErrTimeoutMma);
+                const uint64_t kb = k_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
                 for (int i = 0; i < tiles && ok; ++i) {
-                    if (j < q.end_tile) scores(i);
-                    // The next group is waited for while products are under way.
-                    if (ok && i == tiles - 1 && j < q.end_tile) {
-                        if (j + 1 == q.end_tile) umma_commit_if(q_empty, leads);
-                        wait_for(&kv_full[(g + 1) % kGroups], phase_of(g + 1));
+                    if (taken > 0) ok = wait_bounded(s_free, (taken - 1) & 1, err, kDevErrTimeoutMma);
+                    if (!ok) break;
+                    ++taken;
+                    tmem_fence_after();
+                    const uint64_t qa = q_desc + (uint32_t)(i * S::kTileBytes >> 4);
+#pragma unroll
+                    for (int k = 0; k < kD / 16; ++k)
+                        umma_f16(tmem + kScoreCol, qa + ((k >> 2) * kHalf + (k & 3) * 2),
+                                 kb + ((k >> 2) * kHalf + (k & 3) * 2), idesc, k > 0, leads);
+                    umma_commit_if(&s_full[i], leads);
+                }
+                if (ok) umma_commit_if(&kv_empty[g % kGroups], leads);
+            }
+            if (!ok) break;
+            umma_commit_if(q_empty, leads);
+            umma_commit_if(&kv_empty[g++ % kGroups], leads);  // the part's last group has values alone
+        }
+        // All MMAs issued by this warp complete before TMEM is freed.
+        umma_commit_if(mma_done, leads);
+        drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
+    } else if (warp == 10) {
+        // O_i += P_i V of each group's values.
+        constexpr uint32_t idesc = idesc_f16<T>(kD, true);
+        const bool leads = lane == 0;
+        const uint64_t v_desc = make_mn_desc(smem_u32(ring) + S::kTileBytes);
+        int g = 0;
+        uint32_t part = 0, weights[2] = {0, 0};
+        bool ok = true;
+        Part q;
+        while (ok && part_at(part++, q) && !(q.flags & kEnd)) {
+            const int tiles = q_tiles(q);
+            umma_commit_if(&kv_empty[g++ % kGroups], leads);  // the part's first group has keys alone
+            for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++g) {
+                ok = wait_bounded(&kv_full[g % kGroups], phase_of(g), err, kDevErrTimeoutMma);
+                const uint64_t vb = v_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
+                for (int i = 0; i < tiles && ok; ++i) {
+                    ok = wait_bounded(&p_ready[i], weights[i]++ & 1, err, kDevErrTimeoutMma);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    if (!own[i]) {
+#pragma unroll
+                        for (int k = 0; k < kTile / 16; ++k)
+                            umma_f16_ts(tmem + kOutCol + i * kD, tmem + kWeightCol + i * (kTile / 2) + k * 8,
+                                        vb + k * (2048 >> 4), idesc, j > q.first_tile || k > 0, leads);
                     }
-                    if (ok && j > q.first_tile) values(i, j - 1 == q.first_tile);
+                    umma_commit_if(&o_done[i], leads);
                 }
                 if (ok) umma_commit_if(&kv_empty[g % kGroups], leads);
             }
         }
-        // All MMAs issued by this warp complete before TMEM is freed.
         umma_commit_if(mma_done, leads);
         drain_bounded(mma_done, 0, err, kDevErrTimeoutDrain);
     } else {
