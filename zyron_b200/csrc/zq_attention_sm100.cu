@@ -72,8 +72,10 @@ struct Smem {
     static constexpr int kGroupBytes = 2 * kTileBytes;  // keys, then values
     static constexpr int kGroups = kD == 128 ? 2 : 4;
     static constexpr int kRing = 2 * kTileBytes;  // after the two q tiles
-    static constexpr int kBars = kRing + kGroups * kGroupBytes;
+    static constexpr int kStage = kRing + kGroups * kGroupBytes;  // 4 KiB a softmax warp
+    static constexpr int kBars = kStage + 8 * 4096;
     static constexpr int kTotal = 1024 + kBars + 512;
+    static_assert(kTotal + 1024 <= 227 * 1024, "shared memory, with the static part");
 };
 
 // Instruction descriptor of tcgen05.mma.kind::f16: A and B both fp16 or both bf16,
@@ -228,19 +230,21 @@ __device__ __forceinline__ void clear_rows(uint8_t* v_tile, int from, int to, in
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
 
-// Whether rows [from, to) of a value tile hold an infinity or NaN (this thread's share).
+// Whether rows [from, to) of a value tile hold an infinity or NaN (thread t: row t).
+// An exponent of all ones carries into the sign bit when its lowest bit is added.
 template <class T, int kD>
 __device__ __forceinline__ bool wild_rows(const uint8_t* v_tile, int from, int to, int t) {
-    constexpr uint32_t kOnes = kIsHalf<T> ? 0x7C007C00u : 0x7F807F80u;
-    bool wild = false;
-    for (int i = t; i < (to - from) * (kD / 8); i += 128) {
-        const uint4 w = *reinterpret_cast<const uint4*>(tile_chunk(v_tile, from + i / (kD / 8), i % (kD / 8)));
-        const uint32_t e[4] = {w.x & kOnes, w.y & kOnes, w.z & kOnes, w.w & kOnes};
+    constexpr uint32_t kOnes = kIsHalf<T> ? 0x7C007C00u : 0x7F807F80u, kLowest = kIsHalf<T> ? 0x04000400u : 0x00800080u;
+    uint32_t carry = 0;
+    if (t >= from && t < to) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            wild |= (e[j] & 0xFFFF0000u) == (kOnes & 0xFFFF0000u) || (e[j] & 0xFFFFu) == (kOnes & 0xFFFFu);
+        for (int c = 0; c < kD / 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(tile_chunk(v_tile, t, c));
+            carry |= ((w.x & kOnes) + kLowest) | ((w.y & kOnes) + kLowest) | ((w.z & kOnes) + kLowest) |
+                     ((w.w & kOnes) + kLowest);
+        }
     }
-    return wild;
+    return (carry & 0x80008000u) != 0;
 }
 
 // O += P V of one key tile by the warpgroup itself, every row with the keys that it
@@ -561,13 +565,11 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 }
                 tmem_fence_after();
                 const uint32_t bad = *(volatile uint32_t*)&bad_ring[n % kBadRing];
-                // Masked scores are scaled and masked in their place first, in a loop of
-                // its own (unrolled beside the rest, the code of all warps no longer
-                // stays in the instruction cache, and the MMA warp's steps take 100 to
-                // 200 cycles each); so are all where the scale turns the order around.
                 const bool masked = key0 + kTile > low || bad;
                 float mul = scale;
-                if (masked || scale < 0.0f) {
+                if (bad || !(scale > 0.0f)) {
+                    // Key tiles with pages outside the cache, and scales that turn the
+                    // order around: scaled and masked in their place first.
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
                         uint32_t x[32];
@@ -590,6 +592,12 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 tmem_ld_wait();
                 tmem_fence_before();
                 mbar_arrive(s_free);
+                if (masked) {
+                    const int seen = limit - key0;
+#pragma unroll
+                    for (int k = 0; k < kTile; ++k)
+                        if (k >= seen) s[k / 32][k % 32] = __float_as_uint(-INFINITY);
+                }
                 float m[4];
 #pragma unroll
                 for (int k = 0; k < 64; ++k) {
@@ -676,46 +684,64 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const long long part_at_row = (long long)blockIdx.x * 2 + (r.flags & kSecondSlot ? 1 : 0);
             if (!whole && row_ok)
                 *reinterpret_cast<float2*>(ws.part_stats[1] + 2 * (part_at_row * kManyRows + row)) = make_float2(ref, sum);
-            T* out_row = static_cast<T*>(a.out) + (long long)(r.first + token) * a.ld_out + (long long)head * p.dim;
+            if (final && shape.wide_out) {
+                // 64 columns at a time through the warp's staging block, so that eight
+                // lanes write 128 bytes of a row (a lane its own row: 32 half sectors a
+                // store, 5500 cycles an item).
+                uint8_t* stage = smem + S::kStage + warp * 4096;
+                const long long mine = row_ok ? (long long)(r.first + token) * a.ld_out + (long long)head * p.dim : -1;
 #pragma unroll 1
-            for (int c = 0; c < kD / 32; ++c) {
-                uint32_t o[32];
-                tmem_ld_32x32b_x32(o_addr + c * 32, o);
-                tmem_ld_wait();
-                if (row_ok) {
+                for (int c = 0; c < kD / 64; ++c) {
 #pragma unroll
-                    for (int k = 0; k < 32; k += 8) {
-                        const int d = c * 32 + k;
-                        if (d < p.dim) {
-                            if (final) {
-                                Pack<T, 8> w;
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(o_addr + c * 64 + h * 32, o);
+                        tmem_ld_wait();
 #pragma unroll
-                                for (int e = 0; e < 8; ++e)
-                                    w.e[e] = from_float<T>(sum == 0.0f ? 0.0f : __uint_as_float(o[k + e]) * norm);
-                                if (shape.wide_out) {
-                                    *reinterpret_cast<Pack<T, 8>*>(out_row + d) = w;
-                                } else {
-                                    const uint2* h = reinterpret_cast<const uint2*>(&w);
-                                    reinterpret_cast<uint2*>(out_row + d)[0] = h[0];
-                                    reinterpret_cast<uint2*>(out_row + d)[1] = h[1];
-                                }
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; e += 4) {
-                                    const float v[4] = {__uint_as_float(o[k + e]), __uint_as_float(o[k + e + 1]),
-                                                        __uint_as_float(o[k + e + 2]), __uint_as_float(o[k + e + 3])};
-                                    if (whole)
-                                        put_row<T>(a, ws, r.flags & kPrefix, r.first + token, head, d + e, v, ref, sum);
-                                    else
-                                        *reinterpret_cast<float4*>(
-                                            ws.part_sums[1] + 4 * ((part_at_row * (kD / 4) + (d + e) / 4) * kManyRows + row)) =
-                                            make_float4(v[0], v[1], v[2], v[3]);
-                                }
-                            }
+                        for (int k = 0; k < 4; ++k) {
+                            uint4 w;
+                            const auto two = [&](int e) {
+                                return pack_pair<T>(sum == 0.0f ? 0.0f : __uint_as_float(o[8 * k + e]) * norm,
+                                                    sum == 0.0f ? 0.0f : __uint_as_float(o[8 * k + e + 1]) * norm);
+                            };
+                            w = make_uint4(two(0), two(2), two(4), two(6));
+                            *reinterpret_cast<uint4*>(stage + lane * 128 + (((h * 4 + k) ^ (lane & 7)) << 4)) = w;
                         }
                     }
+                    __syncwarp();
+                    const int d = c * 64 + (lane & 7) * 8;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int rr = i * 4 + (lane >> 3);
+                        const long long to = __shfl_sync(0xffffffffu, mine, rr);
+                        const uint4 w = *reinterpret_cast<const uint4*>(stage + rr * 128 + (((lane & 7) ^ (rr & 7)) << 4));
+                        if (to >= 0 && d < p.dim) *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + to + d) = w;
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < kD / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(o_addr + c * 32, o);
+                    tmem_ld_wait();
+                    if (row_ok) {
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4) {
+                            const int d = c * 32 + k;
+                            const float v[4] = {__uint_as_float(o[k]), __uint_as_float(o[k + 1]), __uint_as_float(o[k + 2]),
+                                                __uint_as_float(o[k + 3])};
+                            if (d >= p.dim) continue;
+                            if (whole)
+                                put_row<T>(a, ws, r.flags & kPrefix, r.first + token, head, d, v, ref, sum);
+                            else
+                                *reinterpret_cast<float4*>(
+                                    ws.part_sums[1] + 4 * ((part_at_row * (kD / 4) + d / 4) * kManyRows + row)) =
+                                    make_float4(v[0], v[1], v[2], v[3]);
+                        }
+                    }
+                    __syncwarp();
+                }
             }
             tmem_fence_before();  // O has been read before the next weights are announced
         }
