@@ -10,19 +10,21 @@
 // Split.  A request's rows of one kv head -- its new tokens times the heads of
 // the group, which all read the same keys -- make an item (more than 256 rows:
 // several); the shared prefix is one more request whose rows are all the call's
-// rows.  Every block takes an equal run of the items' key tiles, whatever the
-// lengths are: it finds its run by a scan over the requests, so the plan lives on
-// the device and a captured call follows the lengths of its replay.  A run covers
-// whole items and at most two parts of items, whose sums it leaves in a slot of
-// its own; a second kernel joins the parts of each item that a border cuts.  With
-// a prefix, own and prefix results stay in fp32 with their maxima and sums, and a
-// third joins the two.
+// rows.  Every worker -- a warp here, a block in the other kernel -- takes an equal
+// run of the items' keys, whatever the lengths are: it finds its run by a scan over
+// the requests, so the plan lives on the device and a captured call follows the
+// lengths of its replay.  A run covers whole items and at most two parts of items,
+// whose sums it leaves in slots of its own; a second kernel joins the parts of each
+// item that a border cuts.  With a prefix, own and prefix results stay in fp32 with
+// their maxima and sums, and a third joins the two.
 //
 // Items of many rows are matrix products for tcgen05 (zq_attention_sm100.cu).
 // This file has the kernel of few rows -- single tokens, drafts: a decode batch
-// reads its cache once, memory bandwidth.  A warp streams its own 16 keys of 64
-// through a ring of cp.async stages, so that no barrier stands between the memory
-// and the products; the products are mma.sync, which at 16 rows take 4 of the 22
+// reads its cache once, memory bandwidth.  A warp streams its run of keys, 16 a
+// stage, through a ring of cp.async stages of its own, so that no barrier stands
+// between the memory and the products, and a warp between two items leaves the
+// memory to the others (four warps an item, their sums joined in shared memory:
+// 96 requests of 20 to 500 tokens took 44 us); the products are mma.sync, which at 16 rows take 4 of the 22
 // cycles that a key's bytes take an SM.  exp(s - m) enters the second product as
 // a sum of two 16-bit parts, so that it is not rounded to the cache's type.
 #include "zq_attention.cuh"
@@ -33,26 +35,21 @@ namespace {
 
 using namespace attn;
 
-constexpr int kWarps = 4;
+constexpr int kWarps = FewPlan::kTeam;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kSlice = 16;              // keys of a warp's stage
-constexpr int kUnit = kSlice * kWarps;  // keys of a unit
-static_assert(kUnit == FewPlan::kKeys, "a unit is one round of the warps");
-constexpr int kStages = 3;
+constexpr int kSlice = FewPlan::kKeys;  // keys of a stage
+constexpr int kLeast = 4;               // stages of a worker, at least
 constexpr int kBlocksPerSm = 2;
 constexpr int kJoinThreads = 256;
 
 template <int kD>
 constexpr int kStageBytes = kSlice * kD * 2 * 2;  // keys, then values
-// The ring of every warp, reused for the warps' sums; q.
+// Two tiles of q take a stage's room.
+template <int kMT>
+constexpr int kStages = kMT == 1 ? 3 : 2;
+// A warp's ring and its q.
 template <int kD, int kMT>
-constexpr int kSmemBytes = kWarps * kStages * kStageBytes<kD> + 16 * kMT * kD * 2;
-
-// Where warp w leaves its sums: the start of its ring.
-template <int kD>
-__device__ __forceinline__ float* warp_sums(uint8_t* smem, int w) {
-    return reinterpret_cast<float*>(smem + w * kStages * kStageBytes<kD>);
-}
+constexpr int kWarpBytes = kStages<kMT> * kStageBytes<kD> + 16 * kMT * kD * 2;
 
 // 16-byte chunk `c` of row `r` of a row-major tile of kD 16-bit elements, chunks
 // XOR-swizzled by row so that eight rows of a column of chunks lie in different banks.
@@ -100,25 +97,26 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 // kMT: 16-row tiles of an item's kRows = 16 kMT rows.
 template <class T, int kD, int kMT>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(const AttentionArgs a, const Workspace ws) {
-    constexpr int kRows = 16 * kMT;
+    constexpr int kRows = 16 * kMT, kS = kStages<kMT>;
     constexpr int kChunks = kD / 8;  // 16-byte chunks of a row
-    static_assert(kStages * kStageBytes<kD> >= kRows * (kD + 2) * 4, "a warp's sums fit in its ring");
+    static_assert(kS * kStageBytes<kD> >= kRows * kD * 4 && kRows * kD * 2 >= kRows * 8, "a warp's sums fit in its ring");
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ long long scratch[kWarps + 2];
+    __shared__ long long scratch[kWarps + 2 * kWarps];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    uint8_t* ring = smem + warp * kStages * kStageBytes<kD>;
+    uint8_t* ring = smem + warp * kWarpBytes<kD, kMT>;
     const uint32_t ring_u = smem_u32(ring);
-    uint8_t* q_tile = smem + kWarps * kStages * kStageBytes<kD>;
+    uint8_t* q_tile = ring + kS * kStageBytes<kD>;
     const uint32_t q_u = smem_u32(q_tile);
     const PagedBatch& p = a.batch;
     const int group = a.heads / p.kv_heads, dim = p.dim;
+    const int worker = blockIdx.x * kWarps + warp;
 
     pdl_wait_primary();
     pdl_launch_dependents();
     const FewPlan plan{a, group, a.prefix_length > 0 ? live_rows(p) : 0};
-    const Found found = find_block<kThreads>(plan, blockIdx.x, gridDim.x, scratch);
-    Cursor<FewPlan> way(plan, found, blockIdx.x);
-    if (threadIdx.x == 0) ws.cuts[0][blockIdx.x] = way.cut(found.share, blockIdx.x, kRows);
+    const Found at = find_workers<kThreads, kWarps>(plan, blockIdx.x * kWarps, warp, gridDim.x * kWarps, kLeast, scratch);
+    Cursor<FewPlan> way(plan, at, worker);
+    if (lane == 0) ws.cuts[0][worker] = way.cut(at.share, worker, kRows);
 
     while (way.next()) {
         const Request r = way.it.r;
@@ -127,17 +125,16 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
         const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)way.it.b * p.ld_pages;
 
         // q of the item: row i is token i / group, head i % group of the kv head's.
-        for (int i = threadIdx.x; i < kRows * kChunks; i += kThreads) {
-            const int row = i / kChunks, c = i % kChunks;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (row < item_rows && c * 8 < dim) {
-                const int token = row / group, head = row % group;
-                v = load_l2(reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) +
-                                                           (long long)(r.first + token) * a.ldq +
-                                                           (long long)(head0 * group + head) * dim + c * 8));
-            }
-            *reinterpret_cast<uint4*>(q_tile + chunk_at<kD>(row, c)) = v;
+#pragma unroll
+        for (int j = 0; j < kRows * kChunks / 32; ++j) {
+            const int i = j * 32 + lane, row = i / kChunks, c = i % kChunks;
+            const bool live = row < item_rows && c * 8 < dim;
+            const T* src = static_cast<const T*>(a.q);
+            if (live)
+                src += (long long)(r.first + row / group) * a.ldq + (long long)(head0 * group + row % group) * dim + c * 8;
+            cp_async16(q_u + chunk_at<kD>(row, c), src, live);
         }
+        cp_async_commit();
 
         // Keys [0, limit) are seen by the thread's rows g and g + 8 of each tile.
         int limit[kMT][2], low = r.length;
@@ -153,11 +150,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
             }
         low = __reduce_min_sync(0xffffffffu, low);
 
-        // Slice i of the warp: keys (c0 + i) * 64 + warp * 16 ... in two halves of
-        // eight, each inside one page.  A lane keeps the pages of half a slice;
-        // a batch of 16 slices is looked up at a time.
-        const int key0 = c0 * kUnit + warp * kSlice;
-        const int slices = key0 < r.length ? min(c1 - c0, (r.length - key0 - 1) / kUnit + 1) : 0;
+        // Slice i: keys key0 + 16 i ... in two halves of eight, each inside one page.
+        // A lane keeps the pages of half a slice; a batch of 16 slices is looked up at
+        // a time.
+        const int key0 = c0 * kSlice;
+        const int slices = key0 < r.length ? min(c1 - c0, (r.length - key0 - 1) / kSlice + 1) : 0;
         int found = -1, offset = 0;
         uint32_t missing = 0;  // two bits a stage: a half on no page of the cache
         const T* kc = static_cast<const T*>(a.k_cache) + (long long)head0 * p.page * dim;
@@ -165,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
         const auto issue = [&](int i) {
             if (i < slices) {
                 if ((i & 15) == 0) {
-                    const int key = key0 + (i + (lane >> 1)) * kUnit + (lane & 1) * 8;
+                    const int key = key0 + (i + (lane >> 1)) * kSlice + (lane & 1) * 8;
                     found = -1;
                     if (key < r.length) {
                         const int index = key / p.page;
@@ -174,14 +171,14 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
                         found = id >= 0 && id < p.cache_pages ? id : -1;
                     }
                 }
-                const int stage = i % kStages;
+                const int stage = i % kS;
                 const uint32_t dst = ring_u + stage * kStageBytes<kD>;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int from = (i & 15) * 2 + half;
                     const int page = __shfl_sync(0xffffffffu, found, from);
                     const int off = __shfl_sync(0xffffffffu, offset, from);
-                    const int keys = r.length - (key0 + i * kUnit + half * 8);  // valid keys of this half
+                    const int keys = r.length - (key0 + i * kSlice + half * 8);  // valid keys of this half
                     missing &= ~(1u << (2 * stage + half));
                     if (page < 0 && keys > 0) missing |= 1u << (2 * stage + half);
                     const T* ks = kc + page * p.ld_k_page + off;
@@ -199,8 +196,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
             cp_async_commit();
         };
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) issue(i);
-        __syncthreads();  // q is there
+        for (int i = 0; i < kS - 1; ++i) issue(i);
+        cp_async_wait<kS - 1>();
+        __syncwarp();  // q is there
 
         // One tile's q stays in registers; two tiles' would not fit beside their sums.
         const auto load_q = [&](int mt, int k, uint32_t (&f)[4]) {
@@ -223,10 +221,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
         }
 
         for (int i = 0; i < slices; ++i) {
-            issue(i + kStages - 1);
-            cp_async_wait<kStages - 1>();
+            issue(i + kS - 1);
+            cp_async_wait<kS - 1>();
             __syncwarp();
-            const int stage = i % kStages, key = key0 + i * kUnit;
+            const int stage = i % kS, key = key0 + i * kSlice;
             const uint32_t k_u = ring_u + stage * kStageBytes<kD>, v_u = k_u + kSlice * kD * 2;
             float s[kMT][2][4];
 #pragma unroll
@@ -342,72 +340,118 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
         cp_async_wait<0>();
         __syncwarp();
 
-        // The warps' sums meet in shared memory: [row][dim], then the row's maximum and sum.
-        float* mine = reinterpret_cast<float*>(ring);
-        float* stats = mine + kRows * kD;
+        if (FewPlan::team_inside(way.it.start, way.it.end, at.share, worker)) {
+            // All the block's warps work on this one item: one part of it, by way of
+            // their rings; maxima and sums where q was.
+            float* mine = reinterpret_cast<float*>(ring);
+            float* stats = reinterpret_cast<float*>(q_tile);
+#pragma unroll
+            for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = mt * 16 + e * 8 + (lane >> 2);
+                    float t = sum[mt][e];
+                    t += __shfl_xor_sync(0xffffffffu, t, 1);
+                    t += __shfl_xor_sync(0xffffffffu, t, 2);
+#pragma unroll
+                    for (int n = 0; n < kD / 8; ++n)
+                        *reinterpret_cast<float2*>(mine + row * kD + n * 8 + (lane & 3) * 2) =
+                            make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
+                    if ((lane & 3) == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(top[mt][e], t);
+                }
+            __syncthreads();
+            const long long part = (long long)blockIdx.x * kWarps * 2 * kRows;
+            for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
+                const int row = i / (kD / 4), d = i % (kD / 4) * 4;
+                Joined j;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float* sums = reinterpret_cast<const float*>(smem + w * kWarpBytes<kD, kMT>);
+                    const float* st = reinterpret_cast<const float*>(smem + w * kWarpBytes<kD, kMT> + kS * kStageBytes<kD>);
+                    j.add(*reinterpret_cast<const float2*>(st + 2 * row),
+                          *reinterpret_cast<const float4*>(sums + row * kD + d));
+                }
+                *reinterpret_cast<float4*>(ws.part_sums[0] + (part + row) * kD + d) =
+                    make_float4(j.v[0], j.v[1], j.v[2], j.v[3]);
+                if (d == 0) *reinterpret_cast<float2*>(ws.part_stats[0] + 2 * (part + row)) = make_float2(j.most, j.total);
+            }
+            break;  // it is the one part of each of them
+        }
+
+        // Rows g and g + 8 of each tile, two elements of every eight a thread.
+        const long long slot = (long long)worker * 2 + way.slot;
 #pragma unroll
         for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int row = mt * 16 + e * 8 + (lane >> 2);
-#pragma unroll
-                for (int n = 0; n < kD / 8; ++n)
-                    *reinterpret_cast<float2*>(mine + row * kD + n * 8 + (lane & 3) * 2) =
-                        make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
                 float t = sum[mt][e];
                 t += __shfl_xor_sync(0xffffffffu, t, 1);
                 t += __shfl_xor_sync(0xffffffffu, t, 2);
-                if ((lane & 3) == 0) {
-                    stats[2 * row] = top[mt][e];
-                    stats[2 * row + 1] = t;
+                if (row >= item_rows) continue;
+                const int token = r.first + row / group, head = head0 * group + row % group;
+                if (way.whole && a.prefix_length == 0) {
+                    const float norm = t == 0.0f ? 0.0f : 1.0f / t;  // a row that sees no key is zero
+                    T* dst = static_cast<T*>(a.out) + (long long)token * a.ld_out + (long long)head * dim;
+#pragma unroll
+                    for (int n = 0; n < kD / 8; ++n)
+                        if (n * 8 < dim) {
+                            Pack<T, 2> w{{from_float<T>(t == 0.0f ? 0.0f : o[mt][n][2 * e] * norm),
+                                          from_float<T>(t == 0.0f ? 0.0f : o[mt][n][2 * e + 1] * norm)}};
+                            *reinterpret_cast<Pack<T, 2>*>(dst + n * 8 + (lane & 3) * 2) = w;
+                        }
+                } else {
+                    const long long at_row = way.whole ? (long long)token * a.heads + head : slot * kRows + row;
+                    float* sums = way.whole ? (prefix ? ws.row_sums[1] : ws.row_sums[0]) : ws.part_sums[0];
+                    float* stats = way.whole ? (prefix ? ws.row_stats[1] : ws.row_stats[0]) : ws.part_stats[0];
+                    float* dst = sums + at_row * (way.whole ? dim : kD);
+#pragma unroll
+                    for (int n = 0; n < kD / 8; ++n)
+                        if (n * 8 < dim)
+                            *reinterpret_cast<float2*>(dst + n * 8 + (lane & 3) * 2) =
+                                make_float2(o[mt][n][2 * e], o[mt][n][2 * e + 1]);
+                    if ((lane & 3) == 0) *reinterpret_cast<float2*>(stats + 2 * at_row) = make_float2(top[mt][e], t);
                 }
             }
-        __syncthreads();
-        for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
-            const int row = i / (kD / 4), d = i % (kD / 4) * 4;
-            float most = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w)
-                most = fmaxf(most, warp_sums<kD>(smem, w)[kRows * kD + 2 * row]);
-            const float ref = most == -INFINITY ? 0.0f : most;
-            float total = 0.0f, v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float* ow = warp_sums<kD>(smem, w);
-                const float keep = exp2_approx(ow[kRows * kD + 2 * row] - ref);
-                total += ow[kRows * kD + 2 * row + 1] * keep;
-                const float4 x = *reinterpret_cast<const float4*>(ow + row * kD + d);
-                v[0] += x.x * keep;
-                v[1] += x.y * keep;
-                v[2] += x.z * keep;
-                v[3] += x.w * keep;
-            }
-            if (d >= dim) continue;
-            const int token = row / group, head = head0 * group + row % group;
-            if (!way.whole)
-                put_part(ws.part_sums[0], ws.part_stats[0], ((long long)blockIdx.x * 2 + way.slot) * kRows + row, kD, d, v,
-                         most, total);
-            else
-                put_row<T>(a, ws, prefix, r.first + token, head, d, v, most, total);
-        }
-        __syncthreads();  // the sums are read: the rings and q may be written again
     }
 }
 
-// Joins the items that borders of the kernel of few rows (the first few_blocks - 1
-// blocks) and of the other kernel (eight blocks a border, 32 rows each) cut.
+// Joins the items that borders of the kernel of few rows (a warp a border, in the
+// first blocks; those of many parts or rows by the whole block) and of the other kernel
+// (eight blocks a border, 32 rows each) cut.
 template <class T, int kD, int kMT>
-__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_blocks) {
-    extern __shared__ int parts[];
+__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_workers) {
+    constexpr int kJoinWarps = kJoinThreads / 32, kSlices = kManyRows / kSliceRows;
     pdl_launch_dependents();
     pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
-    const int borders = max(few_blocks - 1, 0), k = (int)blockIdx.x - borders;
-    constexpr int kSlices = kManyRows / kSliceRows;
-    if (k < 0)
-        join_item<T, FewPlan, 16 * kMT, kD, false, kJoinThreads>(a, ws, 0, blockIdx.x + 1, 0, parts);
-    else
-        join_item<T, ManyPlan, kManyRows, kD, true, kJoinThreads>(a, ws, 1, k / kSlices + 1, k % kSlices * kSliceRows,
-                                                                  parts);
+    const int few_blocks = (few_workers + kJoinWarps - 1) / kJoinWarps;
+    if ((int)blockIdx.x < few_blocks) {
+        const int first = blockIdx.x * kJoinWarps, g = first + (threadIdx.x >> 5);
+        bool long_one = false;
+        if (g > 0 && g < few_workers) {
+            const Cut c = load_cut(ws, 0, g);
+            if (c.rows > 0) {
+                const int lane = threadIdx.x & 31;
+                const long long reach = (c.end - 1) / c.share - (g - 1);
+                const unsigned members = __ballot_sync(0xffffffffu, lane <= reach && FewPlan::holds(c, g - 1 + lane));
+                long_one = reach >= 32 || __popc(members) > kWarpParts || c.rows > kWarpRows<kD>;
+                if (!long_one) join_few<T, 16 * kMT, kD>(a, ws, c, g, members);
+            }
+        }
+        __shared__ bool left[kJoinWarps];
+        if ((threadIdx.x & 31) == 0) left[threadIdx.x >> 5] = long_one;
+        __syncthreads();
+#pragma unroll 1
+        for (int w = 0; w < kJoinWarps; ++w) {
+            if (!left[w]) continue;
+            join_item<T, FewPlan, 16 * kMT, kD, false, kJoinThreads>(a, ws, load_cut(ws, 0, first + w), 0, first + w, 0);
+            __syncthreads();
+        }
+    } else {
+        const int k = (int)blockIdx.x - few_blocks, g = k / kSlices + 1, from = k % kSlices * kSliceRows;
+        const Cut c = load_cut(ws, 1, g);
+        if (from < c.rows) join_item<T, ManyPlan, kManyRows, kD, true, kJoinThreads>(a, ws, c, 1, g, from);
+    }
 }
 
 // Joins the own and the prefix result of every row that a request owns.
@@ -458,17 +502,17 @@ cudaError_t launch_t(const AttentionArgs& a, int dtype, const Shape& s, const Wo
     if (s.many_blocks) e = launch_attend_many(a, dtype, ws, s.many_blocks, stream);
     if (e != cudaSuccess) return e;
     if (s.few_blocks) {
-        constexpr int smem = kSmemBytes<kD, kMT>;
+        constexpr int smem = kWarps * kWarpBytes<kD, kMT>;
+        static_assert(kBlocksPerSm * (smem + 1024 + 256) <= 228 * 1024, "both blocks of an SM");
         e = ensure_smem_attr(attend_few_kernel<T, kD, kMT>, smem);
         if (e != cudaSuccess) return e;
         e = launch_pdl_kernel(attend_few_kernel<T, kD, kMT>, dim3(s.few_blocks), dim3(kThreads), smem, stream, a, ws);
         if (e != cudaSuccess) return e;
     }
-    const int joins = (s.few_blocks ? s.few_blocks - 1 : 0) +
+    const int few_workers = s.few_blocks * kWarps;
+    const int joins = (few_workers + kJoinThreads / 32 - 1) / (kJoinThreads / 32) +
                       (s.many_blocks ? (s.many_blocks - 1) * (kManyRows / kSliceRows) : 0);
-    const size_t parts = sizeof(int) * (size_t)(s.few_blocks > s.many_blocks ? s.few_blocks : s.many_blocks);
-    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(joins), dim3(kJoinThreads), parts, stream, a, ws,
-                          s.few_blocks);
+    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(joins), dim3(kJoinThreads), 0, stream, a, ws, few_workers);
     if (e != cudaSuccess || a.prefix_length == 0) return e;
     return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);
 }
@@ -491,11 +535,11 @@ Workspace layout(const AttentionArgs& a, const Shape& s, uint8_t* base, size_t* 
         at += align256(n * sizeof(float));
         return p;
     };
-    const size_t parts[2] = {(size_t)s.few_blocks * 2 * s.few_rows, (size_t)s.many_blocks * 2 * kManyRows};
+    const size_t parts[2] = {(size_t)s.few_blocks * kWarps * 2 * s.few_rows, (size_t)s.many_blocks * 2 * kManyRows};
     for (int k = 0; k < 2; ++k) {
         ws.part_sums[k] = take(parts[k] * s.width);
         ws.part_stats[k] = take(parts[k] * 2);
-        ws.cuts[k] = reinterpret_cast<Cut*>(take((size_t)(k ? s.many_blocks : s.few_blocks) * (sizeof(Cut) / sizeof(float))));
+        ws.cuts[k] = reinterpret_cast<Cut*>(take((size_t)(k ? s.many_blocks : s.few_blocks * kWarps) * (sizeof(Cut) / sizeof(float))));
     }
     if (a.prefix_length > 0) {
         const size_t rows = (size_t)a.batch.rows * a.heads;

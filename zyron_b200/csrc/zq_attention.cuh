@@ -12,9 +12,9 @@ namespace attn {
 // weights are relative to and their sum.
 struct Cut;
 struct Workspace {
-    // Of the kernel of few rows and of the other: parts of cut items, [block][2][rows][width]
-    // and [block][2][width / 4][rows][4] (a thread a row there), their statistics
-    // [block][2][rows][2], and by block the item that its first unit cuts.
+    // Of the kernel of few rows and of the other: parts of cut items, [worker][2][rows][width]
+    // and [worker][2][width / 4][rows][4] (a thread a row there), their statistics
+    // [worker][2][rows][2], and by worker the item that its first unit cuts.
     float* part_sums[2];
     float* part_stats[2];
     Cut* cuts[2];
@@ -73,8 +73,9 @@ __device__ __forceinline__ int live_rows(const PagedBatch& p) {
 
 // ---- plans ----------------------------------------------------------------------
 //
-// A plan deals the call's work out to the blocks of one kernel.  Work is counted
-// in units; every block takes `share` consecutive ones.  Items (a tile of a
+// A plan deals the call's work out to the workers of one kernel: its warps (few
+// rows) or blocks (many).  Work is counted in units; every worker takes `share`
+// consecutive ones.  Items (a tile of a
 // request's rows of one kv head) follow one another, and a place inside an item
 // stands for a border between its key tiles (cut()).
 struct Item {
@@ -86,10 +87,21 @@ struct Item {
     int key_tiles;
 };
 
-// Requests of at most a.few_rows rows of a kv head: one item a head, units of 64
+// What the join needs to know of an item that the border in front of a worker's
+// first unit cuts; rows 0: none, or an earlier border cuts it too.
+struct alignas(16) Cut {
+    long long start, end, share;
+    int rows;       // of the item
+    int first_row;  // of the request
+    int row0;       // the item's first, among the request's rows of the kv head
+    int head, key_tiles, prefix;
+};
+
+// Requests of at most a.few_rows rows of a kv head: one item a head, units of 16
 // keys, at least one, so that rows that see no key are written too.
 struct FewPlan {
-    static constexpr int kKeys = 64;
+    static constexpr int kKeys = 16;
+    static constexpr int kTeam = 4;  // warps of a block, which leave one part of an item that all of them are inside
     const AttentionArgs& a;
     int group, prefix_rows;
 
@@ -120,6 +132,14 @@ struct FewPlan {
     }
     __device__ static __forceinline__ int cut(long long start, long long end, int, long long unit) {
         return (int)(min(max(unit, start), end) - start);
+    }
+    __device__ static __forceinline__ bool team_inside(long long start, long long end, long long share, int worker) {
+        const long long first = worker / kTeam * kTeam * share;
+        return start <= first && first + kTeam * share <= end;
+    }
+    // Whether worker h (of those that the item reaches) left a part of it.
+    __device__ static __forceinline__ bool holds(const Cut& c, int h) {
+        return h % kTeam == 0 || !team_inside(c.start, c.end, c.share, h);
     }
 };
 
@@ -188,32 +208,26 @@ struct ManyPlan {
     __device__ static __forceinline__ int cut(long long start, long long end, int key_tiles, long long unit) {
         return (int)((min(max(unit, start), end) - start) * key_tiles / (end - start));
     }
+    __device__ static __forceinline__ bool holds(const Cut& c, int h) {
+        return cut(c.start, c.end, c.key_tiles, h * c.share) < cut(c.start, c.end, c.key_tiles, (h + 1) * c.share);
+    }
 };
 __device__ __forceinline__ long long cost_of(const FewPlan& plan, int, const Request& r) { return plan.cost(r); }
 __device__ __forceinline__ long long cost_of(const ManyPlan& plan, int b, const Request& r) { return plan.cost_of(b, r); }
 
-// What the join needs to know of an item that the border in front of a block's
-// first unit cuts; rows 0: none, or an earlier border cuts it too.
-struct alignas(16) Cut {
-    long long start, end, share;
-    int rows;       // of the item
-    int first_row;  // of the request
-    int row0;       // the item's first, among the request's rows of the kv head
-    int head, key_tiles, prefix;
-};
-
 struct Found {
-    long long share;   // units a block
+    long long share;   // units a worker
     long long total;   // units of the call
     long long before;  // units before request b
-    int b;             // the request that holds the block's first unit
+    int b;             // the request that holds the worker's first unit
 };
 
-// Block `g` of `blocks`: its share and where it begins, by a scan of the whole
-// block (kThreads threads) over the requests.  `scratch` is kThreads / 32 + 2
-// words of 64 bits.
-template <int kThreads, class Plan>
-__device__ Found find_block(const Plan& plan, long long g, int blocks, long long* scratch) {
+// Workers g0 .. g0 + kFinds - 1 of `workers` (a worker is a warp or a block): their
+// share, `least` units or more, and where they begin, by a scan of the whole block
+// (kThreads threads) over the requests; for worker g0 + which.  `scratch` is
+// kThreads / 32 + 2 kFinds words of 64 bits.
+template <int kThreads, int kFinds, class Plan>
+__device__ Found find_workers(const Plan& plan, long long g0, int which, int workers, int least, long long* scratch) {
     constexpr int kWarps = kThreads / 32;
     const int n = plan.a.batch.requests;
     const int each = (n + kThreads - 1) / kThreads;
@@ -236,32 +250,38 @@ __device__ Found find_block(const Plan& plan, long long g, int blocks, long long
         if (w < warp) before += scratch[w];
         total += scratch[w];
     }
-    const long long share = (total + blocks - 1) / blocks;
-    const long long unit = g * share;
-    if (unit < head) {
-        if (threadIdx.x == 0) scratch[kWarps] = 0, scratch[kWarps + 1] = -1;
-    } else if (unit >= before && unit < before + mine) {
-        int b = first;
-        long long c = cost_of(plan, b, plan.get(b));
-        while (unit >= before + c) {
-            before += c;
-            ++b;
-            c = cost_of(plan, b, plan.get(b));
+    const long long even = (total + workers - 1) / workers, share = even > least ? even : least;
+    long long* found = scratch + kWarps;
+    int b = first;
+    long long end = before;  // units up to request b
+#pragma unroll 1
+    for (int f = 0; f < kFinds; ++f) {
+        const long long unit = (g0 + f) * share;
+        if (unit < head) {
+            if (threadIdx.x == 0) found[2 * f] = 0, found[2 * f + 1] = -1;
+        } else if (unit >= before && unit < before + mine) {
+            // one request a thread up to kThreads: nothing is read again
+            long long c = each == 1 ? mine : cost_of(plan, b, plan.get(b));
+            while (unit >= end + c) {
+                end += c;
+                ++b;
+                c = cost_of(plan, b, plan.get(b));
+            }
+            found[2 * f] = end;
+            found[2 * f + 1] = b;
         }
-        scratch[kWarps] = before;
-        scratch[kWarps + 1] = b;
     }
     __syncthreads();
-    return Found{share, total, scratch[kWarps], (int)scratch[kWarps + 1]};  // before and b: if unit < total
+    return Found{share, total, found[2 * which], (int)found[2 * which + 1]};  // before and b: if its unit < total
 }
 
-// A block's way through its items: found once, then step by step, without a
+// A worker's way through its items: found once, then step by step, without a
 // division but at the borders that cut an item (a search and 64-bit divisions an
 // item took 12 us a part).
 template <class Plan>
 struct Cursor {
     const Plan& plan;
-    long long unit, last;  // the block's units
+    long long unit, last;  // the worker's units
     // the current part
     Item it;
     int first_tile, end_tile;
@@ -295,7 +315,7 @@ struct Cursor {
         return false;
     }
 
-    // The cut that block g's own first border makes (before the first next()).
+    // The cut that worker g's own first border makes (before the first next()).
     __device__ __forceinline__ Cut cut(long long share, long long g, int tile_rows) const {
         Cut c{};
         if (unit < last && it.start < unit && it.start >= (g - 1) * share) {
@@ -308,13 +328,6 @@ struct Cursor {
   private:
     long long begin;
 };
-
-// Four elements of a part.
-__device__ __forceinline__ void put_part(float* sums, float* stats, long long row, int width, int d, const float (&v)[4],
-                                         float most, float total) {
-    *reinterpret_cast<float4*>(sums + row * width + d) = make_float4(v[0], v[1], v[2], v[3]);
-    if (d == 0) *reinterpret_cast<float2*>(stats + 2 * row) = make_float2(most, total);
-}
 
 // Four elements of a row's output.  A row that sees no key is zero.
 template <class T>
@@ -360,68 +373,195 @@ struct Joined {
     }
 };
 
-// Joins the parts of the item that border g (in front of block g's first unit)
+// Joins the parts of the item that border g (in front of worker g's first unit)
 // cuts: rows [from, from + kSliceRows) of it.  kRows, kWidth: a part's; kByRow: its
-// rows lie side by side (the kernel of many rows).  `parts` has room for the
-// numbers of all parts.
-constexpr int kSliceRows = 32;
-template <class T, class Plan, int kRows, int kWidth, bool kByRow, int kThreads>
-__device__ void join_item(const AttentionArgs& a, const Workspace& ws, int kind, int g, int from, int* parts) {
-    const PagedBatch& p = a.batch;
-    const int group = a.heads / p.kv_heads;
+// rows lie side by side (the kernel of many rows).  Parts are taken 64 workers at a
+// time: their weights first, eight threads a row, then their sums with every load
+// under way at once.
+__device__ __forceinline__ Cut load_cut(const Workspace& ws, int kind, int g) {
     Cut c;
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(Cut) / 16); ++i) {
         const uint4 w = load_l2(reinterpret_cast<const uint4*>(ws.cuts[kind] + g) + i);
         memcpy(reinterpret_cast<char*>(&c) + 16 * i, &w, 16);
     }
-    if (from >= c.rows) return;
-    // Blocks g - 1 .. hold parts of it; those without key tiles wrote none, and an
-    // item that one block holds alone is finished.
-    __shared__ int count;
+    return c;
+}
+constexpr int kSliceRows = 32;
+template <class T, class Plan, int kRows, int kWidth, bool kByRow, int kThreads>
+__device__ void join_item(const AttentionArgs& a, const Workspace& ws, const Cut& c, int kind, int g, int from) {
+    constexpr int kSlice = kRows < kSliceRows ? kRows : kSliceRows, kBatch = 64;
+    static_assert(kThreads == 8 * kSliceRows, "eight threads a row");
+    const PagedBatch& p = a.batch;
+    const int group = a.heads / p.kv_heads;
+    __shared__ int parts[kBatch], count;
+    __shared__ float weights[kBatch][kSlice], totals[kBatch][kSlice];  // maxima, then weights; sums
+    __shared__ float row_most[kSlice], row_total[kSlice], row_keep[kSlice];
+    const int lane = threadIdx.x & 31, h1 = (int)((c.end - 1) / c.share), rows = min(c.rows - from, kSlice);
+    // Workers g - 1 .. h1 may hold parts of it.
+    const auto holds = [&](int h) { return h <= h1 && Plan::holds(c, h); };
     if (threadIdx.x < 32) {
-        const int lane = threadIdx.x, h1 = (int)((c.end - 1) / c.share);
         int n = 0;
-        for (int h0 = g - 1; h0 <= h1; h0 += 32) {
-            const int h = h0 + lane;
-            const bool has = h <= h1 && Plan::cut(c.start, c.end, c.key_tiles, h * c.share) <
-                                            Plan::cut(c.start, c.end, c.key_tiles, (h + 1) * c.share);
-            const unsigned m = __ballot_sync(0xffffffffu, has);
-            // the first block's part may lie in its second slot
-            if (has) parts[n + __popc(m & ((1u << lane) - 1u))] = 2 * h + (h == g - 1 && h * c.share < c.start ? 1 : 0);
-            n += __popc(m);
-        }
+        for (int h = g - 1; h <= h1 && n < 2; h += 32) n += __popc(__ballot_sync(0xffffffffu, holds(h + lane)));
         if (lane == 0) count = n;
     }
+    if (threadIdx.x < kSlice) {
+        row_most[threadIdx.x] = -INFINITY;
+        row_total[threadIdx.x] = 0.0f;
+    }
     __syncthreads();
-    const int n = count;
-    if (n < 2) return;
-    const int rows = min(c.rows - from, kSliceRows);
-    for (int i = threadIdx.x; i < kSliceRows * (kWidth / 4); i += kThreads) {
-        const int in = kByRow ? i % kSliceRows : i / (kWidth / 4);
-        const int d = (kByRow ? i / kSliceRows : i % (kWidth / 4)) * 4, row = from + in;
-        if (d >= p.dim || in >= rows) continue;
-        Joined j;
-        for (int k0 = 0; k0 < n; k0 += 4) {
-            float2 stats[4];
-            float4 sums[4];
+    if (count < 2) return;  // a worker that holds the item alone has finished it
+    constexpr int kElems = kSlice * (kWidth / 4), kEach = (kElems + kThreads - 1) / kThreads;
+    constexpr int kDeep = kEach < 4 ? 16 / kEach : 4;  // parts whose loads are under way at once
+    const auto place = [&](int e, int& in, int& d) {
+        const int i = e * kThreads + threadIdx.x;
+        in = kByRow ? i % kSlice : i / (kWidth / 4);
+        d = (kByRow ? i / kSlice : i % (kWidth / 4)) * 4;
+        return i < kElems && d < p.dim && in < rows;
+    };
+    float v[kEach][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {  // four parts' loads under way at once
-                stats[k] = make_float2(-INFINITY, 0.0f);
-                sums[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (k0 + k < n) {
-                    const long long part = parts[k0 + k];
-                    const long long at = kByRow ? (part * (kWidth / 4) + d / 4) * kRows + row
-                                                : (part * kRows + row) * (kWidth / 4) + d / 4;
-                    stats[k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + part * kRows + row);
-                    sums[k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind]) + at);
-                }
+    for (int e = 0; e < kEach; ++e) v[e][0] = v[e][1] = v[e][2] = v[e][3] = 0.0f;
+    for (int h0 = g - 1; h0 <= h1; h0 += kBatch) {
+        if (threadIdx.x < 32) {
+            int n = 0;
+#pragma unroll
+            for (int b = 0; b < kBatch; b += 32) {
+                const int h = h0 + b + lane;
+                const bool has = holds(h);
+                const unsigned m = __ballot_sync(0xffffffffu, has);
+                // the first worker's part may lie in its second slot
+                if (has) parts[n + __popc(m & ((1u << lane) - 1u))] = 2 * h + (h == g - 1 && h * c.share < c.start ? 1 : 0);
+                n += __popc(m);
             }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) j.add(stats[k], sums[k]);
+            if (lane == 0) count = n;
         }
-        const int token = (c.row0 + row) / group, head = c.head * group + (c.row0 + row) % group;
-        put_row<T>(a, ws, c.prefix, c.first_row + token, head, d, j.v, j.most, j.total);
+        __syncthreads();
+        const int n = count;
+        for (int i = threadIdx.x; i < n * kSlice; i += kThreads) {
+            const int k = i / kSlice, in = i % kSlice;
+            float2 s = make_float2(-INFINITY, 0.0f);
+            if (in < rows)
+                s = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + (long long)parts[k] * kRows + from + in);
+            weights[k][in] = s.x;
+            totals[k][in] = s.y;
+        }
+        __syncthreads();
+        const int in_row = threadIdx.x / 8, sub = threadIdx.x % 8;
+        const bool mine = in_row < kSlice;
+        float most = -INFINITY, total = 0.0f;
+        for (int k = sub; k < n && mine; k += 8) most = fmaxf(most, weights[k][in_row]);
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float before = mine ? row_most[in_row] : 0.0f;
+        most = fmaxf(most, before);
+        const float ref = most == -INFINITY ? 0.0f : most;
+        for (int k = sub; k < n && mine; k += 8) {
+            const float w = exp2_approx(weights[k][in_row] - ref);
+            weights[k][in_row] = w;
+            total += totals[k][in_row] * w;
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+        if (mine && sub == 0) {
+            const float keep = exp2_approx(before - ref);
+            row_keep[in_row] = keep;
+            row_most[in_row] = most;
+            row_total[in_row] = row_total[in_row] * keep + total;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            int in, d;
+            if (place(e, in, d) && h0 > g - 1) {
+                const float keep = row_keep[in];
+#pragma unroll
+                for (int x = 0; x < 4; ++x) v[e][x] *= keep;
+            }
+        }
+        for (int k0 = 0; k0 < n; k0 += kDeep) {
+            float4 x[kDeep][kEach];
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    int in, d;
+                    x[k][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (place(e, in, d) && k0 + k < n) {
+                        const long long part = parts[k0 + k];
+                        const long long at = kByRow ? (part * (kWidth / 4) + d / 4) * kRows + from + in
+                                                    : (part * kRows + from + in) * (kWidth / 4) + d / 4;
+                        x[k][e] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind]) + at);
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < kDeep; ++k)
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) {
+                    int in, d;
+                    if (place(e, in, d) && k0 + k < n) {
+                        const float w = weights[k0 + k][in];
+                        v[e][0] = fmaf(x[k][e].x, w, v[e][0]);
+                        v[e][1] = fmaf(x[k][e].y, w, v[e][1]);
+                        v[e][2] = fmaf(x[k][e].z, w, v[e][2]);
+                        v[e][3] = fmaf(x[k][e].w, w, v[e][3]);
+                    }
+                }
+        }
+        __syncthreads();  // the batch's weights have been used
+    }
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+        int in, d;
+        if (!place(e, in, d)) continue;
+        const int row = c.row0 + from + in;
+        put_row<T>(a, ws, c.prefix, c.first_row + row / group, c.head * group + row % group, d, v[e], row_most[in],
+                   row_total[in]);
+    }
+}
+
+// The same of an item of a row or some in at most kWarpParts parts, `members` of the
+// workers g - 1 ..., by one warp: a lane four elements of a row, all its parts' loads
+// under way at once.
+constexpr int kWarpParts = 8;
+template <int kWidth>
+constexpr int kWarpRows = 4 * 128 / kWidth;
+template <class T, int kRows, int kWidth>
+__device__ void join_few(const AttentionArgs& a, const Workspace& ws, const Cut& c, int g, unsigned members) {
+    constexpr int kLanes = kWidth / 4, kTogether = 32 / kLanes, kSteps = 2;  // lanes of a row, rows at a time
+    const PagedBatch& p = a.batch;
+    const int group = a.heads / p.kv_heads, lane = threadIdx.x & 31;
+    const bool second = (g - 1) * c.share < c.start;  // the first worker's part lies in its second slot
+    for (int row0 = 0; row0 < c.rows; row0 += kSteps * kTogether) {
+        const int d = lane % kLanes * 4;
+        float2 stats[kSteps][kWarpParts];
+        float4 x[kSteps][kWarpParts];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int in = row0 + s * kTogether + lane / kLanes;
+            unsigned m = members;
+#pragma unroll
+            for (int k = 0; k < kWarpParts; ++k) {
+                stats[s][k] = make_float2(-INFINITY, 0.0f);
+                x[s][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (m && in < c.rows && d < p.dim) {
+                    const int h = __ffs(m) - 1;
+                    const long long at = (long long)(2 * (g - 1 + h) + (h == 0 && second ? 1 : 0)) * kRows + in;
+                    stats[s][k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[0]) + at);
+                    x[s][k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[0] + at * kWidth + d));
+                }
+                m &= m - 1;
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int in = row0 + s * kTogether + lane / kLanes;
+            if (in >= c.rows || d >= p.dim) continue;
+            Joined j;
+#pragma unroll
+            for (int k = 0; k < kWarpParts; ++k) j.add(stats[s][k], x[s][k]);
+            put_row<T>(a, ws, c.prefix, c.first_row + in / group, c.head * group + in % group, d, j.v, j.most, j.total);
+        }
     }
 }
 

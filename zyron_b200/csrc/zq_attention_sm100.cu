@@ -371,7 +371,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     pdl_launch_dependents();
 
     const ManyPlan plan{a, shape.group, a.prefix_length > 0 ? live_rows(p) : 0, 2 * shape.tile_tokens};
-    const Found found = find_block<kManyThreads>(plan, blockIdx.x, gridDim.x, scratch);
+    const Found found = find_workers<kManyThreads, 1>(plan, blockIdx.x, 0, gridDim.x, 1, scratch);
     // Tiles of the item that hold rows.
     const auto q_tiles = [&](const Part& q) { return q.rows - q.token0 > shape.tile_tokens ? 2 : 1; };
     // The block's part number `i`; false: the producer gave up.
