@@ -38,7 +38,8 @@ using namespace attn;
 constexpr int kWarps = FewPlan::kTeam;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kSlice = FewPlan::kKeys;  // keys of a stage
-constexpr int kLeast = 4;               // stages of a worker, at least
+constexpr int kLeast = 4;  // units of a worker, at least: all warps of a block inside one item have keys of it
+static_assert(kLeast > FewPlan::kItem, "");
 constexpr int kBlocksPerSm = 2;
 constexpr int kJoinThreads = 256;
 
@@ -361,6 +362,9 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
                 }
             __syncthreads();
             const long long part = (long long)blockIdx.x * kWarps * 2 * kRows;
+            const long long from = blockIdx.x * kWarps * at.share, to = from + kWarps * at.share;
+            const bool all = FewPlan::cut(way.it.start, way.it.end, way.it.key_tiles, from) == 0 &&
+                             FewPlan::cut(way.it.start, way.it.end, way.it.key_tiles, to) == way.it.key_tiles;
             for (int i = threadIdx.x; i < item_rows * (kD / 4); i += kThreads) {
                 const int row = i / (kD / 4), d = i % (kD / 4) * 4;
                 Joined j;
@@ -370,6 +374,11 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
                     const float* st = reinterpret_cast<const float*>(smem + w * kWarpBytes<kD, kMT> + kS * kStageBytes<kD>);
                     j.add(*reinterpret_cast<const float2*>(st + 2 * row),
                           *reinterpret_cast<const float4*>(sums + row * kD + d));
+                }
+                if (d >= dim) continue;
+                if (all) {
+                    put_row<T>(a, ws, prefix, r.first + row / group, head0 * group + row % group, d, j.v, j.most, j.total);
+                    continue;
                 }
                 *reinterpret_cast<float4*>(ws.part_sums[0] + (part + row) * kD + d) =
                     make_float4(j.v[0], j.v[1], j.v[2], j.v[3]);
@@ -416,42 +425,45 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
     }
 }
 
-// Joins the items that borders of the kernel of few rows (a warp a border, in the
-// first blocks; those of many parts or rows by the whole block) and of the other kernel
-// (eight blocks a border, 32 rows each) cut.
+// Joins the items that borders of the kernel of few rows cut: a warp a border, those
+// of many parts or rows by the whole block.
 template <class T, int kD, int kMT>
-__global__ void __launch_bounds__(kJoinThreads) join_parts_kernel(const AttentionArgs a, const Workspace ws, int few_workers) {
-    constexpr int kJoinWarps = kJoinThreads / 32, kSlices = kManyRows / kSliceRows;
+__global__ void __launch_bounds__(kJoinThreads) join_few_kernel(const AttentionArgs a, const Workspace ws, int workers) {
+    constexpr int kJoinWarps = kJoinThreads / 32;
     pdl_launch_dependents();
     pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
-    const int few_blocks = (few_workers + kJoinWarps - 1) / kJoinWarps;
-    if ((int)blockIdx.x < few_blocks) {
-        const int first = blockIdx.x * kJoinWarps, g = first + (threadIdx.x >> 5);
-        bool long_one = false;
-        if (g > 0 && g < few_workers) {
-            const Cut c = load_cut(ws, 0, g);
-            if (c.rows > 0) {
-                const int lane = threadIdx.x & 31;
-                const long long reach = (c.end - 1) / c.share - (g - 1);
-                const unsigned members = __ballot_sync(0xffffffffu, lane <= reach && FewPlan::holds(c, g - 1 + lane));
-                long_one = reach >= 32 || __popc(members) > kWarpParts || c.rows > kWarpRows<kD>;
-                if (!long_one) join_few<T, 16 * kMT, kD>(a, ws, c, g, members);
-            }
+    const int first = blockIdx.x * kJoinWarps, g = first + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    bool left = false;
+    if (g > 0 && g < workers) {
+        const Cut c = load_cut(ws, 0, g);
+        if (c.rows > 0) {
+            const long long reach = (c.end - 1) / c.share - (g - 1);
+            const unsigned members = __ballot_sync(0xffffffffu, lane <= reach && FewPlan::holds(c, g - 1 + lane));
+            left = reach >= 32 || __popc(members) > kWarpParts || c.rows > kWarpRows<kD>;
+            // an item that one worker holds alone is finished
+            if (!left && __popc(members) > 1) join_few<T, 16 * kMT, kD>(a, ws, c, g, members);
         }
-        __shared__ bool left[kJoinWarps];
-        if ((threadIdx.x & 31) == 0) left[threadIdx.x >> 5] = long_one;
-        __syncthreads();
-#pragma unroll 1
-        for (int w = 0; w < kJoinWarps; ++w) {
-            if (!left[w]) continue;
-            join_item<T, FewPlan, 16 * kMT, kD, false, kJoinThreads>(a, ws, load_cut(ws, 0, first + w), 0, first + w, 0);
-            __syncthreads();
-        }
-    } else {
-        const int k = (int)blockIdx.x - few_blocks, g = k / kSlices + 1, from = k % kSlices * kSliceRows;
-        const Cut c = load_cut(ws, 1, g);
-        if (from < c.rows) join_item<T, ManyPlan, kManyRows, kD, true, kJoinThreads>(a, ws, c, 1, g, from);
     }
+    __shared__ bool whole_block[kJoinWarps];
+    if (lane == 0) whole_block[threadIdx.x >> 5] = left;
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < kJoinWarps; ++w) {
+        if (!whole_block[w]) continue;
+        join_item<T, FewPlan, 16 * kMT, kD, false, kJoinThreads>(a, ws, load_cut(ws, 0, first + w), 0, first + w, 0);
+        __syncthreads();
+    }
+}
+
+// The same of the kernel of many rows: eight blocks a border, 32 rows each.
+template <class T, int kD>
+__global__ void __launch_bounds__(kJoinThreads, 4) join_many_kernel(const AttentionArgs a, const Workspace ws) {
+    constexpr int kSlices = kManyRows / kSliceRows;
+    pdl_launch_dependents();
+    pdl_wait_primary();
+    const int g = blockIdx.x / kSlices + 1, from = blockIdx.x % kSlices * kSliceRows;
+    const Cut c = load_cut(ws, 1, g);
+    if (from < c.rows) join_item<T, ManyPlan, kManyRows, kD, true, kJoinThreads>(a, ws, c, 1, g, from);
 }
 
 // Joins the own and the prefix result of every row that a request owns.
@@ -509,10 +521,15 @@ cudaError_t launch_t(const AttentionArgs& a, int dtype, const Shape& s, const Wo
         e = launch_pdl_kernel(attend_few_kernel<T, kD, kMT>, dim3(s.few_blocks), dim3(kThreads), smem, stream, a, ws);
         if (e != cudaSuccess) return e;
     }
-    const int few_workers = s.few_blocks * kWarps;
-    const int joins = (few_workers + kJoinThreads / 32 - 1) / (kJoinThreads / 32) +
-                      (s.many_blocks ? (s.many_blocks - 1) * (kManyRows / kSliceRows) : 0);
-    e = launch_pdl_kernel(join_parts_kernel<T, kD, kMT>, dim3(joins), dim3(kJoinThreads), 0, stream, a, ws, few_workers);
+    if (s.few_blocks) {
+        const int workers = s.few_blocks * kWarps, each = kJoinThreads / 32;
+        e = launch_pdl_kernel(join_few_kernel<T, kD, kMT>, dim3((workers + each - 1) / each), dim3(kJoinThreads), 0, stream,
+                              a, ws, workers);
+        if (e != cudaSuccess) return e;
+    }
+    if (s.many_blocks)
+        e = launch_pdl_kernel(join_many_kernel<T, kD>, dim3((s.many_blocks - 1) * (kManyRows / kSliceRows)),
+                              dim3(kJoinThreads), 0, stream, a, ws);
     if (e != cudaSuccess || a.prefix_length == 0) return e;
     return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);
 }

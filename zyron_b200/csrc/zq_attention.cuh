@@ -97,10 +97,13 @@ struct alignas(16) Cut {
     int head, key_tiles, prefix;
 };
 
-// Requests of at most a.few_rows rows of a kv head: one item a head, units of 16
-// keys, at least one, so that rows that see no key are written too.
+// Requests of at most a.few_rows rows of a kv head: one item a head.  A unit is 16
+// keys, at least one, so that rows that see no key are written too; kItem more stand
+// for what an item takes besides (with none, 51 items of 6 keys took 41 us, four a
+// worker).
 struct FewPlan {
     static constexpr int kKeys = 16;
+    static constexpr int kItem = 3;
     static constexpr int kTeam = 4;  // warps of a block, which leave one part of an item that all of them are inside
     const AttentionArgs& a;
     int group, prefix_rows;
@@ -110,28 +113,29 @@ struct FewPlan {
     }
     __device__ __forceinline__ int key_tiles(const Request& r) const { return r.length > 0 ? (r.length - 1) / kKeys + 1 : 1; }
     __device__ __forceinline__ long long cost(const Request& r) const {
-        return r.rows > 0 && (long long)r.rows * group <= a.few_rows ? (long long)a.batch.kv_heads * key_tiles(r) : 0;
+        return r.rows > 0 && (long long)r.rows * group <= a.few_rows ? (long long)a.batch.kv_heads * (key_tiles(r) + kItem) : 0;
     }
     __device__ __forceinline__ Item item(int b, const Request& r, long long before, long long unit) const {
         const int n = key_tiles(r);
-        const int head = (int)((unit - before) / n);
-        const long long start = before + (long long)head * n;
-        return Item{r, b, head, 0, start, start + n, n};
+        const int head = (int)((unit - before) / (n + kItem));
+        const long long start = before + (long long)head * (n + kItem);
+        return Item{r, b, head, 0, start, start + n + kItem, n};
     }
     // The first item of a request that has some, and the one behind an item of the
     // same request.
     __device__ __forceinline__ Item first(int b, const Request& r, long long unit) const {
         const int n = key_tiles(r);
-        return Item{r, b, 0, 0, unit, unit + n, n};
+        return Item{r, b, 0, 0, unit, unit + n + kItem, n};
     }
     __device__ __forceinline__ bool advance(Item& it) const {
         if (++it.head == a.batch.kv_heads) return false;
         it.start = it.end;
-        it.end += it.key_tiles;
+        it.end += it.key_tiles + kItem;
         return true;
     }
+    // The extra units come first: a border inside them is in front of the keys.
     __device__ static __forceinline__ int cut(long long start, long long end, int, long long unit) {
-        return (int)(min(max(unit, start), end) - start);
+        return (int)max(min(max(unit, start), end) - start - kItem, 0LL);
     }
     __device__ static __forceinline__ bool team_inside(long long start, long long end, long long share, int worker) {
         const long long first = worker / kTeam * kTeam * share;
@@ -139,7 +143,8 @@ struct FewPlan {
     }
     // Whether worker h (of those that the item reaches) left a part of it.
     __device__ static __forceinline__ bool holds(const Cut& c, int h) {
-        return h % kTeam == 0 || !team_inside(c.start, c.end, c.share, h);
+        return cut(c.start, c.end, c.key_tiles, h * c.share) < cut(c.start, c.end, c.key_tiles, (h + 1) * c.share) &&
+               (h % kTeam == 0 || !team_inside(c.start, c.end, c.share, h));
     }
 };
 
@@ -412,7 +417,7 @@ __device__ void join_item(const AttentionArgs& a, const Workspace& ws, const Cut
     __syncthreads();
     if (count < 2) return;  // a worker that holds the item alone has finished it
     constexpr int kElems = kSlice * (kWidth / 4), kEach = (kElems + kThreads - 1) / kThreads;
-    constexpr int kDeep = kEach < 4 ? 16 / kEach : 4;  // parts whose loads are under way at once
+    constexpr int kDeep = kEach < 4 ? 16 / kEach : 2;  // parts whose loads are under way at once
     const auto place = [&](int e, int& in, int& d) {
         const int i = e * kThreads + threadIdx.x;
         in = kByRow ? i % kSlice : i / (kWidth / 4);
