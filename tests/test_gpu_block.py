@@ -671,3 +671,22 @@ def test_decoder_block(zb, torch, new, lengths, prefix):
     graph.replay()
     for got, want in zip(captured[:6], (qkv, q, o, mid, a, y)):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (6, 3, 64)])
+def test_attention_of_many_prompts_gives_the_same_each_time(zb, torch, heads, kv_heads, dim):
+    """Short and long prompts in one call, so that blocks go from parts of many key
+    tiles to parts of one and back: right, and the same bits at every call."""
+    import random
+
+    rng = random.Random(heads)
+    for i in range(6):
+        new = [rng.choice([5, 60, 130, 257, 520, 901]) for _ in range(5)]
+        lengths = [n + rng.choice([0, 0, 1, 100, 700]) for n in new]
+        batch = Batch(torch, 20 + i, new, lengths, 32, kv_heads, dim, torch.bfloat16)
+        q = randn(torch, 30 + i, batch.rows, heads, dim).bfloat16()
+        want, tol = batch.want(q)
+        first = batch.attention(zb, q.cuda())
+        within(torch, first, want, tol, f"prompts {new} in {lengths}")
+        for _ in range(20):
+            assert torch.equal(batch.attention(zb, q.cuda()), first)

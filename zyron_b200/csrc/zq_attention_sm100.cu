@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         for (int i = 0; i < kPartRing; ++i) mbar_init(&part_full[i], 1);
         for (int i = 0; i < kGroups; ++i) {
             mbar_init(&kv_full[i], 1);
-            mbar_init(&kv_empty[i], 2);  // both issuing warps
+            mbar_init(&kv_empty[i], 2);  // keys and values taken
         }
         fence_mbar_init();
         tma_prefetch_desc(&tmap_q);
@@ -381,7 +381,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         return true;
     };
     // A part of T key tiles has T + 1 groups: keys of tile k in group k, values in
-    // the next; groups are counted over the block's parts.
+    // the next; groups are counted over the block's parts.  Who takes the half of a
+    // group that is there alone frees the other half too, so that nobody frees a
+    // group before it has been filled (which would count for the one before it).
     const auto keys_of = [&](int g) { return ring + g % kGroups * S::kGroupBytes; };
     const auto values_of = [&](int g) { return keys_of(g) + S::kTileBytes; };
     const auto phase_of = [](int g) { return (uint32_t)(g / kGroups) & 1u; };
@@ -490,11 +492,13 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                                  kb + ((k >> 2) * kHalf + (k & 3) * 2), idesc, k > 0, leads);
                     umma_commit_if(&s_full[i], leads);
                 }
-                if (ok) umma_commit_if(&kv_empty[g % kGroups], leads);
+                if (!ok) break;
+                umma_commit_if(&kv_empty[g % kGroups], leads);
+                if (j == q.first_tile) umma_commit_if(&kv_empty[g % kGroups], leads);
             }
             if (!ok) break;
             umma_commit_if(q_empty, leads);
-            umma_commit_if(&kv_empty[g++ % kGroups], leads);  // the part's last group has values alone
+            ++g;  // the part's last group has values alone
         }
         // All MMAs issued by this warp complete before TMEM is freed.
         umma_commit_if(mma_done, leads);
@@ -510,7 +514,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
         Part q;
         while (ok && part_at(part++, q) && !(q.flags & kEnd)) {
             const int tiles = q_tiles(q);
-            umma_commit_if(&kv_empty[g++ % kGroups], leads);  // the part's first group has keys alone
+            ++g;  // the part's first group has keys alone
             for (int j = q.first_tile; j < q.end_tile && ok; ++j, ++g) {
                 ok = wait_bounded(&kv_full[g % kGroups], phase_of(g), err, kDevErrTimeoutMma);
                 const uint64_t vb = v_desc + (uint32_t)(g % kGroups * S::kGroupBytes >> 4);
@@ -526,7 +530,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                     umma_commit_if(&o_done[i], leads);
                 }
-                if (ok) umma_commit_if(&kv_empty[g % kGroups], leads);
+                if (!ok) break;
+                umma_commit_if(&kv_empty[g % kGroups], leads);
+                if (j == q.end_tile - 1) umma_commit_if(&kv_empty[g % kGroups], leads);
             }
         }
         umma_commit_if(mma_done, leads);
