@@ -425,8 +425,9 @@ zq_status zq_ipc_close(void* dev_ptr);
  *       ZQ_DECODE_TENSOR_CORE: the tcgen05 decode kernel for m <= 16 (weights
  *         streamed by TMA, work split evenly over the SMs);
  *       ZQ_DECODE_CUDA_CORE: the dp4a warp-per-column GEMV for m <= 8;
- *       ZQ_DECODE_AUTO (default): the GEMV for m <= 4, the tcgen05 kernel for
- *         5 <= m <= 16.
+ *       ZQ_DECODE_AUTO (default): the GEMV for m <= 4; for 5 <= m <= 16 a
+ *         kernel that feeds matrix instructions from registers, or the tcgen05
+ *         kernel where SMs are reserved.
  *     Larger m always runs the tcgen05 GEMM.
  *   ZQ_OPT_RESERVED_SMS: streaming multiprocessors kept out of the matmul
  *     kernels' grids (default 0), so work running concurrently on other

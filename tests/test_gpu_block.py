@@ -124,6 +124,34 @@ def test_epilogue_decode_kernels(zb, torch, m, decode):
     within(torch, zb.matmul(x, w, activation="gelu", residual=r), want, tol, f"decode {decode}")
 
 
+@pytest.mark.parametrize("qtype", ["Int8", "Int4"])
+@pytest.mark.parametrize("m,k,n", [(5, 1000, 9), (7, 129, 1003), (8, 4100, 48), (9, 640, 9477), (12, 2048, 9472), (16, 5000, 8)])
+def test_five_to_sixteen_rows(zb, torch, m, k, n, qtype):
+    """Every decode kernel's integers are exact: the same bits, and the formula's."""
+    w = zb.quantize((randn(torch, 1, k, n) * 0.04).cuda(), getattr(zb.Type, qtype))
+    x, r = randn(torch, 2, m, k).cuda(), randn(torch, 3, m, n).bfloat16().cuda()
+    want, tol = epilogue_want(torch, zb, x, w, None, "silu", r, torch.bfloat16)
+    got, plain = zb.matmul(x, w, activation="silu", residual=r), zb.matmul(x, w)
+    within(torch, got, want, tol, "rows")
+    codes, scale = zb.quantize_rows(x)
+    assert torch.equal(zb.matmul_codes(codes, scale, w, activation="silu", residual=r), got)
+    w.set_decode_kernel(1)
+    assert torch.equal(zb.matmul(x, w), plain) and torch.equal(zb.matmul(x, w, activation="silu", residual=r), got)
+    w.set_decode_kernel(0)
+    w.set_option(2, 8)  # SMs left out
+    assert torch.equal(zb.matmul(x, w), plain)
+
+
+def test_nine_rows_of_a_long_int4_dot(zb, torch):
+    """K past 2^17, where sixteen times the dot would pass 32 bits, at extreme codes."""
+    k = (1 << 17) + 300
+    w = zb.quantize((torch.ones(k, 3) * torch.tensor([1.0, -1.0, 1.0])).cuda(), zb.Type.Int4)
+    x = torch.ones(9, k)
+    x[4] = -1.0
+    want, tol = epilogue_want(torch, zb, x.cuda(), w, None, None, None, torch.float32)
+    within(torch, zb.matmul(x.cuda(), w), want, tol, "long dots")
+
+
 def test_epilogue_plain_is_matmul(zb, torch):
     """float32 without anything else is the plain matmul, bit for bit, at every kernel's size."""
     for m, k, n in EPILOGUE_SIZES:

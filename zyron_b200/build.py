@@ -22,7 +22,7 @@ LIB = os.path.join(HERE, "libzyron_b200.so")
 QLIB = os.path.join(HERE, "libzyron_quant.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 
-CU_SOURCES = ["zq_api.cu", "zq_quant.cu", "zq_gemv.cu", "zq_gemm_sm100.cu", "zq_skinny_sm100.cu", "zq_noalloc.cu",
+CU_SOURCES = ["zq_api.cu", "zq_quant.cu", "zq_gemv.cu", "zq_gemm_sm100.cu", "zq_skinny_sm100.cu", "zq_rows.cu", "zq_noalloc.cu",
               "zq_lm.cu", "zq_sharded.cu", "zq_norm.cu", "zq_lowrank.cu", "zq_logprobs.cu", "zq_append.cu",
               "zq_attention.cu", "zq_attention_sm100.cu", "zq_ops.cu"]
 CU_HEADERS = ["zq_common.cuh", "zq_dot.cuh", "zq_elem.cuh", "zq_epilogue.cuh", "zq_paged.cuh", "zq_attention.cuh",

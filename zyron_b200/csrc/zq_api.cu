@@ -552,8 +552,9 @@ zq::OutDesc single_output(float* y, size_t N) {
 // Whether a plain-output matmul with M rows runs the dp4a GEMV (the weight's
 // ZQ_OPT_DECODE_KERNEL option).  Default: the GEMV for 1-4 rows, where the
 // weight stream alone sets the time and it has the least fixed cost per
-// launch; the tensor cores above that, where dp4a and shared-memory reads of
-// the activation rows limit the GEMV.
+// launch; matrix instructions above that (launch_rows; its grid is not
+// persistent, so the tcgen05 kernel where SMs are reserved), where dp4a and
+// shared-memory reads of the activation rows limit the GEMV.
 bool use_gemv(const zq_weight* w, int M) {
     const int decode = w->opt_decode.load(std::memory_order_relaxed);
     const bool fits = M <= zq::kGemvMaxRows && zq::gemv_smem_bytes(M, w->Kp) <= 200 * 1024;
@@ -590,6 +591,13 @@ zq_status run_codes_out(const zq_weight* w, const int8_t* codes, const float* rs
         a.reserved_sms = reserved;
         a.epi = out.epi;
         ZQ_CUDA(zq::launch_gemv(a, st, pdl));
+        return ZQ_OK;
+    }
+    if (plain && !test && M <= zq::kSkinnyMaxRows && reserved == 0 &&
+        w->opt_decode.load(std::memory_order_relaxed) == ZQ_DECODE_AUTO) {
+        zq::GemvArgs a{w->type, w->panel, N, Kp, w->scales, codes, rs, bias, y, M};
+        a.epi = out.epi;
+        ZQ_CUDA(zq::launch_rows(a, st));
         return ZQ_OK;
     }
     if (plain && M <= zq::kSkinnyMaxRows) {
