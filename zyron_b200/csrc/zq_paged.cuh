@@ -35,10 +35,9 @@ __device__ __forceinline__ Request load_request(const PagedBatch& p, int b) {
     return r;
 }
 
-// The request that owns row t, or -1: a search over starts[0 .. requests] by a
+// The last index of starts[0 .. requests] that is at most t, or -1: a search by a
 // whole warp, 32 places a round (one round up to 32 requests, two up to 1024).
-__device__ __forceinline__ int request_of_row(const PagedBatch& p, int t) {
-    if (!p.starts) return t < p.requests ? t : -1;
+__device__ __forceinline__ int last_start(const PagedBatch& p, int t) {
     const int lane = threadIdx.x & 31;
     // invariant: the last index with starts[i] <= t is in [lo, lo + n), or there is none
     int lo = 0, n = p.requests + 1;
@@ -52,8 +51,30 @@ __device__ __forceinline__ int request_of_row(const PagedBatch& p, int t) {
         n = min(step, n - last * step);
         lo += last * step;
     }
-    if (lo >= p.requests) return -1;
-    return load_l2(p.starts + lo) <= t && t < load_l2(p.starts + lo + 1) ? lo : -1;
+    return lo;
+}
+__device__ __forceinline__ int owner(const PagedBatch& p, int b, int t) {
+    if (b < 0 || b >= p.requests) return -1;
+    return load_l2(p.starts + b) <= t && t < load_l2(p.starts + b + 1) ? b : -1;
+}
+// The request that owns row t, or -1, found by a whole warp.
+__device__ __forceinline__ int request_of_row(const PagedBatch& p, int t) {
+    if (!p.starts) return t < p.requests ? t : -1;
+    return owner(p, last_start(p, t), t);
+}
+// The same of a row a lane, all in [first, last]: the whole warp finds the requests of
+// the two, a lane its own between them.
+__device__ __forceinline__ int request_of_lane(const PagedBatch& p, int first, int last, int t) {
+    if (!p.starts) return t < p.requests ? t : -1;
+    int lo = max(last_start(p, first), 0), hi = max(last_start(p, last), lo);
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (load_l2(p.starts + mid) <= t)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    return owner(p, lo, t);
 }
 
 // The cache page that holds a request's own token `at`, or -1.

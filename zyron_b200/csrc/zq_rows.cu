@@ -138,13 +138,14 @@ cudaError_t launch_t(const GemvArgs& a, cudaStream_t stream) {
                              a.col_scale, a.q, a.row_scale, a.bias, a.y, a.M, a.epi);
 }
 
-// Blocks of 16 columns and 16 warps while 32 columns would leave SMs with fewer than
-// two blocks; of 32 columns and 8 warps above, which read the activations half as
-// often (16 rows, INT4, K = 4096: N = 4096 5.2 us against 6.9, N = 11008 12.0
-// against 11.0; K = 8192, N = 28672 42.6 against 31.8).
+// Blocks of 16 columns and 16 warps while blocks of 32 would leave SMs without one;
+// of 32 columns and 8 warps above, which read the activations half as often (16 rows,
+// INT4, K = 4096: N = 4096 5.2 us against 6.9, N = 5120 7.2 against 7.1, N = 8192 8.9
+// against 7.8, N = 11008 12.0 against 11.0; K = 8192, N = 28672 42.6 against 31.8;
+// INT8 N = 6144 9.4 against 9.5, N = 8192 10.7 against 10.3).
 template <int kType, bool kX16>
 cudaError_t launch_columns(const GemvArgs& a, cudaStream_t stream) {
-    return a.N < 2 * 32 * sm_count() ? launch_t<kType, 16, 2, 2, 2, kX16>(a, stream)
+    return a.N < 32 * sm_count() ? launch_t<kType, 16, 2, 2, 2, kX16>(a, stream)
                                      : launch_t<kType, 8, 4, 1, 4, kX16>(a, stream);
 }
 
