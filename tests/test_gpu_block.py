@@ -718,3 +718,24 @@ def test_attention_of_many_prompts_gives_the_same_each_time(zb, torch, heads, kv
         within(torch, first, want, tol, f"prompts {new} in {lengths}")
         for _ in range(20):
             assert torch.equal(batch.attention(zb, q.cuda()), first)
+
+
+@pytest.mark.parametrize("dim,kv_heads,heads", [(64, 1, 4), (128, 1, 3), (80, 2, 10)])
+def test_attention_split_over_every_block(zb, torch, dim, kv_heads, heads):
+    """One item over all workers: a long cache for one token, for a draft, for a prompt, for a prefix."""
+    batch = Batch(torch, 50, [1], [5000], 16, kv_heads, dim, torch.float16)
+    attention_case(zb, torch, batch, heads)
+    batch = Batch(torch, 51, [5, 1], [3000, 40], 16, kv_heads, dim, torch.bfloat16)
+    attention_case(zb, torch, batch, heads)
+    batch = Batch(torch, 52, [40], [9000], 32, kv_heads, dim, torch.bfloat16)
+    attention_case(zb, torch, batch, heads)
+    batch = Batch(torch, 53, [1, 0, 3], [10, 0, 30], 16, kv_heads, dim, torch.float16, prefix=7001)
+    attention_case(zb, torch, batch, heads)
+
+
+@pytest.mark.parametrize("heads,kv,dim,new,cached", [(8, 1, 24, [70, 0, 2000, 1, 17, 0, 0, 13000, 3, 5000], 40),
+                                                     (3, 1, 128, [5, 0, 0, 700, 31, 1, 2500], 900)])
+def test_append_many_rows(zb, torch, heads, kv, dim, new, cached):
+    """Several rows a block, requests that begin and end inside a block's run, some empty."""
+    batch = Batch(torch, 60, new, [n + cached * (i % 3) for i, n in enumerate(new)], 64, kv, dim, torch.bfloat16)
+    append_case(zb, torch, batch, heads, "bfloat16", 16, False, 3, "bfloat16")

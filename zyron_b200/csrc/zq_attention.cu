@@ -42,6 +42,7 @@ constexpr int kLeast = 4;  // units of a worker, at least: all warps of a block 
 static_assert(kLeast > FewPlan::kItem, "");
 constexpr int kBlocksPerSm = 2;
 constexpr int kJoinThreads = 256;
+constexpr int kMaxManyBlocks = 256;
 
 template <int kD>
 constexpr int kStageBytes = kSlice * kD * 2 * 2;  // keys, then values
@@ -425,45 +426,77 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
     }
 }
 
-// Joins the items that borders of the kernel of few rows cut: a warp a border, those
-// of many parts or rows by the whole block.
+// Joins the items that borders of the kernel of few rows cut: a warp two rows of a
+// border, eight parts at a time, the rows behind them further along the grid's y
+// (17 drafts of up to 6 tokens 9 us; whole blocks after one another 16; four rows a
+// warp: 64 requests' join 16 us against 7).
+constexpr int kJoinRows = 2;
 template <class T, int kD, int kMT>
 __global__ void __launch_bounds__(kJoinThreads) join_few_kernel(const AttentionArgs a, const Workspace ws, int workers) {
-    constexpr int kJoinWarps = kJoinThreads / 32;
+    constexpr int kLanes = kD / 4, kTogether = 32 / kLanes;  // lanes of a row, rows at a time
     pdl_launch_dependents();
     pdl_wait_primary();  // before any return: who waits for this kernel counts on the ones before it too
-    const int first = blockIdx.x * kJoinWarps, g = first + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    bool left = false;
-    if (g > 0 && g < workers) {
-        const Cut c = load_cut(ws, 0, g);
-        if (c.rows > 0) {
-            const long long reach = (c.end - 1) / c.share - (g - 1);
-            const unsigned members = __ballot_sync(0xffffffffu, lane <= reach && FewPlan::holds(c, g - 1 + lane));
-            left = reach >= 32 || __popc(members) > kWarpParts || c.rows > kWarpRows<kD>;
-            // an item that one worker holds alone is finished
-            if (!left && __popc(members) > 1) join_few<T, 16 * kMT, kD>(a, ws, c, g, members);
-        }
-    }
-    __shared__ bool whole_block[kJoinWarps];
-    if (lane == 0) whole_block[threadIdx.x >> 5] = left;
-    __syncthreads();
-#pragma unroll 1
-    for (int w = 0; w < kJoinWarps; ++w) {
-        if (!whole_block[w]) continue;
-        join_item<T, FewPlan, 16 * kMT, kD, false, kJoinThreads>(a, ws, load_cut(ws, 0, first + w), 0, first + w, 0);
-        __syncthreads();
-    }
+    const int g = blockIdx.x * (kJoinThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (g == 0 || g >= workers) return;
+    const Cut c = load_cut(ws, 0, g);
+    for (int row0 = blockIdx.y * kJoinRows; row0 < c.rows; row0 += gridDim.y * kJoinRows)
+        join_rows<T, FewPlan, kJoinRows / kTogether, kTogether, 8>(
+            a, ws, c, 0, g, row0 + lane / kLanes, lane % kLanes * 4,
+            [&](long long slot, int row, long long& stats, long long& sums) {
+                stats = slot * (16 * kMT) + row;
+                sums = stats * kLanes + lane % kLanes;
+            });
 }
 
-// The same of the kernel of many rows: eight blocks a border, 32 rows each.
+// The same of the kernel of many rows, whose parts lie row beside row.  Few borders
+// may cut an item of many parts, or all of them one of two: every block lists the
+// split items and takes its turn at their pieces, 8 rows and 8 parts at a time of few
+// items, 16 and 2 of many (a 16000 key prefix of 96 rows, 16 items of 10 parts, 20 MB:
+// 10 us, by blocks a border 19; prompts, 140 items of 2 parts, 36 MB: 18, was 19).
+template <int kD>
+constexpr int kJoinBlocks = 4 * 128 / kD;  // an SM
 template <class T, int kD>
-__global__ void __launch_bounds__(kJoinThreads, 4) join_many_kernel(const AttentionArgs a, const Workspace ws) {
-    constexpr int kSlices = kManyRows / kSliceRows;
+__global__ void __launch_bounds__(2 * kD, kJoinBlocks<kD>) join_many_kernel(const AttentionArgs a, const Workspace ws, int workers) {
+    constexpr int kThreads = 2 * kD;  // a warp four chunks of four columns
+    __shared__ int split[kMaxManyBlocks], count;
     pdl_launch_dependents();
     pdl_wait_primary();
-    const int g = blockIdx.x / kSlices + 1, from = blockIdx.x % kSlices * kSliceRows;
-    const Cut c = load_cut(ws, 1, g);
-    if (from < c.rows) join_item<T, ManyPlan, kManyRows, kD, true, kJoinThreads>(a, ws, c, 1, g, from);
+    if (threadIdx.x == 0) count = 0;
+    __syncthreads();
+    for (int g0 = 1; g0 < workers; g0 += kThreads) {
+        const int g = g0 + threadIdx.x;
+        const bool is = g < workers && load_l2(&ws.cuts[1][g].rows) > 0;
+        // in order, the same in every block
+        __shared__ int before[kThreads / 32];
+        const unsigned m = __ballot_sync(0xffffffffu, is);
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        if (lane == 0) before[warp] = __popc(m);
+        __syncthreads();
+        int at = count;
+        for (int w = 0; w < warp; ++w) at += before[w];
+        if (is) split[at + __popc(m & ((1u << lane) - 1u))] = g;
+        __syncthreads();
+        if (threadIdx.x == kThreads - 1) count = at + __popc(m);
+        __syncthreads();
+    }
+    const int lane = threadIdx.x & 31, chunk = (threadIdx.x >> 5) * 4 + (lane >> 3);
+    const auto place = [&](long long slot, int row, long long& stats, long long& sums) {
+        stats = slot * kManyRows + row;
+        sums = (slot * (kD / 4) + chunk) * kManyRows + row;
+    };
+    const auto join = [&](auto steps, auto deep) {
+        constexpr int kSteps = decltype(steps)::value, kPieces = kManyRows / (8 * kSteps);
+        for (int i = blockIdx.x; i < count * kPieces; i += gridDim.x) {
+            const int g = split[i / kPieces], row = i % kPieces * 8 * kSteps;
+            const Cut c = load_cut(ws, 1, g);
+            if (row < c.rows)
+                join_rows<T, ManyPlan, kSteps, 8, decltype(deep)::value>(a, ws, c, 1, g, row + (lane & 7), chunk * 4, place);
+        }
+    };
+    if (count * (kManyRows / 8) <= (int)gridDim.x)
+        join(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+    else
+        join(std::integral_constant<int, 2>{}, std::integral_constant<int, 2>{});
 }
 
 // Joins the own and the prefix result of every row that a request owns.
@@ -492,6 +525,7 @@ __global__ void __launch_bounds__(256) join_prefix_kernel(const AttentionArgs a,
 struct Shape {
     int few_rows;     // 16 or 32: the rows of the kernel of few rows; 0: it has none
     int few_blocks;
+    int few_most;     // rows of its items at most
     int many_blocks;  // 0: no item can have more than few_rows
     int width;
 };
@@ -502,8 +536,9 @@ Shape shape_of(const AttentionArgs& a) {
     // the most rows of a kv head that an item may have
     const long long most = a.batch.starts || a.prefix_length > 0 ? all : group;
     if (group <= 32) s.few_rows = most <= 16 || (!a.batch.starts && group <= 16) ? 16 : 32;
+    s.few_most = (int)std::min<long long>(most, s.few_rows);
     s.few_blocks = s.few_rows ? kBlocksPerSm * sm_count() : 0;
-    s.many_blocks = most > s.few_rows ? sm_count() : 0;
+    s.many_blocks = most > s.few_rows ? std::min(sm_count(), kMaxManyBlocks) : 0;
     s.width = a.batch.dim <= 64 ? 64 : 128;
     return s;
 }
@@ -523,13 +558,12 @@ cudaError_t launch_t(const AttentionArgs& a, int dtype, const Shape& s, const Wo
     }
     if (s.few_blocks) {
         const int workers = s.few_blocks * kWarps, each = kJoinThreads / 32;
-        e = launch_pdl_kernel(join_few_kernel<T, kD, kMT>, dim3((workers + each - 1) / each), dim3(kJoinThreads), 0, stream,
-                              a, ws, workers);
+        e = launch_pdl_kernel(join_few_kernel<T, kD, kMT>, dim3((workers + each - 1) / each, std::min(8, (s.few_most + kJoinRows - 1) / kJoinRows)),
+                              dim3(kJoinThreads), 0, stream, a, ws, workers);
         if (e != cudaSuccess) return e;
     }
     if (s.many_blocks)
-        e = launch_pdl_kernel(join_many_kernel<T, kD>, dim3((s.many_blocks - 1) * (kManyRows / kSliceRows)),
-                              dim3(kJoinThreads), 0, stream, a, ws);
+        e = launch_pdl_kernel(join_many_kernel<T, kD>, dim3(kJoinBlocks<kD> * sm_count()), dim3(2 * kD), 0, stream, a, ws, s.many_blocks);
     if (e != cudaSuccess || a.prefix_length == 0) return e;
     return launch_pdl_kernel(join_prefix_kernel<T>, dim3(a.batch.rows), dim3(256), 0, stream, a, ws);
 }

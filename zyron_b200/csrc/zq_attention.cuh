@@ -88,7 +88,8 @@ struct Item {
 };
 
 // What the join needs to know of an item that the border in front of a worker's
-// first unit cuts; rows 0: none, or an earlier border cuts it too.
+// first unit cuts; rows 0: none, or an earlier border cuts it too, or one worker
+// holds all its key tiles and has finished it.
 struct alignas(16) Cut {
     long long start, end, share;
     int rows;       // of the item
@@ -213,7 +214,9 @@ struct ManyPlan {
         return true;
     }
     __device__ static __forceinline__ int cut(long long start, long long end, int key_tiles, long long unit) {
-        return (int)((min(max(unit, start), end) - start) * key_tiles / (end - start));
+        const long long n = (min(max(unit, start), end) - start) * key_tiles;
+        if ((n | (end - start)) >> 32 == 0) return (int)((uint32_t)n / (uint32_t)(end - start));  // a fifth of the time
+        return (int)(n / (end - start));
     }
     __device__ static __forceinline__ bool holds(const Cut& c, int h) {
         return cut(c.start, c.end, c.key_tiles, h * c.share) < cut(c.start, c.end, c.key_tiles, (h + 1) * c.share);
@@ -327,7 +330,9 @@ struct Cursor {
         Cut c{};
         if (unit < last && it.start < unit && it.start >= (g - 1) * share) {
             c = Cut{it.start, it.end, share, 0, it.r.first, it.tile * tile_rows, it.head, it.key_tiles, it.b < 0};
-            c.rows = (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - c.row0);
+            int holders = 0;
+            for (long long h = g - 1; holders < 2 && h * share < it.end; ++h) holders += Plan::holds(c, (int)h);
+            if (holders == 2) c.rows = (int)min((long long)tile_rows, (long long)it.r.rows * plan.group - c.row0);
         }
         return c;
     }
@@ -380,11 +385,6 @@ struct Joined {
     }
 };
 
-// Joins the parts of the item that border g (in front of worker g's first unit)
-// cuts: rows [from, from + kSliceRows) of it.  kRows, kWidth: a part's; kByRow: its
-// rows lie side by side (the kernel of many rows).  Parts are taken 64 workers at a
-// time: their weights first, eight threads a row, then their sums with every load
-// under way at once.
 __device__ __forceinline__ Cut load_cut(const Workspace& ws, int kind, int g) {
     Cut c;
 #pragma unroll
@@ -394,181 +394,62 @@ __device__ __forceinline__ Cut load_cut(const Workspace& ws, int kind, int g) {
     }
     return c;
 }
-constexpr int kSliceRows = 32;
-template <class T, class Plan, int kRows, int kWidth, bool kByRow, int kThreads>
-__device__ void join_item(const AttentionArgs& a, const Workspace& ws, const Cut& c, int kind, int g, int from) {
-    constexpr int kSlice = kRows < kSliceRows ? kRows : kSliceRows, kBatch = 64;
-    static_assert(kThreads == 8 * kSliceRows, "eight threads a row");
-    const PagedBatch& p = a.batch;
-    const int group = a.heads / p.kv_heads;
-    __shared__ int parts[kBatch], count;
-    __shared__ float weights[kBatch][kSlice], totals[kBatch][kSlice];  // maxima, then weights; sums
-    __shared__ float row_most[kSlice], row_total[kSlice], row_keep[kSlice];
-    const int lane = threadIdx.x & 31, h1 = (int)((c.end - 1) / c.share), rows = min(c.rows - from, kSlice);
-    // Workers g - 1 .. h1 may hold parts of it.
-    const auto holds = [&](int h) { return h <= h1 && Plan::holds(c, h); };
-    if (threadIdx.x < 32) {
-        int n = 0;
-        for (int h = g - 1; h <= h1 && n < 2; h += 32) n += __popc(__ballot_sync(0xffffffffu, holds(h + lane)));
-        if (lane == 0) count = n;
-    }
-    if (threadIdx.x < kSlice) {
-        row_most[threadIdx.x] = -INFINITY;
-        row_total[threadIdx.x] = 0.0f;
-    }
-    __syncthreads();
-    if (count < 2) return;  // a worker that holds the item alone has finished it
-    constexpr int kElems = kSlice * (kWidth / 4), kEach = (kElems + kThreads - 1) / kThreads;
-    constexpr int kDeep = kEach < 4 ? 16 / kEach : 2;  // parts whose loads are under way at once
-    const auto place = [&](int e, int& in, int& d) {
-        const int i = e * kThreads + threadIdx.x;
-        in = kByRow ? i % kSlice : i / (kWidth / 4);
-        d = (kByRow ? i / kSlice : i % (kWidth / 4)) * 4;
-        return i < kElems && d < p.dim && in < rows;
-    };
-    float v[kEach][4];
+
+// The parts of the item that border g (in front of worker g's first unit) cuts,
+// kDeep slots a call (-1: none), by the whole warp.
+template <class Plan, int kDeep, class F>
+__device__ __forceinline__ void each_parts(const Cut& c, int g, F f) {
+    const int lane = threadIdx.x & 31, last = (int)((c.end - 1) / c.share);
+    const bool second = (g - 1) * c.share < c.start;  // the first worker's part lies in its second slot
+    for (int h0 = g - 1; h0 <= last; h0 += 32) {
+        unsigned m = __ballot_sync(0xffffffffu, h0 + lane <= last && Plan::holds(c, h0 + lane));
+        while (m) {
+            long long slots[kDeep];
 #pragma unroll
-    for (int e = 0; e < kEach; ++e) v[e][0] = v[e][1] = v[e][2] = v[e][3] = 0.0f;
-    for (int h0 = g - 1; h0 <= h1; h0 += kBatch) {
-        if (threadIdx.x < 32) {
-            int n = 0;
-#pragma unroll
-            for (int b = 0; b < kBatch; b += 32) {
-                const int h = h0 + b + lane;
-                const bool has = holds(h);
-                const unsigned m = __ballot_sync(0xffffffffu, has);
-                // the first worker's part may lie in its second slot
-                if (has) parts[n + __popc(m & ((1u << lane) - 1u))] = 2 * h + (h == g - 1 && h * c.share < c.start ? 1 : 0);
-                n += __popc(m);
+            for (int k = 0; k < kDeep; ++k) {
+                const int h = h0 + __ffs(m) - 1;
+                slots[k] = m ? 2LL * h + (h == g - 1 && second ? 1 : 0) : -1;
+                m &= m - 1;
             }
-            if (lane == 0) count = n;
+            f(slots);
         }
-        __syncthreads();
-        const int n = count;
-        for (int i = threadIdx.x; i < n * kSlice; i += kThreads) {
-            const int k = i / kSlice, in = i % kSlice;
-            float2 s = make_float2(-INFINITY, 0.0f);
-            if (in < rows)
-                s = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + (long long)parts[k] * kRows + from + in);
-            weights[k][in] = s.x;
-            totals[k][in] = s.y;
-        }
-        __syncthreads();
-        const int in_row = threadIdx.x / 8, sub = threadIdx.x % 8;
-        const bool mine = in_row < kSlice;
-        float most = -INFINITY, total = 0.0f;
-        for (int k = sub; k < n && mine; k += 8) most = fmaxf(most, weights[k][in_row]);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        const float before = mine ? row_most[in_row] : 0.0f;
-        most = fmaxf(most, before);
-        const float ref = most == -INFINITY ? 0.0f : most;
-        for (int k = sub; k < n && mine; k += 8) {
-            const float w = exp2_approx(weights[k][in_row] - ref);
-            weights[k][in_row] = w;
-            total += totals[k][in_row] * w;
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-        if (mine && sub == 0) {
-            const float keep = exp2_approx(before - ref);
-            row_keep[in_row] = keep;
-            row_most[in_row] = most;
-            row_total[in_row] = row_total[in_row] * keep + total;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) {
-            int in, d;
-            if (place(e, in, d) && h0 > g - 1) {
-                const float keep = row_keep[in];
-#pragma unroll
-                for (int x = 0; x < 4; ++x) v[e][x] *= keep;
-            }
-        }
-        for (int k0 = 0; k0 < n; k0 += kDeep) {
-            float4 x[kDeep][kEach];
-#pragma unroll
-            for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    int in, d;
-                    x[k][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    if (place(e, in, d) && k0 + k < n) {
-                        const long long part = parts[k0 + k];
-                        const long long at = kByRow ? (part * (kWidth / 4) + d / 4) * kRows + from + in
-                                                    : (part * kRows + from + in) * (kWidth / 4) + d / 4;
-                        x[k][e] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind]) + at);
-                    }
-                }
-#pragma unroll
-            for (int k = 0; k < kDeep; ++k)
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) {
-                    int in, d;
-                    if (place(e, in, d) && k0 + k < n) {
-                        const float w = weights[k0 + k][in];
-                        v[e][0] = fmaf(x[k][e].x, w, v[e][0]);
-                        v[e][1] = fmaf(x[k][e].y, w, v[e][1]);
-                        v[e][2] = fmaf(x[k][e].z, w, v[e][2]);
-                        v[e][3] = fmaf(x[k][e].w, w, v[e][3]);
-                    }
-                }
-        }
-        __syncthreads();  // the batch's weights have been used
-    }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-        int in, d;
-        if (!place(e, in, d)) continue;
-        const int row = c.row0 + from + in;
-        put_row<T>(a, ws, c.prefix, c.first_row + row / group, c.head * group + row % group, d, v[e], row_most[in],
-                   row_total[in]);
     }
 }
 
-// The same of an item of a row or some in at most kWarpParts parts, `members` of the
-// workers g - 1 ..., by one warp: a lane four elements of a row, all its parts' loads
-// under way at once.
-constexpr int kWarpParts = 8;
-template <int kWidth>
-constexpr int kWarpRows = 4 * 128 / kWidth;
-template <class T, int kRows, int kWidth>
-__device__ void join_few(const AttentionArgs& a, const Workspace& ws, const Cut& c, int g, unsigned members) {
-    constexpr int kLanes = kWidth / 4, kTogether = 32 / kLanes, kSteps = 2;  // lanes of a row, rows at a time
-    const PagedBatch& p = a.batch;
-    const int group = a.heads / p.kv_heads, lane = threadIdx.x & 31;
-    const bool second = (g - 1) * c.share < c.start;  // the first worker's part lies in its second slot
-    for (int row0 = 0; row0 < c.rows; row0 += kSteps * kTogether) {
-        const int d = lane % kLanes * 4;
-        float2 stats[kSteps][kWarpParts];
-        float4 x[kSteps][kWarpParts];
+// Joins kSteps rows, kBetween apart, of a split item: a lane four elements of each,
+// the loads of kDeep parts under way at once.  place(slot, row) is where a row of a
+// part lies: its index in the statistics and in the sums.
+template <class T, class Plan, int kSteps, int kBetween, int kDeep, class F>
+__device__ __forceinline__ void join_rows(const AttentionArgs& a, const Workspace& ws, const Cut& c, int kind, int g,
+                                          int row, int d, F place) {
+    const int group = a.heads / a.batch.kv_heads;
+    Joined j[kSteps];
+    each_parts<Plan, kDeep>(c, g, [&](const long long (&slots)[kDeep]) {
+        float2 stats[kDeep][kSteps];
+        float4 x[kDeep][kSteps];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int in = row0 + s * kTogether + lane / kLanes;
-            unsigned m = members;
+        for (int k = 0; k < kDeep; ++k)
 #pragma unroll
-            for (int k = 0; k < kWarpParts; ++k) {
-                stats[s][k] = make_float2(-INFINITY, 0.0f);
-                x[s][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (m && in < c.rows && d < p.dim) {
-                    const int h = __ffs(m) - 1;
-                    const long long at = (long long)(2 * (g - 1 + h) + (h == 0 && second ? 1 : 0)) * kRows + in;
-                    stats[s][k] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[0]) + at);
-                    x[s][k] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[0] + at * kWidth + d));
-                }
-                m &= m - 1;
+            for (int s = 0; s < kSteps; ++s) {
+                stats[k][s] = make_float2(-INFINITY, 0.0f);
+                x[k][s] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (slots[k] < 0 || row + s * kBetween >= c.rows || d >= a.batch.dim) continue;
+                long long stats_at, sums_at;
+                place(slots[k], row + s * kBetween, stats_at, sums_at);
+                stats[k][s] = load_l2(reinterpret_cast<const float2*>(ws.part_stats[kind]) + stats_at);
+                x[k][s] = load_l2(reinterpret_cast<const float4*>(ws.part_sums[kind]) + sums_at);
             }
-        }
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-            const int in = row0 + s * kTogether + lane / kLanes;
-            if (in >= c.rows || d >= p.dim) continue;
-            Joined j;
+        for (int k = 0; k < kDeep; ++k)
 #pragma unroll
-            for (int k = 0; k < kWarpParts; ++k) j.add(stats[s][k], x[s][k]);
-            put_row<T>(a, ws, c.prefix, c.first_row + in / group, c.head * group + in % group, d, j.v, j.most, j.total);
-        }
+            for (int s = 0; s < kSteps; ++s) j[s].add(stats[k][s], x[k][s]);
+    });
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+        const int in = row + s * kBetween;
+        if (in < c.rows && d < a.batch.dim)
+            put_row<T>(a, ws, c.prefix, c.first_row + (c.row0 + in) / group, c.head * group + (c.row0 + in) % group, d,
+                       j[s].v, j[s].most, j[s].total);
     }
 }
 
