@@ -303,8 +303,8 @@ zq_status zq_token_logprobs(const void* logits, int dtype, size_t m, size_t voca
  * starts, lengths and pages are read on the device when the call runs, so a
  * captured call follows what they hold at its replay.  Values that the call's
  * sizes do not allow are clamped or left out, never followed: starts and
- * lengths to [0, rows] and [0, max_pages * page]; a token on a page outside
- * [0, cache_pages) is not stored, and not seen. */
+ * lengths to [0, rows] and [0, max_pages * page] (below 2^31 - 4096); a token
+ * on a page outside [0, cache_pages) is not stored, and not seen. */
 typedef struct zq_paged_batch {
     const int32_t* starts;
     const int32_t* lengths;

@@ -587,6 +587,7 @@ def test_attention_refusals_on_device(zb, torch):
                          ({"prefix_length": 17, "prefix_pages": batch.dev_pages[0, :1].contiguous()}, "hold prefix_length"),
                          ({"prefix_length": -1}, "prefix_length must be"), ({"scale": math.inf}, "scale must be finite"),
                          ({"out": q}, "out overlaps q"), ({"out": q.half()}, "out must have"),
+                         ({"out": batch.k_cache[:1].view(2, 16, 64)[:, :4]}, "out overlaps the caches"),
                          ({"p": batch.dev_pages.cpu()}, "pages is on cpu")):
         with pytest.raises(ValueError, match=message):
             call(**bad)
@@ -596,9 +597,43 @@ def test_attention_refusals_on_device(zb, torch):
     for bad, message in (({"q": q}, "q must be torch.float32"), ({"k": k.double()}, "k must be float32"), ({"v": k.half()}, "of one shape and type"),
                          ({"inv_freq": f}, "rotated must be even and at most dim"), ({"inv_freq": f.float()}, "inv_freq must be"),
                          ({"offset": -1}, "offset must be"), ({"k": k[:, :1], "v": k[:, :1]}, "caches' kv_heads"),
-                         ({"q": k[:, :1]}, "multiple of kv_heads")):
+                         ({"q": k[:, :1]}, "multiple of kv_heads"), ({"offset": 1 << 64}, "offset must be"),
+                         ({"k": batch.v_cache[0, :, :2].transpose(0, 1), "v": k.bfloat16()}, "k overlaps the caches"),
+                         ({"q": batch.k_cache[0, :, :2].transpose(0, 1), "k": k.bfloat16(), "v": k.bfloat16()}, "q overlaps the caches")):
         with pytest.raises(ValueError, match=message):
             app(**bad)
+
+
+def test_caches_without_pages(zb, torch):
+    """Nothing is stored, nothing seen; queries are rotated all the same."""
+    cache = torch.empty(0, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    pages = torch.zeros(3, 4, dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([40, 1, 64], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 40, 41, 45], dtype=torch.int32, device="cuda")
+    q, k = randn(torch, 1, 45, 4, 64).bfloat16().cuda(), randn(torch, 2, 45, 2, 64).bfloat16().cuda()
+    assert torch.equal(zb.append_kv(q, k, k, cache, cache.clone(), pages, lengths, starts), q)
+    out = torch.full_like(q, 7)
+    zb.paged_attention(q, cache, cache.clone(), pages, lengths, starts, prefix_pages=pages[0], prefix_length=60, out=out)
+    assert not out.any()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_lengths_at_the_end_of_32_bits(zb, torch, rows):
+    """2^31 - 1 cached tokens, as far as a table can say: those on a page count, none is read twice."""
+    page = 1024
+    pages = torch.full((1, 1 << 21), -1, dtype=torch.int32, device="cuda")
+    pages[0, 3] = 1
+    lengths = torch.tensor([2**31 - 1], dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, rows], dtype=torch.int32, device="cuda")
+    kc, vc = (randn(torch, 3 + i, 2, 1, page, 64).half().cuda() for i in range(2))
+    q = randn(torch, 1, rows, 4, 64).half().cuda()
+    got = zb.paged_attention(q, kc, vc, pages, lengths, starts)
+    short = zb.paged_attention(q, kc, vc, pages[:, 3:4].contiguous(), torch.full_like(lengths, page), starts, causal=False)
+    within(torch, got, short.double().cpu(), 2.0**-10 * vc[1].abs().max().double().cpu(), "far lengths")
+    k = randn(torch, 9, rows, 1, 64).half().cuda()
+    before = kc.clone()
+    zb.append_kv(None, k, k, kc, vc, pages, lengths, starts)
+    assert torch.equal(kc, before)  # its place is on no page
 
 
 # ---- streams and graphs ------------------------------------------------------------------

@@ -126,12 +126,13 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
         const bool prefix = way.it.b < 0;
         const int32_t* table = prefix ? a.prefix_pages : p.pages + (long long)way.it.b * p.ld_pages;
 
+        const T* q_src = static_cast<const T*>(a.q);  // where a copy of no bytes points: a cache may have no pages
         // q of the item: row i is token i / group, head i % group of the kv head's.
 #pragma unroll
         for (int j = 0; j < kRows * kChunks / 32; ++j) {
             const int i = j * 32 + lane, row = i / kChunks, c = i % kChunks;
             const bool live = row < item_rows && c * 8 < dim;
-            const T* src = static_cast<const T*>(a.q);
+            const T* src = q_src;
             if (live)
                 src += (long long)(r.first + row / group) * a.ldq + (long long)(head0 * group + row % group) * dim + c * 8;
             cp_async16(q_u + chunk_at<kD>(row, c), src, live);
@@ -190,8 +191,8 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
                         const int row = (j * 32 + lane) / kChunks, c = (j * 32 + lane) % kChunks;
                         const bool live = page >= 0 && row < keys && c * 8 < dim;
                         const uint32_t to = chunk_at<kD>(half * 8 + row, c);
-                        cp_async16(dst + to, live ? ks + row * dim + c * 8 : a.k_cache, live);
-                        cp_async16(dst + kSlice * kD * 2 + to, live ? vs + row * dim + c * 8 : a.v_cache, live);
+                        cp_async16(dst + to, live ? ks + row * dim + c * 8 : q_src, live);
+                        cp_async16(dst + kSlice * kD * 2 + to, live ? vs + row * dim + c * 8 : q_src, live);
                     }
                 }
             }

@@ -29,7 +29,8 @@ __device__ __forceinline__ Request load_request(const PagedBatch& p, int b) {
         r.first = b;
         r.rows = 1;
     }
-    const long long most = (long long)p.max_pages * p.page;
+    // a tile's end behind the last token stays an int
+    const long long most = min((long long)p.max_pages * p.page, 0x7FFFFFFFLL - 4096);
     const int n = load_l2(p.lengths + b);
     r.length = (int)(n < 0 ? 0 : n < most ? (long long)n : most);
     return r;

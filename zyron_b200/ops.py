@@ -417,6 +417,20 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=True, stream=None):
     return TokenLogprobs(lp, ent, top_lp, top_ids)
 
 
+def _beside(t, name, k_cache, v_cache):
+    """Refuses a tensor that begins before a cache's end and ends behind its start."""
+    if t is None or t.numel() == 0:
+        return
+    span = lambda x: (x.data_ptr(), x.data_ptr() +  # noqa: E731
+                      (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size())
+    at, end = span(t)
+    for cache in (k_cache, v_cache):
+        if cache.numel():
+            lo, hi = span(cache)
+            if at < hi and lo < end:
+                raise _bad(f"{name} overlaps the caches")
+
+
 def _heads(t, name, rows, dim, dtype=None):
     """A [rows, heads, dim] tensor with contiguous heads: (tensor, row pitch)."""
     if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim:
@@ -508,6 +522,10 @@ def append_kv(q, k, v, k_cache, v_cache, pages, lengths, starts=None, inv_freq=N
         if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
             raise _bad("inv_freq must be contiguous float64 [rotated / 2]")
         rotated = 2 * inv_freq.shape[0]
+    if not 0 <= offset <= 1 << 40:
+        raise _bad("offset must be in [0, 2^40]")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        _beside(t, name, k_cache, v_cache)
     context, ptr = _context(index, stream)
     with context:
         k, ldk = _heads(k, "k", rows, dim)
@@ -567,6 +585,7 @@ def paged_attention(q, k_cache, v_cache, pages, lengths, starts=None, prefix_pag
             if out.stride(2) != 1 or (heads > 1 and out.stride(1) != dim) or (rows > 1 and out.stride(0) < heads * dim):
                 raise _bad("out must have contiguous rows that do not overlap")
             ld_out = out.stride(0) if rows > 1 else heads * dim
+            _beside(out, "out", k_cache, v_cache)
             if rows:
                 _apart(out.flatten(1), ld_out, q.flatten(1), ldq, "q", "out", same=False)
         need = lib().zq_paged_attention_workspace_bytes(C.byref(batch), heads, prefix_length)
