@@ -417,71 +417,96 @@ def token_logprobs(logits, targets=None, top_k=0, entropy=True, stream=None):
     return TokenLogprobs(lp, ent, top_lp, top_ids)
 
 
-def _beside(t, name, k_cache, v_cache):
-    """Refuses a tensor that begins before a cache's end and ends behind its start."""
-    if t is None or t.numel() == 0:
-        return
-    span = lambda x: (x.data_ptr(), x.data_ptr() +  # noqa: E731
-                      (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size())
-    at, end = span(t)
-    for cache in (k_cache, v_cache):
-        if cache.numel():
-            lo, hi = span(cache)
-            if at < hi and lo < end:
-                raise _bad(f"{name} overlaps the caches")
-
-
-def _heads(t, name, rows, dim, dtype=None):
-    """A [rows, heads, dim] tensor with contiguous heads: (tensor, row pitch)."""
-    if t.dim() != 3 or t.shape[0] != rows or t.shape[2] != dim:
+def _heads(t, name, rows, dim, dtype, caches):
+    """A [rows, heads, dim] tensor with contiguous heads, beside the caches:
+    (tensor, its address, heads, row pitch)."""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != rows or shape[2] != dim:
         raise _bad(f"{name} must be [rows, heads, dim] with dim {dim}, and {rows} rows")
-    if dtype is not None and t.dtype != dtype:
+    if t.dtype != dtype:
         raise _bad(f"{name} must be {dtype}")
-    width = t.shape[1] * dim
-    if t.is_contiguous():
-        return t, width
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != dim) or (rows > 1 and t.stride(0) < width):
-        return t.contiguous(), width
-    return t, (t.stride(0) if rows > 1 else width)
+    heads = shape[1]
+    ld = width = heads * dim
+    if not t.is_contiguous():
+        by_row, by_head, by_element = t.stride()
+        if by_element != 1 or heads > 1 and by_head != dim or rows > 1 and by_row < width:
+            if rows:
+                _beside(t.data_ptr(), 1 + (rows - 1) * by_row + (heads - 1) * by_head + (dim - 1) * by_element, t, name, caches)
+            t = t.contiguous()
+        elif rows > 1:
+            ld = by_row
+    at = t.data_ptr()
+    _beside(at, (rows - 1) * ld + width if rows else 0, t, name, caches)
+    return t, at, heads, ld
+
+
+def _beside(at, elements, t, name, caches):
+    """Refuses `elements` of t at `at` that begin before a cache's end and end
+    behind its start."""
+    end = at + elements * t.element_size()
+    for lo, hi in caches:
+        if at < hi and lo < end and at < end:
+            raise _bad(f"{name} overlaps the caches")
 
 
 def _paged_batch(rows, k_cache, v_cache, pages, lengths, starts):
-    """The checked batch of a call over a paged cache."""
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or v_cache.dtype != k_cache.dtype:
+    """The checked batch of a call over a paged cache, (kv_heads, page, dim), and
+    where the caches begin and end."""
+    shape, kind = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape or v_cache.dtype != kind:
         raise _bad("k_cache and v_cache must be [pages, kv_heads, page, dim], of one shape and type")
-    cache_pages, kv_heads, page, dim = k_cache.shape
-    code = _DTYPES.get(k_cache.dtype)
+    cache_pages, kv_heads, page, dim = shape
+    code = _DTYPES.get(kind)
     if code is None or code == 1:
         raise _bad("the cache must be float16 or bfloat16")
     block = kv_heads * page * dim
-    pitch = []
-    for t in (k_cache, v_cache):
-        ok = t.is_contiguous() or (t.stride(3) == 1 and t.stride(2) == dim and
-                                   (kv_heads == 1 or t.stride(1) == page * dim) and
-                                   (cache_pages <= 1 or t.stride(0) >= block))
-        if not ok:
-            raise _bad("each page's [kv_heads, page, dim] must be contiguous in the caches")
-        pitch.append(t.stride(0) if cache_pages > 1 else block)
-    at = (v_cache.data_ptr() - k_cache.data_ptr()) // k_cache.element_size()
-    if cache_pages and -((cache_pages - 1) * pitch[1] + block) < at < (cache_pages - 1) * pitch[0] + block:
-        # interleaved page by page, or one inside the other
-        if pitch[0] != pitch[1] or not block <= at % pitch[0] <= pitch[0] - block:
-            raise _bad("k_cache and v_cache overlap")
-    if pages.dim() != 2 or pages.dtype != torch.int32 or lengths.dtype != torch.int32 or lengths.dim() != 1:
+    k_pitch = v_pitch = block
+    if not k_cache.is_contiguous():
+        k_pitch = _page_pitch(k_cache, block)
+    if not v_cache.is_contiguous():
+        v_pitch = _page_pitch(v_cache, block)
+    k_at, v_at = k_cache.data_ptr(), v_cache.data_ptr()
+    caches = ()
+    if cache_pages:
+        k_end, v_end = k_at + 2 * ((cache_pages - 1) * k_pitch + block), v_at + 2 * ((cache_pages - 1) * v_pitch + block)
+        caches = ((k_at, k_end), (v_at, v_end))
+        if k_at < v_end and v_at < k_end:
+            # interleaved page by page, or one inside the other
+            if k_pitch != v_pitch or not block <= (v_at - k_at) // 2 % k_pitch <= k_pitch - block:
+                raise _bad("k_cache and v_cache overlap")
+    of_pages, of_lengths = pages.shape, lengths.shape
+    if len(of_pages) != 2 or pages.dtype != torch.int32 or lengths.dtype != torch.int32 or len(of_lengths) != 1:
         raise _bad("pages must be int32 [requests, max_pages] and lengths int32 [requests]")
-    requests, max_pages = pages.shape
-    if lengths.shape[0] != requests or not lengths.is_contiguous():
+    requests, max_pages = of_pages
+    if of_lengths[0] != requests or not lengths.is_contiguous():
         raise _bad("lengths must be contiguous int32 [requests], as many as rows of pages")
-    if max_pages > 1 and pages.stride(1) != 1 or requests > 1 and pages.stride(0) < max_pages:
-        raise _bad("pages must have contiguous rows that do not overlap")
+    ld_pages = max_pages
+    if not pages.is_contiguous():
+        by_row, by_page = pages.stride()
+        if max_pages > 1 and by_page != 1 or requests > 1 and by_row < max_pages:
+            raise _bad("pages must have contiguous rows that do not overlap")
+        if requests > 1:
+            ld_pages = by_row
+    start = None
     if starts is None:
         if requests != rows:
             raise _bad(f"without starts every request has one row: {requests} requests, {rows} rows")
     elif starts.dtype != torch.int32 or starts.shape != (requests + 1,) or not starts.is_contiguous():
         raise _bad("starts must be contiguous int32 [requests + 1]")
-    return _lib.PagedBatchC(_ptr(starts), lengths.data_ptr(), pages.data_ptr(),
-                            pages.stride(0) if requests > 1 else max_pages, max_pages, requests, rows, page, cache_pages,
-                            kv_heads, dim, pitch[0], pitch[1], code)
+    else:
+        start = starts.data_ptr()
+    batch = _lib.PagedBatchC(start, lengths.data_ptr(), pages.data_ptr(), ld_pages, max_pages, requests, rows, page,
+                             cache_pages, kv_heads, dim, k_pitch, v_pitch, code)
+    return C.byref(batch), (kv_heads, page, dim), caches, k_at, v_at
+
+
+def _page_pitch(t, block):
+    """Elements from page to page of a cache that is not contiguous as a whole."""
+    pages, kv_heads, page, dim = t.shape
+    by_page, by_head, by_token, by_element = t.stride()
+    if by_element != 1 or by_token != dim or kv_heads > 1 and by_head != page * dim or pages > 1 and by_page < block:
+        raise _bad("each page's [kv_heads, page, dim] must be contiguous in the caches")
+    return by_page if pages > 1 else block
 
 
 def append_kv(q, k, v, k_cache, v_cache, pages, lengths, starts=None, inv_freq=None, interleaved=True, offset=0,
@@ -507,37 +532,37 @@ def append_kv(q, k, v, k_cache, v_cache, pages, lengths, starts=None, inv_freq=N
     stored nor written in the result."""
     if torch is None:
         _setup()
+    kind = k.dtype
     dtype = _dtype(k, "k")
     index = _device(k, "q v k_cache v_cache pages lengths starts inv_freq", q, v, k_cache, v_cache, pages, lengths, starts,
                     inv_freq)
-    if k.dim() != 3 or v.shape != k.shape or v.dtype != k.dtype:
+    shape = k.shape
+    if len(shape) != 3 or v.shape != shape or v.dtype != kind:
         raise _bad("k and v must be [rows, kv_heads, dim], of one shape and type")
-    rows = k.shape[0]
-    batch = _paged_batch(rows, k_cache, v_cache, pages, lengths, starts)
-    if k.shape[1] != k_cache.shape[1]:
+    rows = shape[0]
+    batch, (kv_heads, _, dim), caches, k_at, v_at = _paged_batch(rows, k_cache, v_cache, pages, lengths, starts)
+    if shape[1] != kv_heads:
         raise _bad("k and v must have the caches' kv_heads")
-    dim = k_cache.shape[3]
-    rotated = 0
+    rotated, freq = 0, None
     if inv_freq is not None:
         if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not inv_freq.is_contiguous():
             raise _bad("inv_freq must be contiguous float64 [rotated / 2]")
         rotated = 2 * inv_freq.shape[0]
+        if rotated:
+            freq = inv_freq.data_ptr()
     if not 0 <= offset <= 1 << 40:
         raise _bad("offset must be in [0, 2^40]")
-    for t, name in ((q, "q"), (k, "k"), (v, "v")):
-        _beside(t, name, k_cache, v_cache)
     context, ptr = _context(index, stream)
     with context:
-        k, ldk = _heads(k, "k", rows, dim)
-        v, ldv = _heads(v, "v", rows, dim)
-        out, heads, ldq = None, 0, 0
+        k, at_k, _, ldk = _heads(k, "k", rows, dim, kind, caches)
+        v, at_v, _, ldv = _heads(v, "v", rows, dim, kind, caches)
+        out, at_q, at_out, heads, ldq = None, None, None, 0, 0
         if q is not None:
-            q, ldq = _heads(q, "q", rows, dim, k.dtype)
-            heads = q.shape[1]
+            q, at_q, heads, ldq = _heads(q, "q", rows, dim, kind, caches)
             out = torch.empty_strided((rows, heads, dim), (heads * dim, dim, 1), dtype=k_cache.dtype, device=k.device)
-        check(lib().zq_append_kv(C.byref(batch), _ptr(q), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, dtype, heads,
-                                 k_cache.data_ptr(), v_cache.data_ptr(), _ptr(out), inv_freq.data_ptr() if rotated else None,
-                                 rotated, interleaved, offset, ptr))
+            at_out = out.data_ptr()
+        check(lib().zq_append_kv(batch, at_q, ldq, at_k, ldk, at_v, ldv, dtype, heads, k_at, v_at, at_out, freq, rotated,
+                                 interleaved, offset, ptr))
     return out
 
 
@@ -556,42 +581,50 @@ def paged_attention(q, k_cache, v_cache, pages, lengths, starts=None, prefix_pag
         _setup()
     index = _device(q, "k_cache v_cache pages lengths starts prefix_pages out", k_cache, v_cache, pages, lengths, starts,
                     prefix_pages, out)
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise _bad("q must be [rows, heads, dim]")
-    rows, heads = q.shape[:2]
-    batch = _paged_batch(rows, k_cache, v_cache, pages, lengths, starts)
-    page, dim = k_cache.shape[2:]
+    rows, heads, _ = shape
+    kind = k_cache.dtype
+    batch, (kv_heads, page, dim), caches, k_at, v_at = _paged_batch(rows, k_cache, v_cache, pages, lengths, starts)
     if prefix_length < 0:
         raise _bad("prefix_length must be >= 0")
+    prefix = None
     if prefix_length:
         if prefix_pages is None or prefix_pages.dtype != torch.int32 or prefix_pages.dim() != 1 or \
                 not prefix_pages.is_contiguous() or prefix_pages.shape[0] * page < prefix_length:
             raise _bad("prefix_pages must be contiguous int32 and hold prefix_length tokens")
+        prefix = prefix_pages.data_ptr()
     if scale is None:
         scale = dim**-0.5 if dim else 1.0
-    if heads == 0 or heads % k_cache.shape[1]:
+    if heads == 0 or heads % kv_heads:
         raise _bad("heads must be a multiple of kv_heads")
     context, ptr = _context(index, stream)
     with context:
-        q, ldq = _heads(q, "q", rows, dim, k_cache.dtype)
-        if q.data_ptr() % 16 or ldq % 8:
-            q, ldq = torch.empty((rows, heads, dim), dtype=q.dtype, device=q.device).copy_(q), heads * dim
+        q, at_q, _, ldq = _heads(q, "q", rows, dim, kind, ())
+        device, width = q.device, heads * dim
+        if at_q % 16 or ldq % 8:
+            q, ldq = torch.empty((rows, heads, dim), dtype=kind, device=device).copy_(q), width
+            at_q = q.data_ptr()
+        ld_out = width
         if out is None:
-            out = torch.empty_strided((rows, heads, dim), (heads * dim, dim, 1), dtype=q.dtype, device=q.device)
-            ld_out = heads * dim
+            out = torch.empty_strided((rows, heads, dim), (width, dim, 1), dtype=kind, device=device)
+            at_out = out.data_ptr()
         else:
-            if out.shape != q.shape or out.dtype != q.dtype:
-                raise _bad(f"out must have shape {tuple(q.shape)} and type {q.dtype}")
-            if out.stride(2) != 1 or (heads > 1 and out.stride(1) != dim) or (rows > 1 and out.stride(0) < heads * dim):
+            if out.shape != shape or out.dtype != kind:
+                raise _bad(f"out must have shape {tuple(shape)} and type {kind}")
+            by_row, by_head, by_element = out.stride()
+            if by_element != 1 or (heads > 1 and by_head != dim) or (rows > 1 and by_row < width):
                 raise _bad("out must have contiguous rows that do not overlap")
-            ld_out = out.stride(0) if rows > 1 else heads * dim
-            _beside(out, "out", k_cache, v_cache)
+            if rows > 1:
+                ld_out = by_row
+            at_out = out.data_ptr()
             if rows:
+                _beside(at_out, (rows - 1) * ld_out + width, out, "out", caches)
                 _apart(out.flatten(1), ld_out, q.flatten(1), ldq, "q", "out", same=False)
-        need = lib().zq_paged_attention_workspace_bytes(C.byref(batch), heads, prefix_length)
-        ws = _empty((need + 256,), torch.uint8, q.device)
+        need = lib().zq_paged_attention_workspace_bytes(batch, heads, prefix_length)
+        ws = torch.empty_strided((need + 256,), (1,), dtype=torch.uint8, device=device)
         base = (ws.data_ptr() + 255) & ~255
-        check(lib().zq_paged_attention(C.byref(batch), q.data_ptr(), ldq, heads, k_cache.data_ptr(), v_cache.data_ptr(),
-                                       _ptr(prefix_pages) if prefix_length else None, prefix_length, causal, scale,
-                                       out.data_ptr(), ld_out, base, need, ptr))
+        check(lib().zq_paged_attention(batch, at_q, ldq, heads, k_at, v_at, prefix, prefix_length, causal, scale, at_out,
+                                       ld_out, base, need, ptr))
     return out
