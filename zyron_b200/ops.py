@@ -195,45 +195,45 @@ _ACTIVATIONS = {None: 0, "gelu": 1, "silu": 2, "relu": 3}  # ZQ_ACT_*
 
 
 def _epilogue(shape, index, activation, residual, dtype, out):
-    """The checked epilogue of a matmul with an output of `shape` on device
-    `index`, as the function that makes the call (with that device and the
-    call's stream current)."""
+    """Checks the epilogue of a matmul with an output of `shape` (a tuple) on
+    device `index`; the output's type."""
     if torch is None:
         _setup()
     if activation not in _ACTIVATIONS:
         raise _bad("activation must be None, 'gelu', 'silu' or 'relu'")
     if dtype is None:
         dtype = torch.float32 if residual is None else residual.dtype
-    code = _DTYPES.get(dtype)
-    if code is None:
+    if dtype not in _DTYPES:
         raise _bad("dtype must be float32, float16 or bfloat16")
-    shape = torch.Size(shape)
     if residual is not None:
         if residual.get_device() != index:
             raise _bad(f"residual is on {residual.device}, not on cuda:{index}")
         if residual.shape != shape or residual.dtype != dtype:
-            raise _bad(f"residual must have shape {tuple(shape)} and type {dtype}")
-    n = shape[-1]
+            raise _bad(f"residual must have shape {shape} and type {dtype}")
     if out is not None:
         if out.get_device() != index:
             raise _bad(f"out is on {out.device}, not on cuda:{index}")
         if out.shape != shape or out.dtype != dtype or not out.is_contiguous():
-            raise _bad(f"out must be contiguous, of shape {tuple(shape)} and type {dtype}")
+            raise _bad(f"out must be contiguous, of shape {shape} and type {dtype}")
+    return dtype
 
-    def call(weights, x, codes, scale, bias, ws, ws_bytes, stream):
-        y, res, ld = out, None, 0
-        if residual is not None:
-            res, ld = _rows(residual, "residual")
+
+def _run_epilogue(weights, x, codes, scale, m, device, bias, shape, activation, residual, dtype, out, ws, ws_bytes, stream):
+    """The call that ``_epilogue`` checked, its device and stream current."""
+    n, res, ld = shape[-1], None, 0
+    if residual is not None:
+        if out is None and residual.is_contiguous():
+            res, ld = residual.data_ptr(), n
+        else:
+            rows, ld = _rows(residual, "residual")
             if out is not None:
-                _apart(out.view(-1, n), n, res, ld, "residual", "out")
-        if y is None:
-            y = _empty(shape, dtype, f"cuda:{index}")
-        m = y.numel() // n
-        check(lib().zq_matmul_epilogue(weights.handle, _ptr(x), _ptr(codes), _ptr(scale), m, _ptr(bias),
-                                       _ACTIVATIONS[activation], _ptr(res), ld, y.data_ptr(), code, ws, ws_bytes, stream))
-        return y
-
-    return call
+                _apart(out.view(-1, n), n, rows, ld, "residual", "out")
+            residual, res = rows, rows.data_ptr()  # `residual` holds a copy until the call is made
+    if out is None:
+        out = _empty(shape, dtype, device)
+    check(lib().zq_matmul_epilogue(weights.handle, x, codes, scale, m, None if bias is None else bias.data_ptr(),
+                                   _ACTIVATIONS[activation], res, ld, out.data_ptr(), _DTYPES[dtype], ws, ws_bytes, stream))
+    return out
 
 
 def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None, stream=None, activation=None,
@@ -259,9 +259,9 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
     n = weights.cols()
     if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or not bias.is_contiguous()):
         raise _bad("bias must be contiguous float32 of the output's last dimension")
-    epilogue = None
-    if activation is not None or residual is not None or dtype is not None:
-        epilogue = _epilogue((*lead, n), index, activation, residual, dtype, out)
+    fused = activation is not None or residual is not None or dtype is not None
+    if fused:
+        dtype = _epilogue((*lead, n), index, activation, residual, dtype, out)
     elif out is not None and (out.dtype != torch.float32 or tuple(out.shape) != (*lead, n) or not out.is_contiguous()):
         raise _bad("out must be contiguous float32 [..., N]")
     context, ptr = _context(index, stream)
@@ -275,13 +275,14 @@ def matmul_codes(codes, row_scale, weights: QuantizedMatrix, bias=None, out=None
             padded[:, :k] = q
             q = padded
         scale = row_scale.contiguous()
-        if out is None and epilogue is None:
+        if out is None and not fused:
             out = _empty((*lead, n), torch.float32, q.device)
         need = lib().zq_matmul_workspace_bytes(weights.handle, m)
         ws = _empty((need + 256,), torch.uint8, q.device)
         base = (ws.data_ptr() + 255) & ~255
-        if epilogue is not None:
-            return epilogue(weights, None, q, scale, bias, base, need, ptr)
+        if fused:
+            return _run_epilogue(weights, None, q.data_ptr(), scale.data_ptr(), m, q.device, bias, (*lead, n), activation,
+                                 residual, dtype, out, base, need, ptr)
         check(lib().zq_matmul_codes(weights.handle, q.data_ptr(), scale.data_ptr(), m, _ptr(bias), out.data_ptr(),
                                     base, need, ptr))
     return out

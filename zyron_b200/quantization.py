@@ -324,14 +324,14 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None, ac
                              or not bias.is_contiguous()):
         raise _lib.ZQInvalidArgument("zyron_b200: bias must be contiguous float32 [N] on input's device")
     if fused:
-        from .ops import _epilogue
-
-        epilogue = _epilogue(out_shape, index, activation, residual, dtype, out)
+        dtype = _ops._epilogue(out_shape, index, activation, residual, dtype, out)
         context, ptr = _context(index, stream)
         with context:
-            x = input.contiguous()
-            ws, ws_bytes, _held = workspace(weights, x.numel() // weights.rows(), x.device, ptr)
-            return epilogue(weights, x, None, None, bias, ws, ws_bytes, ptr)
+            x, device = input.contiguous(), input.device
+            m = x.numel() // weights.rows()
+            ws, ws_bytes, _held = workspace(weights, m, device, ptr)
+            return _ops._run_epilogue(weights, x.data_ptr(), None, None, m, device, bias, out_shape, activation, residual,
+                                      dtype, out, ws, ws_bytes, ptr)
     if out is not None and (out.get_device() != index or out.dtype != torch.float32 or not out.is_contiguous()
                             or out.numel() * weights.rows() != input.numel() * n):
         raise _lib.ZQInvalidArgument("zyron_b200: out must be contiguous float32 [..., N] on input's device")
@@ -449,3 +449,6 @@ class QuantizedLinear:
         return y
 
     __call__ = forward
+
+
+from . import ops as _ops  # noqa: E402  (ops imports this module)
