@@ -609,7 +609,7 @@ def run_gemv_workload(args):
                "sample": f"M=1 x K={K} x N={N} INT8, best of 3 (the reference splits work over rows, so M=1 runs on "
                          f"one thread whatever the thread count)"}
     # the default dispatch (ZQ_DECODE_AUTO) runs the dp4a GEMV for M <= 4 and
-    # the tensor-core kernel above; the headline is the kernel it picks
+    # matrix instructions above; the headline is the kernel it picks
     for key, c in cases.items():
         c["default"] = "cuda_core" if key.endswith("_M1") else "tensor_core"
     head = cases["int8_M1"]["cuda_core"]["kernel"]
