@@ -611,7 +611,7 @@ def run_gemv_workload(args):
     # the default dispatch (ZQ_DECODE_AUTO) runs the dp4a GEMV for M <= 4 and
     # matrix instructions above; the headline is the kernel it picks
     for key, c in cases.items():
-        c["default"] = "cuda_core" if key.endswith("_M1") else "tensor_core"
+        c["default"] = "cuda_core" if key.endswith("_M1") else "rows"  # zq_rows.cu, neither of the two
     head = cases["int8_M1"]["cuda_core"]["kernel"]
     line = {"metric": "decode GEMV weight-stream bandwidth (quantization::matmul, M=1 INT8)", "value": head["GBs"],
             "unit": "GB/s", "n_gpus": 1, "steps": args.steps, "warmup": args.warmup, "ms_per_step": head["us"] / 1e3,
@@ -913,7 +913,7 @@ def secondary_block(args):
         cases, peak, peak_src, launches = decode_cases(args)
         out["decode_gemv_K4096_N11008"] = {
             "unit": "GB/s", "peak": peak, "peak_source": peak_src,
-            "dispatch": "zq_matmul default: dp4a GEMV with the quantizer fused for M <= 4, tcgen05 decode kernel "
+            "dispatch": "zq_matmul default: dp4a GEMV with the quantizer fused for M <= 4, mma.sync from registers "
                         "for 5-16 rows",
             "bytes": "payload + 4N scales + M*Kp codes + 4MN outputs per launch; weights rotate over > 2 x L2",
             "cases": {k: v["default"] for k, v in cases.items()}, "gpu_launches": launches}
