@@ -59,8 +59,7 @@ constexpr int kHalfBytes = kTile * 128;  // 128 rows x 64 elements, 128-byte swi
 constexpr int kBadRing = 8;
 constexpr int kPartRing = 4;
 
-// What the producer tells the other warps of a part.  It is at most two parts ahead
-// of the warpgroups (q has one place), so a ring of four is never overrun.
+// What the producer tells the other warps of a part.
 struct Part {
     int first, rows, length;  // of the request
     int token0, head;         // first token of the item, kv head
@@ -336,8 +335,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     volatile uint32_t* own = bad_ring + kBadRing;  // by tile: its warpgroup added the values
     uint32_t* tmem_slot = bad_ring + kBadRing + 2;
     uint64_t* part_full = reinterpret_cast<uint64_t*>(bad_ring + kBadRing + 4);
-    Part* parts = reinterpret_cast<Part*>(part_full + kPartRing);
-    static_assert((10 + 2 * 4 + kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
+    uint64_t* part_empty = part_full + kPartRing;
+    Part* parts = reinterpret_cast<Part*>(part_empty + kPartRing);
+    static_assert((10 + 2 * 4 + 2 * kPartRing) * 8 + (kBadRing + 4) * 4 + kPartRing * sizeof(Part) <= 512, "barriers");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const PagedBatch& p = a.batch;
 
@@ -351,7 +351,10 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             mbar_init(&p_ready[i], 128);
             mbar_init(&o_done[i], 1);
         }
-        for (int i = 0; i < kPartRing; ++i) mbar_init(&part_full[i], 1);
+        for (int i = 0; i < kPartRing; ++i) {
+            mbar_init(&part_full[i], 1);
+            mbar_init(&part_empty[i], 10);  // every warp but the producer
+        }
         for (int i = 0; i < kGroups; ++i) {
             mbar_init(&kv_full[i], 1);
             mbar_init(&kv_empty[i], 2);  // keys and values taken
@@ -382,6 +385,8 @@ __global__ void __launch_bounds__(kManyThreads, 1)
     const auto part_at = [&](uint32_t i, Part& q) {
         if (!wait_bounded(&part_full[i % kPartRing], (i / kPartRing) & 1, err, kDevErrTimeoutMma)) return false;
         q = parts[i % kPartRing];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&part_empty[i % kPartRing]);
         return true;
     };
     // A part of T key tiles has T + 1 groups: keys of tile k in group k, values in
@@ -407,6 +412,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
             const int head = way.it.head;
             const Part q{r.first, r.rows, r.length, way.it.tile * 2 * shape.tile_tokens, head, way.first_tile, way.end_tile,
                          more ? (prefix ? kPrefix : 0) | (way.whole ? kWhole : 0) | (way.slot ? kSecondSlot : 0) : kEnd};
+            if (part >= kPartRing &&
+                !wait_bounded(&part_empty[part % kPartRing], (part / kPartRing - 1) & 1u, err, kDevErrTimeoutProducer))
+                break;
             if (lane == 0) {
                 parts[part % kPartRing] = q;
                 mbar_arrive(&part_full[part % kPartRing]);
