@@ -604,24 +604,32 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     tmem_st_wait();
                     mul = 1.0f;
                 }
+                // Half of the scores at a time: the first half's largest while the second comes.
                 uint32_t s[4][32];
+                float m[4];
+                const auto largest = [&](int half) {
+                    if (masked) {
+                        const int seen = limit - key0 - half * 64;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_addr + c * 32, s[c]);
+                        for (int k = 0; k < 64; ++k)
+                            if (k >= seen) s[2 * half + k / 32][k % 32] = __float_as_uint(-INFINITY);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) {
+                        const float x = fmaxf(__uint_as_float(s[2 * half][k]), __uint_as_float(s[2 * half + 1][k]));
+                        m[k & 3] = half == 0 && k < 4 ? x : fmaxf(m[k & 3], x);
+                    }
+                };
+                tmem_ld_32x32b_x32(s_addr, s[0]);
+                tmem_ld_32x32b_x32(s_addr + 32, s[1]);
+                tmem_ld_wait();
+                tmem_ld_32x32b_x32(s_addr + 64, s[2]);
+                tmem_ld_32x32b_x32(s_addr + 96, s[3]);
+                largest(0);
                 tmem_ld_wait();
                 tmem_fence_before();
                 mbar_arrive(s_free);
-                if (masked) {
-                    const int seen = limit - key0;
-#pragma unroll
-                    for (int k = 0; k < kTile; ++k)
-                        if (k >= seen) s[k / 32][k % 32] = __float_as_uint(-INFINITY);
-                }
-                float m[4];
-#pragma unroll
-                for (int k = 0; k < 64; ++k) {
-                    const float x = fmaxf(__uint_as_float(s[k / 32][k % 32]), __uint_as_float(s[2 + k / 32][k % 32]));
-                    m[k & 3] = k < 4 ? x : fmaxf(m[k & 3], x);
-                }
+                largest(1);
                 const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
                 // The product of the key tile before is in O, and has read its weights.
                 if (!first) {
