@@ -425,9 +425,10 @@ zq_status zq_ipc_close(void* dev_ptr);
  *       ZQ_DECODE_TENSOR_CORE: the tcgen05 decode kernel for m <= 16 (weights
  *         streamed by TMA, work split evenly over the SMs);
  *       ZQ_DECODE_CUDA_CORE: the dp4a warp-per-column GEMV for m <= 8;
- *       ZQ_DECODE_AUTO (default): the GEMV for m <= 4; for 5 <= m <= 16 a
- *         kernel that feeds matrix instructions from registers, or the tcgen05
- *         kernel where SMs are reserved.
+ *       ZQ_DECODE_AUTO (default): the GEMV for m <= 4; above that, up to 64
+ *         rows where it is the faster one, a kernel that feeds matrix
+ *         instructions from registers (not where SMs are reserved: the tcgen05
+ *         kernel up to 16 rows).
  *     Larger m always runs the tcgen05 GEMM.
  *   ZQ_OPT_RESERVED_SMS: streaming multiprocessors kept out of the matmul
  *     kernels' grids (default 0), so work running concurrently on other

@@ -142,6 +142,22 @@ def test_five_to_sixteen_rows(zb, torch, m, k, n, qtype):
     assert torch.equal(zb.matmul(x, w), plain)
 
 
+@pytest.mark.parametrize("qtype", ["Int8", "Int4"])
+@pytest.mark.parametrize("m,k,n", [(17, 1000, 9), (31, 700, 4803), (32, 300, 1003), (20, 128, 14300), (33, 700, 100), (50, 129, 2405),
+                                   (64, 4100, 4000), (64, 200, 4800), (65, 300, 64)])
+def test_rows_up_to_sixty_four(zb, torch, m, k, n, qtype):
+    """The kernel of few rows and the GEMM, by columns and type: the same bits, and the formula's."""
+    w = zb.quantize((randn(torch, 1, k, n) * 0.04).cuda(), getattr(zb.Type, qtype))
+    x, r, b = randn(torch, 2, m, k).cuda(), randn(torch, 3, m, n).bfloat16().cuda(), randn(torch, 4, n).cuda()
+    want, tol = epilogue_want(torch, zb, x, w, b, "gelu", r, torch.bfloat16)
+    got, plain = zb.matmul(x, w, bias=b, activation="gelu", residual=r), zb.matmul(x, w, bias=b)
+    within(torch, got, want, tol, "rows")
+    again = r.clone()
+    assert torch.equal(zb.matmul(x, w, bias=b, activation="gelu", residual=again, out=again), got)
+    w.set_decode_kernel(1)
+    assert torch.equal(zb.matmul(x, w, bias=b), plain)
+
+
 def test_nine_rows_of_a_long_int4_dot(zb, torch):
     """K past 2^17, where sixteen times the dot would pass 32 bits, at extreme codes."""
     k = (1 << 17) + 300

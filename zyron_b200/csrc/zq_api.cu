@@ -593,7 +593,7 @@ zq_status run_codes_out(const zq_weight* w, const int8_t* codes, const float* rs
         ZQ_CUDA(zq::launch_gemv(a, st, pdl));
         return ZQ_OK;
     }
-    if (plain && !test && M <= zq::kSkinnyMaxRows && reserved == 0 &&
+    if (plain && !test && zq::rows_kernel_wins(w->type, M, N) && reserved == 0 &&
         w->opt_decode.load(std::memory_order_relaxed) == ZQ_DECODE_AUTO) {
         zq::GemvArgs a{w->type, w->panel, N, Kp, w->scales, codes, rs, bias, y, M};
         a.epi = out.epi;

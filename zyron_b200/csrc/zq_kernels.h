@@ -142,7 +142,8 @@ cudaError_t launch_dequantize(const uint8_t* panel, int type, int K, int N, int 
 
 size_t gemv_smem_bytes(int M, int Kp);
 cudaError_t launch_gemv(const GemvArgs& a, cudaStream_t stream, bool pdl);
-// 5 to 16 rows of codes (zq_rows.cu).
+// 5 to 64 rows of codes (zq_rows.cu), where that is the fastest kernel.
+bool rows_kernel_wins(int type, int M, int N);
 cudaError_t launch_rows(const GemvArgs& a, cudaStream_t stream);
 
 // Decode-sized matmul on tensor cores (zq_skinny_sm100.cu), M <= 16.

@@ -1,4 +1,4 @@
-// zq_rows.cu -- quantized matmul of 5 to 16 activation rows.
+// zq_rows.cu -- quantized matmul of 5 to 64 activation rows.
 //
 // Computes, for every activation row m and output column n,
 //   acc[m][n] = sum_k q_a[m][k] * q_w[n][k]         (exact int32)
@@ -17,6 +17,9 @@
 // there for tcgen05 (zq_skinny_sm100.cu: a ring of three stages waits for copy, unpack
 // and product in turn): 12 rows, K = 11008, N = 4096, INT4 9.3 us, was 24.1, INT8
 // 11.6, was 23.8; 16 rows, K = 4096, N = 11008 11.0 and 13.5, were 30.6 and 30.0.
+// More rows are more tiles of 16 that the same weights are multiplied by; against the
+// GEMM, whose few tiles stream the weights through a part of the SMs: 32 rows, K =
+// 11008, N = 4096 14.0 and 17.7 us, were 37.2 and 29.2.
 // The activations are what bounds wide ones (16 rows, K = 8192, N = 28672, INT4: 3.7
 // TB/s of weights and as much of codes again, 31.8 us, was 63.7).  A ring of loads
 // in registers that is refilled tile by tile costs registers, so warps, and measured
@@ -40,9 +43,9 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// kTiles: tiles of 8 columns a block.  kDeep: steps of 64 bytes a column that a warp
+// kRowTiles: tiles of 16 rows.  kTiles: tiles of 8 columns a block.  kDeep: steps of 64 bytes a column that a warp
 // has under way.  kBlocks: blocks an SM is to hold.
-template <int kType, int kWarps, int kTiles, int kDeep, int kBlocks, bool kX16, bool kEpi>
+template <int kType, int kRowTiles, int kWarps, int kTiles, int kDeep, int kBlocks, bool kX16, bool kEpi>
 __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_t* __restrict__ panel, int N, int Kp,
                                                                     const float* __restrict__ col_scale, const int8_t* q,
                                                                     const float* row_scale,
@@ -55,7 +58,8 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
     const int col0 = blockIdx.x * kCols;
     const int steps = Kp / (4 * kCodes);
     const size_t col_bytes = (size_t)Kp * 16 / kCodes;
-    __shared__ int sums[kWarps][kRowsTile][kCols + 2];
+    extern __shared__ int sums[];  // [kWarps][rows][kPitch]
+    constexpr int kRows = kRowTiles * kRowsTile, kPitch = kCols + 2;
     const uint8_t* column[kTiles];
 #pragma unroll
     for (int i = 0; i < kTiles; ++i) column[i] = panel + (size_t)min(col0 + i * kColTile + g, N - 1) * col_bytes + t * 16;
@@ -70,24 +74,30 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
     load(warp * kDeep);  // weights depend on no kernel before this one
     pdl_wait_primary();
     pdl_launch_dependents();
-    int acc[kTiles][4];
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0;
-    const bool low = g < M, high = g + 8 < M;
+    int acc[kRowTiles][kTiles][4] = {};
     const int8_t* row = q + (size_t)g * Kp + t * kCodes;
+    // Codes of a step: rows g and g + 8 of each tile.
+    const auto load_x = [&](int s, uint4 (&x)[kRowTiles][2][kParts]) {
+#pragma unroll
+        for (int r = 0; r < 2 * kRowTiles; ++r) {
+            const uint4* p = reinterpret_cast<const uint4*>(row + (size_t)(8 * r) * Kp + s * (4 * kCodes));
+#pragma unroll
+            for (int h = 0; h < kParts; ++h) x[r / 2][r & 1][h] = 8 * r + g < M ? load_l2(p + h) : make_uint4(0, 0, 0, 0);
+        }
+    };
+    // One tile of rows has registers for all its steps' codes at once, more have not.
+    constexpr int kAhead = kRowTiles == 1 ? kDeep : 1;
     for (int at = warp * kDeep; at < steps; at += kDeep * kWarps) {
-        uint4 x[kDeep][2][kParts] = {};
+        uint4 x[kAhead][kRowTiles][2][kParts];
+        if constexpr (kAhead > 1) {
 #pragma unroll
-        for (int d = 0; d < kDeep; ++d)
-#pragma unroll
-            for (int h = 0; h < kParts; ++h) {
-                const int8_t* p = row + (at + d) * (4 * kCodes);
-                if (low && at + d < steps) x[d][0][h] = load_l2(reinterpret_cast<const uint4*>(p) + h);
-                if (high && at + d < steps) x[d][1][h] = load_l2(reinterpret_cast<const uint4*>(p + (size_t)8 * Kp) + h);
-            }
+            for (int d = 0; d < kDeep; ++d)
+                if (at + d < steps) load_x(at + d, x[d % kAhead]);
+        }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if (at + d >= steps) break;
+            if constexpr (kAhead == 1) load_x(at + d, x[0]);
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) {
                 uint4 v[2];
@@ -98,27 +108,32 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
                 else
                     zq_expand_int4x32(w[d][i], v[0], v[1]);
 #pragma unroll
-                for (int h = 0; h < kParts; ++h) {
-                    mma_s8(acc[i], x[d][0][h].x, x[d][1][h].x, x[d][0][h].y, x[d][1][h].y, v[h].x, v[h].y);
-                    mma_s8(acc[i], x[d][0][h].z, x[d][1][h].z, x[d][0][h].w, x[d][1][h].w, v[h].z, v[h].w);
-                }
+                for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+                    for (int h = 0; h < kParts; ++h) {
+                        const uint4 &lo = x[d % kAhead][r][0][h], &hi = x[d % kAhead][r][1][h];
+                        mma_s8(acc[r][i], lo.x, hi.x, lo.y, hi.y, v[h].x, v[h].y);
+                        mma_s8(acc[r][i], lo.z, hi.z, lo.w, hi.w, v[h].z, v[h].w);
+                    }
             }
         }
         load(at + kDeep * kWarps);
     }
 #pragma unroll
-    for (int i = 0; i < kTiles; ++i) {
-        const int c = i * kColTile + 2 * t;
-        *reinterpret_cast<int2*>(&sums[warp][g][c]) = make_int2(acc[i][0], acc[i][1]);
-        *reinterpret_cast<int2*>(&sums[warp][g + 8][c]) = make_int2(acc[i][2], acc[i][3]);
-    }
+    for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+            int* to = sums + (warp * kRows + r * kRowsTile + g) * kPitch + i * kColTile + 2 * t;
+            *reinterpret_cast<int2*>(to) = make_int2(acc[r][i][0], acc[r][i][1]);
+            *reinterpret_cast<int2*>(to + 8 * kPitch) = make_int2(acc[r][i][2], acc[r][i][3]);
+        }
     __syncthreads();
     for (int i = threadIdx.x; i < M * kCols; i += 32 * kWarps) {
         const int m = i / kCols, c = i % kCols, n = col0 + c;
         if (n >= N) continue;
         int sum = 0;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) sum += sums[k][m][c];
+        for (int k = 0; k < kWarps; ++k) sum += sums[(k * kRows + m) * kPitch + c];
         if (kX16) sum >>= 4;
         const float sr = load_l2(row_scale + m), sc = __ldg(col_scale + n);
         const float v = bias ? zq_epilogue_bias(sum, sr, sc, __ldg(bias + n)) : zq_epilogue(sum, sr, sc);
@@ -129,30 +144,52 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
     }
 }
 
-template <int kType, int kWarps, int kTiles, int kDeep, int kBlocks, bool kX16>
+template <int kType, int kRowTiles, int kWarps, int kTiles, int kDeep, int kBlocks, bool kX16>
 cudaError_t launch_t(const GemvArgs& a, cudaStream_t stream) {
-    const auto kernel = a.epi.on ? rows_kernel<kType, kWarps, kTiles, kDeep, kBlocks, kX16, true>
-                                 : rows_kernel<kType, kWarps, kTiles, kDeep, kBlocks, kX16, false>;
-    constexpr int cols = kTiles * kColTile;
-    return launch_pdl_kernel(kernel, dim3((a.N + cols - 1) / cols), dim3(32 * kWarps), 0, stream, a.panel, a.N, a.Kp,
+    const auto kernel = a.epi.on ? rows_kernel<kType, kRowTiles, kWarps, kTiles, kDeep, kBlocks, kX16, true>
+                                 : rows_kernel<kType, kRowTiles, kWarps, kTiles, kDeep, kBlocks, kX16, false>;
+    constexpr int cols = kTiles * kColTile, smem = kWarps * kRowTiles * kRowsTile * (cols + 2) * 4;
+    const cudaError_t e = ensure_smem_attr(kernel, smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl_kernel(kernel, dim3((a.N + cols - 1) / cols), dim3(32 * kWarps), smem, stream, a.panel, a.N, a.Kp,
                              a.col_scale, a.q, a.row_scale, a.bias, a.y, a.M, a.epi);
 }
 
-// Blocks of 16 columns and 16 warps while blocks of 32 would leave SMs without one;
-// of 32 columns and 8 warps above, which read the activations half as often (16 rows,
-// INT4, K = 4096: N = 4096 5.2 us against 6.9, N = 5120 7.2 against 7.1, N = 8192 8.9
-// against 7.8, N = 11008 12.0 against 11.0; K = 8192, N = 28672 42.6 against 31.8;
-// INT8 N = 6144 9.4 against 9.5, N = 8192 10.7 against 10.3).
+// Blocks of 16 columns while blocks of 32 would leave SMs without one, of 32 above,
+// which read the activations half as often.  16 rows (INT4, K = 4096): N = 4096 5.2 us
+// against 6.9, N = 5120 7.2 against 7.1, N = 8192 8.9 against 7.8, N = 11008 12.0
+// against 11.0; K = 8192, N = 28672 42.6 against 31.8; INT8 N = 6144 9.4 against 9.5, N
+// = 8192 10.7 against 10.3.  32 rows: INT4 N = 4096 6.7 against 7.4, N = 11008 16.5
+// against 15.2.  64 rows go to blocks of 32 sooner, from one for two SMs on: N = 1024
+// (K = 1024) 3.8 against 5.6, N = 4096 (K = 4096) 11.7 against 10.4.
+bool narrow(int N) { return N < 32 * sm_count(); }
 template <int kType, bool kX16>
 cudaError_t launch_columns(const GemvArgs& a, cudaStream_t stream) {
-    return a.N < 32 * sm_count() ? launch_t<kType, 16, 2, 2, 2, kX16>(a, stream)
-                                     : launch_t<kType, 8, 4, 1, 4, kX16>(a, stream);
+    if (a.M > 2 * kRowsTile)
+        return a.N < 16 * sm_count() ? launch_t<kType, 4, 8, 2, 2, 2, kX16>(a, stream)
+                                     : launch_t<kType, 4, 8, 4, 2, 1, kX16>(a, stream);
+    if (a.M > kRowsTile)
+        return narrow(a.N) ? launch_t<kType, 2, 8, 2, 2, 2, kX16>(a, stream)
+                           : launch_t<kType, 2, 8, 4, 2, 2, kX16>(a, stream);
+    return narrow(a.N) ? launch_t<kType, 1, 16, 2, 2, 2, kX16>(a, stream)
+                       : launch_t<kType, 1, 8, 4, 1, 4, kX16>(a, stream);
 }
 
 }  // namespace
 
+// Up to 16 rows always.  More rows read more codes a block of columns, so the GEMM's
+// tiles win once there are enough of them.  32 rows: INT8 K = 4096, N = 4096 8.7 us
+// against the GEMM's 15.3, N = 11008 20.7 against 24.0, K = 8192, N = 28672 71 against
+// 55; INT4 6.7 against 18.7, 15.2 against 29.9, 48 against 62.  64 rows: INT8 N = 4096
+// 11.9 against 15.4, N = 11008 31 against 24; INT4 10.4 against 18.7, 27 against 30.
+bool rows_kernel_wins(int type, int M, int N) {
+    if (M <= kRowsTile) return true;
+    if (M <= 2 * kRowsTile) return type == kInt4 || N < 96 * sm_count();
+    return M <= 4 * kRowsTile && narrow(N);
+}
+
 cudaError_t launch_rows(const GemvArgs& a, cudaStream_t stream) {
-    if (a.M < 1 || a.M > kRowsTile) return cudaErrorInvalidValue;
+    if (a.M < 1 || a.M > 4 * kRowsTile) return cudaErrorInvalidValue;
     if (a.type == kInt8) return launch_columns<kInt8, false>(a, stream);
     return int4_x16_fits(a.Kp) ? launch_columns<kInt4, true>(a, stream) : launch_columns<kInt4, false>(a, stream);
 }
