@@ -82,7 +82,10 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
         for (int r = 0; r < 2 * kRowTiles; ++r) {
             const uint4* p = reinterpret_cast<const uint4*>(row + (size_t)(8 * r) * Kp + s * (4 * kCodes));
 #pragma unroll
-            for (int h = 0; h < kParts; ++h) x[r / 2][r & 1][h] = 8 * r + g < M ? load_l2(p + h) : make_uint4(0, 0, 0, 0);
+            for (int h = 0; h < kParts; ++h) {
+                x[r / 2][r & 1][h] = make_uint4(0, 0, 0, 0);
+                if (8 * r + g < M && s < steps) x[r / 2][r & 1][h] = load_l2(p + h);
+            }
         }
     };
     // One tile of rows has registers for all its steps' codes at once, more have not.
@@ -91,8 +94,7 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
         uint4 x[kAhead][kRowTiles][2][kParts];
         if constexpr (kAhead > 1) {
 #pragma unroll
-            for (int d = 0; d < kDeep; ++d)
-                if (at + d < steps) load_x(at + d, x[d % kAhead]);
+            for (int d = 0; d < kDeep; ++d) load_x(at + d, x[d % kAhead]);
         }
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
@@ -128,19 +130,47 @@ __global__ void __launch_bounds__(32 * kWarps, kBlocks) rows_kernel(const uint8_
             *reinterpret_cast<int2*>(to + 8 * kPitch) = make_int2(acc[r][i][2], acc[r][i][3]);
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < M * kCols; i += 32 * kWarps) {
-        const int m = i / kCols, c = i % kCols, n = col0 + c;
-        if (n >= N) continue;
-        int sum = 0;
+    // A thread's outputs, up to four at once, so that their loads are under way together.
+    constexpr int kThreads = 32 * kWarps, kOutputs = (kRows * kCols + kThreads - 1) / kThreads;
+    constexpr int kEach = kOutputs < 4 ? kOutputs : 4;
+    for (int i0 = threadIdx.x; i0 < M * kCols; i0 += kEach * kThreads) {
+        float v[kEach], sr[kEach], sc[kEach], b[kEach], res[kEach];
+        bool live[kEach];
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) sum += sums[(k * kRows + m) * kPitch + c];
-        if (kX16) sum >>= 4;
-        const float sr = load_l2(row_scale + m), sc = __ldg(col_scale + n);
-        const float v = bias ? zq_epilogue_bias(sum, sr, sc, __ldg(bias + n)) : zq_epilogue(sum, sr, sc);
-        if constexpr (kEpi)
-            epi_finish(epi, y, N, m, n, v);
-        else
-            y[(size_t)m * N + n] = v;
+        for (int e = 0; e < kEach; ++e) {
+            const int i = i0 + e * kThreads, m = i / kCols, n = col0 + i % kCols;
+            live[e] = m < M && n < N;
+            sr[e] = live[e] ? load_l2(row_scale + m) : 0.0f;
+            sc[e] = live[e] ? __ldg(col_scale + n) : 0.0f;
+            b[e] = bias && live[e] ? __ldg(bias + n) : 0.0f;
+            res[e] = kEpi && epi.residual && live[e] ? epi_residual(epi, (size_t)m * (size_t)epi.ld_residual + n) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = i0 + e * kThreads, m = min(i / kCols, kRows - 1), c = i % kCols;
+            int sum = 0;
+#pragma unroll
+            for (int k = 0; k < kWarps; ++k) sum += sums[(k * kRows + m) * kPitch + c];
+            if (kX16) sum >>= 4;
+            v[e] = bias ? zq_epilogue_bias(sum, sr[e], sc[e], b[e]) : zq_epilogue(sum, sr[e], sc[e]);
+        }
+        if constexpr (kEpi) {
+            epi_activate(epi.activation, v);
+            if (epi.residual) {
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) v[e] += res[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+            const int i = i0 + e * kThreads;
+            const size_t at = (size_t)(i / kCols) * N + col0 + i % kCols;
+            if (!live[e]) continue;
+            if constexpr (kEpi)
+                epi_store(epi, y, at, v[e]);
+            else
+                y[at] = v[e];
+        }
     }
 }
 
