@@ -31,7 +31,7 @@
 // Bound: 4 dim operations a (row, key) on the tensor cores against one exponential,
 // of which the special function unit makes 16 a cycle and SM: at dim 128 both take
 // 2048 cycles for 256 rows x 128 keys.  Measured: about 2900, and four prompts of
-// 1000 to 2600 tokens (32 heads over 8, dim 128) 226 us with their joins, the tensor
+// 1000 to 2600 tokens (32 heads over 8, dim 128) 224 us with their joins, the tensor
 // cores at 54 %; a 16000 key prefix of 96 rows 41.  Some of the exponentials as a
 // polynomial on the fp32 pipe cost more issue slots than they freed (one in eight
 // 258 us against 251, one in four 268, every other 296).
