@@ -1,0 +1,103 @@
+"""paged_attention, append_kv and the matmul's epilogue where a rounding, an
+infinity or a layout can make them wrong: against plain implementations in 64
+bits, within bounds counted from their roundings."""
+import math
+
+import pytest
+
+from test_gpu_block import CACHES, Batch, half_step, randn, torch, within, zb  # noqa: F401 (torch and zb are fixtures)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- the weights of the attention -------------------------------------------------------
+
+def attention64(torch, batch, q, weight_step, causal=True):
+    """Output and tolerance in 64 bits, of a batch whose values are finite.  Scores: dim / 16
+    tensor-core steps and two more roundings of at most 2^-22 of sum |q k|, the subtraction
+    2^-24 of the scores' range, the exponential 2^-22; a weight's error counts twice (itself
+    and in the sum).  Weights are off by `weight_step` of themselves beside that, sums of
+    products by 2^-22 a step of 16 keys, the output by half a step of its type."""
+    heads, dim = q.shape[1:]
+    out, tol = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(2))
+    x = q.double().cpu()
+    for b, (n, length) in enumerate(zip(batch.new, batch.lens)):
+        rows = slice(batch.starts_host[b], batch.starts_host[b] + n)
+        k, v = (torch.cat([batch.shared[i], batch.own[b][i]], 1).repeat_interleave(heads // batch.kv, 0) for i in (0, 1))
+        key, at = torch.arange(batch.prefix + length) - batch.prefix, length - n + torch.arange(n)
+        seen = (key < 0) | (key <= at[:, None]) | (not causal)
+        mine = x[rows].transpose(0, 1)
+        p = torch.softmax(torch.where(seen, mine @ k.transpose(1, 2) * dim**-0.5, -math.inf), -1)
+        big = (mine.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * dim**-0.5
+        delta = (dim / 16 + 4) * 2.0**-22 * big + 2.0**-21
+        out[rows] = (p @ v).transpose(0, 1)
+        tol[rows] = ((2 * delta + (len(key) / 16 + 8) * 2.0**-22 + weight_step) * (p @ v.abs())).transpose(0, 1)
+    return out, tol + half_step(torch, q.dtype, out) * (1 + 2.0**-7)
+
+
+def put(batch, torch, request, token, key=None, value=None):
+    """Sets the key's first element, or the whole value, of a request's own token (None: the prefix's)."""
+    own = batch.shared if request is None else batch.own[request]
+    table = batch.prefix_pages if request is None else batch.pages[request]
+    page, slot = int(table[token // batch.page]), token % batch.page
+    if key is not None:
+        batch.k_cache[page, :, slot, 0] = key
+        own[0][:, token, 0] = batch.k_cache[page, :, slot, 0].double().cpu()
+    if value is not None:
+        batch.v_cache[page, :, slot] = value
+        own[1][:, token] = batch.v_cache[page, :, slot].double().cpu()
+
+
+def flat(batch, torch, mean):
+    """Takes the first element out of all keys and sets the values around `mean`."""
+    for cache, own in ((batch.k_cache, 0), (batch.v_cache, 1)):
+        if own == 0:
+            cache[..., 0] = 0
+        else:
+            cache += mean
+        for side, table, n in [(batch.shared, batch.prefix_pages, batch.prefix)] + \
+                [(o, batch.pages[b], batch.lens[b]) for b, o in enumerate(batch.own)]:
+            j = torch.arange(n)
+            side[own] = cache[table[j // batch.page].long().cuda(), :, (j % batch.page).cuda()].double().cpu().transpose(0, 1)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("nats", [12, 16, 18])
+@pytest.mark.parametrize("new,dim,prefix", [(1, 64, 0), (5, 128, 0), (1, 128, 300), (5, 64, 300)])
+def test_weights_far_below_the_largest(zb, torch, cache, nats, new, dim, prefix):
+    """A key that takes nearly all weight and has no value: the output is the sum of weights
+    of e^-12 to e^-18, each off by half a step of the cache's type at most."""
+    t = getattr(torch, cache)
+    batch = Batch(torch, nats, [new, 2], [new + 700, 90], 16, 2, dim, t, prefix=prefix)
+    flat(batch, torch, 64.0)
+    sink = nats * dim**0.5 / 8
+    for place in ([(0, 0), (1, 0)], [(0, 300), (1, 50)], [(None, 17)]):
+        if place[0][0] is None and prefix == 0:
+            continue
+        for request, token in place:
+            put(batch, torch, request, token, key=sink, value=0.0)
+        q = 0.05 * randn(torch, new, batch.rows, 4, dim)
+        q[..., 0] = 8.0
+        q = q.to(t)
+        want, tol = attention64(torch, batch, q, torch.finfo(t).eps / 2)
+        assert (want.abs() < 1).all()  # nothing but the small weights
+        within(torch, batch.attention(zb, q.cuda()), want, tol, f"sink at {place}")
+        for request, token in place:
+            put(batch, torch, request, token, key=0.0)
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("scale", [1.0, 2.0**-5, 2.0**-6, 2.0**-7, 2.0**-8, 2.0**-9])
+@pytest.mark.parametrize("new", [1, 5])
+def test_scores_of_many_millions(zb, torch, cache, scale, new):
+    """Scores so large that neighbouring fp32 numbers lie whole powers of two of weight apart:
+    the two largest are equal and the output is their values' mean, exactly."""
+    t = getattr(torch, cache)
+    batch = Batch(torch, 4, [new], [400 + new], 16, 1, 64, t)
+    batch.k_cache[..., 1:] = 0
+    for token in range(400 + new):  # 59392 twice, all others far below
+        put(batch, torch, 0, token, key=59392.0 if token in (17, 300) else 128.0 * (token % 300), value=float(token % 7))
+    q = torch.zeros(new, 4, 64, dtype=t)
+    q[..., 0] = 59392.0
+    got = batch.attention(zb, q.cuda(), scale=scale)
+    assert torch.equal(got, torch.full_like(got, (17 % 7 + 300 % 7) / 2))

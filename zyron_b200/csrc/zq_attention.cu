@@ -27,7 +27,8 @@
 // 96 requests of 20 to 500 tokens took 44 us, now 24); the products are mma.sync,
 // which at 16 rows take 4 of the 22 cycles that a key's bytes take an SM.
 // exp(s - m) enters the second product as a sum of two 16-bit parts, so that it is
-// not rounded to the cache's type.  64 requests of 100 to 6000 tokens, 32 heads over
+// not rounded to the cache's type; with fp16 m lies 2^15 below the largest score, and
+// the parts hold a weight to 2^-22 of itself or 2^-40 of the largest.  64 requests of 100 to 6000 tokens, 32 heads over
 // 8 of 128: 805 MB in 137 us with the join, 5.9 TB/s; one token over 301 keys 10.6.
 #include "zq_attention.cuh"
 
@@ -274,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
                 for (int e = 0; e < 2; ++e) {
                     most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 1));
                     most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 2));
+                    if (kLift<T> != 0.0f) most[e] = __fadd_ru(most[e], -kLift<T>);
                     const float now = fmaxf(top[mt][e], most[e]);
                     ref[e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: every weight is 0
                     const float keep = exp2_approx(top[mt][e] - ref[e]);

@@ -27,14 +27,23 @@ constexpr bool kIsHalf = false;
 template <>
 constexpr bool kIsHalf<__half> = true;
 
+// Weights are taken relative to a reference 2^kLift below the row's largest score:
+// fp16 ends at 2^-24, so weights relative to the largest itself lose digits from
+// 2^-14 down and are gone at e^-18, which counts where one key takes nearly all
+// weight and has no value; fp16's upper end has room for 2^15.  bf16 has the
+// exponents of fp32.  The reference is rounded up, so that no weight is above
+// 2^kLift however large the scores are.
+template <class T>
+constexpr float kLift = kIsHalf<T> ? 15.0f : 0.0f;
+
 __device__ __forceinline__ float exp2_approx(float v) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
 
-// Two fp32 values as packed pairs of 16-bit parts whose sum they are (to 2^-17
-// of bf16, 2^-22 of fp16).
+// Two fp32 values as packed pairs of 16-bit parts whose sum they are: to 2^-17 of
+// the value for bf16, to 2^-22 for fp16, but not below 2^-25, half its smallest step.
 template <class T>
 __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
     const T hx = from_float<T>(x), hy = from_float<T>(y);
