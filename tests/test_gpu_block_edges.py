@@ -63,7 +63,8 @@ def flat(batch, torch, mean):
 
 @pytest.mark.parametrize("cache", CACHES)
 @pytest.mark.parametrize("nats", [12, 16, 18])
-@pytest.mark.parametrize("new,dim,prefix", [(1, 64, 0), (5, 128, 0), (1, 128, 300), (5, 64, 300)])
+@pytest.mark.parametrize("new,dim,prefix", [(1, 64, 0), (5, 128, 0), (1, 128, 300), (5, 64, 300), (200, 128, 0),
+                                            (200, 64, 0), (200, 128, 300)])
 def test_weights_far_below_the_largest(zb, torch, cache, nats, new, dim, prefix):
     """A key that takes nearly all weight and has no value: the output is the sum of weights
     of e^-12 to e^-18, each off by half a step of the cache's type at most."""

@@ -24,9 +24,11 @@
 // in turn: 4500 cycles for 256 rows x 128 keys (5700 in steps of 64 keys, since an
 // MMA of 64 columns takes as long as one of 128), where the softmax takes 2250.
 // A row's reference is raised, and its output in TMEM rescaled, only when its
-// maximum has grown by more than 2^8 since: weights up to 2^8 lose nothing in the
-// sums' 32 bits.  P is rounded to the cache's type for the second product, half a
-// step of each weight.
+// maximum has grown by more than 2^8 since (fp16: 2^3.9): weights up to 2^8 lose
+// nothing in the sums' 32 bits.  P is rounded to the cache's type for the second
+// product, half a step of each weight.  fp16 has no exponents for weights far below
+// the largest, so the reference is set 2^12 below that: half a step down to 2^-26 of
+// the largest (e^-18), 2^-37 of it below.
 //
 // Bound: 4 dim operations a (row, key) on the tensor cores against one exponential,
 // of which the special function unit makes 16 a cycle and SM: at dim 128 both take
@@ -56,6 +58,13 @@ constexpr int kTile = 128;             // rows of a q tile, keys of a key tile
 // TMEM columns: the scores of whichever tile, P (two keys a column), O.
 constexpr int kScoreCol = 0, kWeightCol = 128, kOutCol = 256;
 constexpr int kHalfBytes = kTile * 128;  // 128 rows x 64 elements, 128-byte swizzled
+// How far (base 2) below a new maximum the reference is set, and how far above the
+// reference a maximum may grow.  All rounded so that no weight is above 2^kRoom, the
+// end of fp16, however large the scores are.
+template <class T>
+constexpr float kSetBelow = kIsHalf<T> ? 12.0f : 0.0f;
+template <class T>
+constexpr float kRoom = kIsHalf<T> ? 15.9375f : 8.0f;
 constexpr int kBadRing = 8;
 constexpr int kPartRing = 4;
 
@@ -630,7 +639,7 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                 tmem_fence_before();
                 mbar_arrive(s_free);
                 largest(1);
-                const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * mul;
+                const float top = __fmul_ru(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])), mul);
                 // The product of the key tile before is in O, and has read its weights.
                 if (!first) {
                     if (!wait_bounded(&o_done[wg], (tiles_done - 1) & 1, err, kDevErrTimeoutEpilogue)) {
@@ -639,9 +648,9 @@ __global__ void __launch_bounds__(kManyThreads, 1)
                     }
                     tmem_fence_after();
                 }
-                const bool grown = top > ref + 8.0f;  // from -inf: by anything
+                const bool grown = top > __fadd_rd(ref, kRoom<T>);  // from -inf: by anything
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float now = grown ? top : ref;
+                    const float now = grown ? __fadd_ru(top, -kSetBelow<T>) : ref;
                     const float keep = grown ? exp2_approx(ref - now) : 1.0f;
                     ref = now;
                     sum *= keep;
