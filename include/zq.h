@@ -345,8 +345,13 @@ zq_status zq_append_kv(const zq_paged_batch* batch, const void* q, size_t ldq, c
  * [h * heads / kv_heads, ...) read kv head h; at most ZQ_ATTENTION_MAX_GROUP of
  * them.  q and out are [rows][heads][dim] of the cache's type, ldq and ld_out
  * elements from row to row, q 16-byte aligned with ldq a multiple of 8, out
- * 8-byte aligned with ld_out a multiple of 4; out must not overlap q.  Scores,
- * weights, sums and outputs are fp32, rounded once to out.
+ * 8-byte aligned with ld_out a multiple of 4; out must not overlap q.  Scores (to
+ * 2^27 in size), weights, sums and outputs are fp32, outputs rounded once to out.
+ * One thing is not: a request with more than 32 rows of a kv head (new tokens times
+ * the group's heads), or a prefix with so many in all, multiplies its values by
+ * weights rounded to the cache's type, half a step each (fp16: but not below 2^-37 of
+ * the largest), while their sum is that of the unrounded.  From 17 rows on, either
+ * may happen, as the call's sizes have it.
  * A row that sees no token is zero.  What a row does not see does not reach it,
  * infinities and NaN included; tokens behind a request's length are not read.
  * `workspace` (256-byte aligned) must hold zq_paged_attention_workspace_bytes

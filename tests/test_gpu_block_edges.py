@@ -88,11 +88,11 @@ def test_weights_far_below_the_largest(zb, torch, cache, nats, new, dim, prefix)
 
 
 @pytest.mark.parametrize("cache", CACHES)
-@pytest.mark.parametrize("scale", [1.0, 2.0**-5, 2.0**-6, 2.0**-7, 2.0**-8, 2.0**-9])
-@pytest.mark.parametrize("new", [1, 5])
+@pytest.mark.parametrize("scale", [2.0**-5, 2.0**-6, 2.0**-7, 2.0**-8, 2.0**-9])
+@pytest.mark.parametrize("new", [1, 5, 100])
 def test_scores_of_many_millions(zb, torch, cache, scale, new):
-    """Scores so large that neighbouring fp32 numbers lie whole powers of two of weight apart:
-    the two largest are equal and the output is their values' mean, exactly."""
+    """Scores so large (to 2^27) that neighbouring fp32 numbers lie whole powers of two of
+    weight apart: the two largest are equal and the output is their values' mean, exactly."""
     t = getattr(torch, cache)
     batch = Batch(torch, 4, [new], [400 + new], 16, 1, 64, t)
     batch.k_cache[..., 1:] = 0
@@ -102,3 +102,43 @@ def test_scores_of_many_millions(zb, torch, cache, scale, new):
     q[..., 0] = 59392.0
     got = batch.attention(zb, q.cuda(), scale=scale)
     assert torch.equal(got, torch.full_like(got, (17 % 7 + 300 % 7) / 2))
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("new", [1, 3, 100])
+def test_equal_values_come_back(zb, torch, cache, new):
+    """Where every key has the value 1, the output is 1.  Few rows: products and sums are off
+    by less than a quarter of a step of 16 bits, so 1 is the nearest.  Many: the weights of
+    the products are rounded, half a step each, those of the sum are not.  Keys up to 2^7.2
+    above the first tile's largest, with weights that are no powers of two."""
+    t = getattr(torch, cache)
+    dim = 128
+    batch = Batch(torch, 2, [new], [500 + new], 32, 2, dim, t)
+    flat(batch, torch, 0.0)
+    batch.v_cache[:] = 1.0
+    batch.k_cache[:] *= 0.01
+    for token, nats in ((3, 20), (200, 25), (333, 24), (499, 23.5)):
+        put(batch, torch, 0, token, key=nats * dim**0.5 / 8)
+    q = 0.01 * randn(torch, new, batch.rows, 8, dim)
+    q[..., 0] = torch.linspace(8.0, 6.0, batch.rows * 8).view(batch.rows, 8)
+    got = batch.attention(zb, q.to(t).cuda())
+    if new * 4 <= 16:
+        assert torch.equal(got, torch.ones_like(got))
+    else:
+        one = torch.ones(got.shape, dtype=torch.float64)
+        steps = (600 / 16 + 8) * 2.0**-22
+        within(torch, got, one, steps + torch.finfo(t).eps / 2 + half_step(torch, t, one), "ones")
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("new,heads,prefix", [([1] * 9, 4, 0), ([1] * 9, 4, 200), ([3, 4, 1], 8, 0)])
+def test_weights_of_few_rows_are_not_rounded(zb, torch, cache, new, heads, prefix):
+    """Rows of few-row items alone: the weights' two 16-bit parts hold them to 2^-17.  Values
+    of both signs cancel, so that a weight rounded once (half a step each) would show."""
+    t = getattr(torch, cache)
+    batch = Batch(torch, 31, new, [n + 60 * (i % 3) + 20 for i, n in enumerate(new)], 16, 2, 64, t, prefix=prefix)
+    if prefix:  # one row in all: the prefix's item has few rows too
+        batch = Batch(torch, 31, [1], [80], 16, 2, 64, t, prefix=prefix)
+    q = (0.5 * randn(torch, 5, batch.rows, heads, 64)).to(t)
+    want, tol = attention64(torch, batch, q, 2.0**-17)
+    within(torch, batch.attention(zb, q.cuda()), want, tol, "few rows")
