@@ -142,3 +142,27 @@ def test_weights_of_few_rows_are_not_rounded(zb, torch, cache, new, heads, prefi
     q = (0.5 * randn(torch, 5, batch.rows, heads, 64)).to(t)
     want, tol = attention64(torch, batch, q, 2.0**-17)
     within(torch, batch.attention(zb, q.cuda()), want, tol, "few rows")
+
+
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("new,lengths,dim,prefix", [([1], [700], 64, 0), ([4], [700], 128, 0), ([1, 6], [90, 641], 64, 0),
+                                                    ([2, 1], [500, 65], 128, 200), ([100], [700], 128, 0), ([1] * 3, [3000, 40, 77], 80, 0)])
+def test_infinities_that_are_seen(zb, torch, cache, new, lengths, dim, prefix):
+    """A lone infinity in the values comes out as it is, wherever it lies among the keys; with the
+    opposite one or a NaN beside it in the same element, as NaN."""
+    t = getattr(torch, cache)
+    batch = Batch(torch, 40, new, lengths, 16, 2, dim, t, prefix=prefix)
+    for token, element, value in ((0, 1, math.inf), (11, 2, -math.inf), (33, 3, math.inf), (lengths[0] // 2, 4, -math.inf),
+                                  (20, 5, math.inf), (35, 5, math.inf), (5, 6, math.inf), (lengths[0] - 9, 6, -math.inf),
+                                  (12, 7, math.nan)):
+        page, slot = int(batch.pages[0, token // 16]), token % 16
+        batch.v_cache[page, 0, slot, element] = value
+        batch.own[0][1, 0, token, element] = value
+    if prefix:
+        batch.v_cache[int(batch.prefix_pages[6]), 1, 3, 0] = math.inf
+        batch.shared[1, 1, 6 * 16 + 3, 0] = math.inf
+    q = randn(torch, 3, batch.rows, 8, dim).to(t)
+    want, tol = batch.want(q)
+    got = batch.attention(zb, q.cuda())
+    within(torch, got, want, tol, "seen infinities")
+    assert int(got.isinf().sum()) > 0

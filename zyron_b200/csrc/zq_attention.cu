@@ -201,151 +201,163 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) attend_few_kernel(cons
             }
             cp_async_commit();
         };
-#pragma unroll
-        for (int i = 0; i < kS - 1; ++i) issue(i);
-        cp_async_wait<kS - 1>();
-        __syncwarp();  // q is there
-
-        // One tile's q stays in registers; two tiles' would not fit beside their sums.
-        const auto load_q = [&](int mt, int k, uint32_t (&f)[4]) {
-            ldmatrix4(q_u + chunk_at<kD>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), f);
-        };
-        uint32_t qf[kMT == 1 ? kD / 16 : 1][4];
-        if constexpr (kMT == 1) {
-#pragma unroll
-            for (int k = 0; k < kD / 16; ++k) load_q(0, k, qf[k]);
-        }
         float o[kMT][kD / 8][4], top[kMT][2], sum[kMT][2];
+        // An infinity that a row sees comes out of the products as NaN, since the second part
+        // of a weight may be 0 or below.  An item that ends with a NaN is walked through once
+        // more, its values multiplied by whole weights, slice by slice.
+        for (bool careful = false;; careful = true) {
 #pragma unroll
-        for (int mt = 0; mt < kMT; ++mt) {
-#pragma unroll
-            for (int n = 0; n < kD / 8; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
-            top[mt][0] = top[mt][1] = -INFINITY;
-            sum[mt][0] = sum[mt][1] = 0.0f;
-        }
-
-        for (int i = 0; i < slices; ++i) {
-            issue(i + kS - 1);
+            for (int i = 0; i < kS - 1; ++i) issue(i);
             cp_async_wait<kS - 1>();
+            __syncwarp();  // q is there
+
+            // One tile's q stays in registers; two tiles' would not fit beside their sums.
+            const auto load_q = [&](int mt, int k, uint32_t (&f)[4]) {
+                ldmatrix4(q_u + chunk_at<kD>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), f);
+            };
+            uint32_t qf[kMT == 1 ? kD / 16 : 1][4];
+            if constexpr (kMT == 1) {
+#pragma unroll
+                for (int k = 0; k < kD / 16; ++k) load_q(0, k, qf[k]);
+            }
+#pragma unroll
+            for (int mt = 0; mt < kMT; ++mt) {
+#pragma unroll
+                for (int n = 0; n < kD / 8; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.0f;
+                top[mt][0] = top[mt][1] = -INFINITY;
+                sum[mt][0] = sum[mt][1] = 0.0f;
+            }
+
+            for (int i = 0; i < slices; ++i) {
+                issue(i + kS - 1);
+                cp_async_wait<kS - 1>();
+                __syncwarp();
+                const int stage = i % kS, key = key0 + i * kSlice;
+                const uint32_t k_u = ring_u + stage * kStageBytes<kD>, v_u = k_u + kSlice * kD * 2;
+                float s[kMT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kD / 16; ++k) {
+                    uint32_t f[4];
+                    // lanes 0-7 / 8-15: keys 0-7, low / high half of 16 elements; 16-31: keys 8-15
+                    ldmatrix4(k_u + chunk_at<kD>((lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)), f);
+#pragma unroll
+                    for (int mt = 0; mt < kMT; ++mt) {
+                        if constexpr (kMT > 1) load_q(mt, k, qf[0]);
+                        mma16816<T>(s[mt][0], qf[kMT == 1 ? k : 0], f[0], f[1]);
+                        mma16816<T>(s[mt][1], qf[kMT == 1 ? k : 0], f[2], f[3]);
+                    }
+                }
+                const uint32_t gone = (missing >> (2 * stage)) & 3u;
+                const bool masked = key + kSlice > low || gone;
+                uint32_t hi[kMT][4], lo[kMT][4];
+                float pr[kMT][2][4];
+#pragma unroll
+                for (int mt = 0; mt < kMT; ++mt) {
+                    float most[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float t = s[mt][n][e] * a.scale_log2;
+                            if (masked) {
+                                const int j = key + n * 8 + (lane & 3) * 2 + (e & 1);
+                                if (j >= limit[mt][e >> 1] || ((gone >> n) & 1)) t = -INFINITY;
+                            }
+                            s[mt][n][e] = t;
+                            most[e >> 1] = fmaxf(most[e >> 1], t);
+                        }
+                    float ref[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 1));
+                        most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 2));
+                        if (kLift<T> != 0.0f) most[e] = __fadd_ru(most[e], -kLift<T>);
+                        const float now = fmaxf(top[mt][e], most[e]);
+                        ref[e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: every weight is 0
+                        const float keep = exp2_approx(top[mt][e] - ref[e]);
+                        top[mt][e] = now;
+                        if (keep != 1.0f) {
+                            sum[mt][e] *= keep;
+#pragma unroll
+                            for (int n = 0; n < kD / 8; ++n) {
+                                o[mt][n][2 * e] *= keep;
+                                o[mt][n][2 * e + 1] *= keep;
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            pr[mt][n][e] = exp2_approx(s[mt][n][e] - ref[e >> 1]);
+                            sum[mt][e >> 1] += pr[mt][n][e];
+                        }
+                    // the accumulators' layout is that of the second product's left operand
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            split_pair<T>(pr[mt][n][2 * e], pr[mt][n][2 * e + 1], hi[mt][2 * n + e], lo[mt][2 * n + e]);
+                }
+                if (careful || (masked && wild_values<T, kD>(v_u, lane))) {
+                    // A value that some rows must not see is no number: 0 times it would
+                    // reach them through the product.  Each row takes its own keys' alone,
+                    // with whole weights.
+#pragma unroll 1
+                    for (int kk = 0; kk < kSlice; ++kk) {
+                        const int n = kk >> 3, from = (lane & ~3) | ((kk & 7) >> 1);
+#pragma unroll
+                        for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float w0 = n ? pr[mt][1][2 * e] : pr[mt][0][2 * e];
+                                const float w1 = n ? pr[mt][1][2 * e + 1] : pr[mt][0][2 * e + 1];
+                                const float w = __shfl_sync(0xffffffffu, kk & 1 ? w1 : w0, from);
+                                if (key + kk < limit[mt][e] && !((gone >> n) & 1)) {
+#pragma unroll
+                                    for (int d = 0; d < kD / 8; ++d) {
+                                        const T* v = reinterpret_cast<const T*>(
+                                            ring + (v_u - ring_u) + chunk_at<kD>(kk, d) + (lane & 3) * 4);
+                                        o[mt][d][2 * e] += w * to_float(v[0]);
+                                        o[mt][d][2 * e + 1] += w * to_float(v[1]);
+                                    }
+                                }
+                            }
+                    }
+                } else {
+#pragma unroll
+                    for (int d = 0; d < kD / 16; ++d) {
+                        uint32_t f[4];
+                        // lanes 0-15: keys 0-15 of elements 0-7; 16-31: of elements 8-15
+                        ldmatrix4_trans(v_u + chunk_at<kD>(lane & 15, 2 * d + (lane >> 4)), f);
+#pragma unroll
+                        for (int mt = 0; mt < kMT; ++mt) {
+                            mma16816<T>(o[mt][2 * d], hi[mt], f[0], f[1]);
+                            mma16816<T>(o[mt][2 * d + 1], hi[mt], f[2], f[3]);
+                            mma16816<T>(o[mt][2 * d], lo[mt], f[0], f[1]);
+                            mma16816<T>(o[mt][2 * d + 1], lo[mt], f[2], f[3]);
+                        }
+                    }
+                }
+                __syncwarp();  // the stage may be written again
+            }
+            cp_async_wait<0>();
             __syncwarp();
-            const int stage = i % kS, key = key0 + i * kSlice;
-            const uint32_t k_u = ring_u + stage * kStageBytes<kD>, v_u = k_u + kSlice * kD * 2;
-            float s[kMT][2][4];
+            float off = 0.0f;
 #pragma unroll
             for (int mt = 0; mt < kMT; ++mt)
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kD / 16; ++k) {
-                uint32_t f[4];
-                // lanes 0-7 / 8-15: keys 0-7, low / high half of 16 elements; 16-31: keys 8-15
-                ldmatrix4(k_u + chunk_at<kD>((lane & 7) + (lane >> 4) * 8, 2 * k + ((lane >> 3) & 1)), f);
-#pragma unroll
-                for (int mt = 0; mt < kMT; ++mt) {
-                    if constexpr (kMT > 1) load_q(mt, k, qf[0]);
-                    mma16816<T>(s[mt][0], qf[kMT == 1 ? k : 0], f[0], f[1]);
-                    mma16816<T>(s[mt][1], qf[kMT == 1 ? k : 0], f[2], f[3]);
-                }
-            }
-            const uint32_t gone = (missing >> (2 * stage)) & 3u;
-            const bool masked = key + kSlice > low || gone;
-            uint32_t hi[kMT][4], lo[kMT][4];
-            float pr[kMT][2][4];
-#pragma unroll
-            for (int mt = 0; mt < kMT; ++mt) {
-                float most[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float t = s[mt][n][e] * a.scale_log2;
-                        if (masked) {
-                            const int j = key + n * 8 + (lane & 3) * 2 + (e & 1);
-                            if (j >= limit[mt][e >> 1] || ((gone >> n) & 1)) t = -INFINITY;
-                        }
-                        s[mt][n][e] = t;
-                        most[e >> 1] = fmaxf(most[e >> 1], t);
-                    }
-                float ref[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 1));
-                    most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], 2));
-                    if (kLift<T> != 0.0f) most[e] = __fadd_ru(most[e], -kLift<T>);
-                    const float now = fmaxf(top[mt][e], most[e]);
-                    ref[e] = now == -INFINITY ? 0.0f : now;  // nothing seen yet: every weight is 0
-                    const float keep = exp2_approx(top[mt][e] - ref[e]);
-                    top[mt][e] = now;
-                    if (keep != 1.0f) {
-                        sum[mt][e] *= keep;
-#pragma unroll
-                        for (int n = 0; n < kD / 8; ++n) {
-                            o[mt][n][2 * e] *= keep;
-                            o[mt][n][2 * e + 1] *= keep;
-                        }
-                    }
-                }
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        pr[mt][n][e] = exp2_approx(s[mt][n][e] - ref[e >> 1]);
-                        sum[mt][e >> 1] += pr[mt][n][e];
-                    }
-                // the accumulators' layout is that of the second product's left operand
-#pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-                        split_pair<T>(pr[mt][n][2 * e], pr[mt][n][2 * e + 1], hi[mt][2 * n + e], lo[mt][2 * n + e]);
-            }
-            if (masked && wild_values<T, kD>(v_u, lane)) {
-                // A value that some rows must not see is no number: 0 times it would
-                // reach them through the product.  Each row takes its own keys' alone.
-#pragma unroll 1
-                for (int kk = 0; kk < kSlice; ++kk) {
-                    const int n = kk >> 3, from = (lane & ~3) | ((kk & 7) >> 1);
-#pragma unroll
-                    for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float w0 = n ? pr[mt][1][2 * e] : pr[mt][0][2 * e];
-                            const float w1 = n ? pr[mt][1][2 * e + 1] : pr[mt][0][2 * e + 1];
-                            const float w = __shfl_sync(0xffffffffu, kk & 1 ? w1 : w0, from);
-                            if (key + kk < limit[mt][e] && !((gone >> n) & 1)) {
-#pragma unroll
-                                for (int d = 0; d < kD / 8; ++d) {
-                                    const T* v = reinterpret_cast<const T*>(
-                                        ring + (v_u - ring_u) + chunk_at<kD>(kk, d) + (lane & 3) * 4);
-                                    o[mt][d][2 * e] += w * to_float(v[0]);
-                                    o[mt][d][2 * e + 1] += w * to_float(v[1]);
-                                }
-                            }
-                        }
-                }
-            } else {
-#pragma unroll
-                for (int d = 0; d < kD / 16; ++d) {
-                    uint32_t f[4];
-                    // lanes 0-15: keys 0-15 of elements 0-7; 16-31: of elements 8-15
-                    ldmatrix4_trans(v_u + chunk_at<kD>(lane & 15, 2 * d + (lane >> 4)), f);
-#pragma unroll
-                    for (int mt = 0; mt < kMT; ++mt) {
-                        mma16816<T>(o[mt][2 * d], hi[mt], f[0], f[1]);
-                        mma16816<T>(o[mt][2 * d + 1], hi[mt], f[2], f[3]);
-                        mma16816<T>(o[mt][2 * d], lo[mt], f[0], f[1]);
-                        mma16816<T>(o[mt][2 * d + 1], lo[mt], f[2], f[3]);
-                    }
-                }
-            }
-            __syncwarp();  // the stage may be written again
+                for (int n = 0; n < kD / 8; ++n) off += (o[mt][n][0] + o[mt][n][1]) + (o[mt][n][2] + o[mt][n][3]);
+            if (careful || !__any_sync(0xffffffffu, off != off)) break;
         }
-        cp_async_wait<0>();
-        __syncwarp();
 
         if (FewPlan::team_inside(way.it.start, way.it.end, at.share, worker)) {
             // All the block's warps work on this one item: one part of it, by way of
