@@ -166,3 +166,18 @@ def test_infinities_that_are_seen(zb, torch, cache, new, lengths, dim, prefix):
     got = batch.attention(zb, q.cuda())
     within(torch, got, want, tol, "seen infinities")
     assert int(got.isinf().sum()) > 0
+
+
+# ---- refusals -----------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape,message", [((3, 0, 16, 64), "kv_heads must be in"), ((3, 2, 0, 64), "page must be a multiple of 8"),
+                                           ((3, 2, 16, 0), "dim must be a multiple of 8"), ((0, 0, 16, 64), "kv_heads must be in"),
+                                           ((3, 0, 0, 0), "must be")])
+def test_caches_without_heads_tokens_or_elements(zb, torch, shape, message):
+    cache = torch.zeros(shape, dtype=torch.float16, device="cuda")
+    pages, lengths = torch.zeros(2, 1, dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    q, k = (torch.zeros(2, n, shape[3], dtype=torch.float16, device="cuda") for n in (4, shape[1]))
+    for call in (lambda: zb.paged_attention(q, cache, cache.clone(), pages, lengths),
+                 lambda: zb.append_kv(None, k, k, cache, cache.clone(), pages, lengths)):
+        with pytest.raises(zb.ZQInvalidArgument, match=message):
+            call()

@@ -598,7 +598,7 @@ def paged_attention(q, k_cache, v_cache, pages, lengths, starts=None, prefix_pag
         prefix = prefix_pages.data_ptr()
     if scale is None:
         scale = dim**-0.5 if dim else 1.0
-    if heads == 0 or heads % kv_heads:
+    if heads == 0 or kv_heads and heads % kv_heads:  # no kv heads: refused by the call itself
         raise _bad("heads must be a multiple of kv_heads")
     context, ptr = _context(index, stream)
     with context:
