@@ -297,6 +297,9 @@ zq_status zq_paged_attention(const zq_paged_batch* batch, const void* q, size_t 
     if (s != ZQ_OK) return s;
     if ((s = check_heads(heads, batch->kv_heads)) != ZQ_OK) return s;
     if (!std::isfinite(scale)) return invalid("zyron_b200: scale must be finite");
+    // the kernels' scale, of exponents to base 2; were it infinite, it would make NaN of a score of 0
+    const float scale_log2 = (float)((double)scale * 1.4426950408889634);
+    if (!std::isfinite(scale_log2)) return invalid("zyron_b200: scale is too large");
     if (ldq < heads * batch->dim || ld_out < heads * batch->dim)
         return invalid("zyron_b200: a row pitch is smaller than its row");
     if (ldq % 8 != 0 || ld_out % 4 != 0) return invalid("zyron_b200: ldq must be a multiple of 8, ld_out of 4");
@@ -321,7 +324,7 @@ zq_status zq_paged_attention(const zq_paged_batch* batch, const void* q, size_t 
     a.prefix_length = (int)prefix_length;
     a.heads = (int)heads;
     a.causal = causal != 0;
-    a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+    a.scale_log2 = scale_log2;
     const size_t need = zq::attention_workspace_bytes(a);
     if (!workspace || workspace_bytes < need) {
         char buf[128];
