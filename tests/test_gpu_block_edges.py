@@ -5,7 +5,7 @@ import math
 
 import pytest
 
-from test_gpu_block import CACHES, Batch, half_step, randn, torch, within, zb  # noqa: F401 (torch and zb are fixtures)
+from test_gpu_block import CACHES, Batch, append_case, attention_case, half_step, randn, torch, within, zb  # noqa: F401 (torch and zb are fixtures)
 
 pytestmark = pytest.mark.gpu
 
@@ -181,3 +181,22 @@ def test_caches_without_heads_tokens_or_elements(zb, torch, shape, message):
                  lambda: zb.append_kv(None, k, k, cache, cache.clone(), pages, lengths)):
         with pytest.raises(zb.ZQInvalidArgument, match=message):
             call()
+
+
+# ---- many requests --------------------------------------------------------------------------
+
+@pytest.mark.parametrize("requests,most", [(1500, 5), (1100, 2), (2100, 1)])
+def test_append_of_many_requests(zb, torch, requests, most):
+    """More rows than blocks of one token, more requests (some empty) than two rounds of the
+    search for a row's request tell apart."""
+    new = [(i * 7) % most if most > 1 else int(i % 9 == 4) for i in range(requests)]
+    batch = Batch(torch, 1, new, [n + i % 3 for i, n in enumerate(new)], 8, 1, 16, torch.bfloat16)
+    append_case(zb, torch, batch, 2, "bfloat16", 16, True, 0, "bfloat16")
+
+
+@pytest.mark.parametrize("prefix", [0, 45])
+def test_attention_of_many_requests(zb, torch, prefix):
+    """The same for the attention, and for the rows' two results with a prefix."""
+    new = [(i * 7) % 5 if i % 100 < 60 else 0 for i in range(1500)]
+    batch = Batch(torch, 70, new, [n + i % 30 for i, n in enumerate(new)], 8, 1, 32, torch.bfloat16, prefix=prefix)
+    attention_case(zb, torch, batch, 4)
