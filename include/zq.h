@@ -141,7 +141,9 @@ size_t zq_weight_padded_k(const zq_weight* w);
 /* quantization::matmul (quantization.cpp:177-238) followed, when bias is not
  * NULL, by QuantizedLinear::forward's bias add (quantized_linear.cpp:33-50).
  * x [m][rows], bias [cols] or NULL, y [m][cols]; all device pointers.
- * m <= 8 runs the HBM-bound GEMV, larger m the tcgen05 GEMM.  `workspace`
+ * 1 to 4 rows run the HBM-bound GEMV, more to 16 (where it is faster, to 64)
+ * matrix instructions fed from registers, yet more the tcgen05 GEMM.  y may lie
+ * over x: x is read before y is written.  `workspace`
  * must hold zq_matmul_workspace_bytes(w, m) bytes and must not be shared by
  * calls that may overlap on the GPU.  Results are bit-identical to the
  * reference. */
@@ -207,7 +209,8 @@ zq_status zq_dequantize_host(const zq_weight* w, float* out_host, void* stream);
  * (gelu and silu of -inf are NaN, as the formulas have it).  residual is
  * [m][ld_residual >= cols] of y_dtype or NULL; y is [m][cols] of y_dtype and
  * may be the residual itself (same pointer, ld_residual = cols), but overlap
- * it in no other way.  Same workspace rule as zq_matmul. */
+ * it in no other way; it may lie over x, not over q, row_scale or bias.  Same
+ * workspace rule as zq_matmul. */
 #define ZQ_ACT_NONE 0
 #define ZQ_ACT_GELU 1
 #define ZQ_ACT_SILU 2

@@ -200,3 +200,30 @@ def test_attention_of_many_requests(zb, torch, prefix):
     new = [(i * 7) % 5 if i % 100 < 60 else 0 for i in range(1500)]
     batch = Batch(torch, 70, new, [n + i % 30 for i, n in enumerate(new)], 8, 1, 32, torch.bfloat16, prefix=prefix)
     attention_case(zb, torch, batch, 4)
+
+
+# ---- the matmul in place --------------------------------------------------------------------
+
+@pytest.mark.parametrize("qtype", ["Int8", "Int4"])
+@pytest.mark.parametrize("m", [1, 2, 3, 4, 5, 16, 40, 300])
+def test_matmul_over_its_input(zb, torch, m, qtype):
+    """x = x + W x in place: the output lies over the activations, which every block of the
+    product needs, and over the residual."""
+    k = 2048
+    w = zb.quantize((randn(torch, 1, k, k) * 0.02).cuda(), getattr(zb.Type, qtype))
+    for activation in (None, "gelu"):
+        for _ in range(5):
+            x = randn(torch, m, m, k).cuda()
+            want = zb.matmul(x, w, activation=activation, residual=x)
+            got = zb.matmul(x, w, activation=activation, residual=x, out=x)
+            assert got.data_ptr() == x.data_ptr() and torch.equal(got, want)
+    # without an epilogue, and over a part of it
+    buffer = torch.zeros(m + 1, k, device="cuda")
+    for x, y in ((buffer[:m], buffer[:m]), (buffer[:m], buffer[1:]), (buffer[1:], buffer[:m])):
+        x.copy_(randn(torch, 9, m, k))
+        want = zb.matmul(x, w)
+        assert torch.equal(zb.matmul(x, w, out=y), want)
+    # a 16-bit output in the front half
+    x = randn(torch, 10, m, k).cuda()
+    want = zb.matmul(x, w, dtype=torch.half)
+    assert torch.equal(zb.matmul(x, w, dtype=torch.half, out=x.view(torch.half).flatten()[: m * k].view(m, k)), want)

@@ -673,9 +673,14 @@ zq_status run_codes_out(const zq_weight* w, const int8_t* codes, const float* rs
 zq_status matmul_in_workspace_out(const zq_weight* w, const float* x, size_t m, const float* bias,
                                   const zq::OutDesc& out, uint8_t* ws, cudaStream_t st) {
     const bool plain = out.count == 1 && out.ldy == (long long)w->N && out.col_offset == 0;
-    if (plain && m <= 4 && use_gemv(w, (int)m)) {
+    // Whether the output lies over the input.
+    const size_t y_size = out.epi.on && out.epi.dtype != ZQ_DTYPE_F32 ? 2 : 4;
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(out.base[0]);
+    const bool in_place = x0 < y0 + m * w->N * y_size && y0 < x0 + m * w->K * sizeof(float);
+    if (plain && m <= 4 && !in_place && use_gemv(w, (int)m)) {
         // one launch: the GEMV quantizes the rows itself (same codes and
-        // scales as the standalone quantizer)
+        // scales as the standalone quantizer).  Its blocks read x while others
+        // write y, so an output over x takes the quantizer first.
         zq::GemvArgs a{w->type, w->panel, (int)w->N, w->Kp, w->scales, nullptr, nullptr, bias, out.base[0], (int)m};
         a.x = x;
         a.K = (int)w->K;

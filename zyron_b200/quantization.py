@@ -288,7 +288,8 @@ def matmul(input, weights: QuantizedMatrix, bias=None, out=None, stream=None, ac
     "relu") of the product with its bias, then ``residual`` (the output's shape
     and type) added, all in fp32, then one rounding to ``dtype`` (float32,
     float16 or bfloat16; by default the residual's type, or float32).  ``out``
-    may be the residual itself, and overlap it in no other way.
+    may be the residual itself, and overlap it in no other way; it may lie over
+    ``input``.
     """
     ndim = input.ndim if isinstance(input, np.ndarray) else input.dim()
     if ndim < 2:
