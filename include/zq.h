@@ -355,7 +355,7 @@ zq_status zq_append_kv(const zq_paged_batch* batch, const void* q, size_t ldq, c
  * weights rounded to the cache's type, half a step each (fp16: but not below 2^-37 of
  * the largest), while their sum is that of the unrounded.  From 17 rows on, either
  * may happen, as the call's sizes have it.
- * A row that sees no token is zero.  What a row does not see does not reach it,
+ * A row that sees no token, or whose scores are all -inf, is zero.  What a row does not see does not reach it,
  * infinities and NaN included; an infinite value that it sees stays infinite, or is
  * NaN where its weight has become 0.  Tokens behind a request's length are not read.
  * `workspace` (256-byte aligned) must hold zq_paged_attention_workspace_bytes

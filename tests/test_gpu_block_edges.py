@@ -168,6 +168,28 @@ def test_infinities_that_are_seen(zb, torch, cache, new, lengths, dim, prefix):
     assert int(got.isinf().sum()) > 0
 
 
+@pytest.mark.parametrize("cache", CACHES)
+@pytest.mark.parametrize("new,prefix", [(1, 0), (5, 0), (100, 0), (1, 30), (100, 30)])
+def test_scores_of_minus_infinity(zb, torch, cache, new, prefix):
+    """A key whose score is -inf has no weight; a row that has no other is zero, as one that
+    sees none.  Scores of +inf are NaN."""
+    t = getattr(torch, cache)
+    batch = Batch(torch, 80, [new, 3, 2], [200 + new, 50, 40], 16, 1, 64, t, prefix=prefix)
+    for request, some in ((0, range(200 + new)), (1, range(0, 50, 2)), (None, range(prefix))):
+        for token in some:
+            put(batch, torch, request, token, key=-math.inf)
+    q = randn(torch, 81, batch.rows, 2, 64)
+    q[..., 0] = q[..., 0].abs() + 0.1
+    q[-1, :, 0] *= -1.0  # its last request: the prefix's scores are +inf
+    q = q.to(t)
+    want, tol = batch.want(q)
+    got = batch.attention(zb, q.cuda())
+    if prefix:
+        want[-1] = math.nan
+    within(torch, got, want, tol, "minus infinity")
+    assert not got[:new].any() and got[new:-1].any()
+
+
 # ---- refusals -----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("shape,message", [((3, 0, 16, 64), "kv_heads must be in"), ((3, 2, 0, 64), "page must be a multiple of 8"),

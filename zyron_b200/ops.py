@@ -576,8 +576,10 @@ def paged_attention(q, k_cache, v_cache, pages, lengths, starts=None, prefix_pag
     Every row sees the ``prefix_length`` tokens of a prefix that all requests
     share (on ``prefix_pages``, int32), which is computed once for all of them,
     and its request's own tokens, with ``causal`` those up to its own
-    position.  ``scale`` is 1 / sqrt(dim) by default.  A row that sees no token
-    is zero; rows that no request owns are left as ``out`` has them."""
+    position.  ``scale`` is 1 / sqrt(dim) by default.  A row that sees no token,
+    or whose scores are all -inf, is zero; rows that no request owns are left as
+    ``out`` has them.  Requests (or a prefix) of more than 32 rows of a kv head
+    multiply the values by weights rounded to the cache's type."""
     if torch is None:
         _setup()
     index = _device(q, "k_cache v_cache pages lengths starts prefix_pages out", k_cache, v_cache, pages, lengths, starts,
