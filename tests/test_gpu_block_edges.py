@@ -249,3 +249,16 @@ def test_matmul_over_its_input(zb, torch, m, qtype):
     x = randn(torch, 10, m, k).cuda()
     want = zb.matmul(x, w, dtype=torch.half)
     assert torch.equal(zb.matmul(x, w, dtype=torch.half, out=x.view(torch.half).flatten()[: m * k].view(m, k)), want)
+
+
+@pytest.mark.parametrize("qtype", ["Int8", "Int4"])
+@pytest.mark.parametrize("m,k,n", [(5, 4097, 4736), (16, 4097, 4744), (7, 8200, 9472), (16, 5000, 9488), (9, 4096, 4737)])
+def test_few_rows_at_borders_of_the_column_rule(zb, torch, m, k, n, qtype):
+    """Where blocks of 16 columns end and blocks of 32 begin: the same bits as of the
+    tcgen05 kernel."""
+    w = zb.quantize((randn(torch, k, k, n) * 0.05).cuda(), getattr(zb.Type, qtype))
+    x, b = randn(torch, m, m, k).cuda(), randn(torch, 3, n).cuda()
+    got = zb.matmul(x, w, bias=b), zb.matmul(x, w, bias=b, activation="silu", dtype=torch.half)
+    w.set_decode_kernel(1)
+    assert torch.equal(got[0], zb.matmul(x, w, bias=b))
+    assert torch.equal(got[1], zb.matmul(x, w, bias=b, activation="silu", dtype=torch.half))

@@ -185,14 +185,21 @@ cudaError_t launch_t(const GemvArgs& a, cudaStream_t stream) {
                              a.col_scale, a.q, a.row_scale, a.bias, a.y, a.M, a.epi);
 }
 
-// Blocks of 16 columns while blocks of 32 would leave SMs without one, of 32 above,
-// which read the activations half as often.  16 rows (INT4, K = 4096): N = 4096 5.2 us
-// against 6.9, N = 5120 7.2 against 7.1, N = 8192 8.9 against 7.8, N = 11008 12.0
-// against 11.0; K = 8192, N = 28672 42.6 against 31.8; INT8 N = 6144 9.4 against 9.5, N
-// = 8192 10.7 against 10.3.  32 rows: INT4 N = 4096 6.7 against 7.4, N = 11008 16.5
-// against 15.2.  64 rows go to blocks of 32 sooner, from one for two SMs on: N = 1024
-// (K = 1024) 3.8 against 5.6, N = 4096 (K = 4096) 11.7 against 10.4.
+// Blocks of 16 columns while blocks of 32 would leave SMs without a second one, of 32
+// above, which read the activations half as often.  16 rows (INT4, K = 4096): N = 4096
+// 5.2 us against 6.9, N = 8192 8.9 against 7.8, N = 11008 12.0 against 11.0; INT8 N =
+// 6144 9.4 against 9.5, N = 8192 10.7 against 10.3.  The longer the columns of INT8 the
+// more a block of 32 waits for its own loads (its warps have one step under way), so up
+// to two waves of blocks of 16 go first there (5 rows, calls): K = 8192, N = 8192 19.8
+// us against 21.4, K = 32768, N = 4736 33.3 against 61.1 (16 rows 35.1 and 61.9), N =
+// 9472 59.4 and 81.0; K = 4096, N = 8192 13.0 and 13.2 (14.4 and 13.8).
+// 32 rows: INT4 N = 4096 6.7 against 7.4, N = 11008 16.5 against 15.2.  64 rows go to
+// blocks of 32 sooner, from one for two SMs on: N = 1024 (K = 1024) 3.8 against 5.6, N =
+// 4096 (K = 4096) 11.7 against 10.4.
 bool narrow(int N) { return N < 32 * sm_count(); }
+bool narrow16(int type, int N, int Kp) {
+    return N <= 32 * sm_count() || (type == kInt8 && Kp > 4096 && N <= 64 * sm_count());
+}
 template <int kType, bool kX16>
 cudaError_t launch_columns(const GemvArgs& a, cudaStream_t stream) {
     if (a.M > 2 * kRowsTile)
@@ -201,8 +208,8 @@ cudaError_t launch_columns(const GemvArgs& a, cudaStream_t stream) {
     if (a.M > kRowsTile)
         return narrow(a.N) ? launch_t<kType, 2, 8, 2, 2, 2, kX16>(a, stream)
                            : launch_t<kType, 2, 8, 4, 2, 2, kX16>(a, stream);
-    return narrow(a.N) ? launch_t<kType, 1, 16, 2, 2, 2, kX16>(a, stream)
-                       : launch_t<kType, 1, 8, 4, 1, 4, kX16>(a, stream);
+    return narrow16(kType, a.N, a.Kp) ? launch_t<kType, 1, 16, 2, 2, 2, kX16>(a, stream)
+                                      : launch_t<kType, 1, 8, 4, 1, 4, kX16>(a, stream);
 }
 
 }  // namespace
@@ -211,7 +218,8 @@ cudaError_t launch_columns(const GemvArgs& a, cudaStream_t stream) {
 // tiles win once there are enough of them.  32 rows: INT8 K = 4096, N = 4096 8.7 us
 // against the GEMM's 15.3, N = 11008 20.7 against 24.0, K = 8192, N = 28672 71 against
 // 55; INT4 6.7 against 18.7, 15.2 against 29.9, 48 against 62.  64 rows: INT8 N = 4096
-// 11.9 against 15.4, N = 11008 31 against 24; INT4 10.4 against 18.7, 27 against 30.
+// 11.9 against 15.4, N = 11008 31 against 24; INT4 10.4 against 18.7, 27 against 30 (one
+// rule for both types: INT4 would win up to there by a tenth).
 bool rows_kernel_wins(int type, int M, int N) {
     if (M <= kRowsTile) return true;
     if (M <= 2 * kRowsTile) return type == kInt4 || N < 96 * sm_count();
