@@ -262,3 +262,22 @@ def test_few_rows_at_borders_of_the_column_rule(zb, torch, m, k, n, qtype):
     w.set_decode_kernel(1)
     assert torch.equal(got[0], zb.matmul(x, w, bias=b))
     assert torch.equal(got[1], zb.matmul(x, w, bias=b, activation="silu", dtype=torch.half))
+
+
+# ---- the activation quantizer ----------------------------------------------------------------
+
+@pytest.mark.parametrize("m", [1, 7, 300, 1300, 5000])
+@pytest.mark.parametrize("k", [1, 31, 33, 127, 129, 301, 511, 513, 1003, 1056, 1058, 2050, 2111, 2114, 4097, 4223, 4226, 6001, 8191, 8193])
+def test_quantizer_of_rows_off_the_grid(zb, torch, m, k):
+    """Odd lengths, and rows of whole words that lie off the 16-byte grid: the codes and
+    scales of the same rows with zeros behind them, which lie on it."""
+    x = randn(torch, m + k, m, k).cuda() * torch.linspace(0.0, 3.0, m, device="cuda")[:, None]
+    x[m // 2, k // 2] = math.nan
+    more = -k % 4 + 4
+    codes, scale = zb.quantize_rows(torch.nn.functional.pad(x, (0, more)))
+    got, got_scale = zb.quantize_rows(x)
+    assert torch.equal(got[:, :k], codes[:, :k]) and torch.equal(got_scale, scale)
+    whole = torch.nn.functional.pad(x, (0, more))
+    apart = torch.empty(whole.numel() + 1, device="cuda")[1:].view_as(whole).copy_(whole)
+    got, got_scale = zb.quantize_rows(apart)
+    assert torch.equal(got, codes) and torch.equal(got_scale, scale)

@@ -40,22 +40,28 @@ __device__ __forceinline__ uint32_t code_word(const float4& v, float s, float rc
 }
 
 // Rows longer than a group of warps holds below, or off the 16-byte grid (kVec
-// false: element by element): a block of kT threads a row, the first 32
-// elements of each thread in registers, the rest read again.  One warp a row
-// took 44 us for 12 rows of 11008 (5 so).
-template <int kT, bool kVec>
-__global__ void __launch_bounds__(kT) quantize_long_rows_kernel(const float* __restrict__ x, int K, int Kp,
-                                                                int8_t* __restrict__ q, float* __restrict__ row_scale,
-                                                                int* zero, int n_zero) {
+// false: element by element): kT threads a row, kRows rows a block, the first kHeld
+// loads of each thread in registers, the rest read again.  kStops: for rows that
+// need less than half of them (30000 rows of 127 9.6 us, 32 without; long rows
+// lose by it, 333 of 8190 9.8 us against 7.1).  One warp a row took 44 us
+// for 12 rows of 11008 (5 so); 256 threads a row as many rows of few elements as do
+// not fit a warp's 32 take blocks: 30000 rows of 50 160 us (6.6 by warps), 8192 of
+// 2050 61 (26 by 64 threads).
+template <int kT, int kRows, int kHeld, bool kVec, bool kStops>
+__global__ void __launch_bounds__(kT* kRows) quantize_long_rows_kernel(const float* __restrict__ x, int M, int K, int Kp,
+                                                                       int8_t* __restrict__ q,
+                                                                       float* __restrict__ row_scale, int* zero,
+                                                                       int n_zero) {
+    static_assert(kRows == 1 || kT == 32, "rows that share a block are a warp each");
     pdl_launch_dependents();
     pdl_wait_primary();  // x may come from, and q / counters be read by, the kernels before
     clear_words(zero, n_zero);
     using V = typename std::conditional<kVec, float4, float>::type;
-    constexpr int kHeld = 128 / (int)sizeof(V);
     __shared__ float part[kT / 32];
-    const int t = threadIdx.x;
-    const V* xr = reinterpret_cast<const V*>(x + (size_t)blockIdx.x * K);
-    int8_t* qr = q + (size_t)blockIdx.x * Kp;
+    const int t = threadIdx.x % kT, row = blockIdx.x * kRows + threadIdx.x / kT;
+    if (row >= M) return;
+    const V* xr = reinterpret_cast<const V*>(x + (size_t)row * K);
+    int8_t* qr = q + (size_t)row * Kp;
     const int n = kVec ? K >> 2 : K;
     const auto largest = [](const V& v, float m) {
         if constexpr (kVec)
@@ -66,18 +72,26 @@ __global__ void __launch_bounds__(kT) quantize_long_rows_kernel(const float* __r
     V v[kHeld];
     float m = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) v[i] = t + i * kT < n ? load_l2(xr + t + i * kT) : V{};
+    for (int i = 0; i < kHeld; ++i) {
+        if (kStops && i * kT >= n) break;
+        v[i] = t + i * kT < n ? load_l2(xr + t + i * kT) : V{};
+    }
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) m = largest(v[i], m);
+    for (int i = 0; i < kHeld; ++i) {
+        if (kStops && i * kT >= n) break;
+        m = largest(v[i], m);
+    }
     for (uint32_t i = t + kHeld * kT; i < (uint32_t)n; i += kT) m = largest(load_l2(xr + i), m);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((t & 31) == 0) part[t >> 5] = m;
-    __syncthreads();
+    if constexpr (kT > 32) {
+        if ((t & 31) == 0) part[t >> 5] = m;
+        __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kT / 32; ++w) m = fmaxf(m, part[w]);
+        for (int w = 0; w < kT / 32; ++w) m = fmaxf(m, part[w]);
+    }
     const float s = zq_scale_from_absmax(m, 127.0f);
-    if (t == 0) row_scale[blockIdx.x] = s;
+    if (t == 0) row_scale[row] = s;
     const float rcp = zq_quant_rcp(s);
     const auto put = [&](uint32_t i, const V& e) {
         if constexpr (kVec)
@@ -86,8 +100,10 @@ __global__ void __launch_bounds__(kT) quantize_long_rows_kernel(const float* __r
             qr[i] = (int8_t)zq_quantize_value_rcp(e, s, rcp, 127);
     };
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
+    for (int i = 0; i < kHeld; ++i) {
+        if (kStops && i * kT >= n) break;
         if (t + i * kT < n) put(t + i * kT, v[i]);
+    }
     for (uint32_t i = t + kHeld * kT; i < (uint32_t)n; i += kT) put(i, load_l2(xr + i));
     for (uint32_t i = (uint32_t)K + t; i < (uint32_t)Kp; i += kT) qr[i] = 0;
 }
@@ -169,15 +185,33 @@ cudaError_t launch_quantize_rows(const float* x, int M, int K, int Kp, int8_t* q
                                               Kp, q, row_scale, zero, n_zero);
         }
     }
-    const auto launch = [&](auto kern, int threads) {
-        return launch_pdl_kernel(kern, dim3(M), dim3(threads), 0, stream, x, K, Kp, q, row_scale, zero, n_zero);
+    const auto launch = [&](auto kern, int threads, int rows) {
+        return launch_pdl_kernel(kern, dim3((M + rows - 1) / rows), dim3(threads * rows), 0, stream, x, M, K, Kp, q,
+                                 row_scale, zero, n_zero);
     };
-    if (K <= 8192) return launch(quantize_long_rows_kernel<256, false>, 256);
+    if (K <= 8192) {
+        // As few threads a row as hold it, but more where rows are few, to shorten their way
+        // (one of 1003 elements 2.7 us, 4.2 by a warp).
+        int threads = 32;
+        while (threads < 256 && (K > 33 * threads || (K > 128 && 2LL * threads * M <= 1024 * sm_count()))) threads *= 2;
+        const bool stops = K <= 16 * threads;
+        const auto pick = [&](auto with, auto without, int rows) { return launch(stops ? with : without, threads, rows); };
+        switch (threads) {
+            case 32: return pick(quantize_long_rows_kernel<32, 8, 16, false, true>,
+                                 quantize_long_rows_kernel<32, 8, 32, false, false>, 8);
+            case 64: return pick(quantize_long_rows_kernel<64, 1, 32, false, true>,
+                                 quantize_long_rows_kernel<64, 1, 32, false, false>, 1);
+            case 128: return pick(quantize_long_rows_kernel<128, 1, 32, false, true>,
+                                  quantize_long_rows_kernel<128, 1, 32, false, false>, 1);
+            default: return pick(quantize_long_rows_kernel<256, 1, 32, false, true>,
+                                 quantize_long_rows_kernel<256, 1, 32, false, false>, 1);
+        }
+    }
     if (K <= 16384)
-        return aligned ? launch(quantize_long_rows_kernel<512, true>, 512)
-                       : launch(quantize_long_rows_kernel<512, false>, 512);
-    return aligned ? launch(quantize_long_rows_kernel<1024, true>, 1024)
-                   : launch(quantize_long_rows_kernel<1024, false>, 1024);
+        return aligned ? launch(quantize_long_rows_kernel<512, 1, 8, true, false>, 512, 1)
+                       : launch(quantize_long_rows_kernel<512, 1, 32, false, false>, 512, 1);
+    return aligned ? launch(quantize_long_rows_kernel<1024, 1, 8, true, false>, 1024, 1)
+                   : launch(quantize_long_rows_kernel<1024, 1, 32, false, false>, 1024, 1);
 }
 
 // ---------------------------------------------------------------------------
