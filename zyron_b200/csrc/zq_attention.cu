@@ -29,7 +29,8 @@
 // exp(s - m) enters the second product as a sum of two 16-bit parts, so that it is
 // not rounded to the cache's type; with fp16 m lies 2^15 below the largest score, and
 // the parts hold a weight to 2^-22 of itself or 2^-40 of the largest.  64 requests of 100 to 6000 tokens, 32 heads over
-// 8 of 128: 805 MB in 137 us with the join, 5.9 TB/s; one token over 301 keys 10.6.
+// 8 of 128: 805 MB in 137 us with the join, 5.9 TB/s; one token over 576 keys,
+// 12 heads over 4 of 64, 10.6.  (At dim 128 two tiles spill 8 to 16 bytes a thread.)
 #include "zq_attention.cuh"
 
 namespace zq {

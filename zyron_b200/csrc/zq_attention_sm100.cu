@@ -41,7 +41,8 @@
 // of which the special function unit makes 16 a cycle and SM: at dim 128 both take
 // 2048 cycles for 256 rows x 128 keys.  Measured: about 2900, and four prompts of
 // 1000 to 2600 tokens (32 heads over 8, dim 128) 224 us with their joins, the tensor
-// cores at 54 %; a 16000 key prefix of 96 rows 41.  Some of the exponentials as a
+// cores at 54 % (fp16 247); a 16000 key prefix of 96 rows, fp16, 44.  168 registers a
+// thread are what 11 warps get; 40 bytes spill.  Some of the exponentials as a
 // polynomial on the fp32 pipe cost more issue slots than they freed (one in eight
 // 258 us against 251, one in four 268, every other 296).
 //

@@ -23,7 +23,9 @@
 // The activations are what bounds wide ones (16 rows, K = 8192, N = 28672, INT4: 3.7
 // TB/s of weights and as much of codes again, 31.8 us, was 63.7).  A ring of loads
 // in registers that is refilled tile by tile costs registers, so warps, and measured
-// slower (12.3 us), as did steps dealt out to the warps one by one (9.6).
+// slower (12.3 us), as did steps dealt out to the warps one by one (9.6).  Some of the
+// shapes below are past their registers: 100 bytes a thread spill for INT4 with 33 to 64
+// rows and blocks of 16 columns, 36 for INT8 with up to 16 and blocks of 32.
 #include "zq_common.cuh"
 #include "zq_epilogue.cuh"
 #include "zq_kernels.h"
