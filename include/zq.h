@@ -206,7 +206,8 @@ zq_status zq_dequantize_host(const zq_weight* w, float* out_host, void* stream);
  *   ZQ_ACT_GELU  v / (1 + exp(-2 sqrt(2/pi) (v + 0.044715 v^3))), the tanh form
  *   ZQ_ACT_SILU  v / (1 + exp(-v))
  *   ZQ_ACT_RELU  max(v, 0)
- * (gelu and silu of -inf are NaN, as the formulas have it).  residual is
+ * (gelu and silu of -inf are NaN, as the formulas have it; where they are below
+ * 2^-119 in size, either may be 0).  residual is
  * [m][ld_residual >= cols] of y_dtype or NULL; y is [m][cols] of y_dtype and
  * may be the residual itself (same pointer, ld_residual = cols), but overlap
  * it in no other way; it may lie over x, not over q, row_scale or bias.  Same

@@ -264,6 +264,26 @@ def test_few_rows_at_borders_of_the_column_rule(zb, torch, m, k, n, qtype):
     assert torch.equal(got[1], zb.matmul(x, w, bias=b, activation="silu", dtype=torch.half))
 
 
+@pytest.mark.parametrize("m", [1, 9, 70])
+@pytest.mark.parametrize("activation", ["gelu", "silu"])
+def test_activations_far_below_zero(zb, torch, m, activation):
+    """Down to where the exponential's quotient ends (2^-126): numbers to their precision, 0
+    or the number below 2^-119, never more."""
+    w = zb.quantize(torch.eye(128).cuda())
+    x = torch.full((m, 128), -127.0)
+    x[:, 1:] = -torch.arange(127.0)  # whole codes of scale 1: -0 to -126
+    bias = torch.full((128,), 0.25)
+    got = zb.matmul(x.cuda(), w, bias=bias.cuda(), activation=activation).double().cpu()
+    v = x.double() * float(w.scales()[0]) * 127 + 0.25
+    t = 2 * math.sqrt(2 / math.pi) * (v + 0.044715 * v**3) if activation == "gelu" else v
+    want = v * torch.sigmoid(t)
+    # the product's and the bias's four roundings, by the activation's slope, and its own
+    slope = 1.2 * torch.exp(t).clamp(max=1) * (1 + t.abs())
+    slack = want.abs() * (3 * t.abs() + 8) * 2.0**-24 + 4 * 2.0**-24 * v.abs() * slope
+    within(torch, got, want, slack + half_step(torch, torch.float32, want) + 2.0**-119, activation)
+    assert (got[v <= 0] <= 0).all()
+
+
 # ---- the activation quantizer ----------------------------------------------------------------
 
 @pytest.mark.parametrize("m", [1, 7, 300, 1300, 5000])

@@ -24,7 +24,9 @@ __device__ __forceinline__ float epi_value(int32_t acc, float s_row, float s_col
 }
 
 // v / (1 + 2^t): the base-2 exponential and the reciprocal of the special
-// function unit (2^-22.5 and 2^-23 off), each one instruction.
+// function unit (2^-22.5 and 2^-23 off), each one instruction.  A quotient below
+// 2^-126 is 0, so gelu and silu are 0 from about -10.0 and -87.3 down, where they
+// are 2^-122 and 2^-119.
 __device__ __forceinline__ float epi_logistic(float v, float t) {
     float e, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
